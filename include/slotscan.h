@@ -35,6 +35,7 @@ extern "C" {
 
 #define SLOTSCAN_F32 0
 #define SLOTSCAN_BF16 1
+#define SLOTSCAN_F16 2                             /* slotrope.h and slotattn.h only */
 
 #define SLOTSCAN_MAX_SLOTS 192
 
@@ -267,7 +268,13 @@ int slotscan_gen_bwd(const void* k, const void* q, const void* v, int dtype, con
 #define SLOTSCAN_K_PROJ_DRD 14
 #define SLOTSCAN_K_PROJ_DWO 15
 #define SLOTSCAN_K_PROJ_RED 16
-#define SLOTSCAN_NK 17
+#define SLOTSCAN_K_ROPE 17
+#define SLOTSCAN_K_ROPE_BWD 18
+#define SLOTSCAN_K_ATTN 19
+#define SLOTSCAN_K_ATTN_DQ 20
+#define SLOTSCAN_K_ATTN_DKV 21
+#define SLOTSCAN_K_ATTN_JOIN 22
+#define SLOTSCAN_NK 23
 int slotscan_profile(int enable);
 int slotscan_profile_read(double* total_ms, int64_t* count, int nk);
 

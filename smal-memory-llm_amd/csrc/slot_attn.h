@@ -1,0 +1,235 @@
+// Device helpers shared by the attention kernels, forward (slotattn.hip) and backward (slotattn_bwd.hip).
+//
+// Operands of v_mfma_f32_32x32x16 (16-bit inputs): lane l holds 8 consecutive k values 8 (l >> 5) .. + 7 of row (A) or
+// column (B) l & 31; register r of the result holds row 8 (r >> 2) + 4 (l >> 5) + (r & 3) of column l & 31.  So a score
+// tile with the keys as rows has one query per lane, and its registers 8 m .. 8 m + 7, rounded to 16 bits, are the B
+// operand of the next product over the same 16 keys -- in the order 16 m + 4 h + {0..3}, 16 m + 8 + 4 h + {0..3} for
+// the lane half h -- when the A operand names its keys in that order too: two transposing LDS reads of 4 keys each.
+#pragma once
+#include "slot_common.h"
+
+namespace slotattn {
+
+using namespace slot;
+
+typedef _Float16 f16_t;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+#define LOG2E 1.4426950408889634f
+#define KT 64                                        // keys (or query rows) of a staged tile
+
+template <typename T> __device__ __forceinline__ f32x16 mfma32(const uint4& a, const uint4& b, f32x16 c);
+template <> __device__ __forceinline__ f32x16 mfma32<bf16_t>(const uint4& a, const uint4& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x16 mfma32<f16_t>(const uint4& a, const uint4& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<bf16_t>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack2<f16_t>(float lo, float hi) {
+    const f16x2 x = {(f16_t)lo, (f16_t)hi};          // round to nearest even
+    return __builtin_bit_cast(uint32_t, x);
+}
+// a result tile's registers 8 m .. 8 m + 7 as one operand
+template <typename T> __device__ __forceinline__ uint4 pack8(const f32x16& s, int m) {
+    return make_uint4(pack2<T>(s[8 * m], s[8 * m + 1]), pack2<T>(s[8 * m + 2], s[8 * m + 3]), pack2<T>(s[8 * m + 4], s[8 * m + 5]),
+                      pack2<T>(s[8 * m + 6], s[8 * m + 7]));
+}
+__device__ __forceinline__ uint4 ld16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ uint2 ld_tr(const unsigned char* p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((const lds_void*)p)));
+}
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; r++) z[r] = 0.f;
+    return z;
+}
+// the other half's value (lanes l and l ^ 32), combined
+__device__ __forceinline__ float half_max(float v) {
+    auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// wait until at most n of this wave's vector-memory operations are outstanding.  The direct loads into LDS are not
+// tracked by the compiler; every other vector-memory operation of a wave is younger or tracked, so it can only make
+// these waits longer, never shorter.
+template <int n> __device__ __forceinline__ void wait_vm() {
+    static_assert(n >= 0 && n < 64, "vmcnt is 6 bits");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (n & 15) | ((n >> 4) << 14));
+}
+// workgroup barrier that orders LDS for the compiler and adds no wait for direct loads in flight
+__device__ __forceinline__ void tile_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A staged tile: rows of D 16-bit values, their 16-byte chunks XOR-swizzled so that both kinds of operand reads are free
+// of bank conflicts: 8 consecutive rows at one chunk (row operands, 16 bytes a lane) and 4 rows x 2 chunks (transposing
+// reads).  The swizzle keeps chunk pairs together, so both see 8 distinct pairs in the 64 banks.
+template <int D> struct Tile {
+    static constexpr int CH = D / 8, ROWB = 2 * D, RP = 256 / ROWB;
+    static __device__ __forceinline__ int pos(int r, int c) { return c ^ (2 * ((r / RP) & (CH / 2 - 1))); }
+    static __device__ __forceinline__ int at(int r, int c) { return r * ROWB + 16 * pos(r, c); }
+    // chunk 2 kk + h of row r: the row operand of k step kk
+    static __device__ __forceinline__ uint4 row_op(const unsigned char* s, int r, int kk, int lane) {
+        return ld16(s + at(r + (lane & 31), 2 * kk + (lane >> 5)));
+    }
+    // 8 rows (r + 16 m + 4 h .. + 3 and + 8) of column 32 dt + (l & 31): the operand over rows in a result tile's order
+    static __device__ __forceinline__ uint4 col_op(const unsigned char* s, int r, int dt, int m, int lane) {
+        const int row = r + 16 * m + 4 * (lane >> 5) + ((lane & 15) >> 2);
+        const int c = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), by = 8 * (lane & 1);
+        const uint2 lo = ld_tr(s + at(row, c) + by), hi = ld_tr(s + at(row + 8, c) + by);
+        return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+};
+
+// Direct global -> LDS loads of `rows` rows by one of NW waves: load(i) fills 1 KB.  Rows past `last` repeat it: what they
+// hold never counts (their scores are masked), and nothing outside the tensor is read.
+template <int D, int ROWS, int NW> struct TileLoad {
+    static constexpr int N = ROWS * 2 * D / 1024 / NW;                // loads per wave
+    static_assert(ROWS * 2 * D % (1024 * NW) == 0, "whole loads");
+    template <typename T>
+    static __device__ __forceinline__ void issue(const T* base, int64_t st, int r0, int last, unsigned lds, int w, int lane) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int p = 64 * (N * w + i) + lane, r = p / Tile<D>::CH, c = Tile<D>::pos(r, p % Tile<D>::CH);
+            dma16(base + min(r0 + r, last) * st + 8 * c, lds + 1024u * (N * w + i));
+        }
+    }
+};
+
+// The keys of a tile [j0, j1] that queries of positions [p0, p1] see: none, some or all of the pairs.
+struct Span { int p0, p1, lo, hi; bool one; };       // positions; documents: range of ids, all of one document
+struct Mask {
+    int causal, W, prefix, klen;
+    __device__ __forceinline__ bool band(int p, int j) const {
+        const int d = p - j;
+        return causal ? (d >= 0 && d < W) : (abs(d) < W);
+    }
+    __device__ __forceinline__ bool sees(int p, int j) const { return (band(p, j) || (j < prefix && p >= 0)) && j < klen; }
+    __device__ __forceinline__ bool some(const Span& s, int j0, int j1) const {
+        // the closest pair's distance, p - j
+        const bool b = causal ? (j0 <= s.p1 && s.p0 - j1 < W) : (s.p0 - j1 < W && j0 - s.p1 < W);
+        return (b || j0 < prefix) && j0 < klen;
+    }
+    __device__ __forceinline__ bool all(const Span& s, int j0, int j1) const {
+        const bool b = causal ? (j1 <= s.p0 && s.p1 - j0 < W) : (s.p1 - j0 < W && j1 - s.p0 < W);
+        return (b || (j1 < prefix && s.p0 >= 0)) && j1 < klen;
+    }
+};
+
+struct AttnArgs {
+    const void* q; const void* k; const void* v;
+    int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
+    int B, Tq, Tk, Hq, Hk, R;                        // R = Hq / Hk
+    int causal, W;
+    const float* slopes;
+    const int32_t* ids; const int2* range; int ntd;  // documents: padded ids (B, 64 ntd), ranges (B, ntd)
+    const int32_t* prefix; const int32_t* lens;
+    float sc;                                        // scale log2(e): scores in base 2
+    float ct, c2;                                    // capped: 2 scale log2(e) / cap, cap log2(e)
+    void* out; float* lse;
+    // split rows
+    float* po; float* pm; int chunk, nsplit, tiles;
+    // backward
+    const void* dout; int64_t do_sb, do_sh, do_st;
+    float* delta; void* dq; void* dk; void* dv;
+    float* part; float scale;
+};
+
+// key of register r of a score tile's lane half h, from the tile's first key
+__device__ __forceinline__ constexpr int key_of(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// Scores of 32 keys from key j0 on in base 2, from the products s: scaled, capped and biased.  One query per lane, at
+// position p; slope in base 2.
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ void scores(f32x16& s, const AttnArgs& a, float slope, int p, int j0, int h) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        // cap tanh(x) = cap - 2 cap / (1 + e^2x): off by a few 2^-24 of the cap
+        if constexpr (CAP) s[r] = fmaf(-2.f * a.c2, __builtin_amdgcn_rcpf(1.f + exp2_(s[r] * a.ct)), a.c2);
+        else s[r] *= a.sc;
+    }
+    if constexpr (BIAS) {
+        const float d = (float)(p - j0 - 4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = fmaf(-slope, fabsf(d - (float)key_of(r, 0)), s[r]);
+    }
+}
+
+// Tokens of sequence b that count, and its length that positions are taken from (a length past the keys keeps its positions).
+__device__ __forceinline__ int length_of(const AttnArgs& a, int b) { return a.lens ? min(max(a.lens[b], 0), 1 << 30) : a.Tk; }
+
+// range of the ids of rows [i0, i0 + n) of sequence b (n <= 128), by one wave; one: all rows of one document
+__device__ __forceinline__ void rows_range(const int32_t* ids, int64_t base, int i0, int n, int lane, Span& s) {
+    int lo = 0x7fffffff, hi = -1;
+    bool pad = false;
+    for (int e = lane; e < n; e += 64) {
+        const int x = ids[base + i0 + e];
+        pad |= x < 0;
+        lo = min(lo, x < 0 ? 0x7fffffff : x);
+        hi = max(hi, x);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        lo = min(lo, __shfl_xor(lo, m));
+        hi = max(hi, __shfl_xor(hi, m));
+    }
+    s.lo = lo;
+    s.hi = hi;
+    s.one = lo == hi && __ballot(pad) == 0;
+}
+
+// range of the ids of a document tile as slotattn_docs leaves it: x = smallest (bit 31: some are padding), y = largest
+__device__ __forceinline__ int range_lo(int2 r) { return r.x & 0x7fffffff; }
+__device__ __forceinline__ bool range_one(int2 r) { return r.x == r.y; }
+
+// The walk over the 64-key tiles that a workgroup's queries see.  Each lane tests one of 64 tiles at a time; what a
+// workgroup visits, a wave computes and a wave computes without masks are three ballots.
+struct Walk {
+    const Mask& mk;
+    const Span& sw; const Span& sv;                  // positions of the workgroup's queries and of the wave's
+    const int2* range;                               // documents of this sequence, or null
+    int nt, base, lane;
+    uint64_t act = 0, mine = 0, full = 0;
+    __device__ __forceinline__ Walk(const Mask& m, const Span& w, const Span& v, const int2* r, int l) : mk(m), sw(w), sv(v), range(r), lane(l) {
+        // up to the band's or the prefix' end, from the band's start where there is no prefix
+        const int end = mk.causal ? min(mk.klen, max(sw.p1 + 1, mk.prefix)) : mk.klen;
+        nt = (end + KT - 1) / KT;
+        base = (mk.prefix > 0 ? 0 : (max(0, max(sw.p0, 0) - mk.W + 1) / KT) & ~63) - 64;
+    }
+    // the next visible tile (-1: none), whether this wave's rows see any of it and whether they see all of it
+    __device__ __forceinline__ void next(int& jt, bool& some, bool& all) {
+        while (!act) {
+            base += 64;
+            if (base >= nt) { jt = -1; return; }
+            const int x = base + lane, j0 = x * KT, j1 = j0 + KT - 1;
+            const bool in = x < nt;
+            int2 r = make_int2(0, 0);
+            if (range && in) r = range[x];
+            act = __ballot(in && mk.some(sw, j0, j1) && (!range || (range_lo(r) <= sw.hi && sw.lo <= r.y)));
+            mine = __ballot(in && sv.p0 <= sv.p1 && mk.some(sv, j0, j1) && (!range || (range_lo(r) <= sv.hi && sv.lo <= r.y)));
+            full = __ballot(in && mk.all(sv, j0, j1) && (!range || (sv.one && range_one(r) && r.y == sv.lo)));
+        }
+        const int i = __builtin_ctzll(act);
+        act &= act - 1;
+        jt = base + i;
+        some = mine >> i & 1;
+        all = full >> i & 1;
+    }
+};
+
+}  // namespace slotattn

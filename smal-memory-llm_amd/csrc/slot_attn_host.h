@@ -1,0 +1,57 @@
+// Argument checks and kernel arguments shared by the attention entry points (slotattn.hip, slotattn_bwd.hip).
+#pragma once
+#include "slot_attn.h"
+#include "slot_host.h"
+#include "slotscan.h"
+
+#define SLOTATTN_MAX_T 0x3fffffffLL                  // positions and their differences stay in 31 bits
+
+namespace slotattn_host {
+
+inline int check(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                 const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
+                 int64_t Hk, int64_t D, int64_t window, float cap) {
+    using slothost::fail;
+    using slothost::al16;
+    if (B < 1 || Tq < 1 || Tk < 1 || Hq < 1 || Hk < 1) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: B, Tq, Tk, Hq, Hk must be >= 1");
+    if (Hq % Hk) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: Hq must be a multiple of Hk");
+    if (D != 64 && D != 128) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: D must be 64 or 128");
+    if (window < 1 || window > 0x7fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: window must be in [1, 2^31)");
+    if (!(cap >= 0.f)) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: cap must be >= 0");
+    if (Tq > SLOTATTN_MAX_T || Tk > SLOTATTN_MAX_T || B > 0x7fffffffLL / Hq || Hq / Hk * Tq > SLOTATTN_MAX_T)
+        return fail(SLOTSCAN_ERR_SHAPE, "slotattn: shape too large");
+    if (dtype != SLOTSCAN_BF16 && dtype != SLOTSCAN_F16) return fail(SLOTSCAN_ERR_DTYPE, "slotattn: dtype must be bf16 or fp16");
+    if (!q || !k || !v) return fail(SLOTSCAN_ERR_NULL, "slotattn: a required pointer is NULL");
+    if (!al16(q) || !al16(k) || !al16(v) || (q_sb | q_sh | q_st | k_sb | k_sh | k_st | v_sb | v_sh | v_st) % 8)
+        return fail(SLOTSCAN_ERR_ALIGN, "slotattn: rows of q, k and v must be 16-byte aligned");
+    return 0;
+}
+
+inline slotattn::AttnArgs args(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
+                               int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int64_t B, int64_t Tq, int64_t Tk,
+                               int64_t Hq, int64_t Hk, float scale, int causal, int64_t window, float cap, const float* slopes,
+                               const void* docs, const int32_t* prefix) {
+    slotattn::AttnArgs a{};
+    a.q = q; a.k = k; a.v = v;
+    a.q_sb = q_sb; a.q_sh = q_sh; a.q_st = q_st;
+    a.k_sb = k_sb; a.k_sh = k_sh; a.k_st = k_st;
+    a.v_sb = v_sb; a.v_sh = v_sh; a.v_st = v_st;
+    a.B = (int)B; a.Tq = (int)Tq; a.Tk = (int)Tk; a.Hq = (int)Hq; a.Hk = (int)Hk; a.R = (int)(Hq / Hk);
+    a.causal = causal != 0;
+    a.W = (int)window;
+    a.slopes = slopes;
+    a.ntd = (int)((Tk + KT - 1) / KT);
+    a.ids = (const int32_t*)docs;
+    a.range = docs ? (const int2*)((const int32_t*)docs + B * a.ntd * KT) : nullptr;
+    a.prefix = prefix;
+    a.scale = scale;
+    a.sc = scale * LOG2E;
+    if (cap > 0.f) {
+        a.ct = 2.f * scale * LOG2E / cap;
+        a.c2 = cap * LOG2E;
+    }
+    a.nsplit = 1;
+    return a;
+}
+
+}  // namespace slotattn_host

@@ -1,0 +1,472 @@
+// Exact attention of any range for MI355X (gfx950), forward: scores optionally capped by a tanh and biased by the
+// distance, visible in a band, within documents and in a prefix (semantics: slotattn.h).
+//
+//   attn_fwd    many query rows: 128 queries of one head per workgroup, 32 per wave; one pass over the visible 64-key
+//               tiles with the running maximum and sum of the softmax.
+//   attn_split  few query rows against many keys (a generated token, a short chunk): the rows of a key/value head's query
+//               heads together, the keys split over waves and workgroups; attn_join combines the parts.
+#include "slot_attn.h"
+#include "slotscan.h"
+#include "slotattn.h"
+#include "slot_attn_host.h"
+
+using namespace slotattn;
+using slothost::fail;
+using slothost::hip_fail;
+using slothost::al16;
+
+#define FW 4                                         // waves per workgroup
+#define FT (64 * FW)
+#define FQ (32 * FW)                                 // query rows per workgroup
+
+namespace {
+
+// ------------------------------------------------------------------------------------------- documents
+// One wave per 64 ids: the padded copy (-1 past the end and for every padding id) and the range of the tile's ids.
+__global__ __launch_bounds__(64) void attn_docs(const int32_t* ids, int T, int ntd, int32_t* out, int2* range) {
+    const int b = blockIdx.y, lane = threadIdx.x, i = blockIdx.x * KT + lane;
+    int x = i < T ? ids[(int64_t)b * T + i] : -1;
+    x = x < 0 ? -1 : x;
+    out[((int64_t)b * ntd) * KT + i] = x;
+    int lo = x < 0 ? 0x7fffffff : x, hi = x;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        lo = min(lo, __shfl_xor(lo, m));
+        hi = max(hi, __shfl_xor(hi, m));
+    }
+    const bool pad = __ballot(x < 0) != 0;
+    if (lane == 0) range[(int64_t)b * ntd + blockIdx.x] = make_int2(pad ? (int)((unsigned)lo | 0x80000000u) : lo, hi < 0 ? -2 : hi);
+}
+
+// ------------------------------------------------------------------------------------------- many rows
+template <typename T, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
+    constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
+    typedef TileLoad<D, KT, FW> Load;
+    __shared__ __align__(1024) unsigned char smem[2][2][STAGE];      // [buffer][keys, values]
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // the longest rows (the last tiles under causality) first
+    const int heads = a.B * a.Hq;
+    const int qt = a.tiles - 1 - blockIdx.x / heads, bh = blockIdx.x % heads;
+    const int b = bh / a.Hq, hq = bh - b * a.Hq, hk = hq / a.R;
+    const int len = length_of(a, b), t0 = qt * FQ, off = len - a.Tq;
+    const int t = t0 + 32 * w + (lane & 31), tc = min(t, a.Tq - 1), p = tc + off;
+    Mask mk{a.causal, a.W, a.prefix ? a.prefix[b] : 0, min(len, a.Tk)};
+    // this wave's queries, in operand order
+    uint4 qf[KK];
+    {
+        const T* q = (const T*)a.q + b * a.q_sb + hq * a.q_sh + tc * a.q_st + 8 * h;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) qf[kk] = ld16(q + 16 * kk);
+    }
+    const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
+    const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
+    const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
+    const bool docs = a.ids != nullptr;
+    const int64_t idb = (int64_t)b * a.ntd * KT;
+    Span sw{t0 + off, min(t0 + FQ, a.Tq) - 1 + off, 0, 0, true}, sv{t0 + 32 * w + off, min(t0 + 32 * w + 32, a.Tq) - 1 + off, 0, 0, true};
+    int dq = 0;
+    if (docs) {
+        rows_range(a.ids, idb, sw.p0, sw.p1 - sw.p0 + 1, lane, sw);
+        rows_range(a.ids, idb, min(sv.p0, sw.p1), max(sv.p1 - sv.p0 + 1, 1), lane, sv);
+        dq = a.ids[idb + p];
+        if (dq < 0) dq = -2;
+    }
+    Walk walk(mk, sw, sv, docs ? a.range + (int64_t)b * a.ntd : nullptr, lane);
+    const unsigned lds = lds_addr(smem);
+    auto load = [&](int jt, int buf) {
+        Load::issue(kb, a.k_st, jt * KT, mk.klen - 1, lds + (2 * buf) * STAGE, w, lane);
+        Load::issue(vb, a.v_st, jt * KT, mk.klen - 1, lds + (2 * buf + 1) * STAGE, w, lane);
+    };
+    f32x16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) o[dt] = zero16();
+    float m = -INFINITY, l = 0.f;
+    int jt, jn;
+    bool some, all, some_n = false, all_n = false;
+    walk.next(jt, some, all);
+    if (jt >= 0) load(jt, 0);
+    for (int buf = 0; jt >= 0; buf ^= 1, jt = jn, some = some_n, all = all_n) {
+        walk.next(jn, some_n, all_n);
+        if (jn >= 0) {
+            load(jn, buf ^ 1);
+            wait_vm<2 * Load::N>();
+        } else {
+            wait_vm<0>();
+        }
+        tile_barrier();                               // the tile is there, for every wave
+        if (some) {
+            const unsigned char* sk = smem[buf][0];
+            const unsigned char* sx = smem[buf][1];
+            const int j0 = jt * KT;
+            f32x16 s[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                s[u] = zero16();
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++) s[u] = mfma32<T>(Tile<D>::row_op(sk, 32 * u, kk, lane), qf[kk], s[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++) scores<CAP, BIAS>(s[u], a, slope, p, j0 + 32 * u, h);
+            if (!all) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int j = j0 + 32 * u + key_of(r, h);
+                        bool ok = mk.sees(p, j);
+                        if (docs) ok = ok && a.ids[idb + j] == dq;
+                        s[u][r] = ok ? s[u][r] : -INFINITY;
+                    }
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
+            mx = half_max(mx);
+            const float mn = fmaxf(m, mx);
+            if (__any(mn > m)) {
+                const float f = m == -INFINITY ? 0.f : exp2_(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[dt][r] *= f;
+            }
+            const float mu = m == -INFINITY ? 0.f : m;
+            uint4 pf[2][2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[u][r] = exp2_(s[u][r] - mu);
+                    l += s[u][r];
+                }
+                pf[u][0] = pack8<T>(s[u], 0);
+                pf[u][1] = pack8<T>(s[u], 1);
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(Tile<D>::col_op(sx, 32 * u, dt, mm, lane), pf[u][mm], o[dt]);
+        }
+        tile_barrier();                               // every wave has read the tile
+    }
+    l = half_sum(l);
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    if (t < a.Tq) {
+        T* out = (T*)a.out + (((int64_t)b * a.Tq + t) * a.Hq + hq) * D;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                uint2 x = make_uint2(pack2<T>(o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv), pack2<T>(o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv));
+                *reinterpret_cast<uint2*>(out + 32 * dt + 8 * g + 4 * h) = x;
+            }
+        if (a.lse && h == 0) a.lse[(int64_t)bh * a.Tq + t] = l > 0.f || l != l ? m + __builtin_amdgcn_logf(l) : INFINITY;
+    }
+}
+
+// ------------------------------------------------------------------------------------------- few rows
+// Rows of a key/value head packed as (token, query head of the group); a workgroup takes `chunk` keys of 32 rows, its
+// waves every 4th 32-key tile of them, each with a private ring of two tiles; the waves' results meet in LDS, the
+// workgroups' in attn_join.  Bound by the bytes of the keys and values.
+template <typename T, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
+    constexpr int KK = D / 16, DT = D / 32, ST = 32 * 2 * D;
+    typedef TileLoad<D, 32, 1> Load;
+    __shared__ __align__(1024) unsigned char smem[FW][2][2][ST];     // [wave][buffer][keys, values]
+    __shared__ float s_m[FW][32], s_l[FW][32];
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int sp = blockIdx.x % a.nsplit, rt = blockIdx.x / a.nsplit;
+    const int hk = blockIdx.y, b = blockIdx.z;
+    const int rows = a.Tq * a.R, r0 = rt * 32, row = min(r0 + (lane & 31), rows - 1);
+    const int t = row / a.R, hq = hk * a.R + row - t * a.R;
+    const int len = length_of(a, b), klen = min(len, a.Tk), off = len - a.Tq, p = t + off;
+    Mask mk{a.causal, a.W, a.prefix ? a.prefix[b] : 0, klen};
+    const Span s{r0 / a.R + off, (min(r0 + 32, rows) - 1) / a.R + off, 0, 0, true};
+    // this workgroup's keys
+    const int end = a.causal ? min(klen, max(s.p1 + 1, mk.prefix)) : klen;
+    const int lo = (mk.prefix > 0 ? 0 : max(0, max(s.p0, 0) - a.W + 1) & ~31) + sp * a.chunk, hi = min(end, lo + a.chunk);
+    const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
+    const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
+    const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
+    const unsigned lds = lds_addr(smem[w]);
+    auto load = [&](int j0, int buf) {
+        Load::issue(kb, a.k_st, j0, klen - 1, lds + (2 * buf) * ST, 0, lane);
+        Load::issue(vb, a.v_st, j0, klen - 1, lds + (2 * buf + 1) * ST, 0, lane);
+    };
+    auto seen = [&](int j0) {                         // the next of this wave's tiles that any row sees
+        while (j0 < hi && !mk.some(s, j0, j0 + 31)) j0 += 32 * FW;
+        return j0;
+    };
+    int j0 = seen(lo + 32 * w);
+    if (j0 < hi) load(j0, 0);
+    uint4 qf[KK];
+    {
+        const T* q = (const T*)a.q + b * a.q_sb + hq * a.q_sh + t * a.q_st + 8 * h;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) qf[kk] = ld16(q + 16 * kk);
+    }
+    f32x16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) o[dt] = zero16();
+    float m = -INFINITY, l = 0.f;
+    for (int buf = 0; j0 < hi; buf ^= 1) {
+        const int jn = seen(j0 + 32 * FW);
+        if (jn < hi) {
+            load(jn, buf ^ 1);
+            wait_vm<2 * Load::N>();
+        } else {
+            wait_vm<0>();
+        }
+        asm volatile("" ::: "memory");
+        const unsigned char* sk = smem[w][buf][0];
+        const unsigned char* sx = smem[w][buf][1];
+        f32x16 x = zero16();
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) x = mfma32<T>(Tile<D>::row_op(sk, 0, kk, lane), qf[kk], x);
+        scores<CAP, BIAS>(x, a, slope, p, j0, h);
+        if (j0 + 32 > hi || !mk.all(s, j0, j0 + 31)) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int j = j0 + key_of(r, h);
+                x[r] = j < hi && mk.sees(p, j) ? x[r] : -INFINITY;
+            }
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) mx = fmaxf(mx, x[r]);
+        mx = half_max(mx);
+        const float mn = fmaxf(m, mx);
+        if (__any(mn > m)) {
+            const float f = m == -INFINITY ? 0.f : exp2_(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[dt][r] *= f;
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            x[r] = exp2_(x[r] - mu);
+            l += x[r];
+        }
+        const uint4 pf[2] = {pack8<T>(x, 0), pack8<T>(x, 1)};
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(Tile<D>::col_op(sx, 0, dt, mm, lane), pf[mm], o[dt]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the tile is read before its buffer is filled again
+        j0 = jn;
+    }
+    l = half_sum(l);
+    // the waves' parts: (m, l) of every row to all, then the weighted sums through LDS (its tiles are read)
+    if (h == 0) { s_m[w][lane] = m; s_l[w][lane] = l; }
+    __syncthreads();
+    float M = -INFINITY, Ls = 0.f;
+#pragma unroll
+    for (int i = 0; i < FW; i++) M = fmaxf(M, s_m[i][lane & 31]);
+    const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int i = 0; i < FW; i++) Ls += s_l[i][lane & 31] * exp2_(s_m[i][lane & 31] - Mu);
+    const float f = exp2_(m - Mu);
+    float* so = reinterpret_cast<float*>(smem);       // [wave][row][D + 4]
+    constexpr int SO = D + 4;
+    static_assert(FW * 32 * SO * 4 <= (int)sizeof(smem), "the waves' sums fit");
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *reinterpret_cast<float4*>(so + (w * 32 + (lane & 31)) * SO + 32 * dt + 8 * g + 4 * h) =
+                make_float4(o[dt][4 * g] * f, o[dt][4 * g + 1] * f, o[dt][4 * g + 2] * f, o[dt][4 * g + 3] * f);
+    if (w == 0 && h == 0) { s_m[0][lane] = Ls; s_l[0][lane] = M; }    // read again behind the barrier
+    __syncthreads();
+    // 32 rows x D values: 8 lanes a row
+    const int rr = tid >> 3, c8 = tid & 7, g = r0 + rr;
+    if (g >= rows) return;
+    const float lr = s_m[0][rr], mr = s_l[0][rr];
+    const bool got = lr > 0.f || lr != lr;
+    const float inv = got ? 1.f / lr : 0.f;
+    const int gt = g / a.R, gh = hk * a.R + g - gt * a.R;
+    const int64_t orow = ((int64_t)b * a.Tq + gt) * a.Hq + gh;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+        const int d = 4 * c8 + 32 * i;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int ww = 0; ww < FW; ww++) {
+            const float4 y = *reinterpret_cast<const float4*>(so + (ww * 32 + rr) * SO + d);
+            v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+        }
+        if (a.nsplit == 1) {
+            *reinterpret_cast<uint2*>((T*)a.out + orow * D + d) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+        } else {
+            *reinterpret_cast<float4*>(a.po + (orow * a.nsplit + sp) * D + d) = v;
+        }
+    }
+    if (c8 == 0) {
+        if (a.nsplit == 1) {
+            if (a.lse) a.lse[((int64_t)b * a.Hq + gh) * a.Tq + gt] = got ? mr + __builtin_amdgcn_logf(lr) : INFINITY;
+        } else {
+            *reinterpret_cast<float2*>(a.pm + (orow * a.nsplit + sp) * 2) = make_float2(mr, lr);
+        }
+    }
+}
+
+// One wave per row: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, the parts in order
+template <typename T, int D>
+__global__ __launch_bounds__(FT) void attn_join(AttnArgs a, int64_t nrows) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * FW + (threadIdx.x >> 6);
+    if (row >= nrows) return;
+    const float2* pm = reinterpret_cast<const float2*>(a.pm) + row * a.nsplit;
+    float M = -INFINITY;
+    for (int s = lane; s < a.nsplit; s += 64) M = fmaxf(M, pm[s].x);
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) M = fmaxf(M, __shfl_xor(M, i));
+    const float Mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc[D / 64];
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) acc[i] = 0.f;
+    for (int s = 0; s < a.nsplit; s++) {
+        const float2 x = pm[s];
+        if (x.y == 0.f) continue;                     // nothing visible in this part
+        const float f = exp2_(x.x - Mu);
+        L = fmaf(x.y, f, L);
+        const float* o = a.po + (row * a.nsplit + s) * D + lane * (D / 64);
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) acc[i] = fmaf(o[i], f, acc[i]);
+    }
+    const bool got = L > 0.f || L != L;
+    const float inv = got ? 1.f / L : 0.f;
+    T* out = (T*)a.out + row * D + lane * (D / 64);
+    if constexpr (D == 128) *reinterpret_cast<uint32_t*>(out) = pack2<T>(acc[0] * inv, acc[1] * inv);
+    else *reinterpret_cast<uint16_t*>(out) = (uint16_t)pack2<T>(acc[0] * inv, 0.f);
+    if (a.lse && lane == 0) {
+        const int64_t tok = row / a.Hq;
+        const int hq = (int)(row - tok * a.Hq);
+        const int64_t b = tok / a.Tq;
+        a.lse[(b * a.Hq + hq) * a.Tq + tok - b * a.Tq] = got ? M + __builtin_amdgcn_logf(L) : INFINITY;
+    }
+}
+
+template <typename T, int D, bool CAP, bool BIAS>
+void launch_one(const AttnArgs& a, bool split, hipStream_t st) {
+    if (split) slothost::launch(attn_split<T, D, CAP, BIAS>, dim3((unsigned)(a.nsplit * a.tiles), (unsigned)a.Hk, (unsigned)a.B), dim3(FT), 0, st, a);
+    else slothost::launch(attn_fwd<T, D, CAP, BIAS>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(FT), 0, st, a);
+}
+template <typename T, int D>
+void launch_fwd(const AttnArgs& a, bool cap, bool split, hipStream_t st) {
+    if (cap) a.slopes ? launch_one<T, D, true, true>(a, split, st) : launch_one<T, D, true, false>(a, split, st);
+    else a.slopes ? launch_one<T, D, false, true>(a, split, st) : launch_one<T, D, false, false>(a, split, st);
+}
+template <typename T, int D>
+void launch_join(const AttnArgs& a, hipStream_t st) {
+    const int64_t rows = (int64_t)a.B * a.Tq * a.Hq;
+    slothost::launch(attn_join<T, D>, dim3((unsigned)((rows + FW - 1) / FW)), dim3(FT), 0, st, a, rows);
+}
+
+// How the forward runs.  split: the packed rows and split keys, where 128-row tiles would leave most of the card idle
+// (fewer workgroups than CUs) or most of each tile empty (at most 32 rows of a key/value head).
+struct Plan { bool split; int chunk, nsplit, rtiles; };
+Plan plan(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal, int64_t W, bool docs, bool prefix) {
+    Plan p{false, 0, 1, 0};
+    const int64_t rows = Tq * (Hq / Hk), tiles = (Tq + FQ - 1) / FQ * Hq * B;
+    if (docs || !(rows <= 32 || (tiles < 256 && Tk > 512))) return p;
+    p.split = true;
+    p.rtiles = (int)((rows + 31) / 32);
+    // keys that one row tile can see
+    int64_t keys = Tk;
+    if (causal && !prefix && W < Tk) keys = W + Tq + 32 < Tk ? W + Tq + 32 : Tk;
+    // one workgroup a CU (its rings fill the LDS): two rounds of them, of at least two tiles a wave
+    const int64_t want = (512 + p.rtiles * Hk * B - 1) / (p.rtiles * Hk * B);
+    int64_t chunk = (keys + want - 1) / want;
+    chunk = (chunk + 127) / 128 * 128;
+    if (chunk < 256) chunk = 256;
+    p.chunk = (int)chunk;
+    p.nsplit = (int)((keys + chunk - 1) / chunk);
+    return p;
+}
+size_t split_bytes(const Plan& p, int64_t B, int64_t Tq, int64_t Hq, int64_t D) {
+    return p.nsplit == 1 ? 0 : (size_t)(B * Tq * Hq * p.nsplit) * (D + 2) * sizeof(float);
+}
+
+}  // namespace
+
+// ======================================================================================== C-ABI
+extern "C" size_t slotattn_docs_bytes(int64_t B, int64_t T) {
+    if (B < 1 || T < 1) return 0;
+    const int64_t n = (T + KT - 1) / KT;
+    return (size_t)(B * n) * (KT * 4 + 8);
+}
+
+extern "C" int slotattn_docs(const int32_t* ids, int64_t B, int64_t T, void* docs, void* stream) {
+    if (B < 1 || T < 1 || B > 65535 || T > SLOTATTN_MAX_T) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_docs: B in [1, 65535], T in [1, 2^30)");
+    if (!ids || !docs) return fail(SLOTSCAN_ERR_NULL, "slotattn_docs: a required pointer is NULL");
+    if (!al16(docs)) return fail(SLOTSCAN_ERR_ALIGN, "slotattn_docs: docs must be 16-byte aligned");
+    const int n = (int)((T + KT - 1) / KT);
+    slothost::launch(attn_docs, dim3((unsigned)n, (unsigned)B), dim3(64), 0, (hipStream_t)stream, ids, (int)T, n, (int32_t*)docs,
+                     (int2*)((int32_t*)docs + B * n * KT));
+    hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : hip_fail(e, "attn_docs launch");
+}
+
+extern "C" size_t slotattn_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int causal, int64_t window,
+                                         int has_docs, int has_prefix) {
+    if (B < 1 || Tq < 1 || Tk < 1 || Hk < 1 || Hq < Hk || Hq % Hk) return 0;
+    return split_bytes(plan(B, Tq, Tk, Hq, Hk, causal, window, has_docs, has_prefix), B, Tq, Hq, D);
+}
+
+extern "C" int slotattn_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
+                            int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int dtype, int64_t B, int64_t Tq,
+                            int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal, int64_t window, float cap,
+                            const float* slopes, const void* docs, const int32_t* prefix, const int32_t* lens, void* workspace,
+                            void* out, float* lse, void* stream) {
+    if (int r = slotattn_host::check(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, dtype, B, Tq, Tk, Hq, Hk, D, window, cap)) return r;
+    if (lens && (docs || !causal)) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_fwd: lens goes with causality and without documents");
+    if (!lens && Tq > Tk) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_fwd: more queries than keys");
+    if (!out) return fail(SLOTSCAN_ERR_NULL, "slotattn_fwd: a required pointer is NULL");
+    if (!al16(out) || !al16(workspace) || !al16(docs)) return fail(SLOTSCAN_ERR_ALIGN, "slotattn_fwd: out, docs and workspace must be 16-byte aligned");
+    Plan p = plan(B, Tq, Tk, Hq, Hk, causal, window, docs != nullptr, prefix != nullptr);
+    if (split_bytes(p, B, Tq, Hq, D) && !workspace) return fail(SLOTSCAN_ERR_NULL, "slotattn_fwd: workspace is NULL");
+    AttnArgs a = slotattn_host::args(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, B, Tq, Tk, Hq, Hk, scale, causal, window, cap,
+                                     slopes, docs, prefix);
+    a.lens = lens;
+    a.out = out;
+    a.lse = lse;
+    a.tiles = p.split ? p.rtiles : (int)((Tq + FQ - 1) / FQ);
+    a.chunk = p.chunk;
+    a.nsplit = p.nsplit;
+    a.po = (float*)workspace;
+    a.pm = a.po ? a.po + B * Tq * Hq * p.nsplit * D : nullptr;
+    const bool split = p.split;
+    if ((int64_t)a.tiles * (split ? a.nsplit : B * Hq) > 0x7fffffffLL || (split && (Hk > 65535 || B > 65535)))
+        return fail(SLOTSCAN_ERR_SHAPE, "slotattn_fwd: shape too large");
+    hipStream_t st = (hipStream_t)stream;
+    const bool cp = cap > 0.f;
+    hipError_t e;
+    {
+        slothost::Scope sc(SLOTSCAN_K_ATTN, st);
+        if (dtype == SLOTSCAN_BF16) D == 128 ? launch_fwd<bf16_t, 128>(a, cp, split, st) : launch_fwd<bf16_t, 64>(a, cp, split, st);
+        else D == 128 ? launch_fwd<f16_t, 128>(a, cp, split, st) : launch_fwd<f16_t, 64>(a, cp, split, st);
+        e = hipGetLastError();
+    }
+    if (e != hipSuccess) return hip_fail(e, "attn_fwd launch");
+    if (!split || a.nsplit == 1) return 0;
+    {
+        slothost::Scope sc(SLOTSCAN_K_ATTN_JOIN, st);
+        if (dtype == SLOTSCAN_BF16) D == 128 ? launch_join<bf16_t, 128>(a, st) : launch_join<bf16_t, 64>(a, st);
+        else D == 128 ? launch_join<f16_t, 128>(a, st) : launch_join<f16_t, 64>(a, st);
+        e = hipGetLastError();
+    }
+    return e == hipSuccess ? 0 : hip_fail(e, "attn_join launch");
+}

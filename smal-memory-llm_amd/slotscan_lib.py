@@ -1,5 +1,5 @@
 """ctypes binding of libslotscan.so (declarations: include/slotscan.h, slotread.h, slotmem.h, slotwin.h,
-slotproj.h).
+slotproj.h, slotrope.h, slotattn.h).
 
 torch is imported BEFORE the library is opened: libslotscan.so needs libamdhip64.so.7 by SONAME, and with
 torch loaded first the dynamic loader binds it to torch's own HIP runtime, so the streams and device
@@ -18,8 +18,13 @@ LIB_PATH = os.path.join(HERE, "libslotscan.so")
 
 SLOTSCAN_F32 = 0
 SLOTSCAN_BF16 = 1
+SLOTSCAN_F16 = 2          # the attention of any range and its query and key preparation only
 
 _vp, _i64, _i32, _f32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+
+_ROWS = [_vp, _i64, _i64, _i64]                          # rows by strides: batch, head, token
+_ROPE = _ROWS * 2 + [_i32, _vp, _vp, _i32, _vp, _i64, _i32]
+_ATTN = _ROWS * 3 + [_i32] + [_i64] * 6 + [_f32, _i32, _i64, _f32, _vp]
 
 # name -> (restype, argtypes); every symbol declared in include/*.h appears here
 SIGNATURES = {
@@ -70,6 +75,17 @@ SIGNATURES = {
     "slotwin_fwd": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _vp]),
     "slotwin_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f32,
                            _vp, _vp, _vp, _vp, _vp]),
+    "slotrope_fwd": (_i32, _ROPE + [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _vp]),
+    "slotrope_bwd_workspace": (_sz, [_i64] * 5),
+    "slotrope_bwd": (_i32, _ROPE + [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _f32] + _ROWS * 2 + [_vp] * 6),
+    "slotrope_cache": (_i32, _ROWS * 3 + [_i32, _vp, _vp, _i32, _vp, _i64, _i32, _vp] + [_i64] * 6 + [_f32, _vp]
+                       + _ROWS * 2 + [_vp]),
+    "slotattn_docs_bytes": (_sz, [_i64, _i64]),
+    "slotattn_docs": (_i32, [_vp, _i64, _i64, _vp, _vp]),
+    "slotattn_fwd_workspace": (_sz, [_i64] * 6 + [_i32, _i64, _i32, _i32]),
+    "slotattn_fwd": (_i32, _ATTN + [_vp] * 7),
+    "slotattn_bwd_workspace": (_sz, [_i64] * 6),
+    "slotattn_bwd": (_i32, _ATTN + [_vp] * 4 + _ROWS + [_vp] * 6),
 }
 
 _lib = None
@@ -115,9 +131,33 @@ def dtype_code(dt):
     raise TypeError(f"token dtype {dt} is not supported by the HIP kernels (float32 or bfloat16)")
 
 
+_TYPE_CODES = {torch.float32: SLOTSCAN_F32, torch.bfloat16: SLOTSCAN_BF16, torch.float16: SLOTSCAN_F16}
+
+
+def rows(x):
+    """x (batch, head, token, D) as the kernels read it: D values of a row contiguous, every row 16-byte aligned.  A view
+    that is laid out so costs no copy."""
+    n = 16 // x.element_size()
+    s = x.stride()
+    if s[3] != 1 or s[0] % n or s[1] % n or s[2] % n:
+        x = x.contiguous()
+    return x.clone(memory_format=torch.contiguous_format) if x.data_ptr() % 16 else x
+
+
+def strided(x):
+    """Pointer and strides (batch, head, token) of rows(x), as the entry points take them."""
+    s = x.stride()
+    return x.data_ptr(), s[0], s[1], s[2]
+
+
+def on(device):
+    """Makes `device` the current one around a launch (a no-op where it is)."""
+    return torch.cuda.device(device if device.index != torch.cuda.current_device() else -1)
+
+
 KERNEL_NAMES = ("chain_fwd", "rows_fwd", "rows_bwd", "chain_bwd", "reduce_parts", "read_fwd", "read_bwd", "mem_fwd",
                 "mem_bwd", "win_fwd", "win_bwd", "gen_fwd", "gen_bwd", "proj", "proj_drd", "proj_dwo",
-                "proj_reduce")
+                "proj_reduce", "rope", "rope_bwd", "attn_fwd", "attn_dq", "attn_dkv", "attn_join")
 
 
 def profile(enable, kernels=None):
