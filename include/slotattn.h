@@ -34,7 +34,7 @@ extern "C" {
 size_t slotattn_docs_bytes(int64_t B, int64_t T);
 int slotattn_docs(const int32_t* ids, int64_t B, int64_t T, void* docs, void* stream);
 
-/* Forward.  lse may be NULL where no backward follows.  workspace: slotattn_fwd_workspace(...) bytes, 256-byte aligned: partial results where few query
+/* Forward.  res (as out: what rounding took from it, so that delta is as exact as the sums) and lse may be NULL where no backward follows.  workspace: slotattn_fwd_workspace(...) bytes, 256-byte aligned: partial results where few query
  * rows meet many keys and the keys are split over workgroups (0 bytes otherwise). */
 size_t slotattn_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int causal, int64_t window,
                               int has_docs, int has_prefix);
@@ -42,16 +42,18 @@ int slotattn_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const 
                  int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int dtype, int64_t B, int64_t Tq,
                  int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal, int64_t window, float cap,
                  const float* slopes, const void* docs, const int32_t* prefix, const int32_t* lens, void* workspace,
-                 void* out, float* lse, void* stream);
+                 void* out, void* res, float* lse, void* stream);
 
 /* Backward for the upstream gradient dout (B, Hq, Tq, D) by strides, without lens.  delta is written on the way.  Two kernels, one walking the
- * keys of every query tile (dq), one the queries of every key tile (dk, dv): no atomics, bitwise reproducible. */
-size_t slotattn_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D);
+ * keys of every query tile (dq), one the queries of every key tile (dk, dv; where there are few key tiles, parts of the queries, whose sums a
+ * third kernel adds in order): no atomics, bitwise reproducible.  workspace: slotattn_bwd_workspace(...) bytes, 256-byte aligned. */
+size_t slotattn_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int causal, int64_t window,
+                              int has_prefix);
 int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
                  int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int dtype, int64_t B, int64_t Tq,
                  int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal, int64_t window, float cap,
-                 const float* slopes, const void* docs, const int32_t* prefix, const void* out, const float* lse,
-                 const void* dout, int64_t do_sb, int64_t do_sh, int64_t do_st, void* workspace, float* delta, void* dq,
+                 const float* slopes, const void* docs, const int32_t* prefix, const void* out, const void* res,
+                 const float* lse, const void* dout, int64_t do_sb, int64_t do_sh, int64_t do_st, void* workspace, float* delta, void* dq,
                  void* dk, void* dv, void* stream);
 
 #ifdef __cplusplus

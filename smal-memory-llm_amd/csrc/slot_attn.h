@@ -42,9 +42,6 @@ template <typename T> __device__ __forceinline__ uint4 pack8(const f32x16& s, in
                       pack2<T>(s[8 * m + 6], s[8 * m + 7]));
 }
 __device__ __forceinline__ uint4 ld16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
-__device__ __forceinline__ uint2 ld_tr(const unsigned char* p) {
-    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((const lds_void*)p)));
-}
 __device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
 #pragma unroll
@@ -69,9 +66,9 @@ template <int n> __device__ __forceinline__ void wait_vm() {
     static_assert(n >= 0 && n < 64, "vmcnt is 6 bits");
     __builtin_amdgcn_s_waitcnt(0x0F70 | (n & 15) | ((n >> 4) << 14));
 }
-// workgroup barrier that orders LDS for the compiler and adds no wait for direct loads in flight
+// workgroup barrier behind this wave's LDS accesses; it adds no wait for direct loads in flight
 __device__ __forceinline__ void tile_barrier() {
-    asm volatile("" ::: "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -82,16 +79,33 @@ __device__ __forceinline__ void tile_barrier() {
 template <int D> struct Tile {
     static constexpr int CH = D / 8, ROWB = 2 * D, RP = 256 / ROWB;
     static __device__ __forceinline__ int pos(int r, int c) { return c ^ (2 * ((r / RP) & (CH / 2 - 1))); }
-    static __device__ __forceinline__ int at(int r, int c) { return r * ROWB + 16 * pos(r, c); }
-    // chunk 2 kk + h of row r: the row operand of k step kk
-    static __device__ __forceinline__ uint4 row_op(const unsigned char* s, int r, int kk, int lane) {
-        return ld16(s + at(r + (lane & 31), 2 * kk + (lane >> 5)));
+};
+
+// A lane's operand addresses in a staged tile, as LDS byte addresses: every k step or column block is the same address with
+// a few bits flipped, every 16 rows a constant further, so a lane holds two of them.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) const u32x4 lds_u4;
+typedef __attribute__((address_space(3))) const f32x4 lds_f4;
+__device__ __forceinline__ uint4 lds16(unsigned a) { return __builtin_bit_cast(uint4, *(lds_u4*)(uintptr_t)a); }
+__device__ __forceinline__ f32x4 lds4f(unsigned a) { return *(lds_f4*)(uintptr_t)a; }
+__device__ __forceinline__ uint2 lds_tr(unsigned a) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)a));
+}
+template <int D> struct Ops {
+    typedef Tile<D> Ti;
+    unsigned row, col;                               // relative to a tile's start (1 KB aligned)
+    __device__ __forceinline__ Ops(int lane) {
+        const int l = lane & 31, h = lane >> 5, i = lane & 15, cr = 4 * h + (i >> 2);
+        row = l * Ti::ROWB + 16 * Ti::pos(l, h);
+        col = cr * Ti::ROWB + 16 * Ti::pos(cr, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
     }
-    // 8 rows (r + 16 m + 4 h .. + 3 and + 8) of column 32 dt + (l & 31): the operand over rows in a result tile's order
-    static __device__ __forceinline__ uint4 col_op(const unsigned char* s, int r, int dt, int m, int lane) {
-        const int row = r + 16 * m + 4 * (lane >> 5) + ((lane & 15) >> 2);
-        const int c = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), by = 8 * (lane & 1);
-        const uint2 lo = ld_tr(s + at(row, c) + by), hi = ld_tr(s + at(row + 8, c) + by);
+    // row operand of k step kk: values 16 kk + 8 h .. + 7 of row r + (l & 31), r a multiple of 32
+    static __device__ __forceinline__ uint4 at_row(unsigned base, int r, int kk) { return lds16((base ^ (32 * kk)) + r * Ti::ROWB); }
+    // operand over rows r + 16 m + 4 h .. + 3 and + 8 (a result tile's order) of column 32 dt + (l & 31)
+    static __device__ __forceinline__ uint4 at_col(unsigned base, int r, int dt, int m) {
+        const unsigned a = (base ^ (64 * dt)) + (r + 16 * m) * Ti::ROWB;
+        const uint2 lo = lds_tr(a), hi = lds_tr(a + 8 * Ti::ROWB);
         return make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
 };
@@ -141,14 +155,25 @@ struct AttnArgs {
     const int32_t* prefix; const int32_t* lens;
     float sc;                                        // scale log2(e): scores in base 2
     float ct, c2;                                    // capped: 2 scale log2(e) / cap, cap log2(e)
-    void* out; float* lse;
+    void* out; void* res; float* lse;                // res: what rounding took from out, for the backward's delta
     // split rows
     float* po; float* pm; int chunk, nsplit, tiles;
     // backward
     const void* dout; int64_t do_sb, do_sh, do_st;
     float* delta; void* dq; void* dk; void* dv;
-    float* part; float scale;
+    float* part; int units; float scale;             // split keys of attn_dkv: partial sums, query tiles per workgroup
 };
+
+// a float4 of results and what rounding takes from it
+template <typename T> __device__ __forceinline__ float unpack(uint32_t x, int i);
+template <> __device__ __forceinline__ float unpack<bf16_t>(uint32_t x, int i) { return __uint_as_float(i ? x & 0xffff0000u : x << 16); }
+template <> __device__ __forceinline__ float unpack<f16_t>(uint32_t x, int i) { return (float)__builtin_bit_cast(f16x2, x)[i]; }
+template <typename T> __device__ __forceinline__ void put4(void* out, void* res, int64_t at, float x, float y, float z, float w) {
+    const uint2 o = make_uint2(pack2<T>(x, y), pack2<T>(z, w));
+    *reinterpret_cast<uint2*>((T*)out + at) = o;
+    if (res) *reinterpret_cast<uint2*>((T*)res + at) =
+        make_uint2(pack2<T>(x - unpack<T>(o.x, 0), y - unpack<T>(o.x, 1)), pack2<T>(z - unpack<T>(o.y, 0), w - unpack<T>(o.y, 1)));
+}
 
 // key of register r of a score tile's lane half h, from the tile's first key
 __device__ __forceinline__ constexpr int key_of(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }

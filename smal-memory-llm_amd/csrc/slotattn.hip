@@ -85,27 +85,25 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
     float m = -INFINITY, l = 0.f;
     int jt, jn;
     bool some, all, some_n = false, all_n = false;
+    const Ops<D> ops(lane);
     walk.next(jt, some, all);
     if (jt >= 0) load(jt, 0);
+    // one barrier a tile: behind it the tile is there for every wave and the other buffer is read, so the next one's loads
+    // run during this one's products
     for (int buf = 0; jt >= 0; buf ^= 1, jt = jn, some = some_n, all = all_n) {
         walk.next(jn, some_n, all_n);
-        if (jn >= 0) {
-            load(jn, buf ^ 1);
-            wait_vm<2 * Load::N>();
-        } else {
-            wait_vm<0>();
-        }
-        tile_barrier();                               // the tile is there, for every wave
+        wait_vm<0>();
+        tile_barrier();
+        if (jn >= 0) load(jn, buf ^ 1);
         if (some) {
-            const unsigned char* sk = smem[buf][0];
-            const unsigned char* sx = smem[buf][1];
+            const unsigned sk = lds + (2 * buf) * STAGE + ops.row, sx = lds + (2 * buf + 1) * STAGE + ops.col;
             const int j0 = jt * KT;
             f32x16 s[2];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 s[u] = zero16();
 #pragma unroll
-                for (int kk = 0; kk < KK; kk++) s[u] = mfma32<T>(Tile<D>::row_op(sk, 32 * u, kk, lane), qf[kk], s[u]);
+                for (int kk = 0; kk < KK; kk++) s[u] = mfma32<T>(Ops<D>::at_row(sk, 32 * u, kk), qf[kk], s[u]);
             }
 #pragma unroll
             for (int u = 0; u < 2; u++) scores<CAP, BIAS>(s[u], a, slope, p, j0 + 32 * u, h);
@@ -113,11 +111,13 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int j = j0 + 32 * u + key_of(r, h);
-                        bool ok = mk.sees(p, j);
-                        if (docs) ok = ok && a.ids[idb + j] == dq;
-                        s[u][r] = ok ? s[u][r] : -INFINITY;
+                    for (int g = 0; g < 4; g++) {
+                        const int j = j0 + 32 * u + 8 * g + 4 * h;
+                        const int4 id = docs ? *reinterpret_cast<const int4*>(a.ids + idb + j) : make_int4(0, 0, 0, 0);
+                        s[u][4 * g] = mk.sees(p, j) && id.x == dq ? s[u][4 * g] : -INFINITY;
+                        s[u][4 * g + 1] = mk.sees(p, j + 1) && id.y == dq ? s[u][4 * g + 1] : -INFINITY;
+                        s[u][4 * g + 2] = mk.sees(p, j + 2) && id.z == dq ? s[u][4 * g + 2] : -INFINITY;
+                        s[u][4 * g + 3] = mk.sees(p, j + 3) && id.w == dq ? s[u][4 * g + 3] : -INFINITY;
                     }
             }
             float mx = s[0][0];
@@ -153,21 +153,18 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(Tile<D>::col_op(sx, 32 * u, dt, mm, lane), pf[u][mm], o[dt]);
+                    for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(Ops<D>::at_col(sx, 32 * u, dt, mm), pf[u][mm], o[dt]);
         }
-        tile_barrier();                               // every wave has read the tile
     }
     l = half_sum(l);
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     if (t < a.Tq) {
-        T* out = (T*)a.out + (((int64_t)b * a.Tq + t) * a.Hq + hq) * D;
+        const int64_t at = (((int64_t)b * a.Tq + t) * a.Hq + hq) * D + 4 * h;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                uint2 x = make_uint2(pack2<T>(o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv), pack2<T>(o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv));
-                *reinterpret_cast<uint2*>(out + 32 * dt + 8 * g + 4 * h) = x;
-            }
+            for (int g = 0; g < 4; g++)
+                put4<T>(a.out, a.res, at + 32 * dt + 8 * g, o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv);
         if (a.lse && h == 0) a.lse[(int64_t)bh * a.Tq + t] = l > 0.f || l != l ? m + __builtin_amdgcn_logf(l) : INFINITY;
     }
 }
@@ -206,6 +203,7 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
         while (j0 < hi && !mk.some(s, j0, j0 + 31)) j0 += 32 * FW;
         return j0;
     };
+    const Ops<D> ops(lane);
     int j0 = seen(lo + 32 * w);
     if (j0 < hi) load(j0, 0);
     uint4 qf[KK];
@@ -227,11 +225,10 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
             wait_vm<0>();
         }
         asm volatile("" ::: "memory");
-        const unsigned char* sk = smem[w][buf][0];
-        const unsigned char* sx = smem[w][buf][1];
+        const unsigned sk = lds + (2 * buf) * ST + ops.row, sx = lds + (2 * buf + 1) * ST + ops.col;
         f32x16 x = zero16();
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++) x = mfma32<T>(Tile<D>::row_op(sk, 0, kk, lane), qf[kk], x);
+        for (int kk = 0; kk < KK; kk++) x = mfma32<T>(Ops<D>::at_row(sk, 0, kk), qf[kk], x);
         scores<CAP, BIAS>(x, a, slope, p, j0, h);
         if (j0 + 32 > hi || !mk.all(s, j0, j0 + 31)) {
 #pragma unroll
@@ -264,7 +261,7 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(Tile<D>::col_op(sx, 0, dt, mm, lane), pf[mm], o[dt]);
+            for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(Ops<D>::at_col(sx, 0, dt, mm), pf[mm], o[dt]);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the tile is read before its buffer is filled again
         j0 = jn;
     }
@@ -308,8 +305,8 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
             v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
         }
         if (a.nsplit == 1) {
-            *reinterpret_cast<uint2*>((T*)a.out + orow * D + d) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
-        } else {
+            put4<T>(a.out, a.res, orow * D + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        } else if (got) {
             *reinterpret_cast<float4*>(a.po + (orow * a.nsplit + sp) * D + d) = v;
         }
     }
@@ -322,36 +319,59 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
     }
 }
 
-// One wave per row: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, the parts in order
+// One workgroup per row: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  Groups of D / 4 lanes take every NG-th part,
+// so that a row of hundreds of parts is as many short chains of loads; their sums meet in LDS in order.
 template <typename T, int D>
-__global__ __launch_bounds__(FT) void attn_join(AttnArgs a, int64_t nrows) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * FW + (threadIdx.x >> 6);
-    if (row >= nrows) return;
+__global__ __launch_bounds__(FT) void attn_join(AttnArgs a) {
+    constexpr int LN = D / 4, NG = FT / LN;
+    __shared__ __align__(16) float s_o[NG][D];
+    __shared__ float s_l[NG], s_m[FW];
+    const int tid = threadIdx.x, c = tid % LN, g = tid / LN;
+    const int64_t row = blockIdx.x;
     const float2* pm = reinterpret_cast<const float2*>(a.pm) + row * a.nsplit;
     float M = -INFINITY;
-    for (int s = lane; s < a.nsplit; s += 64) M = fmaxf(M, pm[s].x);
+    for (int s = tid; s < a.nsplit; s += FT) M = fmaxf(M, pm[s].x);
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) M = fmaxf(M, __shfl_xor(M, i));
+    if ((tid & 63) == 0) s_m[tid >> 6] = M;
+    __syncthreads();
+    M = s_m[0];
+#pragma unroll
+    for (int i = 1; i < FW; i++) M = fmaxf(M, s_m[i]);
     const float Mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[D / 64];
-#pragma unroll
-    for (int i = 0; i < D / 64; i++) acc[i] = 0.f;
-    for (int s = 0; s < a.nsplit; s++) {
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = g; s < a.nsplit; s += NG) {
         const float2 x = pm[s];
-        if (x.y == 0.f) continue;                     // nothing visible in this part
-        const float f = exp2_(x.x - Mu);
+        const bool in = x.y != 0.f;                   // otherwise nothing is visible in this part, and no sum was written
+        const float f = in ? exp2_(x.x - Mu) : 0.f;
+        const float4 o = in ? *reinterpret_cast<const float4*>(a.po + (row * a.nsplit + s) * D + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
         L = fmaf(x.y, f, L);
-        const float* o = a.po + (row * a.nsplit + s) * D + lane * (D / 64);
+        acc.x = fmaf(o.x, f, acc.x);
+        acc.y = fmaf(o.y, f, acc.y);
+        acc.z = fmaf(o.z, f, acc.z);
+        acc.w = fmaf(o.w, f, acc.w);
+    }
+    *reinterpret_cast<float4*>(&s_o[g][4 * c]) = acc;
+    if (c == 0) s_l[g] = L;
+    __syncthreads();
+    if (tid >= LN) return;
+    L = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < D / 64; i++) acc[i] = fmaf(o[i], f, acc[i]);
+    for (int i = 0; i < NG; i++) {
+        const float4 o = *reinterpret_cast<const float4*>(&s_o[i][4 * c]);
+        L += s_l[i];
+        acc.x += o.x;
+        acc.y += o.y;
+        acc.z += o.z;
+        acc.w += o.w;
     }
     const bool got = L > 0.f || L != L;
     const float inv = got ? 1.f / L : 0.f;
-    T* out = (T*)a.out + row * D + lane * (D / 64);
-    if constexpr (D == 128) *reinterpret_cast<uint32_t*>(out) = pack2<T>(acc[0] * inv, acc[1] * inv);
-    else *reinterpret_cast<uint16_t*>(out) = (uint16_t)pack2<T>(acc[0] * inv, 0.f);
-    if (a.lse && lane == 0) {
+    put4<T>(a.out, a.res, row * D + 4 * c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (a.lse && c == 0) {
         const int64_t tok = row / a.Hq;
         const int hq = (int)(row - tok * a.Hq);
         const int64_t b = tok / a.Tq;
@@ -371,8 +391,7 @@ void launch_fwd(const AttnArgs& a, bool cap, bool split, hipStream_t st) {
 }
 template <typename T, int D>
 void launch_join(const AttnArgs& a, hipStream_t st) {
-    const int64_t rows = (int64_t)a.B * a.Tq * a.Hq;
-    slothost::launch(attn_join<T, D>, dim3((unsigned)((rows + FW - 1) / FW)), dim3(FT), 0, st, a, rows);
+    slothost::launch(attn_join<T, D>, dim3((unsigned)((int64_t)a.B * a.Tq * a.Hq)), dim3(FT), 0, st, a);
 }
 
 // How the forward runs.  split: the packed rows and split keys, where 128-row tiles would leave most of the card idle
@@ -430,18 +449,19 @@ extern "C" int slotattn_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
                             int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int dtype, int64_t B, int64_t Tq,
                             int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal, int64_t window, float cap,
                             const float* slopes, const void* docs, const int32_t* prefix, const int32_t* lens, void* workspace,
-                            void* out, float* lse, void* stream) {
+                            void* out, void* res, float* lse, void* stream) {
     if (int r = slotattn_host::check(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, dtype, B, Tq, Tk, Hq, Hk, D, window, cap)) return r;
     if (lens && (docs || !causal)) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_fwd: lens goes with causality and without documents");
     if (!lens && Tq > Tk) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_fwd: more queries than keys");
     if (!out) return fail(SLOTSCAN_ERR_NULL, "slotattn_fwd: a required pointer is NULL");
-    if (!al16(out) || !al16(workspace) || !al16(docs)) return fail(SLOTSCAN_ERR_ALIGN, "slotattn_fwd: out, docs and workspace must be 16-byte aligned");
+    if (!al16(out) || !al16(res) || !al16(workspace) || !al16(docs)) return fail(SLOTSCAN_ERR_ALIGN, "slotattn_fwd: out, res, docs and workspace must be 16-byte aligned");
     Plan p = plan(B, Tq, Tk, Hq, Hk, causal, window, docs != nullptr, prefix != nullptr);
     if (split_bytes(p, B, Tq, Hq, D) && !workspace) return fail(SLOTSCAN_ERR_NULL, "slotattn_fwd: workspace is NULL");
     AttnArgs a = slotattn_host::args(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, B, Tq, Tk, Hq, Hk, scale, causal, window, cap,
                                      slopes, docs, prefix);
     a.lens = lens;
     a.out = out;
+    a.res = res;
     a.lse = lse;
     a.tiles = p.split ? p.rtiles : (int)((Tq + FQ - 1) / FQ);
     a.chunk = p.chunk;
@@ -449,7 +469,7 @@ extern "C" int slotattn_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
     a.po = (float*)workspace;
     a.pm = a.po ? a.po + B * Tq * Hq * p.nsplit * D : nullptr;
     const bool split = p.split;
-    if ((int64_t)a.tiles * (split ? a.nsplit : B * Hq) > 0x7fffffffLL || (split && (Hk > 65535 || B > 65535)))
+    if ((int64_t)a.tiles * (split ? a.nsplit : B * Hq) > 0x7fffffffLL || (split && (Hk > 65535 || B > 65535 || B * Tq * Hq > 0x7fffffffLL)))
         return fail(SLOTSCAN_ERR_SHAPE, "slotattn_fwd: shape too large");
     hipStream_t st = (hipStream_t)stream;
     const bool cp = cap > 0.f;

@@ -5,6 +5,8 @@
 //   attn_dq    128 queries of one head per workgroup, walking the visible key tiles (as the forward does); it forms delta
 //   attn_dkv   128 keys of one key/value head per workgroup, walking the query tiles of every head of the group that see them
 // The price is that the scores and dP are formed twice: 7 products where one kernel with atomic dQ would need 5.
+#include <algorithm>
+
 #include "slot_attn.h"
 #include "slotscan.h"
 #include "slotattn.h"
@@ -18,6 +20,7 @@ using slothost::al16;
 #define BW 4                                         // waves per workgroup
 #define BT (64 * BW)
 #define BQ (32 * BW)                                 // queries (attn_dq) or keys (attn_dkv) per workgroup
+#define QT 32                                        // query rows of a tile of attn_dkv
 
 namespace {
 
@@ -35,28 +38,43 @@ __device__ __forceinline__ void dot8(const uint4& x, const uint4& y, float& s, f
     for (int i = 0; i < 8; i++) s = fmaf((float)a[i], (float)b[i], s);
 }
 
-// P and dS of one 32 x 32 tile from its products s = <q, k> and dp = <dO, v>; lse and delta of register r's row through
-// L(r), Dl(r).  dist: the lane's own position; d0: the position of register row 0.  ok(r): visible (only asked if !all).
-template <bool CAP, bool BIAS, class LF, class DF, class OK>
-__device__ __forceinline__ void probs(f32x16& s, f32x16& dp, const AttnArgs& a, float slope, int dist, int d0, int h, bool all, LF L, DF Dl, OK ok) {
-    f32x16 x = s;
-    scores<CAP, BIAS>(x, a, slope, dist, d0, h);
+// P and dS of one 32 x 32 tile, in the place of its products s = <q, k> and dp = <dO, v>; LD(g, L, Dl): log-sum-exp and
+// delta of registers 4 g .. 4 g + 3, so that no more of them are held than a few scores need.  dist: the lane's own position;
+// d0: the position of register row 0.  ok(g, o): which of those four are visible (only asked if !all).
+template <bool CAP, bool BIAS, class LD, class OK>
+__device__ __forceinline__ void probs(f32x16& s, f32x16& dp, const AttnArgs& a, float slope, int dist, int d0, int h, bool all, LD ld, OK ok) {
+    const float d = BIAS ? (float)(dist - d0 - 4 * h) : 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-        float g = 1.f;
-        if constexpr (CAP) {                          // 1 - tanh^2 = 4 z (1 - z), z = 1 / (1 + e^2x)
-            const float z = __builtin_amdgcn_rcpf(1.f + exp2_(s[r] * a.ct));
-            g = 4.f * z * (1.f - z);
+    for (int g = 0; g < 4; g++) {
+        f32x4 L, Dl;
+        ld(g, L, Dl);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = 4 * g + i;
+            float x, t = 1.f;
+            if constexpr (CAP) {                      // tanh = 1 - 2 z, 1 - tanh^2 = 4 z (1 - z), z = 1 / (1 + e^2x)
+                const float z = __builtin_amdgcn_rcpf(1.f + exp2_(s[r] * a.ct));
+                x = fmaf(-2.f * a.c2, z, a.c2) - L[i];
+                t = 4.f * z * (1.f - z);
+            } else {
+                x = fmaf(s[r], a.sc, -L[i]);
+            }
+            if constexpr (BIAS) x = fmaf(-slope, fabsf(d - (float)key_of(r, 0)), x);
+            s[r] = exp2_(x);
+            dp[r] = s[r] * (dp[r] - Dl[i]) * t;
         }
-        float p = exp2_(x[r] - L(r));
-        float ds = p * (dp[r] - Dl(r)) * g;
-        if (!all) {
-            const bool o = ok(r);
-            p = o ? p : 0.f;
-            ds = o ? ds : 0.f;
+    }
+    if (!all) {
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            bool o[4];
+            ok(g, o);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s[4 * g + i] = o[i] ? s[4 * g + i] : 0.f;
+                dp[4 * g + i] = o[i] ? dp[4 * g + i] : 0.f;
+            }
         }
-        s[r] = p;
-        dp[r] = ds;
     }
 }
 
@@ -79,14 +97,17 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
     {
         const T* q = (const T*)a.q + b * a.q_sb + hq * a.q_sh + tc * a.q_st + 8 * h;
         const T* g = (const T*)a.dout + b * a.do_sb + hq * a.do_sh + tc * a.do_st + 8 * h;
-        const T* o = (const T*)a.out + (((int64_t)b * a.Tq + tc) * a.Hq + hq) * D + 8 * h;
+        const int64_t at = (((int64_t)b * a.Tq + tc) * a.Hq + hq) * D + 8 * h;
 #pragma unroll
         for (int kk = 0; kk < KK; kk++) {
             qf[kk] = ld16(q + 16 * kk);
             df[kk] = ld16(g + 16 * kk);
         }
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++) dot8(df[kk], ld16(o + 16 * kk), delta, T{});
+        for (int kk = 0; kk < KK; kk++) {
+            dot8(df[kk], ld16((const T*)a.out + at + 16 * kk), delta, T{});
+            dot8(df[kk], ld16((const T*)a.res + at + 16 * kk), delta, T{});
+        }
     }
     delta = half_sum(delta);
     const int64_t row = (int64_t)bh * a.Tq + tc;
@@ -116,42 +137,41 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
     for (int dt = 0; dt < DT; dt++) acc[dt] = zero16();
     int jt, jn;
     bool some, all, some_n = false, all_n = false;
+    const Ops<D> ops(lane);
     walk.next(jt, some, all);
     if (jt >= 0) load(jt, 0);
     for (int buf = 0; jt >= 0; buf ^= 1, jt = jn, some = some_n, all = all_n) {
         walk.next(jn, some_n, all_n);
-        if (jn >= 0) {
-            load(jn, buf ^ 1);
-            wait_vm<2 * Load::N>();
-        } else {
-            wait_vm<0>();
-        }
+        wait_vm<0>();
         tile_barrier();
+        if (jn >= 0) load(jn, buf ^ 1);
         if (some) {
-            const unsigned char* sk = smem[buf][0];
-            const unsigned char* sx = smem[buf][1];
+            const unsigned sk = lds + (2 * buf) * STAGE + ops.row, sx = sk + STAGE, sc = lds + (2 * buf) * STAGE + ops.col;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int j0 = jt * KT + 32 * u;
                 f32x16 s = zero16(), dp = zero16();
 #pragma unroll
                 for (int kk = 0; kk < KK; kk++) {
-                    s = mfma32<T>(Tile<D>::row_op(sk, 32 * u, kk, lane), qf[kk], s);
-                    dp = mfma32<T>(Tile<D>::row_op(sx, 32 * u, kk, lane), df[kk], dp);
+                    s = mfma32<T>(Ops<D>::at_row(sk, 32 * u, kk), qf[kk], s);
+                    dp = mfma32<T>(Ops<D>::at_row(sx, 32 * u, kk), df[kk], dp);
                 }
-                probs<CAP, BIAS>(s, dp, a, slope, p, j0, h, all, [&](int) { return lse; }, [&](int) { return delta; }, [&](int r) {
-                    const int j = j0 + key_of(r, h);
-                    return mk.sees(p, j) && (!docs || a.ids[idb + j] == dq);
+                probs<CAP, BIAS>(s, dp, a, slope, p, j0, h, all, [&](int, f32x4& L, f32x4& Dl) { L = f32x4{lse, lse, lse, lse}; Dl = f32x4{delta, delta, delta, delta}; }, [&](int g, bool (&o)[4]) {
+                    const int j = j0 + 8 * g + 4 * h;
+                    const int4 id = docs ? *reinterpret_cast<const int4*>(a.ids + idb + j) : make_int4(0, 0, 0, 0);
+                    o[0] = mk.sees(p, j) && id.x == dq;
+                    o[1] = mk.sees(p, j + 1) && id.y == dq;
+                    o[2] = mk.sees(p, j + 2) && id.z == dq;
+                    o[3] = mk.sees(p, j + 3) && id.w == dq;
                 });
 #pragma unroll
                 for (int mm = 0; mm < 2; mm++) {
                     const uint4 ds = pack8<T>(dp, mm);
 #pragma unroll
-                    for (int dt = 0; dt < DT; dt++) acc[dt] = mfma32<T>(Tile<D>::col_op(sk, 32 * u, dt, mm, lane), ds, acc[dt]);
+                    for (int dt = 0; dt < DT; dt++) acc[dt] = mfma32<T>(Ops<D>::at_col(sc, 32 * u, dt, mm), ds, acc[dt]);
                 }
             }
         }
-        tile_barrier();
     }
     if (t < a.Tq) {
         T* out = (T*)a.dq + (((int64_t)b * a.Tq + t) * a.Hq + hq) * D;
@@ -166,30 +186,49 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------- dK, dV
+// the query tiles [x0, x1) of a head that may see keys j0 .. j1
+__device__ __forceinline__ void tile_rows(const AttnArgs& a, const Mask& mk, int j0, int j1, int off, int& x0, int& x1) {
+    x0 = 0;
+    x1 = (a.Tq + QT - 1) / QT;
+    if (j0 >= mk.prefix) {
+        const int lo = a.causal ? j0 : max(0, j0 - a.W + 1);          // the first position
+        x0 = max(0, lo - off) / QT;
+        if (a.W < a.Tk) x1 = min(x1, max(0, j1 + a.W - off + QT - 1) / QT);
+    }
+}
+// whether tiles [x0, x1) of any head, numbered head * nx + tile, fall into [u0, u1)
+__device__ __forceinline__ bool meets(int x0, int x1, int nx, int u0, int u1) {
+    if (x0 >= x1) return false;
+    for (int r = u0 / nx; r * nx < u1; r++)
+        if (max(x0, u0 - r * nx) < min(x1, u1 - r * nx)) return true;
+    return false;
+}
+
 template <typename T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(BT, 1) void attn_dkv(AttnArgs a) {
-    constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
-    typedef TileLoad<D, KT, BW> Load;
-    __shared__ __align__(1024) unsigned char smem[2][2][STAGE];      // [buffer][queries, dout]
-    __shared__ __align__(16) float s_lse[2][KT], s_del[2][KT];
+__global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
+    constexpr int KK = D / 16, DT = D / 32, STAGE = QT * 2 * D, KEYS = BQ * 2 * D;
+    typedef TileLoad<D, QT, BW> Load;
+    __shared__ __align__(1024) unsigned char smem[KEYS + 4 * STAGE]; // the keys; [buffer][queries, dout]
+    __shared__ __align__(16) float s_st[2][2][QT];                   // [buffer][log-sum-exp, delta]
+    __shared__ __align__(16) int s_id[2][QT];                        // the queries' documents
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = a.B * a.Hk;
-    const int jt = blockIdx.x / kvh, bh = blockIdx.x % kvh;           // the first tiles have the most queries under causality
+    // parts of the queries, then key tiles (the first have the most queries under causality), then heads: workgroups that run
+    // at the same time read the same queries
+    const int jt = blockIdx.x / kvh % a.tiles, bh = blockIdx.x % kvh, part = blockIdx.x / (kvh * a.tiles);
     const int b = bh / a.Hk, hk = bh - b * a.Hk;
     const int j0 = jt * BQ, j1 = min(j0 + BQ, a.Tk) - 1, off = a.Tk - a.Tq;
     const int jw = j0 + 32 * w, j = jw + (lane & 31), jc = min(j, a.Tk - 1);
     const int jw1 = min(jw + 31, a.Tk - 1);
     Mask mk{a.causal, a.W, a.prefix ? a.prefix[b] : 0, a.Tk};
-    uint4 kf[KK], vf[KK];
+    const unsigned lds = lds_addr(smem), ldq = lds + KEYS;
+    TileLoad<D, BQ, BW>::issue((const T*)a.k + b * a.k_sb + hk * a.k_sh, a.k_st, j0, a.Tk - 1, lds, w, lane);
+    uint4 vf[KK];
     {
-        const T* k = (const T*)a.k + b * a.k_sb + hk * a.k_sh + jc * a.k_st + 8 * h;
         const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh + jc * a.v_st + 8 * h;
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++) {
-            kf[kk] = ld16(k + 16 * kk);
-            vf[kk] = ld16(v + 16 * kk);
-        }
+        for (int kk = 0; kk < KK; kk++) vf[kk] = ld16(v + 16 * kk);
     }
     const bool docs = a.ids != nullptr;
     const int64_t idb = (int64_t)b * a.ntd * KT;
@@ -201,32 +240,28 @@ __global__ __launch_bounds__(BT, 1) void attn_dkv(AttnArgs a) {
         dk_ = a.ids[idb + jc];
         if (dk_ < 0) dk_ = -2;
     }
-    // query tiles of 64 rows that may see these keys
-    const bool pre = j0 < mk.prefix;
-    int x0 = 0, x1 = (a.Tq + KT - 1) / KT;
-    if (!pre) {
-        const int lo = a.causal ? j0 : max(0, j0 - a.W + 1);          // the first position
-        x0 = max(0, lo - off) / KT;
-        if (a.W < a.Tk) x1 = min(x1, max(0, j1 + a.W - off + KT - 1) / KT);
-    }
+    int x0, x1;
+    tile_rows(a, mk, j0, j1, off, x0, x1);
+    const int nx = (a.Tq + QT - 1) / QT, u0 = part * a.units, u1 = min(u0 + a.units, a.R * nx);
+    if (a.nsplit > 1 && !meets(x0, x1, nx, u0, u1)) return;           // the whole workgroup; attn_add knows it too
     const int2* range = docs ? a.range + (int64_t)b * a.ntd : nullptr;
-    const unsigned lds = lds_addr(smem);
     f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) dk[dt] = dv[dt] = zero16();
-    // the walk: heads of the group x query tiles
-    int r = -1, base = x1;
+    // the walk: heads of the group x query tiles, those of this workgroup's part
+    int r = u0 / nx - 1, base = 0, xe = 0;
     uint64_t act = 0, mine = 0, full = 0;
     auto next = [&](int& hq, int& xt, bool& some, bool& all) {
         while (!act) {
             base += 64;
-            if (base >= x1) {
-                if (++r >= a.R) { xt = -1; return; }
-                base = x0;
+            if (base >= xe) {
+                if (++r * nx >= u1) { xt = -1; return; }
+                base = max(x0, u0 - r * nx);
+                xe = min(x1, u1 - r * nx);
             }
             const int x = base + lane;
-            const bool in = x < x1;
-            Span s{x * KT + off, min(x * KT + KT, a.Tq) - 1 + off, 0, 0, true};
+            const bool in = x < xe;
+            Span s{x * QT + off, min(x * QT + QT, a.Tq) - 1 + off, 0, 0, true};
             if (range && in) {
                 const int2 ra = range[s.p0 / KT], rb = range[s.p1 / KT];
                 s.lo = min(range_lo(ra), range_lo(rb));
@@ -235,7 +270,7 @@ __global__ __launch_bounds__(BT, 1) void attn_dkv(AttnArgs a) {
             }
             act = __ballot(in && mk.some(s, j0, j1) && (!range || (s.lo <= kw.hi && kw.lo <= s.hi)));
             mine = __ballot(in && jw <= jw1 && mk.some(s, jw, jw1) && (!range || (s.lo <= kv.hi && kv.lo <= s.hi)));
-            full = __ballot(in && x * KT + KT <= a.Tq && mk.all(s, jw, jw + 31) && (!range || (s.one && kv.one && s.lo == kv.lo)));
+            full = __ballot(in && x * QT + QT <= a.Tq && mk.all(s, jw, jw + 31) && (!range || (s.one && kv.one && s.lo == kv.lo)));
         }
         const int i = __builtin_ctzll(act);
         act &= act - 1;
@@ -245,76 +280,99 @@ __global__ __launch_bounds__(BT, 1) void attn_dkv(AttnArgs a) {
         all = full >> i & 1;
     };
     auto load = [&](int hq, int xt, int buf) {
-        Load::issue((const T*)a.q + b * a.q_sb + hq * a.q_sh, a.q_st, xt * KT, a.Tq - 1, lds + (2 * buf) * STAGE, w, lane);
-        Load::issue((const T*)a.dout + b * a.do_sb + hq * a.do_sh, a.do_st, xt * KT, a.Tq - 1, lds + (2 * buf + 1) * STAGE, w, lane);
+        Load::issue((const T*)a.q + b * a.q_sb + hq * a.q_sh, a.q_st, xt * QT, a.Tq - 1, ldq + (2 * buf) * STAGE, w, lane);
+        Load::issue((const T*)a.dout + b * a.do_sb + hq * a.do_sh, a.do_st, xt * QT, a.Tq - 1, ldq + (2 * buf + 1) * STAGE, w, lane);
     };
-    auto stat = [&](int hq, int xt) {                 // threads 0..63 the log-sum-exp, 64..127 delta of a row
-        const int t = xt * KT + (tid & 63);
+    auto stat = [&](int hq, int xt) {                 // lanes 0..31 of the first wave the log-sum-exp, 32..63 delta of a row
+        const int t = xt * QT + (lane & 31);
         const int64_t i = ((int64_t)b * a.Hq + hq) * a.Tq + min(t, a.Tq - 1);
-        const float v = tid < 64 ? a.lse[i] : a.delta[i];
-        return t < a.Tq ? v : (tid < 64 ? INFINITY : 0.f);
+        const float v = h ? a.delta[i] : a.lse[i];
+        return t < a.Tq ? v : (h ? 0.f : INFINITY);
     };
     int hq, xt, hn = 0, xn;
     bool some, all, some_n = false, all_n = false;
+    const Ops<D> ops(lane);
+    const unsigned stb = lds_addr(s_st) + 16 * h;
     next(hq, xt, some, all);
+    // the queries' documents (second wave): padding matches no key's
+    auto doc = [&](int xt) { return a.ids[idb + min(xt * QT + (lane & 31) + off, a.Tk - 1)]; };
     float st = 0.f;
+    int sid = 0;
     if (xt >= 0) {
-        if (tid < 128) st = stat(hq, xt);
+        if (w == 0) st = stat(hq, xt);
+        if (w == 1 && docs) sid = doc(xt);
         load(hq, xt, 0);
     }
     for (int buf = 0; xt >= 0; buf ^= 1, hq = hn, xt = xn, some = some_n, all = all_n) {
-        if (tid < 64) s_lse[buf][tid] = st;
-        else if (tid < 128) s_del[buf][tid - 64] = st;
+        if (w == 0) s_st[buf][h][lane & 31] = st;
+        if (w == 1 && docs && h == 0) s_id[buf][lane] = sid;
         next(hn, xn, some_n, all_n);
+        wait_vm<0>();
+        tile_barrier();
         if (xn >= 0) {
-            if (tid < 128) st = stat(hn, xn);
+            if (w == 0) st = stat(hn, xn);
+            if (w == 1 && docs) sid = doc(xn);
             load(hn, xn, buf ^ 1);
-            wait_vm<2 * Load::N>();
-        } else {
-            wait_vm<0>();
         }
-        __syncthreads();
         if (some) {
-            const unsigned char* sq = smem[buf][0];
-            const unsigned char* sd = smem[buf][1];
+            const unsigned sq = ldq + (2 * buf) * STAGE + ops.row, sd = sq + STAGE, sk = lds + 32 * w * Tile<D>::ROWB + ops.row;
+            const unsigned cq = ldq + (2 * buf) * STAGE + ops.col, cd = cq + STAGE;
             const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
+            f32x16 s = zero16(), dp = zero16();
+            uint4 oq = Ops<D>::at_row(sq, 0, 0), ok_ = Ops<D>::at_row(sk, 0, 0), od = Ops<D>::at_row(sd, 0, 0);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-                for (int kk = 0; kk < KK; kk++) {
-                    s = mfma32<T>(Tile<D>::row_op(sq, 32 * u, kk, lane), kf[kk], s);
-                    dp = mfma32<T>(Tile<D>::row_op(sd, 32 * u, kk, lane), vf[kk], dp);
+            for (int kk = 0; kk < KK; kk++) {
+                const uint4 cq_ = oq, ck_ = ok_, cd_ = od;
+                if (kk + 1 < KK) {
+                    oq = Ops<D>::at_row(sq, 0, kk + 1);
+                    ok_ = Ops<D>::at_row(sk, 0, kk + 1);
+                    od = Ops<D>::at_row(sd, 0, kk + 1);
                 }
-                const int t0 = xt * KT + 32 * u;
-                float L[16], Dl[16];
+                s = mfma32<T>(cq_, ck_, s);
+                dp = mfma32<T>(cd_, vf[kk], dp);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const int t0 = xt * QT;
+            probs<CAP, BIAS>(s, dp, a, slope, j, t0 + off, h, all, [&](int g, f32x4& L, f32x4& Dl) {
+                L = lds4f(stb + (2 * buf) * QT * 4 + 32 * g);
+                Dl = lds4f(stb + (2 * buf + 1) * QT * 4 + 32 * g);
+                __builtin_amdgcn_sched_barrier(0);
+            }, [&](int g, bool (&o)[4]) {
+                const int tq = t0 + 8 * g + 4 * h;
+                const int4 id = docs ? *reinterpret_cast<const int4*>(&s_id[buf][8 * g + 4 * h]) : make_int4(0, 0, 0, 0);
+                o[0] = tq < a.Tq && mk.sees(tq + off, j) && id.x == dk_;
+                o[1] = tq + 1 < a.Tq && mk.sees(tq + 1 + off, j) && id.y == dk_;
+                o[2] = tq + 2 < a.Tq && mk.sees(tq + 2 + off, j) && id.z == dk_;
+                o[3] = tq + 3 < a.Tq && mk.sees(tq + 3 + off, j) && id.w == dk_;
+            });
+            __builtin_amdgcn_sched_barrier(0);
+            const uint4 pp[2] = {pack8<T>(s, 0), pack8<T>(s, 1)}, ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
+            uint4 xd = Ops<D>::at_col(cd, 0, 0, 0), xq = Ops<D>::at_col(cq, 0, 0, 0);
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const float4 x = *reinterpret_cast<const float4*>(&s_lse[buf][32 * u + 8 * g + 4 * h]);
-                    const float4 y = *reinterpret_cast<const float4*>(&s_del[buf][32 * u + 8 * g + 4 * h]);
-                    L[4 * g] = x.x; L[4 * g + 1] = x.y; L[4 * g + 2] = x.z; L[4 * g + 3] = x.w;
-                    Dl[4 * g] = y.x; Dl[4 * g + 1] = y.y; Dl[4 * g + 2] = y.z; Dl[4 * g + 3] = y.w;
+            for (int i = 0; i < 2 * DT; i++) {
+                const uint4 yd = xd, yq = xq;
+                if (i + 1 < 2 * DT) {
+                    xd = Ops<D>::at_col(cd, 0, (i + 1) % DT, (i + 1) / DT);
+                    xq = Ops<D>::at_col(cq, 0, (i + 1) % DT, (i + 1) / DT);
                 }
-                probs<CAP, BIAS>(s, dp, a, slope, j, t0 + off, h, all, [&](int r_) { return L[r_]; }, [&](int r_) { return Dl[r_]; }, [&](int r_) {
-                    const int tq = t0 + key_of(r_, h), pq = tq + off;
-                    return tq < a.Tq && mk.sees(pq, j) && (!docs || a.ids[idb + min(pq, a.Tk - 1)] == dk_);
-                });
-#pragma unroll
-                for (int mm = 0; mm < 2; mm++) {
-                    const uint4 pp = pack8<T>(s, mm), ds = pack8<T>(dp, mm);
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) {
-                        dv[dt] = mfma32<T>(Tile<D>::col_op(sd, 32 * u, dt, mm, lane), pp, dv[dt]);
-                        dk[dt] = mfma32<T>(Tile<D>::col_op(sq, 32 * u, dt, mm, lane), ds, dk[dt]);
-                    }
-                }
+                dv[i % DT] = mfma32<T>(yd, pp[i / DT], dv[i % DT]);
+                dk[i % DT] = mfma32<T>(yq, ds[i / DT], dk[i % DT]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        __syncthreads();
     }
-    if (j < a.Tk) {
+    const float f = a.scale;
+    if (a.nsplit > 1) {
+        float* o = a.part + (int64_t)blockIdx.x * 2 * BQ * D + (32 * w + (lane & 31)) * D + 4 * h;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                *reinterpret_cast<float4*>(o + 32 * dt + 8 * g) = make_float4(dk[dt][4 * g] * f, dk[dt][4 * g + 1] * f, dk[dt][4 * g + 2] * f, dk[dt][4 * g + 3] * f);
+                *reinterpret_cast<float4*>(o + BQ * D + 32 * dt + 8 * g) = make_float4(dv[dt][4 * g], dv[dt][4 * g + 1], dv[dt][4 * g + 2], dv[dt][4 * g + 3]);
+            }
+    } else if (j < a.Tk) {
         const int64_t o = (((int64_t)b * a.Tk + j) * a.Hk + hk) * D + 4 * h;
-        const float f = a.scale;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -327,11 +385,34 @@ __global__ __launch_bounds__(BT, 1) void attn_dkv(AttnArgs a) {
     }
 }
 
+// dK and dV of 32 keys from the parts' sums, added in order; 32 rows x D / 4 lanes of 4 values
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_add(AttnArgs a) {
+    const int kvh = a.B * a.Hk, bh = blockIdx.x % kvh, q4 = blockIdx.x / kvh, jt = q4 / (BQ / 32);
+    const int b = bh / a.Hk, hk = bh - b * a.Hk, off = a.Tk - a.Tq;
+    const int j0 = jt * BQ, j1 = min(j0 + BQ, a.Tk) - 1;
+    const Mask mk{a.causal, a.W, a.prefix ? a.prefix[b] : 0, a.Tk};
+    int x0, x1;
+    tile_rows(a, mk, j0, j1, off, x0, x1);
+    const int nx = (a.Tq + QT - 1) / QT;
+    for (int e = threadIdx.x; e < 32 * (D / 4) * 2; e += 256) {
+        const int which = e / (32 * (D / 4)), i = e % (32 * (D / 4)), row = (q4 % (BQ / 32)) * 32 + i / (D / 4), c = 4 * (i % (D / 4));
+        if (j0 + row >= a.Tk) continue;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = 0; p < a.nsplit; p++) {
+            if (!meets(x0, x1, nx, p * a.units, min((p + 1) * a.units, a.R * nx))) continue;
+            const float4 x = *reinterpret_cast<const float4*>(a.part + ((int64_t)(p * a.tiles + jt) * kvh + bh) * 2 * BQ * D + which * BQ * D + row * D + c);
+            s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+        }
+        put4<T>(which ? a.dv : a.dk, nullptr, (((int64_t)b * a.Tk + j0 + row) * a.Hk + hk) * D + c, s.x, s.y, s.z, s.w);
+    }
+}
+
 template <typename T, int D, bool CAP, bool BIAS>
 void launch_one(AttnArgs a, bool keys, hipStream_t st) {
     if (keys) {
         a.tiles = (a.Tk + BQ - 1) / BQ;
-        slothost::launch(attn_dkv<T, D, CAP, BIAS>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hk)), dim3(BT), 0, st, a);
+        slothost::launch(attn_dkv<T, D, CAP, BIAS>, dim3((unsigned)((int64_t)a.tiles * a.nsplit * a.B * a.Hk)), dim3(BT), 0, st, a);
     } else {
         a.tiles = (a.Tq + BQ - 1) / BQ;
         slothost::launch(attn_dq<T, D, CAP, BIAS>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(BT), 0, st, a);
@@ -343,26 +424,57 @@ void launch_bwd(const AttnArgs& a, bool cap, bool keys, hipStream_t st) {
     else a.slopes ? launch_one<T, D, false, true>(a, keys, st) : launch_one<T, D, false, false>(a, keys, st);
 }
 
+template <typename T, int D>
+void launch_add(AttnArgs a, hipStream_t st) {
+    a.tiles = (a.Tk + BQ - 1) / BQ;
+    slothost::launch(attn_add<T, D>, dim3((unsigned)((int64_t)a.tiles * (BQ / 32) * a.B * a.Hk)), dim3(256), 0, st, a);
+}
+
+// Parts of the queries per key tile: where the key tiles alone do not give the card's 512 workgroup slots a round and a half, each
+// workgroup takes about 1 / 1024 of all (key tile, 32-row query tile) pairs, 16 at least (a part costs the write and the read of its sums).
+void parts(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal, int64_t W, bool prefix, int& nsplit, int& units) {
+    const int64_t R = Hq / Hk, nx = (Tq + QT - 1) / QT, tiles = (Tk + BQ - 1) / BQ * B * Hk;
+    nsplit = 1;
+    units = (int)(R * nx);
+    if (tiles >= 768) return;
+    int64_t rows = causal ? Tq - Tq / 2 : Tq;                         // of a head that see a key tile, about
+    if (!prefix && W < Tk) rows = std::min(rows, (causal ? W : 2 * W) + BQ);
+    const int64_t c = std::max<int64_t>(16, tiles * R * ((rows + QT - 1) / QT) / 1024);
+    nsplit = (int)((R * nx + c - 1) / c);
+    units = (int)c;
+}
+
 }  // namespace
 
 // ======================================================================================== C-ABI
-extern "C" size_t slotattn_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) { return 0; }
+extern "C" size_t slotattn_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int causal, int64_t window,
+                                         int has_prefix) {
+    if (B < 1 || Tq < 1 || Tk < 1 || Hk < 1 || Hq < Hk || Hq % Hk) return 0;
+    int n, u;
+    parts(B, Tq, Tk, Hq, Hk, causal, window, has_prefix, n, u);
+    return n == 1 ? 0 : (size_t)((Tk + BQ - 1) / BQ * B * Hk * n) * 2 * BQ * D * sizeof(float);
+}
 
 extern "C" int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
                             int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int dtype, int64_t B, int64_t Tq,
                             int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal, int64_t window, float cap,
-                            const float* slopes, const void* docs, const int32_t* prefix, const void* out, const float* lse,
-                            const void* dout, int64_t do_sb, int64_t do_sh, int64_t do_st, void* workspace, float* delta, void* dq,
+                            const float* slopes, const void* docs, const int32_t* prefix, const void* out, const void* res,
+                            const float* lse, const void* dout, int64_t do_sb, int64_t do_sh, int64_t do_st, void* workspace, float* delta, void* dq,
                             void* dk, void* dv, void* stream) {
     if (int r = slotattn_host::check(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, dtype, B, Tq, Tk, Hq, Hk, D, window, cap)) return r;
     if (Tq > Tk) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: more queries than keys");
-    if (!out || !lse || !dout || !delta || !dq || !dk || !dv) return fail(SLOTSCAN_ERR_NULL, "slotattn_bwd: a required pointer is NULL");
-    if (!al16(out) || !al16(dout) || !al16(dq) || !al16(dk) || !al16(dv) || !al16(docs) || (do_sb | do_sh | do_st) % 8)
-        return fail(SLOTSCAN_ERR_ALIGN, "slotattn_bwd: rows of out, dout, dq, dk and dv, and docs, must be 16-byte aligned");
+    if (!out || !res || !lse || !dout || !delta || !dq || !dk || !dv) return fail(SLOTSCAN_ERR_NULL, "slotattn_bwd: a required pointer is NULL");
+    if (!al16(out) || !al16(res) || !al16(dout) || !al16(dq) || !al16(dk) || !al16(dv) || !al16(docs) || (do_sb | do_sh | do_st) % 8)
+        return fail(SLOTSCAN_ERR_ALIGN, "slotattn_bwd: rows of out, res, dout, dq, dk and dv, and docs, must be 16-byte aligned");
     if ((Tq + BQ - 1) / BQ * B * Hq > 0x7fffffffLL || (Tk + BQ - 1) / BQ * B * Hk > 0x7fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: shape too large");
     AttnArgs a = slotattn_host::args(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, B, Tq, Tk, Hq, Hk, scale, causal, window, cap,
                                      slopes, docs, prefix);
+    parts(B, Tq, Tk, Hq, Hk, causal, window, prefix != nullptr, a.nsplit, a.units);
+    if (a.nsplit > 1 && !workspace) return fail(SLOTSCAN_ERR_NULL, "slotattn_bwd: workspace is NULL");
+    if ((Tk + BQ - 1) / BQ * B * Hk * std::max(a.nsplit, BQ / 32) > 0x7fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: shape too large");
+    a.part = (float*)workspace;
     a.out = (void*)out;
+    a.res = (void*)res;
     a.lse = (float*)lse;
     a.dout = dout;
     a.do_sb = do_sb; a.do_sh = do_sh; a.do_st = do_st;
@@ -377,5 +489,10 @@ extern "C" int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return hip_fail(e, keys ? "attn_dkv launch" : "attn_dq launch");
     }
-    return 0;
+    if (a.nsplit == 1) return 0;
+    slothost::Scope sc(SLOTSCAN_K_ATTN_JOIN, st);
+    if (dtype == SLOTSCAN_BF16) D == 128 ? launch_add<bf16_t, 128>(a, st) : launch_add<bf16_t, 64>(a, st);
+    else D == 128 ? launch_add<f16_t, 128>(a, st) : launch_add<f16_t, 64>(a, st);
+    hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : hip_fail(e, "attn_add launch");
 }

@@ -62,20 +62,21 @@ def _documents(docs, B, T):
 
 
 def _launch_fwd(q_, k_, v_, opts, slopes, dws, prefix, lens, keep):
-    """(out (B, Tq, Hq, D), lse or None) on the current device."""
+    """out (B, Tq, Hq, D) and, to keep for a backward, what rounding took from it and lse; on the current device."""
     scale, causal, window, cap = opts
     B, Hq, Tq, D = q_.shape
     Hk, Tk = k_.shape[1:3]
     dev, lib = q_.device, L.lib()
     out = torch.empty(B, Tq, Hq, D, device=dev, dtype=q_.dtype)
+    res = torch.empty_like(out) if keep else None
     lse = torch.empty(B, Hq, Tq, device=dev, dtype=torch.float32) if keep else None
     n = lib.slotattn_fwd_workspace(B, Tq, Tk, Hq, Hk, D, causal, window, dws is not None, prefix is not None)
     ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
     rc = lib.slotattn_fwd(*L.strided(q_), *L.strided(k_), *L.strided(v_), L._TYPE_CODES[q_.dtype], B, Tq, Tk, Hq, Hk, D, scale,
                           causal, window, cap, L.ptr(slopes), L.ptr(dws), L.ptr(prefix), L.ptr(lens), L.ptr(ws), L.ptr(out),
-                          L.ptr(lse), L.stream_of(dev))
+                          L.ptr(res), L.ptr(lse), L.stream_of(dev))
     L.check(rc, "slotattn_fwd")
-    return out, lse
+    return out, res, lse
 
 
 class _Attend(torch.autograd.Function):
@@ -84,14 +85,14 @@ class _Attend(torch.autograd.Function):
         q_, k_, v_ = L.rows(q), L.rows(k), L.rows(v)
         with L.on(q.device):
             dws = None if docs is None else _documents(docs, k.shape[0], k.shape[2])
-            out, lse = _launch_fwd(q_, k_, v_, opts, slopes, dws, prefix, None, True)
-        ctx.save_for_backward(q_, k_, v_, out, lse, slopes, dws, prefix)
+            out, res, lse = _launch_fwd(q_, k_, v_, opts, slopes, dws, prefix, None, True)
+        ctx.save_for_backward(q_, k_, v_, out, res, lse, slopes, dws, prefix)
         ctx.opts = opts
         return out.transpose(1, 2)
 
     @staticmethod
     def backward(ctx, dout):
-        q_, k_, v_, out, lse, slopes, dws, prefix = ctx.saved_tensors
+        q_, k_, v_, out, res, lse, slopes, dws, prefix = ctx.saved_tensors
         scale, causal, window, cap = ctx.opts
         B, Hq, Tq, D = q_.shape
         Hk, Tk = k_.shape[1:3]
@@ -100,11 +101,11 @@ class _Attend(torch.autograd.Function):
         dq = torch.empty(B, Tq, Hq, D, device=dev, dtype=dt)
         dk, dv = (torch.empty(B, Tk, Hk, D, device=dev, dtype=dt) for _ in range(2))
         delta = torch.empty_like(lse)
-        n = lib.slotattn_bwd_workspace(B, Tq, Tk, Hq, Hk, D)
+        n = lib.slotattn_bwd_workspace(B, Tq, Tk, Hq, Hk, D, causal, window, prefix is not None)
         ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
         with L.on(dev):
             rc = lib.slotattn_bwd(*L.strided(q_), *L.strided(k_), *L.strided(v_), L._TYPE_CODES[dt], B, Tq, Tk, Hq, Hk, D, scale,
-                                  causal, window, cap, L.ptr(slopes), L.ptr(dws), L.ptr(prefix), L.ptr(out), L.ptr(lse),
+                                  causal, window, cap, L.ptr(slopes), L.ptr(dws), L.ptr(prefix), L.ptr(out), L.ptr(res), L.ptr(lse),
                                   *L.strided(do), L.ptr(ws), L.ptr(delta), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.stream_of(dev))
         L.check(rc, "slotattn_bwd")
         return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None, None, None
