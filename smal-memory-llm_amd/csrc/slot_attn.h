@@ -73,16 +73,19 @@ __device__ __forceinline__ void tile_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// A staged tile: rows of D 16-bit values, their 16-byte chunks XOR-swizzled so that both kinds of operand reads are free
-// of bank conflicts: 8 consecutive rows at one chunk (row operands, 16 bytes a lane) and 4 rows x 2 chunks (transposing
-// reads).  The swizzle keeps chunk pairs together, so both see 8 distinct pairs in the 64 banks.
+// A staged tile: rows of D 16-bit values, the 16-byte chunk c of row r at chunk c ^ swz(r).  The 64 banks are 256 bytes wide,
+// a row operand read serves 16 consecutive rows at one chunk at a time, a transposing read 4 rows (4 a .. 4 a + 3) at 4
+// chunks: swz gives the first 16 different places in the banks and the second 4 different groups of 4 (row bits 0, 1 --
+// those that the banks do not see already -- are its high bits, the next two its low ones).  With the row number itself in the place of swz
+// every read took twice its cycles.
 template <int D> struct Tile {
-    static constexpr int CH = D / 8, ROWB = 2 * D, RP = 256 / ROWB;
-    static __device__ __forceinline__ int pos(int r, int c) { return c ^ (2 * ((r / RP) & (CH / 2 - 1))); }
+    static constexpr int CH = D / 8, ROWB = 2 * D;
+    static __device__ __forceinline__ int swz(int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 2) << 1) | ((r >> 2) & 3); }
+    static __device__ __forceinline__ int pos(int r, int c) { return c ^ swz(r); }
 };
 
 // A lane's operand addresses in a staged tile, as LDS byte addresses: every k step or column block is the same address with
-// a few bits flipped, every 16 rows a constant further, so a lane holds two of them.
+// a few bits flipped, every 16 rows a constant further, so a lane holds three of them.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) const u32x4 lds_u4;
@@ -94,18 +97,20 @@ __device__ __forceinline__ uint2 lds_tr(unsigned a) {
 }
 template <int D> struct Ops {
     typedef Tile<D> Ti;
-    unsigned row, col;                               // relative to a tile's start (1 KB aligned)
+    unsigned row, col, col8;                         // relative to a tile's start (1 KB aligned); col8: 8 rows further
     __device__ __forceinline__ Ops(int lane) {
         const int l = lane & 31, h = lane >> 5, i = lane & 15, cr = 4 * h + (i >> 2);
         row = l * Ti::ROWB + 16 * Ti::pos(l, h);
-        col = cr * Ti::ROWB + 16 * Ti::pos(cr, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+        const int c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), by = 8 * (lane & 1);
+        col = cr * Ti::ROWB + 16 * Ti::pos(cr, c) + by;
+        col8 = (cr + 8) * Ti::ROWB + 16 * Ti::pos(cr + 8, c) + by;
     }
     // row operand of k step kk: values 16 kk + 8 h .. + 7 of row r + (l & 31), r a multiple of 32
     static __device__ __forceinline__ uint4 at_row(unsigned base, int r, int kk) { return lds16((base ^ (32 * kk)) + r * Ti::ROWB); }
     // operand over rows r + 16 m + 4 h .. + 3 and + 8 (a result tile's order) of column 32 dt + (l & 31)
-    static __device__ __forceinline__ uint4 at_col(unsigned base, int r, int dt, int m) {
-        const unsigned a = (base ^ (64 * dt)) + (r + 16 * m) * Ti::ROWB;
-        const uint2 lo = lds_tr(a), hi = lds_tr(a + 8 * Ti::ROWB);
+    __device__ __forceinline__ uint4 at_col(unsigned tile, int r, int dt, int m) const {
+        const unsigned o = tile + (r + 16 * m) * Ti::ROWB;
+        const uint2 lo = lds_tr((col ^ (64 * dt)) + o), hi = lds_tr((col8 ^ (64 * dt)) + o);
         return make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
 };
@@ -154,7 +159,8 @@ struct AttnArgs {
     const int32_t* ids; const int2* range; int ntd;  // documents: padded ids (B, 64 ntd), ranges (B, ntd)
     const int32_t* prefix; const int32_t* lens;
     float sc;                                        // scale log2(e): scores in base 2
-    float ct, c2;                                    // capped: 2 scale log2(e) / cap, cap log2(e)
+    float ct, c2, ic2;                               // capped: 2 scale log2(e) / cap, cap log2(e) and its inverse
+    float lim, t0, t1, t2, t3, t4;                   // the polynomial's limit and coefficients, for products <q, k>
     void* out; void* res; float* lse;                // res: what rounding took from out, for the backward's delta
     // split rows
     float* po; float* pm; int chunk, nsplit, tiles;
@@ -178,21 +184,34 @@ template <typename T> __device__ __forceinline__ void put4(void* out, void* res,
 // key of register r of a score tile's lane half h, from the tile's first key
 __device__ __forceinline__ constexpr int key_of(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
-// Scores of 32 keys from key j0 on in base 2, from the products s: scaled, capped and biased.  One query per lane, at
-// position p; slope in base 2.
-template <bool CAP, bool BIAS>
-__device__ __forceinline__ void scores(f32x16& s, const AttnArgs& a, float slope, int p, int j0, int h) {
+// The products s of a 32 x 32 tile as scores in base 2: scaled, or capped.  cap tanh(x) is x times a polynomial in x^2 while
+// |x| <= 3/4 (relative error 7e-7; 6 instructions, none of them a transcendental one), which the scores of a whole tile
+// usually are, else cap - 2 cap / (1 + e^2x) (off by a few 2^-24 of the cap).  attend_long, capped, forward: PLACEHOLDER.
+template <bool CAP> __device__ __forceinline__ void scores(f32x16& s, const AttnArgs& a) {
+    if constexpr (!CAP) {
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-        // cap tanh(x) = cap - 2 cap / (1 + e^2x): off by a few 2^-24 of the cap
-        if constexpr (CAP) s[r] = fmaf(-2.f * a.c2, __builtin_amdgcn_rcpf(1.f + exp2_(s[r] * a.ct)), a.c2);
-        else s[r] *= a.sc;
-    }
-    if constexpr (BIAS) {
-        const float d = (float)(p - j0 - 4 * h);
+        for (int r = 0; r < 16; r++) s[r] *= a.sc;
+    } else {
+        float m = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = fmaf(-slope, fabsf(d - (float)key_of(r, 0)), s[r]);
+        for (int r = 0; r < 16; r++) m = fmaxf(m, fabsf(s[r]));
+        if (__all(m <= a.lim)) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float y = s[r] * s[r];
+                s[r] *= fmaf(fmaf(fmaf(fmaf(a.t4, y, a.t3), y, a.t2), y, a.t1), y, a.t0);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = fmaf(-2.f * a.c2, __builtin_amdgcn_rcpf(1.f + exp2_(s[r] * a.ct)), a.c2);
+        }
     }
+}
+// Minus slope (in base 2) x distance: the lane's own position p against rows j0 + key_of(r, h)
+__device__ __forceinline__ void bias(f32x16& s, float slope, int p, int j0, int h) {
+    const float d = (float)(p - j0 - 4 * h);
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] = fmaf(-slope, fabsf(d - (float)key_of(r, 0)), s[r]);
 }
 
 // Tokens of sequence b that count, and its length that positions are taken from (a length past the keys keeps its positions).

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
         tile_barrier();
         if (jn >= 0) load(jn, buf ^ 1);
         if (some) {
-            const unsigned sk = lds + (2 * buf) * STAGE + ops.row, sx = lds + (2 * buf + 1) * STAGE + ops.col;
+            const unsigned sk = lds + (2 * buf) * STAGE + ops.row, sx = lds + (2 * buf + 1) * STAGE;
             const int j0 = jt * KT;
             f32x16 s[2];
 #pragma unroll
@@ -106,7 +106,10 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
                 for (int kk = 0; kk < KK; kk++) s[u] = mfma32<T>(Ops<D>::at_row(sk, 32 * u, kk), qf[kk], s[u]);
             }
 #pragma unroll
-            for (int u = 0; u < 2; u++) scores<CAP, BIAS>(s[u], a, slope, p, j0 + 32 * u, h);
+            for (int u = 0; u < 2; u++) {
+                scores<CAP>(s[u], a);
+                if constexpr (BIAS) bias(s[u], slope, p, j0 + 32 * u, h);
+            }
             if (!all) {
 #pragma unroll
                 for (int u = 0; u < 2; u++)
@@ -153,7 +156,7 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(Ops<D>::at_col(sx, 32 * u, dt, mm), pf[u][mm], o[dt]);
+                    for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(ops.at_col(sx, 32 * u, dt, mm), pf[u][mm], o[dt]);
         }
     }
     l = half_sum(l);
@@ -225,11 +228,12 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
             wait_vm<0>();
         }
         asm volatile("" ::: "memory");
-        const unsigned sk = lds + (2 * buf) * ST + ops.row, sx = lds + (2 * buf + 1) * ST + ops.col;
+        const unsigned sk = lds + (2 * buf) * ST + ops.row, sx = lds + (2 * buf + 1) * ST;
         f32x16 x = zero16();
 #pragma unroll
         for (int kk = 0; kk < KK; kk++) x = mfma32<T>(Ops<D>::at_row(sk, 0, kk), qf[kk], x);
-        scores<CAP, BIAS>(x, a, slope, p, j0, h);
+        scores<CAP>(x, a);
+        if constexpr (BIAS) bias(x, slope, p, j0, h);
         if (j0 + 32 > hi || !mk.all(s, j0, j0 + 31)) {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
@@ -261,7 +265,7 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(Ops<D>::at_col(sx, 0, dt, mm), pf[mm], o[dt]);
+            for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(ops.at_col(sx, 0, dt, mm), pf[mm], o[dt]);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the tile is read before its buffer is filled again
         j0 = jn;
     }

@@ -43,6 +43,7 @@ __device__ __forceinline__ void dot8(const uint4& x, const uint4& y, float& s, f
 // d0: the position of register row 0.  ok(g, o): which of those four are visible (only asked if !all).
 template <bool CAP, bool BIAS, class LD, class OK>
 __device__ __forceinline__ void probs(f32x16& s, f32x16& dp, const AttnArgs& a, float slope, int dist, int d0, int h, bool all, LD ld, OK ok) {
+    scores<CAP>(s, a);
     const float d = BIAS ? (float)(dist - d0 - 4 * h) : 0.f;
 #pragma unroll
     for (int g = 0; g < 4; g++) {
@@ -51,13 +52,10 @@ __device__ __forceinline__ void probs(f32x16& s, f32x16& dp, const AttnArgs& a, 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = 4 * g + i;
-            float x, t = 1.f;
-            if constexpr (CAP) {                      // tanh = 1 - 2 z, 1 - tanh^2 = 4 z (1 - z), z = 1 / (1 + e^2x)
-                const float z = __builtin_amdgcn_rcpf(1.f + exp2_(s[r] * a.ct));
-                x = fmaf(-2.f * a.c2, z, a.c2) - L[i];
-                t = 4.f * z * (1.f - z);
-            } else {
-                x = fmaf(s[r], a.sc, -L[i]);
+            float t = 1.f, x = s[r] - L[i];
+            if constexpr (CAP) {
+                const float th = s[r] * a.ic2;
+                t = fmaf(-th, th, 1.f);
             }
             if constexpr (BIAS) x = fmaf(-slope, fabsf(d - (float)key_of(r, 0)), x);
             s[r] = exp2_(x);
@@ -146,7 +144,7 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
         tile_barrier();
         if (jn >= 0) load(jn, buf ^ 1);
         if (some) {
-            const unsigned sk = lds + (2 * buf) * STAGE + ops.row, sx = sk + STAGE, sc = lds + (2 * buf) * STAGE + ops.col;
+            const unsigned sk = lds + (2 * buf) * STAGE + ops.row, sx = sk + STAGE, sc = lds + (2 * buf) * STAGE;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int j0 = jt * KT + 32 * u;
@@ -168,7 +166,7 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
                 for (int mm = 0; mm < 2; mm++) {
                     const uint4 ds = pack8<T>(dp, mm);
 #pragma unroll
-                    for (int dt = 0; dt < DT; dt++) acc[dt] = mfma32<T>(Ops<D>::at_col(sc, 32 * u, dt, mm), ds, acc[dt]);
+                    for (int dt = 0; dt < DT; dt++) acc[dt] = mfma32<T>(ops.at_col(sc, 32 * u, dt, mm), ds, acc[dt]);
                 }
             }
         }
@@ -316,7 +314,7 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
         }
         if (some) {
             const unsigned sq = ldq + (2 * buf) * STAGE + ops.row, sd = sq + STAGE, sk = lds + 32 * w * Tile<D>::ROWB + ops.row;
-            const unsigned cq = ldq + (2 * buf) * STAGE + ops.col, cd = cq + STAGE;
+            const unsigned cq = ldq + (2 * buf) * STAGE, cd = cq + STAGE;
             const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
             f32x16 s = zero16(), dp = zero16();
             uint4 oq = Ops<D>::at_row(sq, 0, 0), ok_ = Ops<D>::at_row(sk, 0, 0), od = Ops<D>::at_row(sd, 0, 0);
@@ -347,13 +345,13 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
             });
             __builtin_amdgcn_sched_barrier(0);
             const uint4 pp[2] = {pack8<T>(s, 0), pack8<T>(s, 1)}, ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
-            uint4 xd = Ops<D>::at_col(cd, 0, 0, 0), xq = Ops<D>::at_col(cq, 0, 0, 0);
+            uint4 xd = ops.at_col(cd, 0, 0, 0), xq = ops.at_col(cq, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < 2 * DT; i++) {
                 const uint4 yd = xd, yq = xq;
                 if (i + 1 < 2 * DT) {
-                    xd = Ops<D>::at_col(cd, 0, (i + 1) % DT, (i + 1) / DT);
-                    xq = Ops<D>::at_col(cq, 0, (i + 1) % DT, (i + 1) / DT);
+                    xd = ops.at_col(cd, 0, (i + 1) % DT, (i + 1) / DT);
+                    xq = ops.at_col(cq, 0, (i + 1) % DT, (i + 1) / DT);
                 }
                 dv[i % DT] = mfma32<T>(yd, pp[i / DT], dv[i % DT]);
                 dk[i % DT] = mfma32<T>(yq, ds[i / DT], dk[i % DT]);
