@@ -105,12 +105,14 @@ template <int D> struct Ops {
         col = cr * Ti::ROWB + 16 * Ti::pos(cr, c) + by;
         col8 = (cr + 8) * Ti::ROWB + 16 * Ti::pos(cr + 8, c) + by;
     }
-    // row operand of k step kk: values 16 kk + 8 h .. + 7 of row r + (l & 31), r a multiple of 32
-    static __device__ __forceinline__ uint4 at_row(unsigned base, int r, int kk) { return lds16((base ^ (32 * kk)) + r * Ti::ROWB); }
-    // operand over rows r + 16 m + 4 h .. + 3 and + 8 (a result tile's order) of column 32 dt + (l & 31)
-    __device__ __forceinline__ uint4 at_col(unsigned tile, int r, int dt, int m) const {
-        const unsigned o = tile + (r + 16 * m) * Ti::ROWB;
-        const uint2 lo = lds_tr((col ^ (64 * dt)) + o), hi = lds_tr((col8 ^ (64 * dt)) + o);
+    // A tile's operands, from a lane's address of one of the three kinds plus the tile's start (1 KB aligned): tiles a
+    // constant apart share the flipped address, the rest is the instruction's offset.
+    // row operand of k step kk: values 16 kk + 8 h .. + 7 of row l & 31, `at` bytes further
+    static __device__ __forceinline__ unsigned k_step(unsigned row, int kk) { return row ^ (32 * kk); }
+    static __device__ __forceinline__ unsigned block(unsigned col, int dt) { return col ^ (64 * dt); }
+    // operand over rows r + 16 m + 4 h .. + 3 and + 8 (a result tile's order) of a column block: block() of col and col8
+    static __device__ __forceinline__ uint4 at_col(unsigned c, unsigned c8, int at) {
+        const uint2 lo = lds_tr(c + at), hi = lds_tr(c8 + at);
         return make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
 };
@@ -158,8 +160,8 @@ struct AttnArgs {
     const float* slopes;
     const int32_t* ids; const int2* range; int ntd;  // documents: padded ids (B, 64 ntd), ranges (B, ntd)
     const int32_t* prefix; const int32_t* lens;
-    float sc;                                        // scale log2(e): scores in base 2
-    float ct, c2, ic2;                               // capped: 2 scale log2(e) / cap, cap log2(e) and its inverse
+    float f;                                         // what makes scores() base 2: scale log2(e), or cap log2(e)
+    float ct;                                        // capped: 2 scale log2(e) / cap
     float lim, t0, t1, t2, t3, t4;                   // the polynomial's limit and coefficients, for products <q, k>
     void* out; void* res; float* lse;                // res: what rounding took from out, for the backward's delta
     // split rows
@@ -184,14 +186,12 @@ template <typename T> __device__ __forceinline__ void put4(void* out, void* res,
 // key of register r of a score tile's lane half h, from the tile's first key
 __device__ __forceinline__ constexpr int key_of(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
-// The products s of a 32 x 32 tile as scores in base 2: scaled, or capped.  cap tanh(x) is x times a polynomial in x^2 while
-// |x| <= 3/4 (relative error 7e-7; 6 instructions, none of them a transcendental one), which the scores of a whole tile
-// usually are, else cap - 2 cap / (1 + e^2x) (off by a few 2^-24 of the cap).  attend_long, capped, forward: PLACEHOLDER.
+// The products s of a 32 x 32 tile become scores up to the factor() that makes them base 2: as they are, or tanh of the scaled
+// product where they are capped.  tanh(x) is x times a polynomial in x^2 while |x| <= 3/4 (relative error 7e-7; 6
+// instructions, none of them a transcendental one), which the scores of a whole tile usually are, else 1 - 2 / (1 + e^2x)
+// (off by a few 2^-24).
 template <bool CAP> __device__ __forceinline__ void scores(f32x16& s, const AttnArgs& a) {
-    if constexpr (!CAP) {
-#pragma unroll
-        for (int r = 0; r < 16; r++) s[r] *= a.sc;
-    } else {
+    if constexpr (CAP) {
         float m = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; r++) m = fmaxf(m, fabsf(s[r]));
@@ -203,15 +203,16 @@ template <bool CAP> __device__ __forceinline__ void scores(f32x16& s, const Attn
             }
         } else {
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = fmaf(-2.f * a.c2, __builtin_amdgcn_rcpf(1.f + exp2_(s[r] * a.ct)), a.c2);
+            for (int r = 0; r < 16; r++) s[r] = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp2_(s[r] * a.ct)), 1.f);
         }
     }
 }
-// Minus slope (in base 2) x distance: the lane's own position p against rows j0 + key_of(r, h)
-__device__ __forceinline__ void bias(f32x16& s, float slope, int p, int j0, int h) {
+// Scores in base 2, less slope (in base 2) x distance: the lane's own position p against rows j0 + key_of(r, h); their
+// factor is 1 from here on
+__device__ __forceinline__ void bias(f32x16& s, float f, float slope, int p, int j0, int h) {
     const float d = (float)(p - j0 - 4 * h);
 #pragma unroll
-    for (int r = 0; r < 16; r++) s[r] = fmaf(-slope, fabsf(d - (float)key_of(r, 0)), s[r]);
+    for (int r = 0; r < 16; r++) s[r] = fmaf(-slope, fabsf(d - (float)key_of(r, 0)), s[r] * f);
 }
 
 // Tokens of sequence b that count, and its length that positions are taken from (a length past the keys keeps its positions).

@@ -1,5 +1,8 @@
 // Argument checks and kernel arguments shared by the attention entry points (slotattn.hip, slotattn_bwd.hip).
 #pragma once
+#include <algorithm>
+#include <cmath>
+
 #include "slot_attn.h"
 #include "slot_host.h"
 #include "slotscan.h"
@@ -10,14 +13,15 @@ namespace slotattn_host {
 
 inline int check(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st,
                  const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
-                 int64_t Hk, int64_t D, int64_t window, float cap) {
+                 int64_t Hk, int64_t D, float scale, int64_t window, float cap) {
     using slothost::fail;
     using slothost::al16;
     if (B < 1 || Tq < 1 || Tk < 1 || Hq < 1 || Hk < 1) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: B, Tq, Tk, Hq, Hk must be >= 1");
     if (Hq % Hk) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: Hq must be a multiple of Hk");
     if (D != 64 && D != 128) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: D must be 64 or 128");
     if (window < 1 || window > 0x7fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: window must be in [1, 2^31)");
-    if (!(cap >= 0.f)) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: cap must be >= 0");
+    if (!(cap == 0.f || (cap >= 1e-30f && cap <= 1e30f))) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: cap must be 0 or in [1e-30, 1e30]");
+    if (!(std::fabs(scale) >= 1e-30f && std::fabs(scale) <= 1e30f)) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: |scale| must be in [1e-30, 1e30]");
     if (Tq > SLOTATTN_MAX_T || Tk > SLOTATTN_MAX_T || B > 0x7fffffffLL / Hq || Hq / Hk * Tq > SLOTATTN_MAX_T)
         return fail(SLOTSCAN_ERR_SHAPE, "slotattn: shape too large");
     if (dtype != SLOTSCAN_BF16 && dtype != SLOTSCAN_F16) return fail(SLOTSCAN_ERR_DTYPE, "slotattn: dtype must be bf16 or fp16");
@@ -45,18 +49,17 @@ inline slotattn::AttnArgs args(const void* q, int64_t q_sb, int64_t q_sh, int64_
     a.range = docs ? (const int2*)((const int32_t*)docs + B * a.ntd * KT) : nullptr;
     a.prefix = prefix;
     a.scale = scale;
-    a.sc = scale * LOG2E;
+    a.f = scale * LOG2E;
     if (cap > 0.f) {
-        a.ct = 2.f * scale * LOG2E / cap;
-        a.c2 = cap * LOG2E;
-        a.ic2 = 1.f / a.c2;
-        // tanh(x) / x on [0, 3/4] as a polynomial in x^2, fitted for the smallest largest relative error
-        const double t[5] = {0.99999943, -0.33328252, 0.13258983, -0.05005631, 0.01292964};
-        const double k = (double)scale / cap;
-        double f = (double)cap * 1.4426950408889634 * k;
+        a.f = cap * LOG2E;
+        a.ct = (float)std::min(std::max(2.0 * scale / cap * 1.4426950408889634, -1e37), 1e37);
+        // tanh(x) / x on [0, 3/4] as a polynomial in x^2, fitted for the smallest largest relative error; x = k <q, k>
+        const double t[5] = {0.99999943, -0.33328252, 0.13258983, -0.05005631, 0.01292964}, k = (double)scale / cap;
+        double f = k;
         float* c[5] = {&a.t0, &a.t1, &a.t2, &a.t3, &a.t4};
         for (int i = 0; i < 5; i++, f *= k * k) *c[i] = (float)(t[i] * f);
-        a.lim = (float)(0.75 / (k < 0 ? -k : k));
+        const double m = k < 0 ? -k : k;
+        a.lim = m >= 1e-4 && m <= 1e3 ? (float)(0.75 / m) : -1.f;     // beyond, k^9 leaves fp32: no score takes the polynomial
     }
     a.nsplit = 1;
     return a;

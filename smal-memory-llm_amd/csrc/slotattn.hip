@@ -59,7 +59,11 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
         const T* q = (const T*)a.q + b * a.q_sb + hq * a.q_sh + tc * a.q_st + 8 * h;
 #pragma unroll
         for (int kk = 0; kk < KK; kk++) qf[kk] = ld16(q + 16 * kk);
+        if (a.f < 0.f)                                // a negative scale: of the queries' sign, so that larger products are larger scores
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) { qf[kk].x ^= 0x80008000u; qf[kk].y ^= 0x80008000u; qf[kk].z ^= 0x80008000u; qf[kk].w ^= 0x80008000u; }
     }
+    const float f2 = fabsf(a.f);
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
     const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
@@ -74,6 +78,7 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
         if (dq < 0) dq = -2;
     }
     Walk walk(mk, sw, sv, docs ? a.range + (int64_t)b * a.ntd : nullptr, lane);
+    const float F = BIAS ? 1.f : f2;                  // from a row's values to base 2
     const unsigned lds = lds_addr(smem);
     auto load = [&](int jt, int buf) {
         Load::issue(kb, a.k_st, jt * KT, mk.klen - 1, lds + (2 * buf) * STAGE, w, lane);
@@ -96,19 +101,19 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
         tile_barrier();
         if (jn >= 0) load(jn, buf ^ 1);
         if (some) {
-            const unsigned sk = lds + (2 * buf) * STAGE + ops.row, sx = lds + (2 * buf + 1) * STAGE;
+            const unsigned bo = lds + (2 * buf) * STAGE, rk = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
             const int j0 = jt * KT;
-            f32x16 s[2];
+            f32x16 s[2] = {zero16(), zero16()};
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                s[u] = zero16();
+            for (int kk = 0; kk < KK; kk++) {
+                const unsigned x = Ops<D>::k_step(rk, kk);
 #pragma unroll
-                for (int kk = 0; kk < KK; kk++) s[u] = mfma32<T>(Ops<D>::at_row(sk, 32 * u, kk), qf[kk], s[u]);
+                for (int u = 0; u < 2; u++) s[u] = mfma32<T>(lds16(x + 32 * u * Tile<D>::ROWB), qf[kk], s[u]);
             }
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 scores<CAP>(s[u], a);
-                if constexpr (BIAS) bias(s[u], slope, p, j0 + 32 * u, h);
+                if constexpr (BIAS) bias(s[u], f2, slope, p, j0 + 32 * u, h);
             }
             if (!all) {
 #pragma unroll
@@ -128,10 +133,9 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
-            mx = half_max(mx);
-            const float mn = fmaxf(m, mx);
-            if (__any(mn > m)) {
-                const float f = m == -INFINITY ? 0.f : exp2_(m - mn);
+            mx = half_max(mx) * F;
+            if (__any(mx > m)) {
+                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_(m - mn);
                 m = mn;
                 l *= f;
 #pragma unroll
@@ -145,18 +149,20 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
             for (int u = 0; u < 2; u++) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    s[u][r] = exp2_(s[u][r] - mu);
+                    s[u][r] = exp2_(fmaf(s[u][r], F, -mu));
                     l += s[u][r];
                 }
                 pf[u][0] = pack8<T>(s[u], 0);
                 pf[u][1] = pack8<T>(s[u], 1);
             }
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++)
+            for (int dt = 0; dt < DT; dt++) {
+                const unsigned x = Ops<D>::block(c, dt), x8 = Ops<D>::block(c8, dt);
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(ops.at_col(sx, 32 * u, dt, mm), pf[u][mm], o[dt]);
+                    for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(Ops<D>::at_col(x, x8, STAGE + (32 * u + 16 * mm) * Tile<D>::ROWB), pf[u][mm], o[dt]);
+            }
         }
     }
     l = half_sum(l);
@@ -197,6 +203,7 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
     const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
+    const float f2 = fabsf(a.f), F = BIAS ? 1.f : f2;
     const unsigned lds = lds_addr(smem[w]);
     auto load = [&](int j0, int buf) {
         Load::issue(kb, a.k_st, j0, klen - 1, lds + (2 * buf) * ST, 0, lane);
@@ -214,6 +221,9 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
         const T* q = (const T*)a.q + b * a.q_sb + hq * a.q_sh + t * a.q_st + 8 * h;
 #pragma unroll
         for (int kk = 0; kk < KK; kk++) qf[kk] = ld16(q + 16 * kk);
+        if (a.f < 0.f)                                // a negative scale: of the queries' sign, so that larger products are larger scores
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) { qf[kk].x ^= 0x80008000u; qf[kk].y ^= 0x80008000u; qf[kk].z ^= 0x80008000u; qf[kk].w ^= 0x80008000u; }
     }
     f32x16 o[DT];
 #pragma unroll
@@ -228,12 +238,12 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
             wait_vm<0>();
         }
         asm volatile("" ::: "memory");
-        const unsigned sk = lds + (2 * buf) * ST + ops.row, sx = lds + (2 * buf + 1) * ST;
+        const unsigned bo = lds + (2 * buf) * ST, rk = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
         f32x16 x = zero16();
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++) x = mfma32<T>(Ops<D>::at_row(sk, 0, kk), qf[kk], x);
+        for (int kk = 0; kk < KK; kk++) x = mfma32<T>(lds16(Ops<D>::k_step(rk, kk)), qf[kk], x);
         scores<CAP>(x, a);
-        if constexpr (BIAS) bias(x, slope, p, j0, h);
+        if constexpr (BIAS) bias(x, f2, slope, p, j0, h);
         if (j0 + 32 > hi || !mk.all(s, j0, j0 + 31)) {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
@@ -244,10 +254,9 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
         float mx = x[0];
 #pragma unroll
         for (int r = 1; r < 16; r++) mx = fmaxf(mx, x[r]);
-        mx = half_max(mx);
-        const float mn = fmaxf(m, mx);
-        if (__any(mn > m)) {
-            const float f = m == -INFINITY ? 0.f : exp2_(m - mn);
+        mx = half_max(mx) * F;
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_(m - mn);
             m = mn;
             l *= f;
 #pragma unroll
@@ -258,14 +267,15 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
         const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-            x[r] = exp2_(x[r] - mu);
+            x[r] = exp2_(fmaf(x[r], F, -mu));
             l += x[r];
         }
         const uint4 pf[2] = {pack8<T>(x, 0), pack8<T>(x, 1)};
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(ops.at_col(sx, 0, dt, mm), pf[mm], o[dt]);
+            for (int mm = 0; mm < 2; mm++)
+                o[dt] = mfma32<T>(Ops<D>::at_col(Ops<D>::block(c, dt), Ops<D>::block(c8, dt), ST + 16 * mm * Tile<D>::ROWB), pf[mm], o[dt]);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the tile is read before its buffer is filled again
         j0 = jn;
     }
@@ -454,7 +464,7 @@ extern "C" int slotattn_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
                             int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal, int64_t window, float cap,
                             const float* slopes, const void* docs, const int32_t* prefix, const int32_t* lens, void* workspace,
                             void* out, void* res, float* lse, void* stream) {
-    if (int r = slotattn_host::check(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, dtype, B, Tq, Tk, Hq, Hk, D, window, cap)) return r;
+    if (int r = slotattn_host::check(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, dtype, B, Tq, Tk, Hq, Hk, D, scale, window, cap)) return r;
     if (lens && (docs || !causal)) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_fwd: lens goes with causality and without documents");
     if (!lens && Tq > Tk) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_fwd: more queries than keys");
     if (!out) return fail(SLOTSCAN_ERR_NULL, "slotattn_fwd: a required pointer is NULL");

@@ -38,28 +38,25 @@ __device__ __forceinline__ void dot8(const uint4& x, const uint4& y, float& s, f
     for (int i = 0; i < 8; i++) s = fmaf((float)a[i], (float)b[i], s);
 }
 
-// P and dS of one 32 x 32 tile, in the place of its products s = <q, k> and dp = <dO, v>; LD(g, L, Dl): log-sum-exp and
-// delta of registers 4 g .. 4 g + 3, so that no more of them are held than a few scores need.  dist: the lane's own position;
-// d0: the position of register row 0.  ok(g, o): which of those four are visible (only asked if !all).
+// P and dS of one 32 x 32 tile, in the place of its products s = <q, k> and dp = <dO, v> - delta; ld(g): the log-sum-exp of
+// registers 4 g .. 4 g + 3, so that no more of them are held than a few scores need.  dist: the lane's own position; d0: the
+// position of register row 0.  ok(g, o): which of those four are visible (only asked if !all).
 template <bool CAP, bool BIAS, class LD, class OK>
 __device__ __forceinline__ void probs(f32x16& s, f32x16& dp, const AttnArgs& a, float slope, int dist, int d0, int h, bool all, LD ld, OK ok) {
     scores<CAP>(s, a);
     const float d = BIAS ? (float)(dist - d0 - 4 * h) : 0.f;
 #pragma unroll
     for (int g = 0; g < 4; g++) {
-        f32x4 L, Dl;
-        ld(g, L, Dl);
+        const f32x4 L = ld(g);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = 4 * g + i;
-            float t = 1.f, x = s[r] - L[i];
-            if constexpr (CAP) {
-                const float th = s[r] * a.ic2;
-                t = fmaf(-th, th, 1.f);
-            }
+            const float t = s[r];                     // capped: the tanh, whose slope is 1 - t^2
+            float x = fmaf(t, a.f, -L[i]);
             if constexpr (BIAS) x = fmaf(-slope, fabsf(d - (float)key_of(r, 0)), x);
             s[r] = exp2_(x);
-            dp[r] = s[r] * (dp[r] - Dl[i]) * t;
+            dp[r] *= s[r];
+            if constexpr (CAP) dp[r] *= fmaf(-t, t, 1.f);
         }
     }
     if (!all) {
@@ -144,17 +141,20 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
         tile_barrier();
         if (jn >= 0) load(jn, buf ^ 1);
         if (some) {
-            const unsigned sk = lds + (2 * buf) * STAGE + ops.row, sx = sk + STAGE, sc = lds + (2 * buf) * STAGE;
+            const unsigned bo = lds + (2 * buf) * STAGE, rk = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const int j0 = jt * KT + 32 * u;
-                f32x16 s = zero16(), dp = zero16();
+                const int j0 = jt * KT + 32 * u, at = 32 * u * Tile<D>::ROWB;
+                f32x16 s = zero16(), dp;
+#pragma unroll
+                for (int r = 0; r < 16; r++) dp[r] = -delta;
 #pragma unroll
                 for (int kk = 0; kk < KK; kk++) {
-                    s = mfma32<T>(Ops<D>::at_row(sk, 32 * u, kk), qf[kk], s);
-                    dp = mfma32<T>(Ops<D>::at_row(sx, 32 * u, kk), df[kk], dp);
+                    const unsigned x = Ops<D>::k_step(rk, kk);
+                    s = mfma32<T>(lds16(x + at), qf[kk], s);
+                    dp = mfma32<T>(lds16(x + at + STAGE), df[kk], dp);
                 }
-                probs<CAP, BIAS>(s, dp, a, slope, p, j0, h, all, [&](int, f32x4& L, f32x4& Dl) { L = f32x4{lse, lse, lse, lse}; Dl = f32x4{delta, delta, delta, delta}; }, [&](int g, bool (&o)[4]) {
+                probs<CAP, BIAS>(s, dp, a, slope, p, j0, h, all, [&](int) { return f32x4{lse, lse, lse, lse}; }, [&](int g, bool (&o)[4]) {
                     const int j = j0 + 8 * g + 4 * h;
                     const int4 id = docs ? *reinterpret_cast<const int4*>(a.ids + idb + j) : make_int4(0, 0, 0, 0);
                     o[0] = mk.sees(p, j) && id.x == dq;
@@ -162,11 +162,12 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
                     o[2] = mk.sees(p, j + 2) && id.z == dq;
                     o[3] = mk.sees(p, j + 3) && id.w == dq;
                 });
+                const uint4 ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
 #pragma unroll
-                for (int mm = 0; mm < 2; mm++) {
-                    const uint4 ds = pack8<T>(dp, mm);
+                for (int dt = 0; dt < DT; dt++) {
+                    const unsigned x = Ops<D>::block(c, dt), x8 = Ops<D>::block(c8, dt);
 #pragma unroll
-                    for (int dt = 0; dt < DT; dt++) acc[dt] = mfma32<T>(ops.at_col(sc, 32 * u, dt, mm), ds, acc[dt]);
+                    for (int mm = 0; mm < 2; mm++) acc[dt] = mfma32<T>(Ops<D>::at_col(x, x8, at + 16 * mm * Tile<D>::ROWB), ds[mm], acc[dt]);
                 }
             }
         }
@@ -281,10 +282,10 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
         Load::issue((const T*)a.q + b * a.q_sb + hq * a.q_sh, a.q_st, xt * QT, a.Tq - 1, ldq + (2 * buf) * STAGE, w, lane);
         Load::issue((const T*)a.dout + b * a.do_sb + hq * a.do_sh, a.do_st, xt * QT, a.Tq - 1, ldq + (2 * buf + 1) * STAGE, w, lane);
     };
-    auto stat = [&](int hq, int xt) {                 // lanes 0..31 of the first wave the log-sum-exp, 32..63 delta of a row
+    auto stat = [&](int hq, int xt) {                 // lanes 0..31 of the first wave the log-sum-exp, 32..63 minus delta of a row
         const int t = xt * QT + (lane & 31);
         const int64_t i = ((int64_t)b * a.Hq + hq) * a.Tq + min(t, a.Tq - 1);
-        const float v = h ? a.delta[i] : a.lse[i];
+        const float v = h ? -a.delta[i] : a.lse[i];
         return t < a.Tq ? v : (h ? 0.f : INFINITY);
     };
     int hq, xt, hn = 0, xn;
@@ -313,28 +314,35 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
             load(hn, xn, buf ^ 1);
         }
         if (some) {
-            const unsigned sq = ldq + (2 * buf) * STAGE + ops.row, sd = sq + STAGE, sk = lds + 32 * w * Tile<D>::ROWB + ops.row;
-            const unsigned cq = ldq + (2 * buf) * STAGE, cd = cq + STAGE;
+            const unsigned bo = lds + (2 * buf) * STAGE, rq = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
+            const unsigned rk = lds + 32 * w * Tile<D>::ROWB + ops.row;
             const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
-            f32x16 s = zero16(), dp = zero16();
-            uint4 oq = Ops<D>::at_row(sq, 0, 0), ok_ = Ops<D>::at_row(sk, 0, 0), od = Ops<D>::at_row(sd, 0, 0);
+            f32x16 s = zero16(), dp;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {             // minus delta
+                const f32x4 y = lds4f(stb + (2 * buf + 1) * QT * 4 + 32 * g);
+                dp[4 * g] = y.x; dp[4 * g + 1] = y.y; dp[4 * g + 2] = y.z; dp[4 * g + 3] = y.w;
+            }
+            unsigned x = Ops<D>::k_step(rq, 0);
+            uint4 oq = lds16(x + KEYS), ok = lds16(Ops<D>::k_step(rk, 0)), od = lds16(x + KEYS + STAGE);
 #pragma unroll
             for (int kk = 0; kk < KK; kk++) {
-                const uint4 cq_ = oq, ck_ = ok_, cd_ = od;
+                const uint4 pq = oq, pk = ok, pd = od;
                 if (kk + 1 < KK) {
-                    oq = Ops<D>::at_row(sq, 0, kk + 1);
-                    ok_ = Ops<D>::at_row(sk, 0, kk + 1);
-                    od = Ops<D>::at_row(sd, 0, kk + 1);
+                    x = Ops<D>::k_step(rq, kk + 1);
+                    oq = lds16(x + KEYS);
+                    ok = lds16(Ops<D>::k_step(rk, kk + 1));
+                    od = lds16(x + KEYS + STAGE);
                 }
-                s = mfma32<T>(cq_, ck_, s);
-                dp = mfma32<T>(cd_, vf[kk], dp);
+                s = mfma32<T>(pq, pk, s);
+                dp = mfma32<T>(pd, vf[kk], dp);
                 __builtin_amdgcn_sched_barrier(0);
             }
             const int t0 = xt * QT;
-            probs<CAP, BIAS>(s, dp, a, slope, j, t0 + off, h, all, [&](int g, f32x4& L, f32x4& Dl) {
-                L = lds4f(stb + (2 * buf) * QT * 4 + 32 * g);
-                Dl = lds4f(stb + (2 * buf + 1) * QT * 4 + 32 * g);
+            probs<CAP, BIAS>(s, dp, a, slope, j, t0 + off, h, all, [&](int g) {
+                const f32x4 L = lds4f(stb + (2 * buf) * QT * 4 + 32 * g);
                 __builtin_amdgcn_sched_barrier(0);
+                return L;
             }, [&](int g, bool (&o)[4]) {
                 const int tq = t0 + 8 * g + 4 * h;
                 const int4 id = docs ? *reinterpret_cast<const int4*>(&s_id[buf][8 * g + 4 * h]) : make_int4(0, 0, 0, 0);
@@ -345,16 +353,22 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
             });
             __builtin_amdgcn_sched_barrier(0);
             const uint4 pp[2] = {pack8<T>(s, 0), pack8<T>(s, 1)}, ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
-            uint4 xd = ops.at_col(cd, 0, 0, 0), xq = ops.at_col(cq, 0, 0, 0);
+            unsigned xc = c, x8 = c8;
+            uint4 xq = Ops<D>::at_col(xc, x8, KEYS), xd = Ops<D>::at_col(xc, x8, KEYS + STAGE);
 #pragma unroll
-            for (int i = 0; i < 2 * DT; i++) {
+            for (int i = 0; i < 2 * DT; i++) {        // column block i / 2, 16 rows i % 2
                 const uint4 yd = xd, yq = xq;
                 if (i + 1 < 2 * DT) {
-                    xd = ops.at_col(cd, 0, (i + 1) % DT, (i + 1) / DT);
-                    xq = ops.at_col(cq, 0, (i + 1) % DT, (i + 1) / DT);
+                    const int at = KEYS + 16 * ((i + 1) & 1) * Tile<D>::ROWB;
+                    if (((i + 1) & 1) == 0) {
+                        xc = Ops<D>::block(c, (i + 1) / 2);
+                        x8 = Ops<D>::block(c8, (i + 1) / 2);
+                    }
+                    xq = Ops<D>::at_col(xc, x8, at);
+                    xd = Ops<D>::at_col(xc, x8, at + STAGE);
                 }
-                dv[i % DT] = mfma32<T>(yd, pp[i / DT], dv[i % DT]);
-                dk[i % DT] = mfma32<T>(yq, ds[i / DT], dk[i % DT]);
+                dv[i / 2] = mfma32<T>(yd, pp[i & 1], dv[i / 2]);
+                dk[i / 2] = mfma32<T>(yq, ds[i & 1], dk[i / 2]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -459,7 +473,7 @@ extern "C" int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
                             const float* slopes, const void* docs, const int32_t* prefix, const void* out, const void* res,
                             const float* lse, const void* dout, int64_t do_sb, int64_t do_sh, int64_t do_st, void* workspace, float* delta, void* dq,
                             void* dk, void* dv, void* stream) {
-    if (int r = slotattn_host::check(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, dtype, B, Tq, Tk, Hq, Hk, D, window, cap)) return r;
+    if (int r = slotattn_host::check(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, dtype, B, Tq, Tk, Hq, Hk, D, scale, window, cap)) return r;
     if (Tq > Tk) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: more queries than keys");
     if (!out || !res || !lse || !dout || !delta || !dq || !dk || !dv) return fail(SLOTSCAN_ERR_NULL, "slotattn_bwd: a required pointer is NULL");
     if (!al16(out) || !al16(res) || !al16(dout) || !al16(dq) || !al16(dk) || !al16(dv) || !al16(docs) || (do_sb | do_sh | do_st) % 8)

@@ -18,8 +18,6 @@ fp32; the probabilities and score gradients are rounded to the operands' type fo
 views whose rows are contiguous and 16-byte aligned (others are copied); results and gradients are token-major, seen as
 (B, H, T, D).  Gradients are bitwise reproducible.  No CPU path: a missing library raises.
 """
-import math
-
 import torch
 
 import slotscan_lib as L
@@ -42,10 +40,10 @@ def _check(q, k, v, scale, window, cap, slopes, prefix, what):
         raise NotImplementedError(f"{what} needs D in {_D} (got {q.shape[3]})")
     if window is not None and int(window) < 1:
         raise ValueError(f"{what}: window must be >= 1 or None (got {window})")
-    if cap is not None and not 0.0 < float(cap) < math.inf:
-        raise ValueError(f"{what}: cap must be a positive number or None (got {cap})")
-    if scale is not None and not math.isfinite(scale):
-        raise ValueError(f"{what}: scale must be finite (got {scale})")
+    if cap is not None and not 1e-30 <= float(cap) <= 1e30:
+        raise ValueError(f"{what}: cap must be in [1e-30, 1e30] or None (got {cap})")
+    if scale is not None and not 1e-30 <= abs(scale) <= 1e30:
+        raise ValueError(f"{what}: |scale| must be in [1e-30, 1e30] (got {scale})")
     if slopes is not None:
         if slopes.shape != (q.shape[1],) or slopes.dtype != torch.float32:
             raise ValueError(f"{what}: slopes must be fp32 ({q.shape[1]},) (got {slopes.dtype}, {tuple(slopes.shape)})")
