@@ -117,17 +117,40 @@ template <int D> struct Ops {
     }
 };
 
-// Direct global -> LDS loads of `rows` rows by one of NW waves: load(i) fills 1 KB.  Rows past `last` repeat it: what they
-// hold never counts (their scores are masked), and nothing outside the tensor is read.
+// One direct global -> LDS load as dma16's, the address a wave-uniform base plus a lane's 32-bit offset in bytes.
+__device__ __forceinline__ void dma16s(const void* base, unsigned off, unsigned lds) {
+    const uint64_t p = (uint64_t)base;               // the compiler does not always see that it is one value for the wave
+    base = (const void*)(((uint64_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)p));
+    // five wait states: readfirstlane writes the base from the vector unit, and the hazard before a memory instruction that
+    // reads it is not the compiler's inside of an asm block
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" : : "{m0}"(lds), "v"(off), "s"(base) : "memory");
+}
+// Direct loads of a tile of ROWS rows by wave w of NW.  Load i fills 1 KB: RPL rows from row RPL (NW i + w) on.  A lane's offset
+// is formed once (the swizzle repeats every 16 rows: VAR of them), the loads' bases are scalars: with an address per
+// lane and load the multiplications took 500 of a tile's 3,500 cycles.  Rows past the tensor's last repeat it: what they hold
+// never counts (their scores are masked), and nothing outside the tensor is read.
 template <int D, int ROWS, int NW> struct TileLoad {
-    static constexpr int N = ROWS * 2 * D / 1024 / NW;                // loads per wave
+    static constexpr int N = ROWS * 2 * D / 1024 / NW, RPL = 512 / D;  // loads per wave, rows per load
+    static constexpr int VAR = RPL * NW >= 16 ? 1 : 16 / (RPL * NW);
     static_assert(ROWS * 2 * D % (1024 * NW) == 0, "whole loads");
-    template <typename T>
-    static __device__ __forceinline__ void issue(const T* base, int64_t st, int r0, int last, unsigned lds, int w, int lane) {
+    unsigned off[VAR];
+    int64_t st;
+    int w, lane;
+    __device__ __forceinline__ TileLoad(int64_t stride, int wave, int l) : st(stride), w(wave), lane(l) {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int p = 64 * (N * w + i) + lane, r = p / Tile<D>::CH, c = Tile<D>::pos(r, p % Tile<D>::CH);
-            dma16(base + min(r0 + r, last) * st + 8 * c, lds + 1024u * (N * w + i));
+        for (int i = 0; i < VAR; i++) off[i] = (unsigned)(RPL * w + lane / Tile<D>::CH) * (unsigned)(2 * st) + 16 * chunk(i);
+    }
+    __device__ __forceinline__ int row(int i) const { return RPL * (NW * i + w) + lane / Tile<D>::CH; }
+    __device__ __forceinline__ int chunk(int i) const { return Tile<D>::pos(row(i), lane % Tile<D>::CH); }
+    // rows r0 .. of `base`, `last` the tensor's last row (>= r0)
+    template <typename T> __device__ __forceinline__ void issue(const T* base, int r0, int last, unsigned lds) const {
+        base += r0 * st;
+        if (last - r0 >= ROWS - 1) {
+#pragma unroll
+            for (int i = 0; i < N; i++) dma16s(base + i * (RPL * NW) * st, off[i % VAR], lds + 1024u * (NW * i + w));
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) dma16(base + min(row(i), last - r0) * st + 8 * chunk(i), lds + 1024u * (NW * i + w));
         }
     }
 };

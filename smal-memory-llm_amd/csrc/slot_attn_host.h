@@ -8,6 +8,7 @@
 #include "slotscan.h"
 
 #define SLOTATTN_MAX_T 0x3fffffffLL                  // positions and their differences stay in 31 bits
+#define SLOTATTN_MAX_ST (1LL << 25)                  // elements between tokens: 32 rows' offsets in bytes stay in 32 bits
 
 namespace slotattn_host {
 
@@ -24,6 +25,8 @@ inline int check(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const 
     if (!(std::fabs(scale) >= 1e-30f && std::fabs(scale) <= 1e30f)) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: |scale| must be in [1e-30, 1e30]");
     if (Tq > SLOTATTN_MAX_T || Tk > SLOTATTN_MAX_T || B > 0x7fffffffLL / Hq || Hq / Hk * Tq > SLOTATTN_MAX_T)
         return fail(SLOTSCAN_ERR_SHAPE, "slotattn: shape too large");
+    if (std::max(std::max(q_st, k_st), v_st) >= SLOTATTN_MAX_ST || std::min(std::min(q_st, k_st), v_st) < 0)
+        return fail(SLOTSCAN_ERR_SHAPE, "slotattn: token strides must be in [0, 2^25)");
     if (dtype != SLOTSCAN_BF16 && dtype != SLOTSCAN_F16) return fail(SLOTSCAN_ERR_DTYPE, "slotattn: dtype must be bf16 or fp16");
     if (!q || !k || !v) return fail(SLOTSCAN_ERR_NULL, "slotattn: a required pointer is NULL");
     if (!al16(q) || !al16(k) || !al16(v) || (q_sb | q_sh | q_st | k_sb | k_sh | k_st | v_sb | v_sh | v_st) % 8)

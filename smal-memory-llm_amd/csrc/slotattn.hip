@@ -18,6 +18,9 @@ using slothost::al16;
 #define FW 4                                         // waves per workgroup
 #define FT (64 * FW)
 #define FQ (32 * FW)                                 // query rows per workgroup
+// A row's sums keep their reference maximum until a score passes it by this much (base 2): probabilities then reach 2^8, far
+// from any type's end, and the sums are rescaled a few times a row instead of in most tiles.
+#define LAZY 8.f
 
 namespace {
 
@@ -80,9 +83,10 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
     Walk walk(mk, sw, sv, docs ? a.range + (int64_t)b * a.ntd : nullptr, lane);
     const float F = BIAS ? 1.f : f2;                  // from a row's values to base 2
     const unsigned lds = lds_addr(smem);
+    const Load lk(a.k_st, w, lane), lv(a.v_st, w, lane);
     auto load = [&](int jt, int buf) {
-        Load::issue(kb, a.k_st, jt * KT, mk.klen - 1, lds + (2 * buf) * STAGE, w, lane);
-        Load::issue(vb, a.v_st, jt * KT, mk.klen - 1, lds + (2 * buf + 1) * STAGE, w, lane);
+        lk.issue(kb, jt * KT, mk.klen - 1, lds + (2 * buf) * STAGE);
+        lv.issue(vb, jt * KT, mk.klen - 1, lds + (2 * buf + 1) * STAGE);
     };
     f32x16 o[DT];
 #pragma unroll
@@ -134,7 +138,7 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
             mx = half_max(mx) * F;
-            if (__any(mx > m)) {
+            if (__any(mx > m + LAZY)) {
                 const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_(m - mn);
                 m = mn;
                 l *= f;
@@ -205,9 +209,10 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
     const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
     const float f2 = fabsf(a.f), F = BIAS ? 1.f : f2;
     const unsigned lds = lds_addr(smem[w]);
+    const Load lk(a.k_st, 0, lane), lv(a.v_st, 0, lane);
     auto load = [&](int j0, int buf) {
-        Load::issue(kb, a.k_st, j0, klen - 1, lds + (2 * buf) * ST, 0, lane);
-        Load::issue(vb, a.v_st, j0, klen - 1, lds + (2 * buf + 1) * ST, 0, lane);
+        lk.issue(kb, j0, klen - 1, lds + (2 * buf) * ST);
+        lv.issue(vb, j0, klen - 1, lds + (2 * buf + 1) * ST);
     };
     auto seen = [&](int j0) {                         // the next of this wave's tiles that any row sees
         while (j0 < hi && !mk.some(s, j0, j0 + 31)) j0 += 32 * FW;
@@ -255,7 +260,7 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
 #pragma unroll
         for (int r = 1; r < 16; r++) mx = fmaxf(mx, x[r]);
         mx = half_max(mx) * F;
-        if (__any(mx > m)) {
+        if (__any(mx > m + LAZY)) {
             const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_(m - mn);
             m = mn;
             l *= f;

@@ -123,9 +123,10 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
     }
     Walk walk(mk, sw, sv, docs ? a.range + (int64_t)b * a.ntd : nullptr, lane);
     const unsigned lds = lds_addr(smem);
+    const Load lk(a.k_st, w, lane), lv(a.v_st, w, lane);
     auto load = [&](int jt, int buf) {
-        Load::issue(kb, a.k_st, jt * KT, mk.klen - 1, lds + (2 * buf) * STAGE, w, lane);
-        Load::issue(vb, a.v_st, jt * KT, mk.klen - 1, lds + (2 * buf + 1) * STAGE, w, lane);
+        lk.issue(kb, jt * KT, mk.klen - 1, lds + (2 * buf) * STAGE);
+        lv.issue(vb, jt * KT, mk.klen - 1, lds + (2 * buf + 1) * STAGE);
     };
     f32x16 acc[DT];
 #pragma unroll
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
     const int jw1 = min(jw + 31, a.Tk - 1);
     Mask mk{a.causal, a.W, a.prefix ? a.prefix[b] : 0, a.Tk};
     const unsigned lds = lds_addr(smem), ldq = lds + KEYS;
-    TileLoad<D, BQ, BW>::issue((const T*)a.k + b * a.k_sb + hk * a.k_sh, a.k_st, j0, a.Tk - 1, lds, w, lane);
+    TileLoad<D, BQ, BW>(a.k_st, w, lane).issue((const T*)a.k + b * a.k_sb + hk * a.k_sh, j0, a.Tk - 1, lds);
     uint4 vf[KK];
     {
         const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh + jc * a.v_st + 8 * h;
@@ -278,9 +279,10 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
         some = mine >> i & 1;
         all = full >> i & 1;
     };
+    const Load lq(a.q_st, w, lane), ld(a.do_st, w, lane);
     auto load = [&](int hq, int xt, int buf) {
-        Load::issue((const T*)a.q + b * a.q_sb + hq * a.q_sh, a.q_st, xt * QT, a.Tq - 1, ldq + (2 * buf) * STAGE, w, lane);
-        Load::issue((const T*)a.dout + b * a.do_sb + hq * a.do_sh, a.do_st, xt * QT, a.Tq - 1, ldq + (2 * buf + 1) * STAGE, w, lane);
+        lq.issue((const T*)a.q + b * a.q_sb + hq * a.q_sh, xt * QT, a.Tq - 1, ldq + (2 * buf) * STAGE);
+        ld.issue((const T*)a.dout + b * a.do_sb + hq * a.do_sh, xt * QT, a.Tq - 1, ldq + (2 * buf + 1) * STAGE);
     };
     auto stat = [&](int hq, int xt) {                 // lanes 0..31 of the first wave the log-sum-exp, 32..63 minus delta of a row
         const int t = xt * QT + (lane & 31);
@@ -478,6 +480,7 @@ extern "C" int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
     if (!out || !res || !lse || !dout || !delta || !dq || !dk || !dv) return fail(SLOTSCAN_ERR_NULL, "slotattn_bwd: a required pointer is NULL");
     if (!al16(out) || !al16(res) || !al16(dout) || !al16(dq) || !al16(dk) || !al16(dv) || !al16(docs) || (do_sb | do_sh | do_st) % 8)
         return fail(SLOTSCAN_ERR_ALIGN, "slotattn_bwd: rows of out, res, dout, dq, dk and dv, and docs, must be 16-byte aligned");
+    if (do_st < 0 || do_st >= SLOTATTN_MAX_ST) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: token strides must be in [0, 2^25)");
     if ((Tq + BQ - 1) / BQ * B * Hq > 0x7fffffffLL || (Tk + BQ - 1) / BQ * B * Hk > 0x7fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: shape too large");
     AttnArgs a = slotattn_host::args(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, B, Tq, Tk, Hq, Hk, scale, causal, window, cap,
                                      slopes, docs, prefix);
