@@ -30,6 +30,26 @@ template <> __device__ __forceinline__ f32x16 mfma32<bf16_t>(const uint4& a, con
 template <> __device__ __forceinline__ f32x16 mfma32<f16_t>(const uint4& a, const uint4& b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+// The same in place, with the registers' kind fixed: sums in accumulation registers, scores in vector registers.  Left to the
+// compiler, a kernel whose sums and scores pass 256 registers moved all of them from one kind to the other in every
+// iteration.  The compiler does not know these for matrix instructions: before anything else reads a result, mfma_settle().
+template <typename T> __device__ __forceinline__ void mfma_acc(f32x16& c, const uint4& a, const uint4& b);
+template <> __device__ __forceinline__ void mfma_acc<bf16_t>(f32x16& c, const uint4& a, const uint4& b) {
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(bf16x8, a)), "v"(__builtin_bit_cast(bf16x8, b)));
+}
+template <> __device__ __forceinline__ void mfma_acc<f16_t>(f32x16& c, const uint4& a, const uint4& b) {
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(f16x8, a)), "v"(__builtin_bit_cast(f16x8, b)));
+}
+template <typename T> __device__ __forceinline__ void mfma_vec(f32x16& c, const uint4& a, const uint4& b);
+template <> __device__ __forceinline__ void mfma_vec<bf16_t>(f32x16& c, const uint4& a, const uint4& b) {
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(__builtin_bit_cast(bf16x8, a)), "v"(__builtin_bit_cast(bf16x8, b)));
+}
+template <> __device__ __forceinline__ void mfma_vec<f16_t>(f32x16& c, const uint4& a, const uint4& b) {
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(__builtin_bit_cast(f16x8, a)), "v"(__builtin_bit_cast(f16x8, b)));
+}
+// the results of earlier mfma_acc / mfma_vec can be read, and registers written just before be read by later ones: 20 wait
+// states (a 16-pass matrix instruction needs 18)
+__device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 3" ::: "memory"); }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<bf16_t>(float lo, float hi) { return pack_bf16x2(lo, hi); }
 template <> __device__ __forceinline__ uint32_t pack2<f16_t>(float lo, float hi) {
@@ -125,6 +145,10 @@ __device__ __forceinline__ void dma16s(const void* base, unsigned off, unsigned 
     // reads it is not the compiler's inside of an asm block
     asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" : : "{m0}"(lds), "v"(off), "s"(base) : "memory");
 }
+// One direct global -> LDS load of 4 bytes per lane from g into LDS at lds + 4 * lane.
+__device__ __forceinline__ void dma4(const void* g, unsigned lds) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" : : "{m0}"(lds), "v"(g) : "memory");
+}
 // Direct loads of a tile of ROWS rows by wave w of NW.  Load i fills 1 KB: RPL rows from row RPL (NW i + w) on.  A lane's offset
 // is formed once (the swizzle repeats every 16 rows: VAR of them), the loads' bases are scalars: with an address per
 // lane and load the multiplications took 500 of a tile's 3,500 cycles.  Rows past the tensor's last repeat it: what they hold
@@ -213,20 +237,25 @@ __device__ __forceinline__ constexpr int key_of(int r, int h) { return 8 * (r >>
 // product where they are capped.  tanh(x) is x times a polynomial in x^2 while |x| <= 3/4 (relative error 7e-7; 6
 // instructions, none of them a transcendental one), which the scores of a whole tile usually are, else 1 - 2 / (1 + e^2x)
 // (off by a few 2^-24).
+__device__ __forceinline__ float tanh_poly(float s, const AttnArgs& a) {
+    const float y = s * s;
+    return s * fmaf(fmaf(fmaf(fmaf(a.t4, y, a.t3), y, a.t2), y, a.t1), y, a.t0);
+}
+__device__ __forceinline__ float tanh_any(float s, const AttnArgs& a) { return fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp2_(s * a.ct)), 1.f); }
+__device__ __forceinline__ bool poly_holds(const f32x16& s, const AttnArgs& a) {
+    float m = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; r++) m = fmaxf(m, fabsf(s[r]));
+    return __all(m <= a.lim);
+}
 template <bool CAP> __device__ __forceinline__ void scores(f32x16& s, const AttnArgs& a) {
     if constexpr (CAP) {
-        float m = 0.f;
+        if (poly_holds(s, a)) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) m = fmaxf(m, fabsf(s[r]));
-        if (__all(m <= a.lim)) {
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const float y = s[r] * s[r];
-                s[r] *= fmaf(fmaf(fmaf(fmaf(a.t4, y, a.t3), y, a.t2), y, a.t1), y, a.t0);
-            }
+            for (int r = 0; r < 16; r++) s[r] = tanh_poly(s[r], a);
         } else {
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp2_(s[r] * a.ct)), 1.f);
+            for (int r = 0; r < 16; r++) s[r] = tanh_any(s[r], a);
         }
     }
 }
