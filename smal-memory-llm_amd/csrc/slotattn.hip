@@ -51,11 +51,11 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the longest rows (the last tiles under causality) first
     const int heads = a.B * a.Hq;
-    const int qt = a.tiles - 1 - blockIdx.x / heads, bh = blockIdx.x % heads;
-    const int b = bh / a.Hq, hq = bh - b * a.Hq, hk = hq / a.R;
+    const int qt = uni((int)(a.tiles - 1 - blockIdx.x / heads)), bh = uni((int)(blockIdx.x % heads));
+    const int b = uni(bh / a.Hq), hq = bh - b * a.Hq, hk = uni(hq / a.R);
     const int len = length_of(a, b), t0 = qt * FQ, off = len - a.Tq;
     const int t = t0 + 32 * w + (lane & 31), tc = min(t, a.Tq - 1), p = tc + off;
-    Mask mk{a.causal, a.W, a.prefix ? a.prefix[b] : 0, min(len, a.Tk)};
+    Mask mk{a.causal, a.W, prefix_of(a, b), min(len, a.Tk)};
     // this wave's queries, in operand order
     uint4 qf[KK];
     {
@@ -107,13 +107,32 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
         if (some) {
             const unsigned bo = lds + (2 * buf) * STAGE, rk = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
             const int j0 = jt * KT;
+            // operands are read PRE products ahead: an LDS read takes as long as four or five of them
             f32x16 s[2] = {zero16(), zero16()};
+            uint4 kr[4][2];
+            auto rows = [&](int kk) {
+                const unsigned x = Ops<D>::k_step(rk, kk);
+                kr[kk & 3][0] = lds16(x);
+                kr[kk & 3][1] = lds16(x + 32 * Tile<D>::ROWB);
+            };
+            rows(0);
+            rows(1);
+            rows(2);
 #pragma unroll
             for (int kk = 0; kk < KK; kk++) {
-                const unsigned x = Ops<D>::k_step(rk, kk);
-#pragma unroll
-                for (int u = 0; u < 2; u++) s[u] = mfma32<T>(lds16(x + 32 * u * Tile<D>::ROWB), qf[kk], s[u]);
+                if (kk + 3 < KK) rows(kk + 3);
+                s[0] = mfma32<T>(kr[kk & 3][0], qf[kk], s[0]);
+                s[1] = mfma32<T>(kr[kk & 3][1], qf[kk], s[1]);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            uint4 vr[5];                              // operand i: column block i % DT of 16 keys i / DT
+            auto cols = [&](int i) {
+                vr[i % 5] = Ops<D>::at_col(Ops<D>::block(c, i % DT), Ops<D>::block(c8, i % DT), STAGE + 16 * (i / DT) * Tile<D>::ROWB);
+            };
+            cols(0);
+            cols(1);
+            cols(2);
+            cols(3);
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 scores<CAP>(s[u], a);
@@ -160,12 +179,10 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
                 pf[u][1] = pack8<T>(s[u], 1);
             }
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                const unsigned x = Ops<D>::block(c, dt), x8 = Ops<D>::block(c8, dt);
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int mm = 0; mm < 2; mm++) o[dt] = mfma32<T>(Ops<D>::at_col(x, x8, STAGE + (32 * u + 16 * mm) * Tile<D>::ROWB), pf[u][mm], o[dt]);
+            for (int i = 0; i < 4 * DT; i++) {
+                o[i % DT] = mfma32<T>(vr[i % 5], pf[i / DT >> 1][i / DT & 1], o[i % DT]);
+                if (i + 4 < 4 * DT) cols(i + 4);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -199,7 +216,7 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
     const int rows = a.Tq * a.R, r0 = rt * 32, row = min(r0 + (lane & 31), rows - 1);
     const int t = row / a.R, hq = hk * a.R + row - t * a.R;
     const int len = length_of(a, b), klen = min(len, a.Tk), off = len - a.Tq, p = t + off;
-    Mask mk{a.causal, a.W, a.prefix ? a.prefix[b] : 0, klen};
+    Mask mk{a.causal, a.W, prefix_of(a, b), klen};
     const Span s{r0 / a.R + off, (min(r0 + 32, rows) - 1) / a.R + off, 0, 0, true};
     // this workgroup's keys
     const int end = a.causal ? min(klen, max(s.p1 + 1, mk.prefix)) : klen;

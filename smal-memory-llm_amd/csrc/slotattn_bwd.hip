@@ -20,7 +20,7 @@ using slothost::al16;
 #define BW 4                                         // waves per workgroup
 #define BT (64 * BW)
 #define BQ (32 * BW)                                 // queries (attn_dq) or keys (attn_dkv) per workgroup
-#define QT 64                                        // query rows of a tile of attn_dkv
+#define QT 32                                        // query rows of a tile of attn_dkv
 
 namespace {
 
@@ -82,11 +82,11 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int heads = a.B * a.Hq;
-    const int qt = a.tiles - 1 - blockIdx.x / heads, bh = blockIdx.x % heads;
-    const int b = bh / a.Hq, hq = bh - b * a.Hq, hk = hq / a.R;
+    const int qt = uni((int)(a.tiles - 1 - blockIdx.x / heads)), bh = uni((int)(blockIdx.x % heads));
+    const int b = uni(bh / a.Hq), hq = bh - b * a.Hq, hk = uni(hq / a.R);
     const int t0 = qt * BQ, off = a.Tk - a.Tq;
     const int t = t0 + 32 * w + (lane & 31), tc = min(t, a.Tq - 1), p = tc + off;
-    Mask mk{a.causal, a.W, a.prefix ? a.prefix[b] : 0, a.Tk};
+    Mask mk{a.causal, a.W, prefix_of(a, b), a.Tk};
     uint4 qf[KK], df[KK];
     float delta = 0.f;
     {
@@ -143,18 +143,36 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
         if (jn >= 0) load(jn, buf ^ 1);
         if (some) {
             const unsigned bo = lds + (2 * buf) * STAGE, rk = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
+            // operands are read ahead of their products, the columns' before the probabilities, the second half's rows before the first
+            // half's last products
+            uint4 kr[4], vr[4], cr[5];
+            auto rows = [&](int u, int kk) {
+                const unsigned x = Ops<D>::k_step(rk, kk) + 32 * u * Tile<D>::ROWB;
+                kr[kk & 3] = lds16(x);
+                vr[kk & 3] = lds16(x + STAGE);
+            };
+            auto cols = [&](int u, int i) {           // operand i: column block i % DT of 16 keys i / DT
+                cr[i % 5] = Ops<D>::at_col(Ops<D>::block(c, i % DT), Ops<D>::block(c8, i % DT), (32 * u + 16 * (i / DT)) * Tile<D>::ROWB);
+            };
+            rows(0, 0);
+            rows(0, 1);
+            rows(0, 2);
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const int j0 = jt * KT + 32 * u, at = 32 * u * Tile<D>::ROWB;
+                const int j0 = jt * KT + 32 * u;
                 f32x16 s = zero16(), dp;
 #pragma unroll
                 for (int r = 0; r < 16; r++) dp[r] = -delta;
 #pragma unroll
                 for (int kk = 0; kk < KK; kk++) {
-                    const unsigned x = Ops<D>::k_step(rk, kk);
-                    s = mfma32<T>(lds16(x + at), qf[kk], s);
-                    dp = mfma32<T>(lds16(x + at + STAGE), df[kk], dp);
+                    if (kk + 3 < KK) rows(u, kk + 3);
+                    s = mfma32<T>(kr[kk & 3], qf[kk], s);
+                    dp = mfma32<T>(vr[kk & 3], df[kk], dp);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                cols(u, 0);
+                cols(u, 1);
+                cols(u, 2);
                 probs<CAP, BIAS>(s, dp, a, slope, p, j0, h, all, [&](int) { return f32x4{lse, lse, lse, lse}; }, [&](int g, bool (&o)[4]) {
                     const int j = j0 + 8 * g + 4 * h;
                     const int4 id = docs ? *reinterpret_cast<const int4*>(a.ids + idb + j) : make_int4(0, 0, 0, 0);
@@ -164,11 +182,13 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
                     o[3] = mk.sees(p, j + 3) && id.w == dq;
                 });
                 const uint4 ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    const unsigned x = Ops<D>::block(c, dt), x8 = Ops<D>::block(c8, dt);
-#pragma unroll
-                    for (int mm = 0; mm < 2; mm++) acc[dt] = mfma32<T>(Ops<D>::at_col(x, x8, at + 16 * mm * Tile<D>::ROWB), ds[mm], acc[dt]);
+                for (int i = 0; i < 2 * DT; i++) {
+                    acc[i % DT] = mfma32<T>(cr[i % 5], ds[i / DT], acc[i % DT]);
+                    if (i + 3 < 2 * DT) cols(u, i + 3);
+                    else if (u == 0) rows(1, i + 3 - 2 * DT);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
@@ -204,22 +224,13 @@ __device__ __forceinline__ bool meets(int x0, int x1, int nx, int u0, int u1) {
     return false;
 }
 
-// Each wave holds 32 keys and values as operands and their dK, dV as sums, one wave per SIMD.  A step interleaves three
-// blocks of 32 queries: the products of block m + 1, P and dS of block m, the sums of block m - 1, which do not depend on each
-// other, so the matrix and the vector units run at the same time within the wave.  The queries' and dout's tiles of 64 rows
-// come through a ring of RING, up to FLY of them in flight behind the one that is needed next.
-#define RING 4
-#define FLY 2
-
 template <typename T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(BT, 1) void attn_dkv(AttnArgs a) {
-    constexpr int KK = D / 16, DT = D / 32, STAGE = QT * 2 * D, SLOT = 2 * STAGE, RC = 16 / KK, HALF = 32 * 2 * D;
-    static_assert(KK == 2 * DT, "a step's chunks: one k step of the next tile's products, one operand of the last one's sums");
+__global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
+    constexpr int KK = D / 16, DT = D / 32, STAGE = QT * 2 * D, KEYS = BQ * 2 * D;
     typedef TileLoad<D, QT, BW> Load;
-    constexpr int PER = 2 * Load::N;
-    __shared__ __align__(1024) unsigned char smem[RING * SLOT];      // [slot][queries, dout]
-    __shared__ __align__(16) float s_st[RING][2][QT];                // log-sum-exp, minus delta
-    __shared__ __align__(16) int s_id[RING][QT];                     // the queries' documents
+    __shared__ __align__(1024) unsigned char smem[KEYS + 4 * STAGE]; // the keys; [buffer][queries, dout]
+    __shared__ __align__(16) float s_st[2][2][QT];                   // [buffer][log-sum-exp, delta]
+    __shared__ __align__(16) int s_id[2][2 * QT];                    // the queries' documents (twice)
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = a.B * a.Hk;
@@ -236,24 +247,21 @@ __global__ __launch_bounds__(BT, 1) void attn_dkv(AttnArgs a) {
         bh = blockIdx.x % kvh;
         part = blockIdx.x / (kvh * a.tiles);
     }
-    const int b = bh / a.Hk, hk = bh - b * a.Hk;
+    jt = uni(jt);
+    bh = uni(bh);
+    part = uni(part);
+    const int b = uni(bh / a.Hk), hk = bh - b * a.Hk;
     const int j0 = jt * BQ, j1 = min(j0 + BQ, a.Tk) - 1, off = a.Tk - a.Tq;
     const int jw = j0 + 32 * w, j = jw + (lane & 31), jc = min(j, a.Tk - 1);
     const int jw1 = min(jw + 31, a.Tk - 1);
-    Mask mk{a.causal, a.W, a.prefix ? a.prefix[b] : 0, a.Tk};
-    int x0, x1;
-    tile_rows(a, mk, j0, j1, off, x0, x1);
-    const int nx = (a.Tq + QT - 1) / QT, u0 = part * a.units, u1 = min(u0 + a.units, a.R * nx);
-    if (a.nsplit > 1 && !meets(x0, x1, nx, u0, u1)) return;           // the whole workgroup; attn_add knows it too
-    uint4 kf[KK], vf[KK];
+    Mask mk{a.causal, a.W, prefix_of(a, b), a.Tk};
+    const unsigned lds = lds_addr(smem), ldq = lds + KEYS;
+    TileLoad<D, BQ, BW>(a.k_st, w, lane).issue((const T*)a.k + b * a.k_sb + hk * a.k_sh, j0, a.Tk - 1, lds);
+    uint4 vf[KK];
     {
-        const T* k = (const T*)a.k + b * a.k_sb + hk * a.k_sh + jc * a.k_st + 8 * h;
         const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh + jc * a.v_st + 8 * h;
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++) {
-            kf[kk] = ld16(k + 16 * kk);
-            vf[kk] = ld16(v + 16 * kk);
-        }
+        for (int kk = 0; kk < KK; kk++) vf[kk] = ld16(v + 16 * kk);
     }
     const bool docs = a.ids != nullptr;
     const int64_t idb = (int64_t)b * a.ntd * KT;
@@ -265,16 +273,22 @@ __global__ __launch_bounds__(BT, 1) void attn_dkv(AttnArgs a) {
         dk_ = a.ids[idb + jc];
         if (dk_ < 0) dk_ = -2;
     }
+    int x0, x1;
+    tile_rows(a, mk, j0, j1, off, x0, x1);
+    const int nx = (a.Tq + QT - 1) / QT, u0 = part * a.units, u1 = min(u0 + a.units, a.R * nx);
+    if (a.nsplit > 1 && !meets(x0, x1, nx, u0, u1)) return;           // the whole workgroup; attn_add knows it too
     const int2* range = docs ? a.range + (int64_t)b * a.ntd : nullptr;
-    // the walk: heads of the group x query tiles, those of this workgroup's part.  A tile as one number: head of the group,
-    // tile, whether every pair of the wave's keys is visible; -1: none
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) dk[dt] = dv[dt] = zero16();
+    // the walk: heads of the group x query tiles, those of this workgroup's part
     int r = u0 / nx - 1, base = 0, xe = 0;
-    uint64_t act = 0, full = 0;
-    auto next = [&]() -> int2 {
+    uint64_t act = 0, mine = 0, full = 0;
+    auto next = [&](int& hq, int& xt, bool& some, bool& all) {
         while (!act) {
             base += 64;
             if (base >= xe) {
-                if (++r * nx >= u1) return make_int2(-1, 0);
+                if (++r * nx >= u1) { xt = -1; return; }
                 base = max(x0, u0 - r * nx);
                 xe = min(x1, u1 - r * nx);
             }
@@ -288,186 +302,93 @@ __global__ __launch_bounds__(BT, 1) void attn_dkv(AttnArgs a) {
                 s.one = range_one(ra) && range_one(rb) && ra.y == rb.y;
             }
             act = __ballot(in && mk.some(s, j0, j1) && (!range || (s.lo <= kw.hi && kw.lo <= s.hi)));
+            mine = __ballot(in && jw <= jw1 && mk.some(s, jw, jw1) && (!range || (s.lo <= kv.hi && kv.lo <= s.hi)));
             full = __ballot(in && x * QT + QT <= a.Tq && mk.all(s, jw, jw + 31) && (!range || (s.one && kv.one && s.lo == kv.lo)));
         }
         const int i = __builtin_ctzll(act);
         act &= act - 1;
-        return make_int2(2 * (base + i) + (int)(full >> i & 1), r);
+        xt = base + i;
+        hq = hk * a.R + r;
+        some = mine >> i & 1;
+        all = full >> i & 1;
     };
-    const unsigned lds = lds_addr(smem), lst = lds_addr(s_st), lid = lds_addr(s_id);
     const Load lq(a.q_st, w, lane), ld(a.do_st, w, lane);
-    const T* qb = (const T*)a.q + b * a.q_sb + (int64_t)hk * a.R * a.q_sh;
-    const T* db = (const T*)a.dout + b * a.do_sb + (int64_t)hk * a.R * a.do_sh;
-    const int64_t sb = ((int64_t)b * a.Hq + hk * a.R) * a.Tq;
-    auto load = [&](int2 c, int slot) {
-        const int t0 = (c.x >> 1) * QT;
-        lq.issue(qb + c.y * a.q_sh, t0, a.Tq - 1, lds + slot * SLOT);
-        ld.issue(db + c.y * a.do_sh, t0, a.Tq - 1, lds + slot * SLOT + STAGE);
-        const int t = min(t0 + lane, a.Tq - 1);                       // rows past the last repeat it and are masked
-        if (w < 2) dma4((w ? a.delta : a.lse) + sb + (int64_t)c.y * a.Tq + t, lst + (2 * slot + w) * QT * 4);
-        if (w == 2 && docs) dma4(a.ids + idb + t + off, lid + slot * QT * 4);
+    auto load = [&](int hq, int xt, int buf) {
+        lq.issue((const T*)a.q + b * a.q_sb + hq * a.q_sh, xt * QT, a.Tq - 1, ldq + (2 * buf) * STAGE);
+        ld.issue((const T*)a.dout + b * a.do_sb + hq * a.do_sh, xt * QT, a.Tq - 1, ldq + (2 * buf + 1) * STAGE);
+        const int t = min(xt * QT + (lane & 31), a.Tq - 1);           // rows past the last repeat it and are masked
+        if (w == 0) dma4((h ? a.delta : a.lse) + ((int64_t)b * a.Hq + hq) * a.Tq + t, lds_addr(s_st[buf]));
+        if (w == 1 && docs) dma4(a.ids + idb + t + off, lds_addr(s_id[buf]));
     };
-    f32x16 dk[DT], dv[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; dt++) dk[dt] = dv[dt] = zero16();
+    int hq, xt, hn = 0, xn;
+    bool some, all, some_n = false, all_n = false;
     const Ops<D> ops(lane);
-    uint4 pp[2], ds[2];                               // P and dS of the last tile as operands
-    // a block of 32 query rows: its tile's slot and which half.  Its products start from 0 and minus delta.
-    auto start = [&](f32x16& s, f32x16& dp, int blk) {
-        s = zero16();
+    const unsigned stb = lds_addr(s_st) + 16 * h;
+    next(hq, xt, some, all);
+    if (xt >= 0) load(hq, xt, 0);
+    for (int buf = 0; xt >= 0; buf ^= 1, hq = hn, xt = xn, some = some_n, all = all_n) {
+        next(hn, xn, some_n, all_n);
+        wait_vm<0>();
+        tile_barrier();
+        if (xn >= 0) load(hn, xn, buf ^ 1);
+        if (some) {
+            const unsigned bo = lds + (2 * buf) * STAGE, rq = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
+            const unsigned rk = lds + 32 * w * Tile<D>::ROWB + ops.row;
+            const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
+            f32x16 s = zero16(), dp;
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const f32x4 y = lds4f(lst + (blk >> 1) * 2 * QT * 4 + QT * 4 + (blk & 1) * 128 + 32 * g + 16 * h);
-            dp[4 * g] = y.x; dp[4 * g + 1] = y.y; dp[4 * g + 2] = y.z; dp[4 * g + 3] = y.w;
-        }
-        asm volatile("s_nop 3" : "+v"(s), "+v"(dp)); // between a register's write and a matrix instruction of an asm block
-    };
-    auto at = [&](int blk) { return lds + (blk >> 1) * SLOT + (blk & 1) * HALF; };
-    // P and dS of a block whose pairs are not all visible: 0 for the others
-    auto mask = [&](f32x16& s, f32x16& dp, int blk, int t0) {
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const int tq = t0 + 8 * g + 4 * h;
-            const int4 id = docs ? *reinterpret_cast<const int4*>(&s_id[blk >> 1][(blk & 1) * 32 + 8 * g + 4 * h]) : make_int4(0, 0, 0, 0);
-            const int ids[4] = {id.x, id.y, id.z, id.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const bool o = tq + i < a.Tq && mk.sees(tq + i + off, j) && ids[i] == dk_;
-                s[4 * g + i] = o ? s[4 * g + i] : 0.f;
-                dp[4 * g + i] = o ? dp[4 * g + i] : 0.f;
+            for (int g = 0; g < 4; g++) {             // minus delta
+                const f32x4 y = lds4f(stb + (2 * buf + 1) * QT * 4 + 32 * g);
+                dp[4 * g] = y.x; dp[4 * g + 1] = y.y; dp[4 * g + 2] = y.z; dp[4 * g + 3] = y.w;
             }
-        }
-    };
-    // One step: the products of block bn into (sN, dN), P and dS of block bc (rows from t0, head r of the group) from (s, dp), the
-    // sums of block bp.
-    auto step = [&](f32x16& s, f32x16& dp, f32x16& sN, f32x16& dN, int bp, int bc, int bn, int t0, int r, bool all) {
-        const unsigned rn = at(bn) + ops.row, cp = at(bp) + ops.col, cp8 = at(bp) + ops.col8;
-        float c0 = 1.f, c1 = 0.f, c2 = 0.f, c3 = 0.f, c4 = 0.f;
-        if constexpr (CAP) {
-            if (poly_holds(s, a)) {
-                c0 = a.t0; c1 = a.t1; c2 = a.t2; c3 = a.t3; c4 = a.t4;
-            } else {                                  // the polynomial below then is its argument
+            uint4 oq[3], ok[3], od[3];                // operands of three k steps: two of them on their way
+            auto rows = [&](int kk) {
+                const unsigned x = Ops<D>::k_step(rq, kk);
+                oq[kk % 3] = lds16(x + KEYS);
+                ok[kk % 3] = lds16(Ops<D>::k_step(rk, kk));
+                od[kk % 3] = lds16(x + KEYS + STAGE);
+            };
+            rows(0);
+            rows(1);
 #pragma unroll
-                for (int e = 0; e < 16; e++) s[e] = tanh_any(s[e], a);
+            for (int kk = 0; kk < KK; kk++) {
+                if (kk + 2 < KK) rows(kk + 2);
+                s = mfma32<T>(oq[kk % 3], ok[kk % 3], s);
+                dp = mfma32<T>(od[kk % 3], vf[kk], dp);
+                __builtin_amdgcn_sched_barrier(0);
             }
-        }
-        f32x4 L[4];
+            const int t0 = xt * QT;
+            probs<CAP, BIAS>(s, dp, a, slope, j, t0 + off, h, all, [&](int g) {
+                const f32x4 L = lds4f(stb + (2 * buf) * QT * 4 + 32 * g);
+                __builtin_amdgcn_sched_barrier(0);
+                return L;
+            }, [&](int g, bool (&o)[4]) {
+                const int tq = t0 + 8 * g + 4 * h;
+                const int4 id = docs ? *reinterpret_cast<const int4*>(&s_id[buf][8 * g + 4 * h]) : make_int4(0, 0, 0, 0);
+                o[0] = tq < a.Tq && mk.sees(tq + off, j) && id.x == dk_;
+                o[1] = tq + 1 < a.Tq && mk.sees(tq + 1 + off, j) && id.y == dk_;
+                o[2] = tq + 2 < a.Tq && mk.sees(tq + 2 + off, j) && id.z == dk_;
+                o[3] = tq + 3 < a.Tq && mk.sees(tq + 3 + off, j) && id.w == dk_;
+            });
+            __builtin_amdgcn_sched_barrier(0);
+            const uint4 pp[2] = {pack8<T>(s, 0), pack8<T>(s, 1)}, ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
+            uint4 xq[4], xd[4];                       // column block i / 2, 16 rows i % 2
+            auto cols = [&](int i) {
+                const unsigned xc = Ops<D>::block(c, i / 2), x8 = Ops<D>::block(c8, i / 2);
+                xq[i % 4] = Ops<D>::at_col(xc, x8, KEYS + 16 * (i & 1) * Tile<D>::ROWB);
+                xd[i % 4] = Ops<D>::at_col(xc, x8, KEYS + 16 * (i & 1) * Tile<D>::ROWB + STAGE);
+            };
+            cols(0);
+            cols(1);
+            cols(2);
 #pragma unroll
-        for (int g = 0; g < 4; g++) L[g] = lds4f(lst + (bc >> 1) * 2 * QT * 4 + (bc & 1) * 128 + 32 * g + 16 * h);
-        start(sN, dN, bn);
-        const float slope = BIAS ? a.slopes[hk * a.R + r] * LOG2E : 0.f, d = (float)(j - t0 - off - 4 * h);
-        uint4 oq = lds16(Ops<D>::k_step(rn, 0)), od = lds16(Ops<D>::k_step(rn, 0) + STAGE);
-        uint4 xq = Ops<D>::at_col(cp, cp8, 0), xd = Ops<D>::at_col(cp, cp8, STAGE);
-        float t;
-        // half of a score's way to P and dS: its tanh where it is capped, then the rest
-        auto half = [&](int x) {
-            const int e = x >> 1;
-            if ((x & 1) == 0) {
-                t = s[e];                             // capped: the tanh, whose slope is 1 - t^2
-                if constexpr (CAP) {
-                    const float y = t * t;
-                    t *= fmaf(fmaf(fmaf(fmaf(c4, y, c3), y, c2), y, c1), y, c0);
-                }
-                return;
-            }
-            float z = fmaf(t, a.f, -L[e >> 2][e & 3]);
-            if constexpr (BIAS) z = fmaf(-slope, fabsf(d - (float)key_of(e, 0)), z);
-            s[e] = exp2_(z);
-            dp[e] *= s[e];
-            if constexpr (CAP) dp[e] *= fmaf(-t, t, 1.f);
-        };
-#pragma unroll
-        for (int i = 0; i < KK; i++) {
-            const uint4 pq = oq, pd = od, yq = xq, yd = xd;
-            // one matrix instruction, then as much of the vector work as hides it
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                if (x == 0) mfma_vec<T>(sN, pq, kf[i]);
-                if (x == 1) mfma_acc<T>(dv[i / 2], yd, pp[i & 1]);
-                if (x == 2) mfma_vec<T>(dN, pd, vf[i]);
-                if (x == 3) mfma_acc<T>(dk[i / 2], yq, ds[i & 1]);
-                if (i + 1 < KK) {
-                    // column block (i + 1) / 2, rows 16 ((i + 1) % 2) ..
-                    const int ro = 16 * ((i + 1) & 1) * Tile<D>::ROWB;
-                    if (x == 0) oq = lds16(Ops<D>::k_step(rn, i + 1));
-                    if (x == 1) xd = Ops<D>::at_col(Ops<D>::block(cp, (i + 1) / 2), Ops<D>::block(cp8, (i + 1) / 2), ro + STAGE);
-                    if (x == 2) od = lds16(Ops<D>::k_step(rn, i + 1) + STAGE);
-                    if (x == 3) xq = Ops<D>::at_col(Ops<D>::block(cp, (i + 1) / 2), Ops<D>::block(cp8, (i + 1) / 2), ro);
-                }
-#pragma unroll
-                for (int y = 0; y < RC / 2; y++) half(2 * RC * i + x * (RC / 2) + y);
+            for (int i = 0; i < 2 * DT; i++) {
+                if (i + 3 < 2 * DT) cols(i + 3);
+                dv[i / 2] = mfma32<T>(xd[i % 4], pp[i & 1], dv[i / 2]);
+                dk[i / 2] = mfma32<T>(xq[i % 4], ds[i & 1], dk[i / 2]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (!all) mask(s, dp, bc, t0);
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-            pp[m] = pack8<T>(s, m);
-            ds[m] = pack8<T>(dp, m);
-        }
-        mfma_settle();
-    };
-    // tiles n (at hand), n + 1 .. n + 1 + FLY (loaded or on their way)
-    int2 tile[FLY + 2];
-    int fly = 0;                                      // tiles issued and not yet waited for
-#pragma unroll
-    for (int i = 0; i < FLY + 1; i++) {
-        tile[i] = i && tile[i - 1].x < 0 ? make_int2(-1, 0) : next();
-        if (tile[i].x >= 0) {
-            load(tile[i], i);
-            fly++;
-        }
-    }
-    // the oldest of the tiles in flight has landed: at most the younger ones' loads are outstanding
-    auto landed = [&]() {
-        fly--;
-        if (fly >= 2) wait_vm<2 * PER>();
-        else if (fly == 1) wait_vm<PER>();
-        else wait_vm<0>();
-        tile_barrier();
-    };
-    if (tile[0].x >= 0) {
-        f32x16 s, dp, sN, dN;
-        // the step before the first: nothing, from a slot of zeros (the ring reaches it only behind another barrier)
-        pp[0] = pp[1] = ds[0] = ds[1] = make_uint4(0u, 0u, 0u, 0u);
-        for (int i = tid; i < SLOT / 16; i += BT) *reinterpret_cast<uint4*>(smem + (RING - 1) * SLOT + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
-        landed();
-        start(s, dp, 0);
-#pragma unroll
-        for (int kk = 0; kk < KK; kk++) {
-            const unsigned x = Ops<D>::k_step(lds + ops.row, kk);
-            mfma_vec<T>(s, lds16(x), kf[kk]);
-            mfma_vec<T>(dp, lds16(x + STAGE), vf[kk]);
-        }
-        mfma_settle();
-        int n = 0;
-        for (bool more = true; more; n++) {
-            const int b0 = 2 * (n & (RING - 1)), t0 = (tile[0].x >> 1) * QT, rr = tile[0].y;
-            const bool all = tile[0].x & 1;
-            step(s, dp, sN, dN, (b0 - 1) & (2 * RING - 1), b0, b0 + 1, t0, rr, all);
-            more = tile[1].x >= 0;
-            if (more) {
-                landed();                             // tile n + 1 is there, tile n - 1 is read
-                tile[FLY + 1] = tile[FLY].x < 0 ? make_int2(-1, 0) : next();
-                if (tile[FLY + 1].x >= 0) {
-                    load(tile[FLY + 1], (n + FLY + 1) & (RING - 1));
-                    fly++;
-                }
-#pragma unroll
-                for (int i = 0; i <= FLY; i++) tile[i] = tile[i + 1];
-            }
-            step(sN, dN, s, dp, b0, b0 + 1, more ? (b0 + 2) & (2 * RING - 1) : b0, t0 + 32, rr, all);
-        }
-        // the sums of the last block
-        const int bl = 2 * ((n - 1) & (RING - 1)) + 1;
-        const unsigned cp = at(bl) + ops.col, cp8 = at(bl) + ops.col8;
-#pragma unroll
-        for (int i = 0; i < KK; i++) {
-            const unsigned xc = Ops<D>::block(cp, i / 2), x8 = Ops<D>::block(cp8, i / 2);
-            mfma_acc<T>(dv[i / 2], Ops<D>::at_col(xc, x8, 16 * (i & 1) * Tile<D>::ROWB + STAGE), pp[i & 1]);
-            mfma_acc<T>(dk[i / 2], Ops<D>::at_col(xc, x8, 16 * (i & 1) * Tile<D>::ROWB), ds[i & 1]);
-        }
-        mfma_settle();
     }
     const float f = a.scale;
     if (a.nsplit > 1) {
@@ -499,7 +420,7 @@ __global__ __launch_bounds__(256) void attn_add(AttnArgs a) {
     const int kvh = a.B * a.Hk, bh = blockIdx.x % kvh, q4 = blockIdx.x / kvh, jt = q4 / (BQ / 32);
     const int b = bh / a.Hk, hk = bh - b * a.Hk, off = a.Tk - a.Tq;
     const int j0 = jt * BQ, j1 = min(j0 + BQ, a.Tk) - 1;
-    const Mask mk{a.causal, a.W, a.prefix ? a.prefix[b] : 0, a.Tk};
+    const Mask mk{a.causal, a.W, prefix_of(a, b), a.Tk};
     int x0, x1;
     tile_rows(a, mk, j0, j1, off, x0, x1);
     const int nx = (a.Tq + QT - 1) / QT;
@@ -539,7 +460,7 @@ void launch_add(AttnArgs a, hipStream_t st) {
 }
 
 // Parts of the queries per key tile: where the key tiles alone do not give the card's 512 workgroup slots a round and a half, each
-// workgroup takes about 1 / 1024 of all (key tile, query tile) pairs, 8 at least (a part costs the write and the read of its sums).
+// workgroup takes about 1 / 1024 of all (key tile, 32-row query tile) pairs, 16 at least (a part costs the write and the read of its sums).
 void parts(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal, int64_t W, bool prefix, int& nsplit, int& units) {
     const int64_t R = Hq / Hk, nx = (Tq + QT - 1) / QT, tiles = (Tk + BQ - 1) / BQ * B * Hk;
     nsplit = 1;
@@ -547,7 +468,7 @@ void parts(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal
     if (tiles >= 768) return;
     int64_t rows = causal ? Tq - Tq / 2 : Tq;                         // of a head that see a key tile, about
     if (!prefix && W < Tk) rows = std::min(rows, (causal ? W : 2 * W) + BQ);
-    const int64_t c = std::max<int64_t>(8, tiles * R * ((rows + QT - 1) / QT) / 1024);
+    const int64_t c = std::max<int64_t>(16, tiles * R * ((rows + QT - 1) / QT) / 1024);
     nsplit = (int)((R * nx + c - 1) / c);
     units = (int)c;
 }
