@@ -198,11 +198,6 @@ template <int D, int ROWS, int NW> struct TileLoad {
 struct Span { int p0, p1, lo, hi; bool one; };       // positions; documents: range of ids, all of one document
 struct Mask {
     int causal, W, prefix, klen;
-    __device__ __forceinline__ bool band(int p, int j) const {
-        const int d = p - j;
-        return causal ? (d >= 0 && d < W) : (abs(d) < W);
-    }
-    __device__ __forceinline__ bool sees(int p, int j) const { return (band(p, j) || (j < prefix && p >= 0)) && j < klen; }
     __device__ __forceinline__ bool some(const Span& s, int j0, int j1) const {
         // the closest pair's distance, p - j
         const bool b = causal ? (j0 <= s.p1 && s.p0 - j1 < W) : (s.p0 - j1 < W && j0 - s.p1 < W);
@@ -227,7 +222,7 @@ struct AttnArgs {
     float lim, t0, t1, t2, t3, t4;                   // the polynomial's limit and coefficients, for products <q, k>
     void* out; void* res; float* lse;                // res: what rounding took from out, for the backward's delta
     // split rows
-    float* po; float* pm; int chunk, nsplit, tiles;
+    float* po; float* pm; int chunk, nsplit, tiles, groups;
     // backward
     const void* dout; int64_t do_sb, do_sh, do_st;
     float* delta; void* dq; void* dk; void* dv;
@@ -287,32 +282,76 @@ __device__ __forceinline__ void bias(f32x16& s, float f, float slope, int p, int
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ float uni(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 // Tokens of sequence b that count, and its length that positions are taken from (a length past the keys keeps its positions).
-__device__ __forceinline__ int length_of(const AttnArgs& a, int b) { return uni(a.lens ? min(max(a.lens[b], 0), 1 << 30) : a.Tk); }
+__device__ __forceinline__ int length_of(const AttnArgs& a, int b) { return uni(a.lens ? min(max(a.lens[b], 0), (1 << 30) - 1) : a.Tk); }
 __device__ __forceinline__ int prefix_of(const AttnArgs& a, int b) { return uni(a.prefix ? a.prefix[b] : 0); }
-
-// range of the ids of rows [i0, i0 + n) of sequence b (n <= 128), by one wave; one: all rows of one document
-__device__ __forceinline__ void rows_range(const int32_t* ids, int64_t base, int i0, int n, int lane, Span& s) {
-    int lo = 0x7fffffff, hi = -1;
-    bool pad = false;
-    for (int e = lane; e < n; e += 64) {
-        const int x = ids[base + i0 + e];
-        pad |= x < 0;
-        lo = min(lo, x < 0 ? 0x7fffffff : x);
-        hi = max(hi, x);
-    }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        lo = min(lo, __shfl_xor(lo, m));
-        hi = max(hi, __shfl_xor(hi, m));
-    }
-    s.lo = uni(lo);
-    s.hi = uni(hi);
-    s.one = s.lo == s.hi && __ballot(pad) == 0;
-}
 
 // range of the ids of a document tile as slotattn_docs leaves it: x = smallest (bit 31: some are padding), y = largest
 __device__ __forceinline__ int range_lo(int2 r) { return r.x & 0x7fffffff; }
 __device__ __forceinline__ bool range_one(int2 r) { return r.x == r.y; }
+// The ids of positions [s.p0, s.p1] (at most 128 of them), from the ranges of the 64-id tiles that they touch: wider than
+// they are where they fill no whole tile.
+__device__ __forceinline__ void doc_span(const int2* range, Span& s) {
+    const int x0 = uni(s.p0 / KT), x1 = uni(max(s.p0, s.p1) / KT);
+    int lo = 0x7fffffff, hi = -2;
+    bool one = true;
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        const int2 r = range[min(x0 + i, x1)];
+        lo = min(lo, range_lo(r));
+        hi = max(hi, r.y);
+        one = one && range_one(r);
+    }
+    s.lo = uni(lo);
+    s.hi = uni(hi);
+    s.one = uni((int)(one && lo == hi));
+}
+// What one lane sees of the other side's rows: those with i - first <= count (unsigned), first + count inclusive; and, for a
+// query that a prefix reaches behind the band, those below `below`.
+struct Sees {
+    unsigned first, count, below;
+    // a query at position p (negative: sees nothing), against keys
+    static __device__ __forceinline__ Sees query(const Mask& m, int p) {
+        int lo = p - m.W + 1, hi = min(m.causal ? p : p + m.W - 1, m.klen - 1);
+        int b = p >= 0 ? min(m.prefix, m.klen) : 0;
+        if (lo <= b && b > 0) {                       // one interval
+            lo = 0;
+            hi = max(hi, b - 1);
+            b = 0;
+        }
+        lo = max(lo, 0);
+        if (hi < lo || p < 0) { lo = 0x7fffffff; hi = lo; }
+        return {(unsigned)lo, (unsigned)(hi - lo), (unsigned)max(b, 0)};
+    }
+    // a key at position j, against queries of positions up to `last`
+    static __device__ __forceinline__ Sees key(const Mask& m, int j, int last) {
+        int lo = m.causal ? j : j - m.W + 1, hi = min(j + m.W - 1, last);
+        if (j < m.prefix) { lo = 0; hi = last; }
+        lo = max(lo, 0);
+        if (hi < lo) { lo = 0x7fffffff; hi = lo; }
+        return {(unsigned)lo, (unsigned)(hi - lo), 0u};
+    }
+};
+// The 16 rows of a result tile from row j0 on (rows j0 + key_of(r, h)) that a lane sees, as bits: by its interval, by the prefix
+// where a lane's does not join it (pre), by the document ids (at ids + 8 g + 4 h; null: none)
+__device__ __forceinline__ uint32_t seen16(const Sees& v, int j0, int h, bool pre, const int* ids, int id) {
+    const unsigned x = (unsigned)(j0 + 4 * h) - v.first, y = (unsigned)(j0 + 4 * h);
+    uint32_t m = 0;
+#pragma unroll
+    for (int r = 0; r < 16; r++) m |= (x + key_of(r, 0) <= v.count ? 1u : 0u) << r;
+    if (pre) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) m |= (y + key_of(r, 0) < v.below ? 1u : 0u) << r;
+    }
+    if (ids) {
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int4 d = *reinterpret_cast<const int4*>(ids + 8 * g + 4 * h);
+            m &= ~(((d.x != id ? 1u : 0u) | (d.y != id ? 2u : 0u) | (d.z != id ? 4u : 0u) | (d.w != id ? 8u : 0u)) << (4 * g));
+        }
+    }
+    return m;
+}
+__device__ __forceinline__ bool bit(uint32_t m, int r) { return (m >> r & 1) != 0; }
 
 // The walk over the 64-key tiles that a workgroup's queries see.  Each lane tests one of 64 tiles at a time; what a
 // workgroup visits, a wave computes and a wave computes without masks are three ballots.

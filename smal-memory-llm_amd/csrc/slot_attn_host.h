@@ -45,7 +45,7 @@ inline slotattn::AttnArgs args(const void* q, int64_t q_sb, int64_t q_sh, int64_
     a.v_sb = v_sb; a.v_sh = v_sh; a.v_st = v_st;
     a.B = (int)B; a.Tq = (int)Tq; a.Tk = (int)Tk; a.Hq = (int)Hq; a.Hk = (int)Hk; a.R = (int)(Hq / Hk);
     a.causal = causal != 0;
-    a.W = (int)window;
+    a.W = (int)std::min<int64_t>(window, 1 << 30);      // any distance is less
     a.slopes = slopes;
     a.ntd = (int)((Tk + KT - 1) / KT);
     a.ids = (const int32_t*)docs;

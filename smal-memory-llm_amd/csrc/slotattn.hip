@@ -42,13 +42,16 @@ __global__ __launch_bounds__(64) void attn_docs(const int32_t* ids, int T, int n
 }
 
 // ------------------------------------------------------------------------------------------- many rows
-template <typename T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
+// GR groups of 4 waves share a workgroup's rows, each taking every GR-th of their key tiles; their sums meet in LDS.  With two
+// groups the longest rows take half the steps: under causality 128 rows of 8,192 tokens see up to 128 tiles, 49 on average
+// would fill the card's time.
+template <typename T, int D, bool CAP, bool BIAS, int GR>
+__global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
     constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
     typedef TileLoad<D, KT, FW> Load;
-    __shared__ __align__(1024) unsigned char smem[2][2][STAGE];      // [buffer][keys, values]
-    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __shared__ __align__(1024) unsigned char smem[GR][2][2][STAGE];  // [group][buffer][keys, values]
+    const int tid = threadIdx.x & (FT - 1), lane = tid & 63, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), grp = GR == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / FT);
     // the longest rows (the last tiles under causality) first
     const int heads = a.B * a.Hq;
     const int qt = uni((int)(a.tiles - 1 - blockIdx.x / heads)), bh = uni((int)(blockIdx.x % heads));
@@ -75,14 +78,16 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
     Span sw{t0 + off, min(t0 + FQ, a.Tq) - 1 + off, 0, 0, true}, sv{t0 + 32 * w + off, min(t0 + 32 * w + 32, a.Tq) - 1 + off, 0, 0, true};
     int dq = 0;
     if (docs) {
-        rows_range(a.ids, idb, sw.p0, sw.p1 - sw.p0 + 1, lane, sw);
-        rows_range(a.ids, idb, min(sv.p0, sw.p1), max(sv.p1 - sv.p0 + 1, 1), lane, sv);
+        const int2* range = a.range + (int64_t)b * a.ntd;
+        doc_span(range, sw);
+        if (sv.p0 <= sv.p1) doc_span(range, sv);
         dq = a.ids[idb + p];
         if (dq < 0) dq = -2;
     }
+    const Sees see = Sees::query(mk, p);
     Walk walk(mk, sw, sv, docs ? a.range + (int64_t)b * a.ntd : nullptr, lane);
     const float F = BIAS ? 1.f : f2;                  // from a row's values to base 2
-    const unsigned lds = lds_addr(smem);
+    const unsigned lds = lds_addr(smem[grp]);
     const Load lk(a.k_st, w, lane), lv(a.v_st, w, lane);
     auto load = [&](int jt, int buf) {
         lk.issue(kb, jt * KT, mk.klen - 1, lds + (2 * buf) * STAGE);
@@ -92,15 +97,28 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) o[dt] = zero16();
     float m = -INFINITY, l = 0.f;
+    // this group's next tile, and whether any group has one
+    auto next = [&](int& jt, bool& some, bool& all) -> bool {
+        walk.next(jt, some, all);
+        const bool any = jt >= 0;
+        if constexpr (GR == 2) {
+            int j1 = -1;
+            bool s1 = false, a1 = false;
+            if (any) walk.next(j1, s1, a1);
+            if (grp) { jt = j1; some = s1; all = a1; }
+        }
+        some = some && jt >= 0;
+        return any;
+    };
     int jt, jn;
-    bool some, all, some_n = false, all_n = false;
+    bool some = false, all = false, some_n = false, all_n = false;
     const Ops<D> ops(lane);
-    walk.next(jt, some, all);
+    bool go = next(jt, some, all), more;
     if (jt >= 0) load(jt, 0);
     // one barrier a tile: behind it the tile is there for every wave and the other buffer is read, so the next one's loads
     // run during this one's products
-    for (int buf = 0; jt >= 0; buf ^= 1, jt = jn, some = some_n, all = all_n) {
-        walk.next(jn, some_n, all_n);
+    for (int buf = 0; go; buf ^= 1, jt = jn, some = some_n, all = all_n, go = more) {
+        more = next(jn, some_n, all_n);
         wait_vm<0>();
         tile_barrier();
         if (jn >= 0) load(jn, buf ^ 1);
@@ -140,16 +158,11 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
             }
             if (!all) {
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+                for (int u = 0; u < 2; u++) {
+                    const uint32_t ok = seen16(see, j0 + 32 * u, h, j0 < mk.prefix, docs ? a.ids + idb + j0 + 32 * u : nullptr, dq);
 #pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        const int j = j0 + 32 * u + 8 * g + 4 * h;
-                        const int4 id = docs ? *reinterpret_cast<const int4*>(a.ids + idb + j) : make_int4(0, 0, 0, 0);
-                        s[u][4 * g] = mk.sees(p, j) && id.x == dq ? s[u][4 * g] : -INFINITY;
-                        s[u][4 * g + 1] = mk.sees(p, j + 1) && id.y == dq ? s[u][4 * g + 1] : -INFINITY;
-                        s[u][4 * g + 2] = mk.sees(p, j + 2) && id.z == dq ? s[u][4 * g + 2] : -INFINITY;
-                        s[u][4 * g + 3] = mk.sees(p, j + 3) && id.w == dq ? s[u][4 * g + 3] : -INFINITY;
-                    }
+                    for (int r = 0; r < 16; r++) s[u][r] = bit(ok, r) ? s[u][r] : -INFINITY;
+                }
             }
             float mx = s[0][0];
 #pragma unroll
@@ -187,6 +200,36 @@ __global__ __launch_bounds__(FT, 2) void attn_fwd(AttnArgs a) {
         }
     }
     l = half_sum(l);
+    if constexpr (GR == 2) {
+        float4* so = reinterpret_cast<float4*>(smem);                 // [4 DT][thread], then the rows' maxima and sums
+        float* sm = reinterpret_cast<float*>(so + 4 * DT * FT);
+        static_assert((16 * DT + 2) * FT * 4 <= (int)sizeof(smem), "a group's sums fit");
+        __syncthreads();
+        if (grp) {
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) so[(4 * dt + g) * FT + tid] = make_float4(o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]);
+            sm[tid] = m;
+            sm[FT + tid] = l;
+        }
+        __syncthreads();
+        if (grp) return;
+        const float m1 = sm[tid], l1 = sm[FT + tid], M = fmaxf(m, m1), Mu = M == -INFINITY ? 0.f : M;
+        const float f0 = exp2_(m - Mu), f1 = exp2_(m1 - Mu);
+        m = M;
+        l = l * f0 + l1 * f1;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const float4 x = so[(4 * dt + g) * FT + tid];
+                o[dt][4 * g] = fmaf(x.x, f1, o[dt][4 * g] * f0);
+                o[dt][4 * g + 1] = fmaf(x.y, f1, o[dt][4 * g + 1] * f0);
+                o[dt][4 * g + 2] = fmaf(x.z, f1, o[dt][4 * g + 2] * f0);
+                o[dt][4 * g + 3] = fmaf(x.w, f1, o[dt][4 * g + 3] * f0);
+            }
+    }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     if (t < a.Tq) {
         const int64_t at = (((int64_t)b * a.Tq + t) * a.Hq + hq) * D + 4 * h;
@@ -236,6 +279,7 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
         return j0;
     };
     const Ops<D> ops(lane);
+    const Sees see = Sees::query(mk, p);
     int j0 = seen(lo + 32 * w);
     if (j0 < hi) load(j0, 0);
     uint4 qf[KK];
@@ -267,11 +311,9 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
         scores<CAP>(x, a);
         if constexpr (BIAS) bias(x, f2, slope, p, j0, h);
         if (j0 + 32 > hi || !mk.all(s, j0, j0 + 31)) {
+            const uint32_t ok = seen16(see, j0, h, j0 < mk.prefix, nullptr, 0);
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int j = j0 + key_of(r, h);
-                x[r] = j < hi && mk.sees(p, j) ? x[r] : -INFINITY;
-            }
+            for (int r = 0; r < 16; r++) x[r] = j0 + key_of(r, h) < hi && bit(ok, r) ? x[r] : -INFINITY;
         }
         float mx = x[0];
 #pragma unroll
@@ -418,7 +460,8 @@ __global__ __launch_bounds__(FT) void attn_join(AttnArgs a) {
 template <typename T, int D, bool CAP, bool BIAS>
 void launch_one(const AttnArgs& a, bool split, hipStream_t st) {
     if (split) slothost::launch(attn_split<T, D, CAP, BIAS>, dim3((unsigned)(a.nsplit * a.tiles), (unsigned)a.Hk, (unsigned)a.B), dim3(FT), 0, st, a);
-    else slothost::launch(attn_fwd<T, D, CAP, BIAS>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(FT), 0, st, a);
+    else if (a.groups == 2) slothost::launch(attn_fwd<T, D, CAP, BIAS, 2>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(2 * FT), 0, st, a);
+    else slothost::launch(attn_fwd<T, D, CAP, BIAS, 1>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(FT), 0, st, a);
 }
 template <typename T, int D>
 void launch_fwd(const AttnArgs& a, bool cap, bool split, hipStream_t st) {
@@ -502,6 +545,7 @@ extern "C" int slotattn_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
     a.tiles = p.split ? p.rtiles : (int)((Tq + FQ - 1) / FQ);
     a.chunk = p.chunk;
     a.nsplit = p.nsplit;
+    a.groups = getenv("GR") ? atoi(getenv("GR")) : 1;
     a.po = (float*)workspace;
     a.pm = a.po ? a.po + B * Tq * Hq * p.nsplit * D : nullptr;
     const bool split = p.split;

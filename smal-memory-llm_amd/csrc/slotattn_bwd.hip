@@ -40,7 +40,7 @@ __device__ __forceinline__ void dot8(const uint4& x, const uint4& y, float& s, f
 
 // P and dS of one 32 x 32 tile, in the place of its products s = <q, k> and dp = <dO, v> - delta; ld(g): the log-sum-exp of
 // registers 4 g .. 4 g + 3, so that no more of them are held than a few scores need.  dist: the lane's own position; d0: the
-// position of register row 0.  ok(g, o): which of those four are visible (only asked if !all).
+// position of register row 0.  ok(): which rows are visible, as bits (only asked if !all).
 template <bool CAP, bool BIAS, class LD, class OK>
 __device__ __forceinline__ void probs(f32x16& s, f32x16& dp, const AttnArgs& a, float slope, int dist, int d0, int h, bool all, LD ld, OK ok) {
     scores<CAP>(s, a);
@@ -60,27 +60,24 @@ __device__ __forceinline__ void probs(f32x16& s, f32x16& dp, const AttnArgs& a, 
         }
     }
     if (!all) {
+        const uint32_t m = ok();
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            bool o[4];
-            ok(g, o);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                s[4 * g + i] = o[i] ? s[4 * g + i] : 0.f;
-                dp[4 * g + i] = o[i] ? dp[4 * g + i] : 0.f;
-            }
+        for (int r = 0; r < 16; r++) {
+            s[r] = bit(m, r) ? s[r] : 0.f;
+            dp[r] = bit(m, r) ? dp[r] : 0.f;
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------- dQ
-template <typename T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
+// (GR groups of waves as in the forward)
+template <typename T, int D, bool CAP, bool BIAS, int GR>
+__global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
     constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
     typedef TileLoad<D, KT, BW> Load;
-    __shared__ __align__(1024) unsigned char smem[2][2][STAGE];
-    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __shared__ __align__(1024) unsigned char smem[GR][2][2][STAGE];
+    const int tid = threadIdx.x & (BT - 1), lane = tid & 63, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), grp = GR == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / BT);
     const int heads = a.B * a.Hq;
     const int qt = uni((int)(a.tiles - 1 - blockIdx.x / heads)), bh = uni((int)(blockIdx.x % heads));
     const int b = uni(bh / a.Hq), hq = bh - b * a.Hq, hk = uni(hq / a.R);
@@ -107,7 +104,7 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
     delta = half_sum(delta);
     const int64_t row = (int64_t)bh * a.Tq + tc;
     const float lse = a.lse[row];
-    if (t < a.Tq && h == 0) a.delta[row] = -delta;  // as attn_dkv starts its products
+    if (t < a.Tq && h == 0 && grp == 0) a.delta[row] = -delta;  // as attn_dkv starts its products
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
     const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
@@ -116,13 +113,15 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
     Span sw{t0 + off, min(t0 + BQ, a.Tq) - 1 + off, 0, 0, true}, sv{t0 + 32 * w + off, min(t0 + 32 * w + 32, a.Tq) - 1 + off, 0, 0, true};
     int dq = 0;
     if (docs) {
-        rows_range(a.ids, idb, sw.p0, sw.p1 - sw.p0 + 1, lane, sw);
-        rows_range(a.ids, idb, min(sv.p0, sw.p1), max(sv.p1 - sv.p0 + 1, 1), lane, sv);
+        const int2* range = a.range + (int64_t)b * a.ntd;
+        doc_span(range, sw);
+        if (sv.p0 <= sv.p1) doc_span(range, sv);
         dq = a.ids[idb + p];
         if (dq < 0) dq = -2;
     }
+    const Sees see = Sees::query(mk, p);
     Walk walk(mk, sw, sv, docs ? a.range + (int64_t)b * a.ntd : nullptr, lane);
-    const unsigned lds = lds_addr(smem);
+    const unsigned lds = lds_addr(smem[grp]);
     const Load lk(a.k_st, w, lane), lv(a.v_st, w, lane);
     auto load = [&](int jt, int buf) {
         lk.issue(kb, jt * KT, mk.klen - 1, lds + (2 * buf) * STAGE);
@@ -131,13 +130,25 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
     f32x16 acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) acc[dt] = zero16();
+    auto next = [&](int& jt, bool& some, bool& all) -> bool {
+        walk.next(jt, some, all);
+        const bool any = jt >= 0;
+        if constexpr (GR == 2) {
+            int j1 = -1;
+            bool s1 = false, a1 = false;
+            if (any) walk.next(j1, s1, a1);
+            if (grp) { jt = j1; some = s1; all = a1; }
+        }
+        some = some && jt >= 0;
+        return any;
+    };
     int jt, jn;
-    bool some, all, some_n = false, all_n = false;
+    bool some = false, all = false, some_n = false, all_n = false;
     const Ops<D> ops(lane);
-    walk.next(jt, some, all);
+    bool go = next(jt, some, all), more;
     if (jt >= 0) load(jt, 0);
-    for (int buf = 0; jt >= 0; buf ^= 1, jt = jn, some = some_n, all = all_n) {
-        walk.next(jn, some_n, all_n);
+    for (int buf = 0; go; buf ^= 1, jt = jn, some = some_n, all = all_n, go = more) {
+        more = next(jn, some_n, all_n);
         wait_vm<0>();
         tile_barrier();
         if (jn >= 0) load(jn, buf ^ 1);
@@ -173,14 +184,7 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
                 cols(u, 0);
                 cols(u, 1);
                 cols(u, 2);
-                probs<CAP, BIAS>(s, dp, a, slope, p, j0, h, all, [&](int) { return f32x4{lse, lse, lse, lse}; }, [&](int g, bool (&o)[4]) {
-                    const int j = j0 + 8 * g + 4 * h;
-                    const int4 id = docs ? *reinterpret_cast<const int4*>(a.ids + idb + j) : make_int4(0, 0, 0, 0);
-                    o[0] = mk.sees(p, j) && id.x == dq;
-                    o[1] = mk.sees(p, j + 1) && id.y == dq;
-                    o[2] = mk.sees(p, j + 2) && id.z == dq;
-                    o[3] = mk.sees(p, j + 3) && id.w == dq;
-                });
+                probs<CAP, BIAS>(s, dp, a, slope, p, j0, h, all, [&](int) { return f32x4{lse, lse, lse, lse}; }, [&]() { return seen16(see, j0, h, j0 < mk.prefix, docs ? a.ids + idb + j0 : nullptr, dq); });
                 const uint4 ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -192,6 +196,28 @@ __global__ __launch_bounds__(BT, 2) void attn_dq(AttnArgs a) {
                 }
             }
         }
+    }
+    if constexpr (GR == 2) {
+        float4* so = reinterpret_cast<float4*>(smem);                 // [4 DT][thread]
+        __syncthreads();
+        if (grp) {
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) so[(4 * dt + g) * BT + tid] = make_float4(acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
+        }
+        __syncthreads();
+        if (grp) return;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const float4 x = so[(4 * dt + g) * BT + tid];
+                acc[dt][4 * g] += x.x;
+                acc[dt][4 * g + 1] += x.y;
+                acc[dt][4 * g + 2] += x.z;
+                acc[dt][4 * g + 3] += x.w;
+            }
     }
     if (t < a.Tq) {
         T* out = (T*)a.dq + (((int64_t)b * a.Tq + t) * a.Hq + hq) * D;
@@ -268,8 +294,9 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
     Span kw{j0, j1, 0, 0, true}, kv{jw, jw1, 0, 0, true};             // document ranges of the keys
     int dk_ = 0;
     if (docs) {
-        rows_range(a.ids, idb, j0, j1 - j0 + 1, lane, kw);
-        rows_range(a.ids, idb, min(jw, j1), max(jw1 - jw + 1, 1), lane, kv);
+        const int2* range = a.range + (int64_t)b * a.ntd;
+        doc_span(range, kw);
+        if (jw <= jw1) doc_span(range, kv);
         dk_ = a.ids[idb + jc];
         if (dk_ < 0) dk_ = -2;
     }
@@ -278,6 +305,7 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
     const int nx = (a.Tq + QT - 1) / QT, u0 = part * a.units, u1 = min(u0 + a.units, a.R * nx);
     if (a.nsplit > 1 && !meets(x0, x1, nx, u0, u1)) return;           // the whole workgroup; attn_add knows it too
     const int2* range = docs ? a.range + (int64_t)b * a.ntd : nullptr;
+    const Sees see = Sees::key(mk, j, a.Tk - 1);
     f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) dk[dt] = dv[dt] = zero16();
@@ -362,14 +390,7 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
                 const f32x4 L = lds4f(stb + (2 * buf) * QT * 4 + 32 * g);
                 __builtin_amdgcn_sched_barrier(0);
                 return L;
-            }, [&](int g, bool (&o)[4]) {
-                const int tq = t0 + 8 * g + 4 * h;
-                const int4 id = docs ? *reinterpret_cast<const int4*>(&s_id[buf][8 * g + 4 * h]) : make_int4(0, 0, 0, 0);
-                o[0] = tq < a.Tq && mk.sees(tq + off, j) && id.x == dk_;
-                o[1] = tq + 1 < a.Tq && mk.sees(tq + 1 + off, j) && id.y == dk_;
-                o[2] = tq + 2 < a.Tq && mk.sees(tq + 2 + off, j) && id.z == dk_;
-                o[3] = tq + 3 < a.Tq && mk.sees(tq + 3 + off, j) && id.w == dk_;
-            });
+            }, [&]() { return seen16(see, t0 + off, h, false, docs ? s_id[buf] : nullptr, dk_); });
             __builtin_amdgcn_sched_barrier(0);
             const uint4 pp[2] = {pack8<T>(s, 0), pack8<T>(s, 1)}, ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
             uint4 xq[4], xd[4];                       // column block i / 2, 16 rows i % 2
@@ -444,7 +465,8 @@ void launch_one(AttnArgs a, bool keys, hipStream_t st) {
         slothost::launch(attn_dkv<T, D, CAP, BIAS>, dim3((unsigned)((int64_t)a.tiles * a.nsplit * a.B * a.Hk)), dim3(BT), 0, st, a);
     } else {
         a.tiles = (a.Tq + BQ - 1) / BQ;
-        slothost::launch(attn_dq<T, D, CAP, BIAS>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(BT), 0, st, a);
+        if (a.groups == 2) slothost::launch(attn_dq<T, D, CAP, BIAS, 2>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(2 * BT), 0, st, a);
+        else slothost::launch(attn_dq<T, D, CAP, BIAS, 1>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(BT), 0, st, a);
     }
 }
 template <typename T, int D>
@@ -459,18 +481,17 @@ void launch_add(AttnArgs a, hipStream_t st) {
     slothost::launch(attn_add<T, D>, dim3((unsigned)((int64_t)a.tiles * (BQ / 32) * a.B * a.Hk)), dim3(256), 0, st, a);
 }
 
-// Parts of the queries per key tile: where the key tiles alone do not give the card's 512 workgroup slots a round and a half, each
-// workgroup takes about 1 / 1024 of all (key tile, 32-row query tile) pairs, 16 at least (a part costs the write and the read of its sums).
+// Parts of the queries per key tile.  A part costs the write and the read of its sums, about as long as 20 query tiles take, so keys are
+// split only where the key tiles alone do not fill the card's 512 workgroup slots, and into parts of 48 query tiles at least.
 void parts(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal, int64_t W, bool prefix, int& nsplit, int& units) {
     const int64_t R = Hq / Hk, nx = (Tq + QT - 1) / QT, tiles = (Tk + BQ - 1) / BQ * B * Hk;
-    nsplit = 1;
-    units = (int)(R * nx);
-    if (tiles >= 768) return;
     int64_t rows = causal ? Tq - Tq / 2 : Tq;                         // of a head that see a key tile, about
     if (!prefix && W < Tk) rows = std::min(rows, (causal ? W : 2 * W) + BQ);
-    const int64_t c = std::max<int64_t>(16, tiles * R * ((rows + QT - 1) / QT) / 1024);
-    nsplit = (int)((R * nx + c - 1) / c);
-    units = (int)c;
+    const int64_t work = R * ((rows + QT - 1) / QT);
+    static const int want = getenv("NP") ? atoi(getenv("NP")) : 1024;
+    const int64_t n = tiles >= 512 ? 1 : std::max<int64_t>(1, std::min((want + tiles - 1) / tiles, work / 48));
+    units = (int)((R * nx + n - 1) / n);
+    nsplit = (int)((R * nx + units - 1) / units);
 }
 
 }  // namespace
@@ -503,6 +524,7 @@ extern "C" int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
     if (a.nsplit > 1 && !workspace) return fail(SLOTSCAN_ERR_NULL, "slotattn_bwd: workspace is NULL");
     if ((Tk + BQ - 1) / BQ * B * Hk * std::max(a.nsplit, BQ / 32) > 0x7fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: shape too large");
     a.part = (float*)workspace;
+    a.groups = getenv("GR") ? atoi(getenv("GR")) : 1;
     a.out = (void*)out;
     a.res = (void*)res;
     a.lse = (float*)lse;
