@@ -334,7 +334,9 @@ struct Sees {
 // The 16 rows of a result tile from row j0 on (rows j0 + key_of(r, h)) that a lane sees, as bits: by its interval, by the prefix
 // where a lane's does not join it (pre), by the document ids (at ids + 8 g + 4 h; null: none)
 __device__ __forceinline__ uint32_t seen16(const Sees& v, int j0, int h, bool pre, const int* ids, int id) {
-    const unsigned x = (unsigned)(j0 + 4 * h) - v.first, y = (unsigned)(j0 + 4 * h);
+    unsigned x = (unsigned)(j0 + 4 * h) - v.first;
+    const unsigned y = (unsigned)(j0 + 4 * h);
+    asm volatile("" : "+v"(x));                       // only where it is asked for: not computed ahead of the branch around it
     uint32_t m = 0;
 #pragma unroll
     for (int r = 0; r < 16; r++) m |= (x + key_of(r, 0) <= v.count ? 1u : 0u) << r;

@@ -250,15 +250,22 @@ __device__ __forceinline__ bool meets(int x0, int x1, int nx, int u0, int u1) {
     return false;
 }
 
+// Two waves share 32 keys, on one SIMD: the first forms the scores and P, and sums dV = P^T dO; the second dP and dS, and sums
+// dK = dS^T Q, a tile behind, with P (times the cap's slope) handed over in LDS.  Each holds one operand and one sum -- one wave
+// with both had 250 registers and no room to read operands ahead: 3,100 cycles a tile of 32 x 32 pairs, with 1,024 of
+// matrix work -- and one's matrix instructions run beside the other's vector ones.
+#define RING 4                                       // tiles: the two at work, two on their way
+
 template <typename T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
-    constexpr int KK = D / 16, DT = D / 32, STAGE = QT * 2 * D, KEYS = BQ * 2 * D;
+__global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
+    constexpr int KK = D / 16, DT = D / 32, STAGE = QT * 2 * D, SLOT = 2 * STAGE, EX = 4096;
     typedef TileLoad<D, QT, BW> Load;
-    __shared__ __align__(1024) unsigned char smem[KEYS + 4 * STAGE]; // the keys; [buffer][queries, dout]
-    __shared__ __align__(16) float s_st[2][2][QT];                   // [buffer][log-sum-exp, delta]
-    __shared__ __align__(16) int s_id[2][2 * QT];                    // the queries' documents (twice)
-    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __shared__ __align__(1024) unsigned char smem[RING * SLOT];      // [slot][queries, dout]
+    __shared__ __align__(1024) unsigned char s_ex[2][BW][EX];        // P on its way: [tile % 2][pair][register quad][lane]
+    __shared__ __align__(16) float s_st[RING][2][QT];                // log-sum-exp, minus delta
+    __shared__ __align__(16) int s_id[RING][2 * QT];                 // the queries' documents (twice)
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int role = uni((int)threadIdx.x / BT), w = uni((int)(threadIdx.x & (BT - 1)) >> 6);
     const int kvh = a.B * a.Hk;
     // Workgroups that read the same queries -- one part of one key/value head's -- run on one XCD, at the same time, so that its L2
     // serves them: XCD i % 8 takes every 8th (part, head).  Where those are no multiple of 8, heads alternate.
@@ -281,42 +288,37 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
     const int jw = j0 + 32 * w, j = jw + (lane & 31), jc = min(j, a.Tk - 1);
     const int jw1 = min(jw + 31, a.Tk - 1);
     Mask mk{a.causal, a.W, prefix_of(a, b), a.Tk};
-    const unsigned lds = lds_addr(smem), ldq = lds + KEYS;
-    TileLoad<D, BQ, BW>(a.k_st, w, lane).issue((const T*)a.k + b * a.k_sb + hk * a.k_sh, j0, a.Tk - 1, lds);
-    uint4 vf[KK];
-    {
-        const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh + jc * a.v_st + 8 * h;
-#pragma unroll
-        for (int kk = 0; kk < KK; kk++) vf[kk] = ld16(v + 16 * kk);
-    }
-    const bool docs = a.ids != nullptr;
-    const int64_t idb = (int64_t)b * a.ntd * KT;
-    Span kw{j0, j1, 0, 0, true}, kv{jw, jw1, 0, 0, true};             // document ranges of the keys
-    int dk_ = 0;
-    if (docs) {
-        const int2* range = a.range + (int64_t)b * a.ntd;
-        doc_span(range, kw);
-        if (jw <= jw1) doc_span(range, kv);
-        dk_ = a.ids[idb + jc];
-        if (dk_ < 0) dk_ = -2;
-    }
     int x0, x1;
     tile_rows(a, mk, j0, j1, off, x0, x1);
     const int nx = (a.Tq + QT - 1) / QT, u0 = part * a.units, u1 = min(u0 + a.units, a.R * nx);
     if (a.nsplit > 1 && !meets(x0, x1, nx, u0, u1)) return;           // the whole workgroup; attn_add knows it too
-    const int2* range = docs ? a.range + (int64_t)b * a.ntd : nullptr;
-    const Sees see = Sees::key(mk, j, a.Tk - 1);
-    f32x16 dk[DT], dv[DT];
+    uint4 of[KK];                                     // this wave's keys, or values, as operands
+    {
+        const T* x = (role ? (const T*)a.v + b * a.v_sb + hk * a.v_sh + jc * a.v_st : (const T*)a.k + b * a.k_sb + hk * a.k_sh + jc * a.k_st) + 8 * h;
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++) dk[dt] = dv[dt] = zero16();
-    // the walk: heads of the group x query tiles, those of this workgroup's part
+        for (int kk = 0; kk < KK; kk++) of[kk] = ld16(x + 16 * kk);
+    }
+    const bool docs = a.ids != nullptr;
+    const int64_t idb = (int64_t)b * a.ntd * KT;
+    Span kw{j0, j1, 0, 0, true}, kv{jw, jw1, 0, 0, true};             // document ranges of the keys
+    const int2* range = docs ? a.range + (int64_t)b * a.ntd : nullptr;
+    int id = 0;
+    if (docs) {
+        doc_span(range, kw);
+        if (jw <= jw1) doc_span(range, kv);
+        id = a.ids[idb + jc];
+        if (id < 0) id = -2;
+    }
+    const Sees see = Sees::key(mk, j, a.Tk - 1);
+    // the walk: heads of the group x query tiles, those of this workgroup's part.  A tile: its number, twice, plus whether every
+    // pair of the wave's keys is visible, and its head; -1: none
     int r = u0 / nx - 1, base = 0, xe = 0;
-    uint64_t act = 0, mine = 0, full = 0;
-    auto next = [&](int& hq, int& xt, bool& some, bool& all) {
+    uint64_t act = 0, full = 0;
+    auto next = [&]() -> int2 {
         while (!act) {
             base += 64;
             if (base >= xe) {
-                if (++r * nx >= u1) { xt = -1; return; }
+                if (++r * nx >= u1) return make_int2(-1, 0);
                 base = max(x0, u0 - r * nx);
                 xe = min(x1, u1 - r * nx);
             }
@@ -330,108 +332,169 @@ __global__ __launch_bounds__(BT, 2) void attn_dkv(AttnArgs a) {
                 s.one = range_one(ra) && range_one(rb) && ra.y == rb.y;
             }
             act = __ballot(in && mk.some(s, j0, j1) && (!range || (s.lo <= kw.hi && kw.lo <= s.hi)));
-            mine = __ballot(in && jw <= jw1 && mk.some(s, jw, jw1) && (!range || (s.lo <= kv.hi && kv.lo <= s.hi)));
             full = __ballot(in && x * QT + QT <= a.Tq && mk.all(s, jw, jw + 31) && (!range || (s.one && kv.one && s.lo == kv.lo)));
         }
         const int i = __builtin_ctzll(act);
         act &= act - 1;
-        xt = base + i;
-        hq = hk * a.R + r;
-        some = mine >> i & 1;
-        all = full >> i & 1;
+        return make_int2(2 * (base + i) + (int)(full >> i & 1), r);
     };
-    const Load lq(a.q_st, w, lane), ld(a.do_st, w, lane);
-    auto load = [&](int hq, int xt, int buf) {
-        lq.issue((const T*)a.q + b * a.q_sb + hq * a.q_sh, xt * QT, a.Tq - 1, ldq + (2 * buf) * STAGE);
-        ld.issue((const T*)a.dout + b * a.do_sb + hq * a.do_sh, xt * QT, a.Tq - 1, ldq + (2 * buf + 1) * STAGE);
-        const int t = min(xt * QT + (lane & 31), a.Tq - 1);           // rows past the last repeat it and are masked
-        if (w == 0) dma4((h ? a.delta : a.lse) + ((int64_t)b * a.Hq + hq) * a.Tq + t, lds_addr(s_st[buf]));
-        if (w == 1 && docs) dma4(a.ids + idb + t + off, lds_addr(s_id[buf]));
+    const unsigned lds = lds_addr(smem), lst = lds_addr(s_st), lid = lds_addr(s_id), lex = lds_addr(s_ex) + w * EX + 16 * lane;
+    // the first kind of wave loads the queries, the second dout
+    const int64_t xst = role ? a.do_st : a.q_st, xsh = role ? a.do_sh : a.q_sh;
+    const Load ldx(xst, w, lane);
+    const T* xb = role ? (const T*)a.dout + b * a.do_sb + (int64_t)hk * a.R * xsh : (const T*)a.q + b * a.q_sb + (int64_t)hk * a.R * xsh;
+    const int64_t sb = ((int64_t)b * a.Hq + hk * a.R) * a.Tq;
+    auto load = [&](int2 c, int slot) {
+        const int t0 = (c.x >> 1) * QT;
+        ldx.issue(xb + c.y * xsh, t0, a.Tq - 1, lds + slot * SLOT + role * STAGE);
+        const int t = min(t0 + (lane & 31), a.Tq - 1);                // rows past the last repeat it and are masked
+        if (w == 0 && !role) dma4((h ? a.delta : a.lse) + sb + (int64_t)c.y * a.Tq + t, lst + slot * 2 * QT * 4);
+        if (w == 0 && role && docs) dma4(a.ids + idb + t + off, lid + slot * 2 * QT * 4);
     };
-    int hq, xt, hn = 0, xn;
-    bool some, all, some_n = false, all_n = false;
+    f32x16 sum[DT];                                   // dV, or dK
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) sum[dt] = zero16();
     const Ops<D> ops(lane);
-    const unsigned stb = lds_addr(s_st) + 16 * h;
-    next(hq, xt, some, all);
-    if (xt >= 0) load(hq, xt, 0);
-    for (int buf = 0; xt >= 0; buf ^= 1, hq = hn, xt = xn, some = some_n, all = all_n) {
-        next(hn, xn, some_n, all_n);
-        wait_vm<0>();
+    // x = sum over D of the tile's rows (the queries', or dout's) and this wave's operands, read three products ahead
+    auto product = [&](f32x16& x, unsigned rows) {
+        uint4 o[4];
+#pragma unroll
+        for (int kk = 0; kk < 3; kk++) o[kk] = lds16(Ops<D>::k_step(rows, kk));
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            if (kk + 3 < KK) o[(kk + 3) & 3] = lds16(Ops<D>::k_step(rows, kk + 3));
+            x = mfma32<T>(o[kk & 3], of[kk], x);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // sum += the tile's columns times y; the first operands come with the tile
+    struct Cols { uint4 o[5]; } cols;
+    auto col = [&](unsigned tile, int i) {            // operand i: column block i % DT of 16 rows i / DT
+        cols.o[i % 5] = Ops<D>::at_col(Ops<D>::block(tile + ops.col, i % DT), Ops<D>::block(tile + ops.col8, i % DT), 16 * (i / DT) * Tile<D>::ROWB);
+    };
+    auto add = [&](unsigned tile, const uint4 (&y)[2]) {
+#pragma unroll
+        for (int i = 0; i < 2 * DT; i++) {
+            sum[i % DT] = mfma32<T>(cols.o[i % 5], y[i / DT], sum[i % DT]);
+            if (i + 4 < 2 * DT) col(tile, i + 4);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // tiles n - 1 (the second wave's), n (the first's), n + 1, n + 2
+    int2 last = make_int2(-1, 0), cur = next(), nxt = make_int2(-1, 0), nn;
+    if (cur.x >= 0) {
+        load(cur, 0);
+        nxt = next();
+        if (nxt.x >= 0) load(nxt, 1);
+    }
+    int n = 0;
+    // tile n is there, tile n - 2 is read, P of tile n - 1 handed over; the next one's loads on their way
+    auto arrive = [&]() {
+        if (nxt.x >= 0) wait_vm<Load::N>();
+        else wait_vm<0>();
         tile_barrier();
-        if (xn >= 0) load(hn, xn, buf ^ 1);
-        if (some) {
-            const unsigned bo = lds + (2 * buf) * STAGE, rq = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
-            const unsigned rk = lds + 32 * w * Tile<D>::ROWB + ops.row;
-            const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
-            f32x16 s = zero16(), dp;
+        nn = nxt.x >= 0 ? next() : make_int2(-1, 0);
+        if (nn.x >= 0) load(nn, (n + 2) & (RING - 1));
+    };
+    auto leave = [&]() {
+        n++;
+        last = cur;
+        cur = nxt;
+        nxt = nn;
+    };
+    // (a loop for each kind of wave, with the same barriers: in one loop the sums were copied where its branches meet)
+    if (!role) {
+        while (cur.x >= 0) {
+            arrive();
+            const int slot = n & (RING - 1), t0 = (cur.x >> 1) * QT;
+            const unsigned tile = lds + slot * SLOT;
+            f32x16 s = zero16();
+            product(s, tile + ops.row);
+#pragma unroll
+            for (int i = 0; i < 4; i++) col(tile + STAGE, i);
+            f32x4 L[4];
+#pragma unroll
+            for (int g = 0; g < 4; g++) L[g] = lds4f(lst + slot * 2 * QT * 4 + 32 * g + 16 * h);
+            __builtin_amdgcn_sched_barrier(0);
+            scores<CAP>(s, a);
+            const float slope = BIAS ? a.slopes[hk * a.R + cur.y] * LOG2E : 0.f, d = (float)(j - t0 - off - 4 * h);
+            f32x16 g;                                 // what dP becomes dS by
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float t = s[e];                 // capped: the tanh, whose slope is 1 - t^2
+                float x = fmaf(t, a.f, -L[e >> 2][e & 3]);
+                if constexpr (BIAS) x = fmaf(-slope, fabsf(d - (float)key_of(e, 0)), x);
+                s[e] = exp2_(x);
+                g[e] = CAP ? s[e] * fmaf(-t, t, 1.f) : s[e];
+            }
+            if (!(cur.x & 1)) {
+                const uint32_t m = seen16(see, t0 + off, h, false, docs ? s_id[slot] : nullptr, id);
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[e] = bit(m, e) ? s[e] : 0.f;
+                    g[e] = bit(m, e) ? g[e] : 0.f;
+                }
+            }
+            unsigned char* ex = s_ex[n & 1][w] + 16 * lane;
+#pragma unroll
+            for (int q = 0; q < 4; q++) *reinterpret_cast<float4*>(ex + 1024 * q) = make_float4(g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]);
+            const uint4 y[2] = {pack8<T>(s, 0), pack8<T>(s, 1)};
+            __builtin_amdgcn_sched_barrier(0);
+            add(tile + STAGE, y);
+            leave();
+        }
+        if (n) arrive();                              // the second wave's last tile
+    } else if (cur.x >= 0) {
+        arrive();
+        leave();
+        while (last.x >= 0) {
+            arrive();
+            const int slot = (n - 1) & (RING - 1);
+            const unsigned tile = lds + slot * SLOT;
+            f32x16 dp;
 #pragma unroll
             for (int g = 0; g < 4; g++) {             // minus delta
-                const f32x4 y = lds4f(stb + (2 * buf + 1) * QT * 4 + 32 * g);
+                const f32x4 y = lds4f(lst + slot * 2 * QT * 4 + QT * 4 + 32 * g + 16 * h);
                 dp[4 * g] = y.x; dp[4 * g + 1] = y.y; dp[4 * g + 2] = y.z; dp[4 * g + 3] = y.w;
             }
-            uint4 oq[3], ok[3], od[3];                // operands of three k steps: two of them on their way
-            auto rows = [&](int kk) {
-                const unsigned x = Ops<D>::k_step(rq, kk);
-                oq[kk % 3] = lds16(x + KEYS);
-                ok[kk % 3] = lds16(Ops<D>::k_step(rk, kk));
-                od[kk % 3] = lds16(x + KEYS + STAGE);
-            };
-            rows(0);
-            rows(1);
+            product(dp, tile + STAGE + ops.row);
+            f32x4 p[4];
 #pragma unroll
-            for (int kk = 0; kk < KK; kk++) {
-                if (kk + 2 < KK) rows(kk + 2);
-                s = mfma32<T>(oq[kk % 3], ok[kk % 3], s);
-                dp = mfma32<T>(od[kk % 3], vf[kk], dp);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            const int t0 = xt * QT;
-            probs<CAP, BIAS>(s, dp, a, slope, j, t0 + off, h, all, [&](int g) {
-                const f32x4 L = lds4f(stb + (2 * buf) * QT * 4 + 32 * g);
-                __builtin_amdgcn_sched_barrier(0);
-                return L;
-            }, [&]() { return seen16(see, t0 + off, h, false, docs ? s_id[buf] : nullptr, dk_); });
+            for (int q = 0; q < 4; q++) p[q] = lds4f(lex + ((n - 1) & 1) * BW * EX + 1024 * q);
+#pragma unroll
+            for (int i = 0; i < 4; i++) col(tile, i);
             __builtin_amdgcn_sched_barrier(0);
-            const uint4 pp[2] = {pack8<T>(s, 0), pack8<T>(s, 1)}, ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
-            uint4 xq[4], xd[4];                       // column block i / 2, 16 rows i % 2
-            auto cols = [&](int i) {
-                const unsigned xc = Ops<D>::block(c, i / 2), x8 = Ops<D>::block(c8, i / 2);
-                xq[i % 4] = Ops<D>::at_col(xc, x8, KEYS + 16 * (i & 1) * Tile<D>::ROWB);
-                xd[i % 4] = Ops<D>::at_col(xc, x8, KEYS + 16 * (i & 1) * Tile<D>::ROWB + STAGE);
-            };
-            cols(0);
-            cols(1);
-            cols(2);
 #pragma unroll
-            for (int i = 0; i < 2 * DT; i++) {
-                if (i + 3 < 2 * DT) cols(i + 3);
-                dv[i / 2] = mfma32<T>(xd[i % 4], pp[i & 1], dv[i / 2]);
-                dk[i / 2] = mfma32<T>(xq[i % 4], ds[i & 1], dk[i / 2]);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int e = 0; e < 16; e++) dp[e] *= p[e >> 2][e & 3];
+            if (!(last.x & 1)) {                      // a masked pair's dP may be anything
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    asm volatile("" : "+v"(dp[e]));   // (not ahead of the branch)
+                    dp[e] = p[e >> 2][e & 3] == 0.f ? 0.f : dp[e];
+                }
             }
+            const uint4 y[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
+            __builtin_amdgcn_sched_barrier(0);
+            add(tile, y);
+            leave();
         }
     }
-    const float f = a.scale;
+    const float f = role ? a.scale : 1.f;
     if (a.nsplit > 1) {
-        float* o = a.part + ((int64_t)(part * a.tiles + jt) * kvh + bh) * 2 * BQ * D + (32 * w + (lane & 31)) * D + 4 * h;
+        float* o = a.part + ((int64_t)(part * a.tiles + jt) * kvh + bh) * 2 * BQ * D + (role ? 0 : BQ * D) + (32 * w + (lane & 31)) * D + 4 * h;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                *reinterpret_cast<float4*>(o + 32 * dt + 8 * g) = make_float4(dk[dt][4 * g] * f, dk[dt][4 * g + 1] * f, dk[dt][4 * g + 2] * f, dk[dt][4 * g + 3] * f);
-                *reinterpret_cast<float4*>(o + BQ * D + 32 * dt + 8 * g) = make_float4(dv[dt][4 * g], dv[dt][4 * g + 1], dv[dt][4 * g + 2], dv[dt][4 * g + 3]);
-            }
+            for (int g = 0; g < 4; g++)
+                *reinterpret_cast<float4*>(o + 32 * dt + 8 * g) = make_float4(sum[dt][4 * g] * f, sum[dt][4 * g + 1] * f, sum[dt][4 * g + 2] * f, sum[dt][4 * g + 3] * f);
     } else if (j < a.Tk) {
-        const int64_t o = (((int64_t)b * a.Tk + j) * a.Hk + hk) * D + 4 * h;
+        T* o = (T*)(role ? a.dk : a.dv) + (((int64_t)b * a.Tk + j) * a.Hk + hk) * D + 4 * h;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                *reinterpret_cast<uint2*>((T*)a.dk + o + 32 * dt + 8 * g) =
-                    make_uint2(pack2<T>(dk[dt][4 * g] * f, dk[dt][4 * g + 1] * f), pack2<T>(dk[dt][4 * g + 2] * f, dk[dt][4 * g + 3] * f));
-                *reinterpret_cast<uint2*>((T*)a.dv + o + 32 * dt + 8 * g) =
-                    make_uint2(pack2<T>(dv[dt][4 * g], dv[dt][4 * g + 1]), pack2<T>(dv[dt][4 * g + 2], dv[dt][4 * g + 3]));
-            }
+            for (int g = 0; g < 4; g++)
+                *reinterpret_cast<uint2*>(o + 32 * dt + 8 * g) =
+                    make_uint2(pack2<T>(sum[dt][4 * g] * f, sum[dt][4 * g + 1] * f), pack2<T>(sum[dt][4 * g + 2] * f, sum[dt][4 * g + 3] * f));
     }
 }
 
@@ -462,7 +525,7 @@ template <typename T, int D, bool CAP, bool BIAS>
 void launch_one(AttnArgs a, bool keys, hipStream_t st) {
     if (keys) {
         a.tiles = (a.Tk + BQ - 1) / BQ;
-        slothost::launch(attn_dkv<T, D, CAP, BIAS>, dim3((unsigned)((int64_t)a.tiles * a.nsplit * a.B * a.Hk)), dim3(BT), 0, st, a);
+        slothost::launch(attn_dkv<T, D, CAP, BIAS>, dim3((unsigned)((int64_t)a.tiles * a.nsplit * a.B * a.Hk)), dim3(2 * BT), 0, st, a);
     } else {
         a.tiles = (a.Tq + BQ - 1) / BQ;
         if (a.groups == 2) slothost::launch(attn_dq<T, D, CAP, BIAS, 2>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(2 * BT), 0, st, a);
