@@ -37,7 +37,7 @@ int slotattn_docs(const int32_t* ids, int64_t B, int64_t T, void* docs, void* st
 /* Forward.  res (as out: what rounding took from it, so that delta is as exact as the sums) and lse may be NULL where no backward follows.  workspace: slotattn_fwd_workspace(...) bytes, 256-byte aligned: partial results where few query
  * rows meet many keys and the keys are split over workgroups (0 bytes otherwise). */
 size_t slotattn_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int causal, int64_t window,
-                              int has_docs, int has_prefix);
+                              int has_docs, int has_prefix, int has_lens);
 int slotattn_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
                  int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int dtype, int64_t B, int64_t Tq,
                  int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal, int64_t window, float cap,

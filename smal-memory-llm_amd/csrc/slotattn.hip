@@ -18,6 +18,7 @@ using slothost::al16;
 #define FW 4                                         // waves per workgroup
 #define FT (64 * FW)
 #define FQ (32 * FW)                                 // query rows per workgroup
+#define SW 2                                         // waves per workgroup where the keys are split
 // A row's sums keep their reference maximum until a score passes it by this much (base 2): probabilities then reach 2^8, far
 // from any type's end, and the sums are rescaled a few times a row instead of in most tiles.
 #define LAZY 8.f
@@ -247,11 +248,11 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
 // waves every 4th 32-key tile of them, each with a private ring of two tiles; the waves' results meet in LDS, the
 // workgroups' in attn_join.  Bound by the bytes of the keys and values.
 template <typename T, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
+__global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
     constexpr int KK = D / 16, DT = D / 32, ST = 32 * 2 * D;
     typedef TileLoad<D, 32, 1> Load;
-    __shared__ __align__(1024) unsigned char smem[FW][2][2][ST];     // [wave][buffer][keys, values]
-    __shared__ float s_m[FW][32], s_l[FW][32];
+    __shared__ __align__(1024) unsigned char smem[SW][2][2][ST];     // [wave][buffer][keys, values]
+    __shared__ float s_m[SW][32], s_l[SW][32];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sp = blockIdx.x % a.nsplit, rt = blockIdx.x / a.nsplit;
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
         lv.issue(vb, j0, klen - 1, lds + (2 * buf + 1) * ST);
     };
     auto seen = [&](int j0) {                         // the next of this wave's tiles that any row sees
-        while (j0 < hi && !mk.some(s, j0, j0 + 31)) j0 += 32 * FW;
+        while (j0 < hi && !mk.some(s, j0, j0 + 31)) j0 += 32 * SW;
         return j0;
     };
     const Ops<D> ops(lane);
@@ -295,19 +296,21 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) o[dt] = zero16();
     float m = -INFINITY, l = 0.f;
+    // Keys and values are fetched two tiles ahead, each into the place that it has just been read from: a wave has one and a
+    // half to two tiles (24 to 32 KB at D = 128) on their way while it computes.
+    int j1 = j0 < hi ? seen(j0 + 32 * SW) : hi;
+    if (j1 < hi) load(j1, 1);
     for (int buf = 0; j0 < hi; buf ^= 1) {
-        const int jn = seen(j0 + 32 * FW);
-        if (jn < hi) {
-            load(jn, buf ^ 1);
-            wait_vm<2 * Load::N>();
-        } else {
-            wait_vm<0>();
-        }
+        const int j2 = j1 < hi ? seen(j1 + 32 * SW) : hi;
+        if (j1 < hi) wait_vm<3 * Load::N>();          // behind this tile's keys: its values, the next keys and values
+        else wait_vm<Load::N>();
         asm volatile("" ::: "memory");
         const unsigned bo = lds + (2 * buf) * ST, rk = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
         f32x16 x = zero16();
 #pragma unroll
         for (int kk = 0; kk < KK; kk++) x = mfma32<T>(lds16(Ops<D>::k_step(rk, kk)), qf[kk], x);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the keys are read before their place is filled again
+        if (j2 < hi) lk.issue(kb, j2, klen - 1, lds + (2 * buf) * ST);
         scores<CAP>(x, a);
         if constexpr (BIAS) bias(x, f2, slope, p, j0, h);
         if (j0 + 32 > hi || !mk.all(s, j0, j0 + 31)) {
@@ -335,13 +338,19 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
             l += x[r];
         }
         const uint4 pf[2] = {pack8<T>(x, 0), pack8<T>(x, 1)};
+        if (j2 < hi) wait_vm<3 * Load::N>();          // behind the values: the next tile, the keys after it
+        else if (j1 < hi) wait_vm<2 * Load::N>();
+        else wait_vm<0>();
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int mm = 0; mm < 2; mm++)
                 o[dt] = mfma32<T>(Ops<D>::at_col(Ops<D>::block(c, dt), Ops<D>::block(c8, dt), ST + 16 * mm * Tile<D>::ROWB), pf[mm], o[dt]);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the tile is read before its buffer is filled again
-        j0 = jn;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // the values, too
+        if (j2 < hi) lv.issue(vb, j2, klen - 1, lds + (2 * buf + 1) * ST);
+        j0 = j1;
+        j1 = j2;
     }
     l = half_sum(l);
     // the waves' parts: (m, l) of every row to all, then the weighted sums through LDS (its tiles are read)
@@ -349,14 +358,14 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
     __syncthreads();
     float M = -INFINITY, Ls = 0.f;
 #pragma unroll
-    for (int i = 0; i < FW; i++) M = fmaxf(M, s_m[i][lane & 31]);
+    for (int i = 0; i < SW; i++) M = fmaxf(M, s_m[i][lane & 31]);
     const float Mu = M == -INFINITY ? 0.f : M;
 #pragma unroll
-    for (int i = 0; i < FW; i++) Ls += s_l[i][lane & 31] * exp2_(s_m[i][lane & 31] - Mu);
+    for (int i = 0; i < SW; i++) Ls += s_l[i][lane & 31] * exp2_(s_m[i][lane & 31] - Mu);
     const float f = exp2_(m - Mu);
     float* so = reinterpret_cast<float*>(smem);       // [wave][row][D + 4]
     constexpr int SO = D + 4;
-    static_assert(FW * 32 * SO * 4 <= (int)sizeof(smem), "the waves' sums fit");
+    static_assert(SW * 32 * SO * 4 <= (int)sizeof(smem), "the waves' sums fit");
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -366,33 +375,35 @@ __global__ __launch_bounds__(FT) void attn_split(AttnArgs a) {
     if (w == 0 && h == 0) { s_m[0][lane] = Ls; s_l[0][lane] = M; }    // read again behind the barrier
     __syncthreads();
     // 32 rows x D values: 8 lanes a row
-    const int rr = tid >> 3, c8 = tid & 7, g = r0 + rr;
-    if (g >= rows) return;
-    const float lr = s_m[0][rr], mr = s_l[0][rr];
-    const bool got = lr > 0.f || lr != lr;
-    const float inv = got ? 1.f / lr : 0.f;
-    const int gt = g / a.R, gh = hk * a.R + g - gt * a.R;
-    const int64_t orow = ((int64_t)b * a.Tq + gt) * a.Hq + gh;
+    for (int rr = tid >> 3; rr < 32; rr += 8 * SW) {
+        const int c8 = tid & 7, g = r0 + rr;
+        if (g >= rows) break;
+        const float lr = s_m[0][rr], mr = s_l[0][rr];
+        const bool got = lr > 0.f || lr != lr;
+        const float inv = got ? 1.f / lr : 0.f;
+        const int gt = g / a.R, gh = hk * a.R + g - gt * a.R;
+        const int64_t orow = ((int64_t)b * a.Tq + gt) * a.Hq + gh;
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) {
-        const int d = 4 * c8 + 32 * i;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < D / 32; i++) {
+            const int d = 4 * c8 + 32 * i;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int ww = 0; ww < FW; ww++) {
-            const float4 y = *reinterpret_cast<const float4*>(so + (ww * 32 + rr) * SO + d);
-            v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+            for (int ww = 0; ww < SW; ww++) {
+                const float4 y = *reinterpret_cast<const float4*>(so + (ww * 32 + rr) * SO + d);
+                v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+            }
+            if (a.nsplit == 1) {
+                put4<T>(a.out, a.res, orow * D + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            } else if (got) {
+                *reinterpret_cast<float4*>(a.po + (orow * a.nsplit + sp) * D + d) = v;
+            }
         }
-        if (a.nsplit == 1) {
-            put4<T>(a.out, a.res, orow * D + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-        } else if (got) {
-            *reinterpret_cast<float4*>(a.po + (orow * a.nsplit + sp) * D + d) = v;
-        }
-    }
-    if (c8 == 0) {
-        if (a.nsplit == 1) {
-            if (a.lse) a.lse[((int64_t)b * a.Hq + gh) * a.Tq + gt] = got ? mr + __builtin_amdgcn_logf(lr) : INFINITY;
-        } else {
-            *reinterpret_cast<float2*>(a.pm + (orow * a.nsplit + sp) * 2) = make_float2(mr, lr);
+        if (c8 == 0) {
+            if (a.nsplit == 1) {
+                if (a.lse) a.lse[((int64_t)b * a.Hq + gh) * a.Tq + gt] = got ? mr + __builtin_amdgcn_logf(lr) : INFINITY;
+            } else {
+                *reinterpret_cast<float2*>(a.pm + (orow * a.nsplit + sp) * 2) = make_float2(mr, lr);
+            }
         }
     }
 }
@@ -459,7 +470,7 @@ __global__ __launch_bounds__(FT) void attn_join(AttnArgs a) {
 
 template <typename T, int D, bool CAP, bool BIAS>
 void launch_one(const AttnArgs& a, bool split, hipStream_t st) {
-    if (split) slothost::launch(attn_split<T, D, CAP, BIAS>, dim3((unsigned)(a.nsplit * a.tiles), (unsigned)a.Hk, (unsigned)a.B), dim3(FT), 0, st, a);
+    if (split) slothost::launch(attn_split<T, D, CAP, BIAS>, dim3((unsigned)(a.nsplit * a.tiles), (unsigned)a.Hk, (unsigned)a.B), dim3(64 * SW), 0, st, a);
     else if (a.groups == 2) slothost::launch(attn_fwd<T, D, CAP, BIAS, 2>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(2 * FT), 0, st, a);
     else slothost::launch(attn_fwd<T, D, CAP, BIAS, 1>, dim3((unsigned)((int64_t)a.tiles * a.B * a.Hq)), dim3(FT), 0, st, a);
 }
@@ -473,22 +484,28 @@ void launch_join(const AttnArgs& a, hipStream_t st) {
     slothost::launch(attn_join<T, D>, dim3((unsigned)((int64_t)a.B * a.Tq * a.Hq)), dim3(FT), 0, st, a);
 }
 
-// How the forward runs.  split: the packed rows and split keys, where 128-row tiles would leave most of the card idle
-// (fewer workgroups than CUs) or most of each tile empty (at most 32 rows of a key/value head).
-struct Plan { bool split; int chunk, nsplit, rtiles; };
-Plan plan(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal, int64_t W, bool docs, bool prefix) {
-    Plan p{false, 0, 1, 0};
+// How the forward runs.  split: the packed rows and split keys, where a key/value head has at most 32 rows (a tile of 128 would be
+// mostly empty), or where under 128 tiles meet so many keys that the idle CUs matter more than the rows that a tile shares
+// its operands with.  groups: two groups of waves per tile while every tile has a CU of its own anyway.
+struct Plan { bool split; int chunk, nsplit, rtiles, groups; };
+Plan plan(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal, int64_t W, bool docs, bool prefix, bool ragged) {
+    Plan p{false, 0, 1, 0, 1};
     const int64_t rows = Tq * (Hq / Hk), tiles = (Tq + FQ - 1) / FQ * Hq * B;
-    if (docs || !(rows <= 32 || (tiles < 256 && Tk > 512))) return p;
-    p.split = true;
-    p.rtiles = (int)((rows + 31) / 32);
     // keys that one row tile can see
     int64_t keys = Tk;
     if (causal && !prefix && W < Tk) keys = W + Tq + 32 < Tk ? W + Tq + 32 : Tk;
-    // one workgroup a CU (its rings fill the LDS): two rounds of them, of at least two tiles a wave
-    const int64_t want = (512 + p.rtiles * Hk * B - 1) / (p.rtiles * Hk * B);
+    if (docs || !(rows <= 32 || (tiles < 128 && keys >= 4096))) {
+        if (tiles <= 256) p.groups = 2;
+        return p;
+    }
+    p.split = true;
+    p.rtiles = (int)((rows + 31) / 32);
+    // Two workgroups a CU (their rings fill the LDS).  One round of them where the lengths are equal; where they may be ragged, pieces
+    // small enough that the last round is short, not so small that a workgroup's start (about 5 us) counts: 32 sequences of
+    // 1,024 to 8,192 keys, pieces of 512 / 768 / 1,024 / 2,048 keys: 81 / 62 / 77 / 70 us.
+    const int64_t total = ragged && B > 1 ? 1408 : 512, want = (total + p.rtiles * Hk * B - 1) / (p.rtiles * Hk * B);
     int64_t chunk = (keys + want - 1) / want;
-    chunk = (chunk + 127) / 128 * 128;
+    chunk = (chunk + 63) / 64 * 64;
     if (chunk < 256) chunk = 256;
     p.chunk = (int)chunk;
     p.nsplit = (int)((keys + chunk - 1) / chunk);
@@ -519,9 +536,9 @@ extern "C" int slotattn_docs(const int32_t* ids, int64_t B, int64_t T, void* doc
 }
 
 extern "C" size_t slotattn_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D, int causal, int64_t window,
-                                         int has_docs, int has_prefix) {
+                                         int has_docs, int has_prefix, int has_lens) {
     if (B < 1 || Tq < 1 || Tk < 1 || Hk < 1 || Hq < Hk || Hq % Hk) return 0;
-    return split_bytes(plan(B, Tq, Tk, Hq, Hk, causal, window, has_docs, has_prefix), B, Tq, Hq, D);
+    return split_bytes(plan(B, Tq, Tk, Hq, Hk, causal, window, has_docs, has_prefix, has_lens), B, Tq, Hq, D);
 }
 
 extern "C" int slotattn_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
@@ -534,7 +551,7 @@ extern "C" int slotattn_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
     if (!lens && Tq > Tk) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_fwd: more queries than keys");
     if (!out) return fail(SLOTSCAN_ERR_NULL, "slotattn_fwd: a required pointer is NULL");
     if (!al16(out) || !al16(res) || !al16(workspace) || !al16(docs)) return fail(SLOTSCAN_ERR_ALIGN, "slotattn_fwd: out, res, docs and workspace must be 16-byte aligned");
-    Plan p = plan(B, Tq, Tk, Hq, Hk, causal, window, docs != nullptr, prefix != nullptr);
+    Plan p = plan(B, Tq, Tk, Hq, Hk, causal, window, docs != nullptr, prefix != nullptr, lens != nullptr);
     if (split_bytes(p, B, Tq, Hq, D) && !workspace) return fail(SLOTSCAN_ERR_NULL, "slotattn_fwd: workspace is NULL");
     AttnArgs a = slotattn_host::args(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, B, Tq, Tk, Hq, Hk, scale, causal, window, cap,
                                      slopes, docs, prefix);
@@ -545,7 +562,7 @@ extern "C" int slotattn_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
     a.tiles = p.split ? p.rtiles : (int)((Tq + FQ - 1) / FQ);
     a.chunk = p.chunk;
     a.nsplit = p.nsplit;
-    a.groups = getenv("GR") ? atoi(getenv("GR")) : 1;
+    a.groups = p.groups;
     a.po = (float*)workspace;
     a.pm = a.po ? a.po + B * Tq * Hq * p.nsplit * D : nullptr;
     const bool split = p.split;

@@ -545,14 +545,13 @@ void launch_add(AttnArgs a, hipStream_t st) {
 }
 
 // Parts of the queries per key tile.  A part costs the write and the read of its sums, about as long as 20 query tiles take, so keys are
-// split only where the key tiles alone do not fill the card's 512 workgroup slots, and into parts of 48 query tiles at least.
+// split only where the key tiles alone do not fill the card, and into parts of 48 query tiles at least.
 void parts(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal, int64_t W, bool prefix, int& nsplit, int& units) {
     const int64_t R = Hq / Hk, nx = (Tq + QT - 1) / QT, tiles = (Tk + BQ - 1) / BQ * B * Hk;
     int64_t rows = causal ? Tq - Tq / 2 : Tq;                         // of a head that see a key tile, about
     if (!prefix && W < Tk) rows = std::min(rows, (causal ? W : 2 * W) + BQ);
     const int64_t work = R * ((rows + QT - 1) / QT);
-    static const int want = getenv("NP") ? atoi(getenv("NP")) : 1024;
-    const int64_t n = tiles >= 512 ? 1 : std::max<int64_t>(1, std::min((want + tiles - 1) / tiles, work / 48));
+    const int64_t n = tiles >= 512 ? 1 : std::max<int64_t>(1, std::min((1023 + tiles) / tiles, work / 48));
     units = (int)((R * nx + n - 1) / n);
     nsplit = (int)((R * nx + units - 1) / units);
 }
@@ -587,7 +586,7 @@ extern "C" int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
     if (a.nsplit > 1 && !workspace) return fail(SLOTSCAN_ERR_NULL, "slotattn_bwd: workspace is NULL");
     if ((Tk + BQ - 1) / BQ * B * Hk * std::max(a.nsplit, BQ / 32) > 0x7fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: shape too large");
     a.part = (float*)workspace;
-    a.groups = getenv("GR") ? atoi(getenv("GR")) : 1;
+    a.groups = (Tq + BQ - 1) / BQ * B * Hq <= 256 ? 2 : 1;           // as in the forward
     a.out = (void*)out;
     a.res = (void*)res;
     a.lse = (float*)lse;

@@ -68,7 +68,8 @@ def _launch_fwd(q_, k_, v_, opts, slopes, dws, prefix, lens, keep):
     out = torch.empty(B, Tq, Hq, D, device=dev, dtype=q_.dtype)
     res = torch.empty_like(out) if keep else None
     lse = torch.empty(B, Hq, Tq, device=dev, dtype=torch.float32) if keep else None
-    n = lib.slotattn_fwd_workspace(B, Tq, Tk, Hq, Hk, D, causal, window, dws is not None, prefix is not None)
+    n = lib.slotattn_fwd_workspace(B, Tq, Tk, Hq, Hk, D, causal, window, dws is not None, prefix is not None,
+                                   lens is not None)
     ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
     rc = lib.slotattn_fwd(*L.strided(q_), *L.strided(k_), *L.strided(v_), L._TYPE_CODES[q_.dtype], B, Tq, Tk, Hq, Hk, D, scale,
                           causal, window, cap, L.ptr(slopes), L.ptr(dws), L.ptr(prefix), L.ptr(lens), L.ptr(ws), L.ptr(out),

@@ -82,7 +82,7 @@ SIGNATURES = {
                        + _ROWS * 2 + [_vp]),
     "slotattn_docs_bytes": (_sz, [_i64, _i64]),
     "slotattn_docs": (_i32, [_vp, _i64, _i64, _vp, _vp]),
-    "slotattn_fwd_workspace": (_sz, [_i64] * 6 + [_i32, _i64, _i32, _i32]),
+    "slotattn_fwd_workspace": (_sz, [_i64] * 6 + [_i32, _i64, _i32, _i32, _i32]),
     "slotattn_fwd": (_i32, _ATTN + [_vp] * 8),
     "slotattn_bwd_workspace": (_sz, [_i64] * 6 + [_i32, _i64, _i32]),
     "slotattn_bwd": (_i32, _ATTN + [_vp] * 5 + _ROWS + [_vp] * 6),
