@@ -355,6 +355,79 @@ __device__ __forceinline__ uint32_t seen16(const Sees& v, int j0, int h, bool pr
 }
 __device__ __forceinline__ bool bit(uint32_t m, int r) { return (m >> r & 1) != 0; }
 
+// ---- rows next to infinities and NaN -----------------------------------------------------------------------
+// A masked pair has the weight 0 in its product, and 0 times an infinity or a NaN of the other operand is a NaN: a row whose
+// sums come out so is formed again by its wave, one row at a time, from its visible pairs alone.  Where all is finite that
+// costs the tests, about 1 instruction per value of the accumulators; a row whose scores hold a NaN of their own is left at the first.
+__device__ __forceinline__ float nonfinite(const f32x16& x, float t) {            // t + 0 if all of x is finite, else NaN
+#pragma unroll
+    for (int r = 0; r < 16; r++) t = fmaf(x[r], 0.f, t);
+    return t;
+}
+__device__ __forceinline__ int lane_of(int x, int i) { return __builtin_amdgcn_readlane(x, i); }
+__device__ __forceinline__ float lane_of(float x, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)); }
+__device__ __forceinline__ Sees lane_of(const Sees& v, int i) {
+    return {(unsigned)lane_of((int)v.first, i), (unsigned)lane_of((int)v.count, i), (unsigned)lane_of((int)v.below, i)};
+}
+__device__ __forceinline__ float widen1(bf16_t x) { return bf2f(x); }
+__device__ __forceinline__ float widen1(f16_t x) { return (float)x; }
+template <typename T, int D> __device__ __forceinline__ float dot_row(const T* x, const T* y) {
+    float s = 0.f;
+    for (int d = 0; d < D; d++) s = fmaf(widen1(x[d]), widen1(y[d]), s);
+    return s;
+}
+// the score of one pair in base 2, and the slope of the cap
+template <bool CAP, bool BIAS> __device__ __forceinline__ float score1(float x, const AttnArgs& a, float slope, int dist, float& tang) {
+    tang = 1.f;
+    if constexpr (CAP) {
+        x = fabsf(x) <= a.lim ? tanh_poly(x, a) : tanh_any(x, a);
+        tang = fmaf(-x, x, 1.f);
+    }
+    x *= a.f;
+    if constexpr (BIAS) x = fmaf(-slope, fabsf((float)dist), x);
+    return x;
+}
+__device__ __forceinline__ bool sees1(const Sees& v, int j, const int* ids, int id) {
+    return ((unsigned)j - v.first <= v.count || (unsigned)j < v.below) && (!ids || ids[j] == id);
+}
+// One query's softmax over keys [lo, hi): maximum, sum and unnormalised output, values lane D / 64 .. of it per lane
+template <typename T, int D, bool CAP, bool BIAS>
+__device__ __forceinline__ void exact_row(const AttnArgs& a, const T* q, const T* kb, const T* vb, const Sees& v, const int* ids, int id, float slope,
+                                          int p, int lo, int hi, int lane, float& m, float& l, float (&o)[D / 64]) {
+    m = -INFINITY;
+    l = 0.f;
+    for (int i = 0; i < D / 64; i++) o[i] = 0.f;
+    for (int j0 = lo; j0 < hi; j0 += 64) {
+        const int j = j0 + lane;
+        const bool ok = j < hi && sees1(v, j, ids, id);
+        uint64_t b = __ballot(ok);
+        if (!b) continue;
+        float x = -INFINITY, tang;
+        if (ok) x = score1<CAP, BIAS>(dot_row<T, D>(q, kb + j * a.k_st), a, slope, p - j, tang);
+        if (__ballot(x != x)) {
+            l = NAN;
+            for (int i = 0; i < D / 64; i++) o[i] = NAN;
+            return;
+        }
+        float mx = x;
+        for (int i = 1; i < 64; i <<= 1) mx = fmaxf(mx, __shfl_xor(mx, i));
+        const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, f = m == -INFINITY ? 0.f : exp2_(m - mn);
+        const float e = ok ? exp2_(x - mu) : 0.f;
+        m = mn;
+        l = l * f + wavesum(e);
+        for (int i = 0; i < D / 64; i++) o[i] *= f;
+        for (; b; b &= b - 1) {
+            const int k = __builtin_ctzll(b);
+            const float w = lane_of(e, k);
+            for (int i = 0; i < D / 64; i++) o[i] = fmaf(w, widen1(vb[(j0 + k) * a.v_st + lane * (D / 64) + i]), o[i]);
+        }
+    }
+}
+template <typename T, int D> __device__ __forceinline__ void put_row(T* out, int lane, const float (&o)[D / 64]) {
+    if constexpr (D == 128) *reinterpret_cast<uint32_t*>(out + 2 * lane) = pack2<T>(o[0], o[1]);
+    else *reinterpret_cast<uint16_t*>(out + lane) = (uint16_t)pack2<T>(o[0], 0.f);
+}
+
 // The walk over the 64-key tiles that a workgroup's queries see.  Each lane tests one of 64 tiles at a time; what a
 // workgroup visits, a wave computes and a wave computes without masks are three ballots.
 struct Walk {

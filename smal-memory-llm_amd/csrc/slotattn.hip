@@ -231,8 +231,28 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
                 o[dt][4 * g + 3] = fmaf(x.w, f1, o[dt][4 * g + 3] * f0);
             }
     }
+    float bad = l * 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) bad = nonfinite(o[dt], bad);
+    const uint64_t odd = __ballot(bad != 0.f && t < a.Tq);
+    const uint32_t rows = (uint32_t)(odd | odd >> 32);
+    for (uint32_t left = rows; left; left &= left - 1) {
+        const int i = __builtin_ctz(left), ti = t0 + 32 * w + i;
+        float m1, l1, o1[D / 64], rest[D / 64];
+        exact_row<T, D, CAP, BIAS>(a, (const T*)a.q + b * a.q_sb + hq * a.q_sh + ti * a.q_st, kb, vb, lane_of(see, i), docs ? a.ids + idb : nullptr,
+                                   lane_of(dq, i), slope, ti + off, 0, mk.klen, lane, m1, l1, o1);
+        const float inv1 = l1 > 0.f || l1 != l1 ? 1.f / l1 : 0.f;
+        const int64_t at = (((int64_t)b * a.Tq + ti) * a.Hq + hq) * D;
+        for (int e = 0; e < D / 64; e++) {
+            o1[e] *= inv1;
+            rest[e] = o1[e] - unpack<T>(pack2<T>(o1[e], 0.f), 0);
+        }
+        put_row<T, D>((T*)a.out + at, lane, o1);
+        if (a.res) put_row<T, D>((T*)a.res + at, lane, rest);
+        if (a.lse && lane == 0) a.lse[(int64_t)bh * a.Tq + ti] = l1 > 0.f || l1 != l1 ? m1 + __builtin_amdgcn_logf(l1) : INFINITY;
+    }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    if (t < a.Tq) {
+    if (t < a.Tq && !bit(rows, lane & 31)) {
         const int64_t at = (((int64_t)b * a.Tq + t) * a.Hq + hq) * D + 4 * h;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
@@ -253,6 +273,7 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
     typedef TileLoad<D, 32, 1> Load;
     __shared__ __align__(1024) unsigned char smem[SW][2][2][ST];     // [wave][buffer][keys, values]
     __shared__ float s_m[SW][32], s_l[SW][32];
+    __shared__ uint32_t s_bad[SW];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sp = blockIdx.x % a.nsplit, rt = blockIdx.x / a.nsplit;
@@ -373,7 +394,28 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
             *reinterpret_cast<float4*>(so + (w * 32 + (lane & 31)) * SO + 32 * dt + 8 * g + 4 * h) =
                 make_float4(o[dt][4 * g] * f, o[dt][4 * g + 1] * f, o[dt][4 * g + 2] * f, o[dt][4 * g + 3] * f);
     if (w == 0 && h == 0) { s_m[0][lane] = Ls; s_l[0][lane] = M; }    // read again behind the barrier
+    float bad = l * 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) bad = nonfinite(o[dt], bad);
+    const uint64_t odd = __ballot(bad != 0.f && r0 + (lane & 31) < rows);
+    if (lane == 0) s_bad[w] = (uint32_t)(odd | odd >> 32);
     __syncthreads();
+    uint32_t left = 0;
+#pragma unroll
+    for (int i = 0; i < SW; i++) left |= s_bad[i];
+    if (left) {                                       // the same in every wave
+        for (; left; left &= left - 1) {
+            const int i = __builtin_ctz(left);
+            if (i % SW != w) continue;
+            float m1, l1, o1[D / 64];
+            exact_row<T, D, CAP, BIAS>(a, (const T*)a.q + b * a.q_sb + lane_of(hq, i) * a.q_sh + lane_of(t, i) * a.q_st, kb, vb, lane_of(see, i),
+                                       nullptr, 0, lane_of(slope, i), lane_of(p, i), lo, hi, lane, m1, l1, o1);
+            for (int ww = 0; ww < SW; ww++)
+                for (int e = 0; e < D / 64; e++) so[(ww * 32 + i) * SO + lane * (D / 64) + e] = ww ? 0.f : o1[e];
+            if (lane == 0) { s_m[0][i] = l1; s_l[0][i] = m1; }
+        }
+        __syncthreads();
+    }
     // 32 rows x D values: 8 lanes a row
     for (int rr = tid >> 3; rr < 32; rr += 8 * SW) {
         const int c8 = tid & 7, g = r0 + rr;

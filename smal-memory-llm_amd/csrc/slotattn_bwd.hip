@@ -219,7 +219,43 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
                 acc[dt][4 * g + 3] += x.w;
             }
     }
-    if (t < a.Tq) {
+    float bad = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) bad = nonfinite(acc[dt], bad);
+    const uint64_t odd = __ballot(bad != 0.f && t < a.Tq);
+    const uint32_t rows = (uint32_t)(odd | odd >> 32);
+    for (uint32_t left = rows; left; left &= left - 1) {              // (exact_row's, with dS in the place of P)
+        const int i = __builtin_ctz(left), ti = t0 + 32 * w + i, pi = ti + off, id = lane_of(dq, i);
+        const T* q = (const T*)a.q + b * a.q_sb + hq * a.q_sh + ti * a.q_st;
+        const T* g = (const T*)a.dout + b * a.do_sb + hq * a.do_sh + ti * a.do_st;
+        const Sees v = Sees::query(mk, pi);
+        const float L = a.lse[(int64_t)bh * a.Tq + ti], de = lane_of(delta, i);
+        float o1[D / 64];
+        for (int e = 0; e < D / 64; e++) o1[e] = 0.f;
+        for (int j1 = 0; j1 < mk.klen; j1 += 64) {
+            const int j = j1 + lane;
+            const bool ok = j < mk.klen && sees1(v, j, docs ? a.ids + idb : nullptr, id);
+            uint64_t m = __ballot(ok);
+            if (!m) continue;
+            float d = 0.f, tang;
+            if (ok) {
+                d = exp2_(score1<CAP, BIAS>(dot_row<T, D>(q, kb + j * a.k_st), a, slope, pi - j, tang) - L);
+                d *= (dot_row<T, D>(g, vb + j * a.v_st) - de) * tang;
+            }
+            if (__ballot(d != d)) {
+                for (int e = 0; e < D / 64; e++) o1[e] = NAN;
+                break;
+            }
+            for (; m; m &= m - 1) {
+                const int k = __builtin_ctzll(m);
+                const float x = lane_of(d, k);
+                for (int e = 0; e < D / 64; e++) o1[e] = fmaf(x, widen1(kb[(j1 + k) * a.k_st + lane * (D / 64) + e]), o1[e]);
+            }
+        }
+        for (int e = 0; e < D / 64; e++) o1[e] *= a.scale;
+        put_row<T, D>((T*)a.dq + (((int64_t)b * a.Tq + ti) * a.Hq + hq) * D, lane, o1);
+    }
+    if (t < a.Tq && !bit(rows, lane & 31)) {
         T* out = (T*)a.dq + (((int64_t)b * a.Tq + t) * a.Hq + hq) * D;
         const float f = a.scale;
 #pragma unroll
@@ -480,8 +516,59 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
         }
     }
     const float f = role ? a.scale : 1.f;
+    float bad = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) bad = nonfinite(sum[dt], bad);
+    const uint64_t odd = __ballot(bad != 0.f && j < a.Tk);
+    const uint32_t rows = (uint32_t)(odd | odd >> 32);
+    float* const po = a.part + ((int64_t)(part * a.tiles + jt) * kvh + bh) * 2 * BQ * D + (role ? 0 : BQ * D) + 32 * w * D;
+    for (uint32_t left = rows; left; left &= left - 1) {              // a key's sums from the queries that see it, of this part
+        const int i = __builtin_ctz(left), ji = jw + i, idi = lane_of(id, i);
+        const T* k = (const T*)a.k + b * a.k_sb + hk * a.k_sh + ji * a.k_st;
+        const T* v = (const T*)a.v + b * a.v_sb + hk * a.v_sh + ji * a.v_st;
+        const Sees se = lane_of(see, i);
+        float o1[D / 64];
+        for (int e = 0; e < D / 64; e++) o1[e] = 0.f;
+        for (int rr = u0 / nx; rr * nx < u1; rr++) {
+            const int hq = hk * a.R + rr;
+            const T* qh = (const T*)a.q + b * a.q_sb + hq * a.q_sh;
+            const T* gh = (const T*)a.dout + b * a.do_sb + hq * a.do_sh;
+            const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
+            const int te = min(min(x1, u1 - rr * nx) * QT, a.Tq);
+            for (int t1 = max(x0, u0 - rr * nx) * QT; t1 < te; t1 += 64) {
+                const int t = t1 + lane;
+                const bool ok = t < te && sees1(se, t + off, docs ? a.ids + idb : nullptr, idi);
+                uint64_t m = __ballot(ok);
+                if (!m) continue;
+                float d = 0.f, tang;
+                if (ok) {
+                    const int64_t at = ((int64_t)b * a.Hq + hq) * a.Tq + t;
+                    d = exp2_(score1<CAP, BIAS>(dot_row<T, D>(qh + t * a.q_st, k), a, slope, t + off - ji, tang) - a.lse[at]);
+                    if (role) d *= (dot_row<T, D>(gh + t * a.do_st, v) + a.delta[at]) * tang;
+                }
+                if (__ballot(d != d)) {
+                    for (int e = 0; e < D / 64; e++) o1[e] = NAN;
+                    rr = a.R;
+                    break;
+                }
+                for (; m; m &= m - 1) {
+                    const int x = __builtin_ctzll(m);
+                    const T* row = role ? qh + (t1 + x) * a.q_st : gh + (t1 + x) * a.do_st;
+                    const float y = lane_of(d, x);
+                    for (int e = 0; e < D / 64; e++) o1[e] = fmaf(y, widen1(row[lane * (D / 64) + e]), o1[e]);
+                }
+            }
+        }
+        for (int e = 0; e < D / 64; e++) o1[e] *= f;
+        if (a.nsplit > 1) {
+            for (int e = 0; e < D / 64; e++) po[i * D + lane * (D / 64) + e] = o1[e];
+        } else {
+            put_row<T, D>((T*)(role ? a.dk : a.dv) + (((int64_t)b * a.Tk + ji) * a.Hk + hk) * D, lane, o1);
+        }
+    }
+    if (bit(rows, lane & 31)) return;
     if (a.nsplit > 1) {
-        float* o = a.part + ((int64_t)(part * a.tiles + jt) * kvh + bh) * 2 * BQ * D + (role ? 0 : BQ * D) + (32 * w + (lane & 31)) * D + 4 * h;
+        float* o = po + (lane & 31) * D + 4 * h;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
