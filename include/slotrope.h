@@ -31,7 +31,7 @@ int slotrope_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const 
                  int64_t Hk, int64_t D, float eps, void* qo, void* ko, void* stream);
 
 /* Backward: the gradients dqo, dko of the two outputs (by strides) in; dq (B, T, Hq, D), dk (B, T, Hk, D) and dwq, dwk
- * (D, in wdtype; NULL where the gain is) out.  The gains' gradients are summed in fp32 in a fixed order (no atomics).
+ * (D, in wdtype; NULL: not wanted) out.  The gains' gradients are summed in fp32 in a fixed order (no atomics).
  * workspace: slotrope_bwd_workspace(B, T, Hq, Hk, D) bytes, 16-byte aligned. */
 size_t slotrope_bwd_workspace(int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D);
 int slotrope_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,

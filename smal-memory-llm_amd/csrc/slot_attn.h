@@ -30,41 +30,6 @@ template <> __device__ __forceinline__ f32x16 mfma32<bf16_t>(const uint4& a, con
 template <> __device__ __forceinline__ f32x16 mfma32<f16_t>(const uint4& a, const uint4& b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-// The same in place, with the registers' kind fixed: sums in accumulation registers, scores in vector registers.  Left to the
-// compiler, a kernel whose sums and scores pass 256 registers moved all of them from one kind to the other in every
-// iteration.  The compiler does not know these for matrix instructions: before anything else reads a result, mfma_settle().
-template <typename T> __device__ __forceinline__ void mfma_acc(f32x16& c, const uint4& a, const uint4& b);
-template <> __device__ __forceinline__ void mfma_acc<bf16_t>(f32x16& c, const uint4& a, const uint4& b) {
-    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(bf16x8, a)), "v"(__builtin_bit_cast(bf16x8, b)));
-}
-template <> __device__ __forceinline__ void mfma_acc<f16_t>(f32x16& c, const uint4& a, const uint4& b) {
-    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(f16x8, a)), "v"(__builtin_bit_cast(f16x8, b)));
-}
-template <typename T> __device__ __forceinline__ void mfma_vec(f32x16& c, const uint4& a, const uint4& b);
-template <> __device__ __forceinline__ void mfma_vec<bf16_t>(f32x16& c, const uint4& a, const uint4& b) {
-    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(__builtin_bit_cast(bf16x8, a)), "v"(__builtin_bit_cast(bf16x8, b)));
-}
-template <> __device__ __forceinline__ void mfma_vec<f16_t>(f32x16& c, const uint4& a, const uint4& b) {
-    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(__builtin_bit_cast(f16x8, a)), "v"(__builtin_bit_cast(f16x8, b)));
-}
-// The first product of a sum: c = a b + from, or a b alone
-template <typename T> __device__ __forceinline__ void mfma_from(f32x16& c, const uint4& a, const uint4& b, const f32x16& from);
-template <> __device__ __forceinline__ void mfma_from<bf16_t>(f32x16& c, const uint4& a, const uint4& b, const f32x16& from) {
-    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %3" : "=&v"(c) : "v"(__builtin_bit_cast(bf16x8, a)), "v"(__builtin_bit_cast(bf16x8, b)), "v"(from));
-}
-template <> __device__ __forceinline__ void mfma_from<f16_t>(f32x16& c, const uint4& a, const uint4& b, const f32x16& from) {
-    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %3" : "=&v"(c) : "v"(__builtin_bit_cast(f16x8, a)), "v"(__builtin_bit_cast(f16x8, b)), "v"(from));
-}
-template <typename T> __device__ __forceinline__ void mfma_first(f32x16& c, const uint4& a, const uint4& b);
-template <> __device__ __forceinline__ void mfma_first<bf16_t>(f32x16& c, const uint4& a, const uint4& b) {
-    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(__builtin_bit_cast(bf16x8, a)), "v"(__builtin_bit_cast(bf16x8, b)));
-}
-template <> __device__ __forceinline__ void mfma_first<f16_t>(f32x16& c, const uint4& a, const uint4& b) {
-    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(c) : "v"(__builtin_bit_cast(f16x8, a)), "v"(__builtin_bit_cast(f16x8, b)));
-}
-// Behind it the results of earlier ones can be read, and registers written just before be read by later ones: 20 wait states
-// (a 16-pass matrix instruction needs 18)
-__device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 3" ::: "memory"); }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<bf16_t>(float lo, float hi) { return pack_bf16x2(lo, hi); }
 template <> __device__ __forceinline__ uint32_t pack2<f16_t>(float lo, float hi) {
@@ -280,7 +245,6 @@ __device__ __forceinline__ void bias(f32x16& s, float f, float slope, int p, int
 // A value that is the same in every lane, in a scalar register.  (Loads behind the asm blocks' memory clobbers go through
 // vector registers, and what is computed from them -- a tile's base address -- would stay there.)
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ float uni(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 // Tokens of sequence b that count, and its length that positions are taken from (a length past the keys keeps its positions).
 __device__ __forceinline__ int length_of(const AttnArgs& a, int b) { return uni(a.lens ? min(max(a.lens[b], 0), (1 << 30) - 1) : a.Tk); }
 __device__ __forceinline__ int prefix_of(const AttnArgs& a, int b) { return uni(a.prefix ? a.prefix[b] : 0); }

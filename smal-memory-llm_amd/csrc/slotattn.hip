@@ -43,9 +43,14 @@ __global__ __launch_bounds__(64) void attn_docs(const int32_t* ids, int T, int n
 }
 
 // ------------------------------------------------------------------------------------------- many rows
-// GR groups of 4 waves share a workgroup's rows, each taking every GR-th of their key tiles; their sums meet in LDS.  With two
-// groups the longest rows take half the steps: under causality 128 rows of 8,192 tokens see up to 128 tiles, 49 on average
-// would fill the card's time.
+// Per 64 keys a wave has 2 D / 16 + D / 8 matrix instructions of 32 cycles (S = K Q^T, O += V^T P^T; 1,024 cycles at D = 128) and
+// about 350 vector ones for the softmax of 32 x 64 scores; both share a SIMD's issue, so two waves a SIMD (64 KB of LDS a
+// workgroup) fill one's gaps with the other's work.  Measured: 8,192 causal tokens, 12 query heads of 128 on 4, capped: 284 us
+// (1.45e12 bits of arithmetic in products: 726 TFLOP/s; the two products alone would take 149 us at the rate of a large
+// library product); 4 x 2,000 tokens with prefixes, capped: 98 us.
+// GR groups of 4 waves share a workgroup's rows, each taking every GR-th of their key tiles; their sums meet in LDS.  Two
+// groups halve the longest rows' steps where every tile has a CU of its own (up to 256 tiles); with more tiles their
+// lockstep costs more than the balance gives (8,192 tokens: 340 against 295 us).
 template <typename T, int D, bool CAP, bool BIAS, int GR>
 __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
     constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
@@ -126,7 +131,7 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
         if (some) {
             const unsigned bo = lds + (2 * buf) * STAGE, rk = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
             const int j0 = jt * KT;
-            // operands are read PRE products ahead: an LDS read takes as long as four or five of them
+            // operands are read three steps (six products) ahead: an LDS read takes as long as four or five products
             f32x16 s[2] = {zero16(), zero16()};
             uint4 kr[4][2];
             auto rows = [&](int kk) {
@@ -264,9 +269,12 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------- few rows
-// Rows of a key/value head packed as (token, query head of the group); a workgroup takes `chunk` keys of 32 rows, its
-// waves every 4th 32-key tile of them, each with a private ring of two tiles; the waves' results meet in LDS, the
-// workgroups' in attn_join.  Bound by the bytes of the keys and values.
+// Rows of a key/value head packed as (token, query head of the group); a workgroup takes `chunk` keys of 32 rows, its waves every
+// SW-th 32-key tile of them, each through a ring of its own of two tiles (no barrier in the loop); the waves' results meet
+// in LDS, the workgroups' in attn_join.  Bound by the bytes of the keys and values: two workgroups a CU keep about 100 KB
+// on their way.  Measured: 32 sequences of up to 8,192 tokens, 12 query heads of 128 on 4: 63 + 4 us (join), 4.6 TB/s;
+// one of 131,072: 43 + 8 us, 6.2 TB/s in the kernel.  (Four waves a workgroup, one workgroup a CU, tiles fetched one
+// ahead: 92 and 57 us.)
 template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
     constexpr int KK = D / 16, DT = D / 32, ST = 32 * 2 * D;

@@ -14,11 +14,13 @@ are not enough -- packed documents, long windows, prompts read both ways, capped
         is not read.  A query of negative position (lens[b] < T) gets 0.
 
 bf16 or fp16, D in {64, 128}; docs, prefix (B,) and lens (B,) int32, slopes fp32.  Scores, softmax statistics and sums are
-fp32; the probabilities and score gradients are rounded to the operands' type for their products.  Operands may be any
-views whose rows are contiguous and 16-byte aligned (others are copied); results and gradients are token-major, seen as
-(B, H, T, D).  Gradients are bitwise reproducible.  No CPU path: a missing library raises.
+fp32; the probabilities and score gradients are rounded to the operands' type for their products.  What a query does not see
+never reaches its row, infinities and NaN included.  Operands may be any views whose rows are contiguous and 16-byte aligned
+(others are copied: a cache should not need that); results and gradients are token-major, seen as (B, H, T, D).  Gradients
+are bitwise reproducible; there is no second derivative.  No CPU path: a missing library raises.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 import slotscan_lib as L
 from slotrope_hip import _same_device, check_caches, check_lens
@@ -90,6 +92,7 @@ class _Attend(torch.autograd.Function):
         return out.transpose(1, 2)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q_, k_, v_, out, res, lse, slopes, dws, prefix = ctx.saved_tensors
         scale, causal, window, cap = ctx.opts

@@ -19,6 +19,7 @@ a fixed order.  Operands may be any views whose rows are contiguous and 16-byte 
 projection (others are copied); results are token-major, seen as (B, H, T, D).  No CPU path: a missing library raises.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 import slotscan_lib as L
 
@@ -104,6 +105,7 @@ class _Rope(torch.autograd.Function):
         return _launch_fwd(q_, k_, wq_, wk_, wt, freqs, positions, eps, inter)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dqo, dko):
         q_, k_, wq_, wk_, freqs, positions = ctx.saved_tensors
         wt, eps, inter, tq, tk = ctx.meta
@@ -152,6 +154,16 @@ def check_caches(kcache, vcache, like, Hk, what):
         raise NotImplementedError(f"{what}: the caches must have the queries' type {like.dtype} (got {kcache.dtype}, {vcache.dtype})")
 
 
+def _apart(c):
+    """Whether no two rows of c (B, H, S, D) share memory: every dimension steps over all that the closer ones reach."""
+    reach = c.size(3)
+    for st, n in sorted((c.stride(i), c.size(i)) for i in range(3) if c.size(i) > 1):
+        if st < reach:
+            return False
+        reach += st * (n - 1)
+    return True
+
+
 def check_lens(lens, B, what):
     if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
         raise ValueError(f"{what}: lens must be a contiguous int32 ({B},) (got {lens.dtype}, {tuple(lens.shape)})")
@@ -170,7 +182,7 @@ def qk_rope_cache(q, k, v, wq, wk, freqs, lens, kcache, vcache, eps=1e-6, interl
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, wq, wk, kcache, vcache)):
         raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
     for c in (kcache, vcache):
-        if any(c.size(i) > 1 and c.stride(i) < D for i in range(3)) or c.data_ptr() != L.rows(c).data_ptr():
+        if not _apart(c) or not L.in_place(c):
             raise ValueError(f"{what}: a cache is written in place: its rows must be contiguous, 16-byte aligned and apart")
     _same_device(what, q, k, v, wq, wk, freqs, lens, kcache, vcache)
     q_, k_, v_ = L.rows(q), L.rows(k), L.rows(v)

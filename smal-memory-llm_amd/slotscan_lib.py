@@ -134,13 +134,19 @@ def dtype_code(dt):
 _TYPE_CODES = {torch.float32: SLOTSCAN_F32, torch.bfloat16: SLOTSCAN_BF16, torch.float16: SLOTSCAN_F16}
 
 
-def rows(x):
-    """x (batch, head, token, D) as the kernels read it: D values of a row contiguous, every row 16-byte aligned and
-    tokens fewer than 2^25 elements apart.  A view that is laid out so costs no copy."""
+def in_place(x):
+    """Whether x (batch, head, token, D) is as the kernels read it: D values of a row contiguous, every row 16-byte aligned and
+    tokens fewer than 2^25 elements apart."""
     n = 16 // x.element_size()
     s = x.stride()
-    if s[3] != 1 or s[0] % n or s[1] % n or s[2] % n or s[2] >= 1 << 25:
-        x = x.contiguous()
+    return s[3] == 1 and not (s[0] % n or s[1] % n or s[2] % n) and s[2] < 1 << 25 and not x.data_ptr() % 16
+
+
+def rows(x):
+    """x as the kernels read it (in_place), itself or a copy."""
+    if in_place(x):
+        return x
+    x = x.contiguous()
     return x.clone(memory_format=torch.contiguous_format) if x.data_ptr() % 16 else x
 
 
