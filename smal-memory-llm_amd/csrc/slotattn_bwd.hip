@@ -69,6 +69,16 @@ __device__ __forceinline__ void probs(f32x16& s, f32x16& dp, const AttnArgs& a, 
     }
 }
 
+// what rounding took from x to y = pack8() of it
+template <typename T> __device__ __forceinline__ void minus(f32x16& x, const uint4 (&y)[2]) {
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+        const uint32_t w[4] = {y[m].x, y[m].y, y[m].z, y[m].w};
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[8 * m + i] -= unpack<T>(w[i / 2], i & 1);
+    }
+}
+
 // ------------------------------------------------------------------------------------------- dQ
 // Three products of 32 x 32 x D per wave and half tile (S, dP, dQ) beside about 10 vector instructions a score; K and V tiles are
 // staged once for 128 queries, two workgroups a CU.  8,192 causal tokens, 12 query heads of 128 on 4, capped: 368 us (610
@@ -187,13 +197,18 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
                 cols(u, 1);
                 cols(u, 2);
                 probs<CAP, BIAS>(s, dp, a, slope, p, j0, h, all, [&](int) { return f32x4{lse, lse, lse, lse}; }, [&]() { return seen16(see, j0, h, j0 < mk.prefix, docs ? a.ids + idb + j0 : nullptr, dq); });
+                // dS in two parts, its rounding and what that took away: a row's dS sum to zero, so that what the keys with the large
+                // weights have in common (they lie along the query) cancels in dQ, but not the roundings of their dS.
                 const uint4 ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
+                minus<T>(dp, ds);
+                const uint4 dl[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 2 * DT; i++) {
-                    acc[i % DT] = mfma32<T>(cr[i % 5], ds[i / DT], acc[i % DT]);
+                for (int i = 0; i <= 2 * DT; i++) {   // the second part a step behind, so that no product waits for the one before
+                    if (i < 2 * DT) acc[i % DT] = mfma32<T>(cr[i % 5], ds[i / DT], acc[i % DT]);
+                    if (i > 0) acc[(i - 1) % DT] = mfma32<T>(cr[(i - 1) % 5], dl[(i - 1) / DT], acc[(i - 1) % DT]);
                     if (i + 3 < 2 * DT) cols(u, i + 3);
-                    else if (u == 0) rows(1, i + 3 - 2 * DT);
+                    else if (u == 0 && i < 2 * DT) rows(1, i + 3 - 2 * DT);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
