@@ -4,7 +4,7 @@
 // P comes back from the rows' log-sum-exp.  Two kernels, each of which owns what it sums, so nothing is added atomically:
 //   attn_dq    128 queries of one head per workgroup, walking the visible key tiles (as the forward does); it forms delta
 //   attn_dkv   128 keys of one key/value head per workgroup, walking the query tiles of every head of the group that see them
-// The price is that the scores and dP are formed twice: 7 products where one kernel with atomic dQ would need 5.
+// The price is that the scores and dP are formed twice (with dQ's in two parts 8 products, where one kernel with atomic dQ would need 5 or 6).
 #include <algorithm>
 
 #include "slot_attn.h"
@@ -80,9 +80,10 @@ template <typename T> __device__ __forceinline__ void minus(f32x16& x, const uin
 }
 
 // ------------------------------------------------------------------------------------------- dQ
-// Three products of 32 x 32 x D per wave and half tile (S, dP, dQ) beside about 10 vector instructions a score; K and V tiles are
-// staged once for 128 queries, two workgroups a CU.  8,192 causal tokens, 12 query heads of 128 on 4, capped: 368 us (610
-// TFLOP/s; 224 us at a large library product's rate).  (GR groups of waves as in the forward.)
+// Four products of 32 x 32 x D per wave and half tile (S, dP, dQ twice) beside about 12 vector instructions a score; K and V tiles are
+// staged once for 128 queries, two workgroups a CU.  8,192 causal tokens, 12 query heads of 128 on 4, capped: 425 us (the three products
+// that cannot be left out take 224 us at a large library product's rate; with dS rounded once 370 us).  (GR groups of waves as in
+// the forward.)
 template <typename T, int D, bool CAP, bool BIAS, int GR>
 __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
     constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
