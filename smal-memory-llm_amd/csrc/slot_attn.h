@@ -320,9 +320,10 @@ __device__ __forceinline__ uint32_t seen16(const Sees& v, int j0, int h, bool pr
 __device__ __forceinline__ bool bit(uint32_t m, int r) { return (m >> r & 1) != 0; }
 
 // ---- rows next to infinities and NaN -----------------------------------------------------------------------
-// A masked pair has the weight 0 in its product, and 0 times an infinity or a NaN of the other operand is a NaN: a row whose
-// sums come out so is formed again by its wave, one row at a time, from its visible pairs alone.  Where all is finite that
-// costs the tests, about 1 instruction per value of the accumulators; a row whose scores hold a NaN of their own is left at the first.
+// A masked pair has the weight 0 in its product, and 0 times an infinity or a NaN of the other operand is a NaN.  So a row whose
+// sums come out so, though all that it sees is finite, is formed again by its wave, one row at a time, from its visible pairs
+// alone; one that sees such a value keeps its sums.  Where all is finite that costs the tests, about 1 instruction per
+// value of the accumulators; a value seen by every row costs each wave one pass over the keys.
 __device__ __forceinline__ float nonfinite(const f32x16& x, float t) {            // t + 0 if all of x is finite, else NaN
 #pragma unroll
     for (int r = 0; r < 16; r++) t = fmaf(x[r], 0.f, t);
@@ -340,6 +341,20 @@ template <typename T, int D> __device__ __forceinline__ float dot_row(const T* x
     for (int d = 0; d < D; d++) s = fmaf(widen1(x[d]), widen1(y[d]), s);
     return s;
 }
+template <typename T, int D> __device__ __forceinline__ bool finite_row(const T* x) {
+    float t = 0.f;
+    for (int d = 0; d < D; d++) t = fmaf(widen1(x[d]), 0.f, t);
+    return t == 0.f;
+}
+// o += sum over the rows k of m, at most n of them, of lane k's w times the row; values D / 64 lane .. of it per lane
+template <typename T, int D> __device__ __forceinline__ void add_rows(float (&o)[D / 64], float w, uint64_t m, const T* rows, int64_t st, int n, int lane) {
+#pragma unroll 8
+    for (int k = 0; k < 64; k++) {
+        const T* r = rows + min(k, n - 1) * st + lane * (D / 64);
+        const float y = lane_of(w, k);
+        for (int i = 0; i < D / 64; i++) o[i] = fmaf(y, m >> k & 1 ? widen1(r[i]) : 0.f, o[i]);
+    }
+}
 // the score of one pair in base 2, and the slope of the cap
 template <bool CAP, bool BIAS> __device__ __forceinline__ float score1(float x, const AttnArgs& a, float slope, int dist, float& tang) {
     tang = 1.f;
@@ -354,6 +369,22 @@ template <bool CAP, bool BIAS> __device__ __forceinline__ float score1(float x, 
 __device__ __forceinline__ bool sees1(const Sees& v, int j, const int* ids, int id) {
     return ((unsigned)j - v.first <= v.count || (unsigned)j < v.below) && (!ids || ids[j] == id);
 }
+// Whether the lane's row sees one of keys [lo, hi) whose two rows are not finite.  (In a wave: all lanes.)
+template <typename T, int D>
+__device__ __forceinline__ bool sees_nonfinite(const Sees& v, const int* ids, int id, const T* kb, int64_t k_st, const T* vb, int64_t v_st, int lo, int hi, int lane) {
+    bool hit = false;
+    for (int j0 = lo; j0 < hi; j0 += 64) {
+        const int j = j0 + lane;
+        for (uint64_t b = __ballot(j < hi && !(finite_row<T, D>(kb + j * k_st) && finite_row<T, D>(vb + j * v_st))); b; b &= b - 1)
+            hit = hit || sees1(v, j0 + __builtin_ctzll(b), ids, id);
+    }
+    return hit;
+}
+// rows of the wave (lanes l and l + 32 have row l) for which x holds, as bits
+__device__ __forceinline__ uint32_t row_bits(bool x) {
+    const uint64_t b = __ballot(x);
+    return (uint32_t)(b | b >> 32);
+}
 // One query's softmax over keys [lo, hi): maximum, sum and unnormalised output, values lane D / 64 .. of it per lane
 template <typename T, int D, bool CAP, bool BIAS>
 __device__ __forceinline__ void exact_row(const AttnArgs& a, const T* q, const T* kb, const T* vb, const Sees& v, const int* ids, int id, float slope,
@@ -364,15 +395,10 @@ __device__ __forceinline__ void exact_row(const AttnArgs& a, const T* q, const T
     for (int j0 = lo; j0 < hi; j0 += 64) {
         const int j = j0 + lane;
         const bool ok = j < hi && sees1(v, j, ids, id);
-        uint64_t b = __ballot(ok);
+        const uint64_t b = __ballot(ok);
         if (!b) continue;
         float x = -INFINITY, tang;
         if (ok) x = score1<CAP, BIAS>(dot_row<T, D>(q, kb + j * a.k_st), a, slope, p - j, tang);
-        if (__ballot(x != x)) {
-            l = NAN;
-            for (int i = 0; i < D / 64; i++) o[i] = NAN;
-            return;
-        }
         float mx = x;
         for (int i = 1; i < 64; i <<= 1) mx = fmaxf(mx, __shfl_xor(mx, i));
         const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, f = m == -INFINITY ? 0.f : exp2_(m - mn);
@@ -380,11 +406,11 @@ __device__ __forceinline__ void exact_row(const AttnArgs& a, const T* q, const T
         m = mn;
         l = l * f + wavesum(e);
         for (int i = 0; i < D / 64; i++) o[i] *= f;
-        for (; b; b &= b - 1) {
-            const int k = __builtin_ctzll(b);
-            const float w = lane_of(e, k);
-            for (int i = 0; i < D / 64; i++) o[i] = fmaf(w, widen1(vb[(j0 + k) * a.v_st + lane * (D / 64) + i]), o[i]);
+        if (l != l) {                                 // its own query, or an overflow
+            for (int i = 0; i < D / 64; i++) o[i] = NAN;
+            return;
         }
+        add_rows<T, D>(o, e, b, vb + j0 * a.v_st, a.v_st, hi - j0, lane);
     }
 }
 template <typename T, int D> __device__ __forceinline__ void put_row(T* out, int lane, const float (&o)[D / 64]) {

@@ -239,8 +239,8 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
     float bad = l * 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) bad = nonfinite(o[dt], bad);
-    const uint64_t odd = __ballot(bad != 0.f && t < a.Tq);
-    const uint32_t rows = (uint32_t)(odd | odd >> 32);
+    uint32_t rows = row_bits(bad != 0.f && t < a.Tq);
+    if (rows) rows &= ~row_bits(sees_nonfinite<T, D>(see, docs ? a.ids + idb : nullptr, dq, kb, a.k_st, vb, a.v_st, 0, mk.klen, lane));
     for (uint32_t left = rows; left; left &= left - 1) {
         const int i = __builtin_ctz(left), ti = t0 + 32 * w + i;
         float m1, l1, o1[D / 64], rest[D / 64];
@@ -405,13 +405,14 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
     float bad = l * 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) bad = nonfinite(o[dt], bad);
-    const uint64_t odd = __ballot(bad != 0.f && r0 + (lane & 31) < rows);
-    if (lane == 0) s_bad[w] = (uint32_t)(odd | odd >> 32);
+    const uint32_t odd = row_bits(bad != 0.f && r0 + (lane & 31) < rows);
+    if (lane == 0) s_bad[w] = odd;
     __syncthreads();
     uint32_t left = 0;
 #pragma unroll
     for (int i = 0; i < SW; i++) left |= s_bad[i];
     if (left) {                                       // the same in every wave
+        left &= ~row_bits(sees_nonfinite<T, D>(see, nullptr, 0, kb, a.k_st, vb, a.v_st, lo, hi, lane));
         for (; left; left &= left - 1) {
             const int i = __builtin_ctz(left);
             if (i % SW != w) continue;

@@ -240,8 +240,8 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
     float bad = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) bad = nonfinite(acc[dt], bad);
-    const uint64_t odd = __ballot(bad != 0.f && t < a.Tq);
-    const uint32_t rows = (uint32_t)(odd | odd >> 32);
+    uint32_t rows = row_bits(bad != 0.f && t < a.Tq);
+    if (rows) rows &= ~row_bits(sees_nonfinite<T, D>(see, docs ? a.ids + idb : nullptr, dq, kb, a.k_st, vb, a.v_st, 0, mk.klen, lane));
     for (uint32_t left = rows; left; left &= left - 1) {              // (exact_row's, with dS in the place of P)
         const int i = __builtin_ctz(left), ti = t0 + 32 * w + i, pi = ti + off, id = lane_of(dq, i);
         const T* q = (const T*)a.q + b * a.q_sb + hq * a.q_sh + ti * a.q_st;
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
         for (int j1 = 0; j1 < mk.klen; j1 += 64) {
             const int j = j1 + lane;
             const bool ok = j < mk.klen && sees1(v, j, docs ? a.ids + idb : nullptr, id);
-            uint64_t m = __ballot(ok);
+            const uint64_t m = __ballot(ok);
             if (!m) continue;
             float d = 0.f, tang;
             if (ok) {
@@ -264,11 +264,7 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
                 for (int e = 0; e < D / 64; e++) o1[e] = NAN;
                 break;
             }
-            for (; m; m &= m - 1) {
-                const int k = __builtin_ctzll(m);
-                const float x = lane_of(d, k);
-                for (int e = 0; e < D / 64; e++) o1[e] = fmaf(x, widen1(kb[(j1 + k) * a.k_st + lane * (D / 64) + e]), o1[e]);
-            }
+            add_rows<T, D>(o1, d, m, kb + j1 * a.k_st, a.k_st, mk.klen - j1, lane);
         }
         for (int e = 0; e < D / 64; e++) o1[e] *= a.scale;
         put_row<T, D>((T*)a.dq + (((int64_t)b * a.Tq + ti) * a.Hq + hq) * D, lane, o1);
@@ -539,8 +535,27 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
     float bad = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) bad = nonfinite(sum[dt], bad);
-    const uint64_t odd = __ballot(bad != 0.f && j < a.Tk);
-    const uint32_t rows = (uint32_t)(odd | odd >> 32);
+    uint32_t rows = row_bits(bad != 0.f && j < a.Tk);
+    if (rows) {                                       // keys that see a query with something not finite keep their sums, too
+        bool hit = false;
+        for (int rr = u0 / nx; rr * nx < u1; rr++) {
+            const int hq = hk * a.R + rr, te = min(min(x1, u1 - rr * nx) * QT, a.Tq);
+            const T* qh = (const T*)a.q + b * a.q_sb + hq * a.q_sh;
+            const T* gh = (const T*)a.dout + b * a.do_sb + hq * a.do_sh;
+            const int64_t at = ((int64_t)b * a.Hq + hq) * a.Tq;
+            for (int t1 = max(x0, u0 - rr * nx) * QT; t1 < te; t1 += 64) {
+                const int t = t1 + lane;
+                bool ill = false;
+                if (t < te) {
+                    const float s = a.lse[at + t] * 0.f + (role ? a.delta[at + t] * 0.f : 0.f);   // (an infinite log-sum-exp: a query that sees nothing)
+                    ill = s != s || !finite_row<T, D>(qh + t * a.q_st) || !finite_row<T, D>(gh + t * a.do_st);
+                }
+                for (uint64_t m = __ballot(ill); m; m &= m - 1)
+                    hit = hit || sees1(see, t1 + __builtin_ctzll(m) + off, docs ? a.ids + idb : nullptr, id);
+            }
+        }
+        rows &= ~row_bits(hit);
+    }
     float* const po = a.part + ((int64_t)(part * a.tiles + jt) * kvh + bh) * 2 * BQ * D + (role ? 0 : BQ * D) + 32 * w * D;
     for (uint32_t left = rows; left; left &= left - 1) {              // a key's sums from the queries that see it, of this part
         const int i = __builtin_ctz(left), ji = jw + i, idi = lane_of(id, i);
@@ -558,7 +573,7 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
             for (int t1 = max(x0, u0 - rr * nx) * QT; t1 < te; t1 += 64) {
                 const int t = t1 + lane;
                 const bool ok = t < te && sees1(se, t + off, docs ? a.ids + idb : nullptr, idi);
-                uint64_t m = __ballot(ok);
+                const uint64_t m = __ballot(ok);
                 if (!m) continue;
                 float d = 0.f, tang;
                 if (ok) {
@@ -571,12 +586,7 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
                     rr = a.R;
                     break;
                 }
-                for (; m; m &= m - 1) {
-                    const int x = __builtin_ctzll(m);
-                    const T* row = role ? qh + (t1 + x) * a.q_st : gh + (t1 + x) * a.do_st;
-                    const float y = lane_of(d, x);
-                    for (int e = 0; e < D / 64; e++) o1[e] = fmaf(y, widen1(row[lane * (D / 64) + e]), o1[e]);
-                }
+                add_rows<T, D>(o1, d, m, role ? qh + t1 * a.q_st : gh + t1 * a.do_st, role ? a.q_st : a.do_st, te - t1, lane);
             }
         }
         for (int e = 0; e < D / 64; e++) o1[e] *= f;

@@ -122,3 +122,32 @@ def test_cache_newest_token(case):
         out = A.attend_cache(q.cuda(), k.cuda(), v.cuda(), lens.cuda(), **opt).cpu()
     near(out[:, :, :-1], *(x[:, :, :-1] for x in ref), "out")
     assert bool(out[:, :, -1].isnan().all())
+
+
+@pytest.mark.parametrize("T,D,where", [(2000, 128, "v"), (700, 64, "k"), (2000, 64, "q"), (700, 128, "do")])
+def test_one_early_value(T, D, where):
+    """A single value that many rows see: they may be anything there, those before it and another document are as they were."""
+    print("one value", T, D, where, flush=True)
+    xs = dict(zip(("q", "k", "v", "do"), attn_inputs(2, 4, 2, T, T, D, BF, 25)))
+    docs = torch.zeros(2, T, dtype=torch.int32)
+    docs[:, T - 300:] = 1
+    ref = AO.attention(xs["q"], xs["k"], xs["v"], dout=xs["do"], docs=docs, u=U[BF])
+    xs[where] = xs[where].clone()
+    xs[where][:, :, 70, 3] = NAN
+    got = dict(zip(("out", "dq", "dk", "dv"), _run(*xs.values(), dict(docs=docs))))
+    clean = torch.ones(T, dtype=torch.bool)
+    clean[70:T - 300] = False
+    later = torch.arange(T) >= T - 300
+    for name, g in got.items():
+        keep = clean.clone()
+        if name in ("dk", "dv"):                         # earlier keys are seen by the queries that it reaches
+            keep = later.clone()
+            if where in ("q", "do"):
+                keep |= (torch.arange(T) > 70)
+        elif where in ("q", "do"):
+            keep = torch.ones(T, dtype=torch.bool)
+            keep[70] = name == "out" and where == "do"
+        near(g[:, :, keep], *(x[:, :, keep] for x in ref[name]), name)
+    seen = {"v": ("out", slice(70, T - 300), 3), "k": ("out", slice(70, T - 300), slice(None)), "q": ("out", slice(70, 71), slice(None)),
+            "do": ("dq", slice(70, 71), slice(None))}[where]
+    assert bool(got[seen[0]][:, :, seen[1], seen[2]].isnan().all())
