@@ -624,15 +624,26 @@ __global__ __launch_bounds__(256) void attn_add(AttnArgs a) {
     const Mask mk{a.causal, a.W, prefix_of(a, b), a.Tk};
     int x0, x1;
     tile_rows(a, mk, j0, j1, off, x0, x1);
-    const int nx = (a.Tq + QT - 1) / QT;
+    const int nx = (a.Tq + QT - 1) / QT, lane = threadIdx.x & 63;
+    const uint64_t parts = __ballot(lane < a.nsplit && meets(x0, x1, nx, lane * a.units, min((lane + 1) * a.units, a.R * nx)));
     for (int e = threadIdx.x; e < 32 * (D / 4) * 2; e += 256) {
         const int which = e / (32 * (D / 4)), i = e % (32 * (D / 4)), row = (q4 % (BQ / 32)) * 32 + i / (D / 4), c = 4 * (i % (D / 4));
         if (j0 + row >= a.Tk) continue;
+        const float* from = a.part + ((int64_t)jt * kvh + bh) * 2 * BQ * D + which * BQ * D + row * D + c;
+        const int64_t st = (int64_t)a.tiles * kvh * 2 * BQ * D;
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p = 0; p < a.nsplit; p++) {
-            if (!meets(x0, x1, nx, p * a.units, min((p + 1) * a.units, a.R * nx))) continue;
-            const float4 x = *reinterpret_cast<const float4*>(a.part + ((int64_t)(p * a.tiles + jt) * kvh + bh) * 2 * BQ * D + which * BQ * D + row * D + c);
-            s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+        for (uint64_t m = parts; m;) {                // in order, four loads on their way
+            float4 x[4];
+            bool in[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                in[k] = m != 0;
+                x[k] = *reinterpret_cast<const float4*>(from + (in[k] ? __builtin_ctzll(m) : __builtin_ctzll(parts)) * st);
+                m &= m - 1;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (in[k]) { s.x += x[k].x; s.y += x[k].y; s.z += x[k].z; s.w += x[k].w; }
         }
         put4<T>(which ? a.dv : a.dk, nullptr, (((int64_t)b * a.Tk + j0 + row) * a.Hk + hk) * D + c, s.x, s.y, s.z, s.w);
     }
@@ -661,14 +672,16 @@ void launch_add(AttnArgs a, hipStream_t st) {
     slothost::launch(attn_add<T, D>, dim3((unsigned)((int64_t)a.tiles * (BQ / 32) * a.B * a.Hk)), dim3(256), 0, st, a);
 }
 
-// Parts of the queries per key tile.  A part costs the write and the read of its sums, about as long as 20 query tiles take, so keys are
-// split only where the key tiles alone do not fill the card, and into parts of 48 query tiles at least.
+// Parts of the queries per key tile, 64 at most.  A part costs the write and the read of its sums, about as long as 20 query tiles take, so
+// where the key tiles fill the card, keys are split into parts of 48 query tiles at least.  Where they leave CUs idle (under 400 / 2 tiles), a part
+// of 8 pays already: 4 heads of 128 x 4,096 tokens 145 -> 78 us with the addition, 12 heads on 4 x 1,024 tokens 111 -> 41, 2 heads of 64 on
+// 1 x 2,048 tokens 109 -> 29, 3 x 6 heads of 64 x 1,111 tokens 36 -> 30.
 void parts(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal, int64_t W, bool prefix, int& nsplit, int& units) {
     const int64_t R = Hq / Hk, nx = (Tq + QT - 1) / QT, tiles = (Tk + BQ - 1) / BQ * B * Hk;
     int64_t rows = causal ? Tq - Tq / 2 : Tq;                         // of a head that see a key tile, about
     if (!prefix && W < Tk) rows = std::min(rows, (causal ? W : 2 * W) + BQ);
     const int64_t work = R * ((rows + QT - 1) / QT);
-    const int64_t n = tiles >= 512 ? 1 : std::max<int64_t>(1, std::min((1023 + tiles) / tiles, work / 48));
+    const int64_t n = tiles >= 512 ? 1 : std::max({(int64_t)1, std::min({(int64_t)64, (1023 + tiles) / tiles, work / 48}), std::min({(int64_t)64, 400 / tiles, work / 8})});
     units = (int)((R * nx + n - 1) / n);
     nsplit = (int)((R * nx + units - 1) / units);
 }
