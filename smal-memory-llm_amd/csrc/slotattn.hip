@@ -536,8 +536,10 @@ void launch_join(const AttnArgs& a, hipStream_t st) {
 }
 
 // How the forward runs.  split: the packed rows and split keys, where a key/value head has at most 32 rows (a tile of 128 would be
-// mostly empty), or where under 128 tiles meet so many keys that the idle CUs matter more than the rows that a tile shares
-// its operands with.  groups: two groups of waves per tile while every tile has a CU of its own anyway.
+// mostly empty), or where few rows in all meet many keys: unsplit, a call takes about 8 us and 15 ns a key while CUs idle (D = 128; 128
+// to 512 rows of 12 heads alike), split about 14 us and 2.5 ns for 1,000 rows and a key.  Measured, split / unsplit: 768 rows (64 tokens of 12
+// heads) x 1,024 / 3,500 keys 16 / 22 and 18 / 55 us, 1,536 rows x 1,024 / 2,048 keys 17 / 22 and 19 / 35, 6,144 rows x 2,048 / 3,500 keys 43 / 37 and
+// 65 / 60; 256 rows x 512 keys 16 / 14.  groups: two groups of waves per tile while every tile has a CU of its own anyway.
 struct Plan { bool split; int chunk, nsplit, rtiles, groups; };
 Plan plan(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal, int64_t W, bool docs, bool prefix, bool ragged) {
     Plan p{false, 0, 1, 0, 1};
@@ -545,7 +547,8 @@ Plan plan(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int causal,
     // keys that one row tile can see
     int64_t keys = Tk;
     if (causal && !prefix && W < Tk) keys = W + Tq + 32 < Tk ? W + Tq + 32 : Tk;
-    if (docs || !(rows <= 32 || (tiles < 128 && keys >= 4096))) {
+    const int64_t all = rows * Hk * B;
+    if (docs || !(rows <= 32 || (all <= 4096 && keys >= 1024 && 3 * keys >= 2 * all))) {
         if (tiles <= 256) p.groups = 2;
         return p;
     }
