@@ -280,7 +280,8 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
     constexpr int KK = D / 16, DT = D / 32, ST = 32 * 2 * D;
     typedef TileLoad<D, 32, 1> Load;
     __shared__ __align__(1024) unsigned char smem[SW][2][2][ST];     // [wave][buffer][keys, values]
-    __shared__ float s_m[SW][32], s_l[SW][32];
+    __shared__ float s_m[SW][32], s_l[SW][32];                       // the waves' maxima and sums of every row
+    __shared__ float s_M[32], s_L[32];                               // the workgroup's
     __shared__ uint32_t s_bad[SW];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
         for (int g = 0; g < 4; g++)
             *reinterpret_cast<float4*>(so + (w * 32 + (lane & 31)) * SO + 32 * dt + 8 * g + 4 * h) =
                 make_float4(o[dt][4 * g] * f, o[dt][4 * g + 1] * f, o[dt][4 * g + 2] * f, o[dt][4 * g + 3] * f);
-    if (w == 0 && h == 0) { s_m[0][lane] = Ls; s_l[0][lane] = M; }    // read again behind the barrier
+    if (w == 0 && h == 0) { s_M[lane] = M; s_L[lane] = Ls; }          // not over s_m and s_l, which the other waves may still read
     float bad = l * 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) bad = nonfinite(o[dt], bad);
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
                                        nullptr, 0, lane_of(slope, i), lane_of(p, i), lo, hi, lane, m1, l1, o1);
             for (int ww = 0; ww < SW; ww++)
                 for (int e = 0; e < D / 64; e++) so[(ww * 32 + i) * SO + lane * (D / 64) + e] = ww ? 0.f : o1[e];
-            if (lane == 0) { s_m[0][i] = l1; s_l[0][i] = m1; }
+            if (lane == 0) { s_M[i] = m1; s_L[i] = l1; }
         }
         __syncthreads();
     }
@@ -429,7 +430,7 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
     for (int rr = tid >> 3; rr < 32; rr += 8 * SW) {
         const int c8 = tid & 7, g = r0 + rr;
         if (g >= rows) break;
-        const float lr = s_m[0][rr], mr = s_l[0][rr];
+        const float lr = s_L[rr], mr = s_M[rr];
         const bool got = lr > 0.f || lr != lr;
         const float inv = got ? 1.f / lr : 0.f;
         const int gt = g / a.R, gh = hk * a.R + g - gt * a.R;
