@@ -15,7 +15,7 @@
  *   dtype   SLOTSCAN_BF16 or SLOTSCAN_F16; scores, softmax statistics and sums are fp32
  *   q (B, Hq, Tq, D), k, v (B, Hk, Tk, D) by strides in elements (batch, head, token), every row 16-byte aligned; D = 64 or 128;
  *           Hq a multiple of Hk: query head h reads key/value head h / (Hq / Hk)
- *   |scale| in [1e-30, 1e30], cap too, or 0: none; window >= 1 (2^31 - 1: none); slopes (Hq) fp32, prefix (B), lens (B) int32 or NULL
+ *   |scale| in [1e-30, 1e30], cap too and at most 1e36 |scale|, or 0: none; window >= 1 (2^31 - 1: none); slopes (Hq) fp32, prefix (B), lens (B) int32 or NULL
  *   out, dq (B, Tq, Hq, D), dk, dv (B, Tk, Hk, D) contiguous;  lse, delta (B, Hq, Tq) fp32, the rows' log-sum-exp in base 2
  *           (+inf where nothing is visible) and sum(dout o out), kept between the calls
  *   docs    what slotattn_docs left: slotattn_docs_bytes(B, Tk) bytes, or NULL

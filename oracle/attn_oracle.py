@@ -10,6 +10,8 @@ by the chain rule.  `u` is half a step of the operands' type.  The bounds, per e
           delta' = rowsum |dO o out|;  dk alike
 and 32-bit sums: a dot product over D values is off by D 2^-24 of its absolute sum at most, which moves a probability by that
 much of itself (times the scale) and dS by that much of P (|dO| |V|^T + delta').
+
+A capped score may be off by 2^-21 of the cap; with `strict` by 2^-20 of itself and no more, however far the cap is.
 """
 import torch
 
@@ -37,7 +39,7 @@ def visible(B, Tq, Tk, causal=True, window=None, docs=None, prefix=None, lens=No
 
 
 def attention(q, k, v, scale=None, causal=True, window=None, cap=None, slopes=None, docs=None, prefix=None, lens=None,
-              dout=None, u=0.0):
+              dout=None, u=0.0, strict=False):
     """{"out": (value, bound)} and with dout also dq, dk, dv; all (B, H, T, D) float64."""
     B, Hq, Tq, D = q.shape
     Hk, Tk = k.shape[1:3]
@@ -52,6 +54,7 @@ def attention(q, k, v, scale=None, causal=True, window=None, cap=None, slopes=No
     raw = scale * (q @ k.transpose(-1, -2))
     th = torch.tanh(raw / cap) if cap else None
     s = cap * th if cap else raw
+    tanh_err = 0.0 if not cap else 2.0 ** -20 * s.abs() if strict else 2.0 ** -21 * cap
     if slopes is not None:
         s = s - slopes.double().view(-1, 1, 1) * dist.abs().double().unsqueeze(1)
     s = torch.where(ok, s, float("-inf"))
@@ -61,8 +64,10 @@ def attention(q, k, v, scale=None, causal=True, window=None, cap=None, slopes=No
     out = p @ v
     f = D * 2.0 ** -24
     # how far a probability may be off, relative: its score's absolute sum, the exponential's argument (2^-23 of it), both for
-    # the score and for the row's log-sum-exp; a cap's tanh by a few 2^-24 of the cap
-    amp = f * scale * (q.abs() @ k.abs().transpose(-1, -2)) + 2.0 ** -21 * torch.where(ok, s, 0.0).abs() + 2.0 ** -21 * (cap or 0.0)
+    # the score and for the row's log-sum-exp; and what the cap's tanh is off by
+    amp = f * scale * (q.abs() @ k.abs().transpose(-1, -2)) + 2.0 ** -21 * torch.where(ok, s, 0.0).abs() + tanh_err
+    if strict and cap:                                   # a capped score is off by the cap's range at most
+        amp = amp.clamp_max(2.0 * cap)
     amp = torch.where(ok, amp, 0.0)
     amp = 1.05 * (amp + amp.amax(-1, keepdim=True)) + 2.0 ** -18
     half = u < 2.0 ** -9 and u > 0                       # fp16: probabilities below 2^-14 of the row's largest lose bits

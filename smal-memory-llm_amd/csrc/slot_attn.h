@@ -21,6 +21,12 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 #define LOG2E 1.4426950408889634f
+// tanh(x) / x on [0, 3/4] as a polynomial in x^2, fitted for the smallest largest relative error
+#define TANH0 0.99999943f
+#define TANH1 -0.33328252f
+#define TANH2 0.13258983f
+#define TANH3 -0.05005631f
+#define TANH4 0.01292964f
 #define KT 64                                        // keys (or query rows) of a staged tile
 
 template <typename T> __device__ __forceinline__ f32x16 mfma32(const uint4& a, const uint4& b, f32x16 c);
@@ -183,7 +189,8 @@ struct AttnArgs {
     const int32_t* ids; const int2* range; int ntd;  // documents: padded ids (B, 64 ntd), ranges (B, ntd)
     const int32_t* prefix; const int32_t* lens;
     float f;                                         // what makes scores() base 2: scale log2(e), or cap log2(e)
-    float ct;                                        // capped: 2 scale log2(e) / cap
+    float kc, ct;                                    // capped: scale / cap, and 2 log2(e) of it
+    int mix;                                         // a cap so far above that small scores need a form of their own
     float lim, t0, t1, t2, t3, t4;                   // the polynomial's limit and coefficients, for products <q, k>
     void* out; void* res; float* lse;                // res: what rounding took from out, for the backward's delta
     // split rows
@@ -208,15 +215,21 @@ template <typename T> __device__ __forceinline__ void put4(void* out, void* res,
 // key of register r of a score tile's lane half h, from the tile's first key
 __device__ __forceinline__ constexpr int key_of(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
-// The products s of a 32 x 32 tile become scores up to the factor() that makes them base 2: as they are, or tanh of the scaled
-// product where they are capped.  tanh(x) is x times a polynomial in x^2 while |x| <= 3/4 (relative error 7e-7; 6
-// instructions, none of them a transcendental one), which the scores of a whole tile usually are, else 1 - 2 / (1 + e^2x)
-// (off by a few 2^-24).
+// The products s of a 32 x 32 tile become scores up to the factor() that makes them base 2: as they are, or tanh(x), x = kc s, where
+// they are capped.  tanh(x) is x times a polynomial in x^2 while |x| <= 3/4 (relative error 7e-7; 6 instructions, none of them a
+// transcendental one), which the scores of a whole tile usually are, else 1 - 2 / (1 + e^2x).  That is off by a few 2^-24 of 1, not
+// of itself, and a score is cap tanh(x): up to a cap of 64 less than 2^-16, but 0.1 at 1e6.  Above 64 each x takes the form that is exact for it
+// (8,192 tokens, forward, tiles that all hold scores past the cap: 371 us against 281 by the exponential form alone); the polynomial
+// with x formed first, as the powers of a small kc in the shorter one's coefficients would leave 32 bits.
 __device__ __forceinline__ float tanh_poly(float s, const AttnArgs& a) {
     const float y = s * s;
     return s * fmaf(fmaf(fmaf(fmaf(a.t4, y, a.t3), y, a.t2), y, a.t1), y, a.t0);
 }
-__device__ __forceinline__ float tanh_any(float s, const AttnArgs& a) { return fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp2_(s * a.ct)), 1.f); }
+__device__ __forceinline__ float tanh_exp(float s, const AttnArgs& a) { return fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp2_(s * a.ct)), 1.f); }
+__device__ __forceinline__ float tanh_mix(float s, const AttnArgs& a) {
+    const float x = s * a.kc, y = x * x, t = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp2_(x * (2.f * LOG2E))), 1.f);
+    return fabsf(x) <= 0.75f ? x * fmaf(fmaf(fmaf(fmaf(TANH4, y, TANH3), y, TANH2), y, TANH1), y, TANH0) : t;
+}
 __device__ __forceinline__ bool poly_holds(const f32x16& s, const AttnArgs& a) {
     float m = 0.f;
 #pragma unroll
@@ -228,9 +241,12 @@ template <bool CAP> __device__ __forceinline__ void scores(f32x16& s, const Attn
         if (poly_holds(s, a)) {
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = tanh_poly(s[r], a);
+        } else if (a.mix) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = tanh_mix(s[r], a);
         } else {
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = tanh_any(s[r], a);
+            for (int r = 0; r < 16; r++) s[r] = tanh_exp(s[r], a);
         }
     }
 }
@@ -382,7 +398,7 @@ template <typename T, int D> __device__ __forceinline__ void add_rows(float (&o)
 template <bool CAP, bool BIAS> __device__ __forceinline__ float score1(float x, const AttnArgs& a, float slope, int dist, float& tang) {
     tang = 1.f;
     if constexpr (CAP) {
-        x = fabsf(x) <= a.lim ? tanh_poly(x, a) : tanh_any(x, a);
+        x = fabsf(x) <= a.lim ? tanh_poly(x, a) : a.mix ? tanh_mix(x, a) : tanh_exp(x, a);
         tang = fmaf(-x, x, 1.f);
     }
     x *= a.f;

@@ -23,6 +23,8 @@ inline int check(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const 
     if (window < 1 || window > 0x7fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: window must be in [1, 2^31)");
     if (!(cap == 0.f || (cap >= 1e-30f && cap <= 1e30f))) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: cap must be 0 or in [1e-30, 1e30]");
     if (!(std::fabs(scale) >= 1e-30f && std::fabs(scale) <= 1e30f)) return fail(SLOTSCAN_ERR_SHAPE, "slotattn: |scale| must be in [1e-30, 1e30]");
+    if (cap > 1.000001e36 * std::fabs((double)scale))                 // (both are rounded to 32 bits here)
+        return fail(SLOTSCAN_ERR_SHAPE, "slotattn: cap must be at most 1e36 |scale|");
     if (Tq > SLOTATTN_MAX_T || Tk > SLOTATTN_MAX_T || B > 0x7fffffffLL / Hq || Hq / Hk * Tq > SLOTATTN_MAX_T)
         return fail(SLOTSCAN_ERR_SHAPE, "slotattn: shape too large");
     if (std::max(std::max(q_st, k_st), v_st) >= SLOTATTN_MAX_ST || std::min(std::min(q_st, k_st), v_st) < 0)
@@ -55,14 +57,18 @@ inline slotattn::AttnArgs args(const void* q, int64_t q_sb, int64_t q_sh, int64_
     a.f = scale * LOG2E;
     if (cap > 0.f) {
         a.f = cap * LOG2E;
-        a.ct = (float)std::min(std::max(2.0 * scale / cap * 1.4426950408889634, -1e37), 1e37);
-        // tanh(x) / x on [0, 3/4] as a polynomial in x^2, fitted for the smallest largest relative error; x = k <q, k>
-        const double t[5] = {0.99999943, -0.33328252, 0.13258983, -0.05005631, 0.01292964}, k = (double)scale / cap;
-        double f = k;
-        float* c[5] = {&a.t0, &a.t1, &a.t2, &a.t3, &a.t4};
-        for (int i = 0; i < 5; i++, f *= k * k) *c[i] = (float)(t[i] * f);
-        const double m = k < 0 ? -k : k;
-        a.lim = m >= 1e-4 && m <= 1e3 ? (float)(0.75 / m) : -1.f;     // beyond, k^9 leaves fp32: no score takes the polynomial
+        const double k = std::min(std::max((double)scale / cap, -1e37), 1e37), m = std::fabs(k);       // (at the ends tanh is 1, or its argument 0)
+        a.kc = (float)k;
+        a.ct = (float)(2.0 * k * 1.4426950408889634);
+        a.mix = cap > 64.f;
+        a.lim = -1.f;                                 // powers of k that leave fp32: no score takes the shorter polynomial
+        if (m >= 1e-4 && m <= 1e3) {                  // in the products <q, k> themselves
+            const double t[5] = {TANH0, TANH1, TANH2, TANH3, TANH4};
+            double f = k;
+            float* c[5] = {&a.t0, &a.t1, &a.t2, &a.t3, &a.t4};
+            for (int i = 0; i < 5; i++, f *= k * k) *c[i] = (float)(t[i] * f);
+            a.lim = (float)(0.75 / m);
+        }
     }
     a.nsplit = 1;
     return a;

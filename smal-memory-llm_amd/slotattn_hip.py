@@ -46,6 +46,8 @@ def _check(q, k, v, scale, window, cap, slopes, prefix, what):
         raise ValueError(f"{what}: cap must be in [1e-30, 1e30] or None (got {cap})")
     if scale is not None and not 1e-30 <= abs(scale) <= 1e30:
         raise ValueError(f"{what}: |scale| must be in [1e-30, 1e30] (got {scale})")
+    if cap is not None and float(cap) > 1e36 * (q.shape[3] ** -0.5 if scale is None else abs(scale)):
+        raise ValueError(f"{what}: cap must be at most 1e36 |scale| (got {cap}, scale {scale})")
     if slopes is not None:
         if slopes.shape != (q.shape[1],) or slopes.dtype != torch.float32:
             raise ValueError(f"{what}: slopes must be fp32 ({q.shape[1]},) (got {slopes.dtype}, {tuple(slopes.shape)})")
