@@ -11,7 +11,9 @@ by the chain rule.  `u` is half a step of the operands' type.  The bounds, per e
 and 32-bit sums: a dot product over D values is off by D 2^-24 of its absolute sum at most, which moves a probability by that
 much of itself (times the scale) and dS by that much of P (|dO| |V|^T + delta').
 
-A capped score may be off by 2^-21 of the cap; with `strict` by 2^-20 of itself and no more, however far the cap is.
+A capped score may be off by 2^-21 of the cap; with `strict` by 2^-20 of itself and no more, however far the cap is.  In fp16 small
+probabilities and dS lose bits, by half a step of 2^-24 each; with `strict` that step counts from the largest dS of a query (for dq) or of a key (for
+dk) at 2^10, P for dv from 1 at 2^14, and delta is off only by what two roundings of the output leave.
 """
 import torch
 
@@ -96,6 +98,18 @@ def attention(q, k, v, scale=None, causal=True, window=None, cap=None, slopes=No
     res["dq"] = (dq, sc * (e @ k.abs()) + u * dq.abs() * 1.02 + tiny)
     res["dk"] = (dk, share(sc * (e.transpose(-1, -2) @ q.abs())) + u * dk.abs() * 1.02 + tiny)
     ep = p * (u * 1.02 + amp) + sub * ok.double()
+    if strict:
+        step = 2.0 ** -25 if half else 0.0
+        d = ok.double()
+        e0 = u * 1.02 * ds.abs() + p * (2 * u * u * d1 + step * g.abs().sum(-1, keepdim=True)
+                                        + f * (pa + d1) + (amp + (2 * amp / cap if cap else 0.0)) * (dp.abs() + d1))
+        at = lambda dim: step * 2.0 ** -10 * d * ds.abs().amax(dim, keepdim=True)
+        res["dq"] = (dq, sc * ((e0 + at(-1)) @ k.abs()) + u * dq.abs() * 1.02 + tiny)
+        # (heads that share a key share its power of two)
+        top = share(ds.abs().amax(-2, keepdim=True)).repeat_interleave(R, 1) if R > 1 else ds.abs().amax(-2, keepdim=True)
+        e1 = e0 + step * 2.0 ** -10 * d * top
+        res["dk"] = (dk, share(sc * (e1.transpose(-1, -2) @ q.abs())) + u * dk.abs() * 1.02 + tiny)
+        ep = p * (u * 1.02 + amp) + step * 2.0 ** -14 * d
     res["dv"] = (dv, share(ep.transpose(-1, -2) @ g.abs()) + u * dv.abs() * 1.02 + tiny)
     return res
 

@@ -79,6 +79,28 @@ template <typename T> __device__ __forceinline__ void minus(f32x16& x, const uin
     }
 }
 
+// fp16 has 30 powers of two, and dS is about 1/T of dP: unscaled it falls among the subnormals, or to zero, long before the
+// gradients do.  So each sum's dS -- a query's for dQ, a key's for dK -- is held at a power of two of its own: large at first, lowered
+// when the largest |dS| passes fp16's range, to where that one has the exponent DS_AT, and taken out at the end: half a step of the
+// smallest dS is then 2^-35 of the sum's largest.  P, at most 1, enters dV's product at 2^P_UP.  Measured, 2,048 tokens, an upstream gradient of
+// 1e-4: dQ and dK off by 7.5e-4 and 7.8e-4 (2-norm; the results' own rounding is 7.5e-4), unscaled 3.9e-3; 8,192 tokens, 12 heads of 128 on 4:
+// attn_dq 404 and attn_dkv 610 us, unscaled 371 and 573.  bf16 has fp32's range and needs none of it.
+#define DS_FROM 60
+#define DS_AT 10
+#define DS_TOP 32768.f
+#define P_UP 14
+template <typename T> struct Half { static constexpr bool value = false; };
+template <> struct Half<f16_t> { static constexpr bool value = true; };
+__device__ __forceinline__ float max_abs(const f32x16& x) {
+    float m = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; r++) m = fmaxf(m, fabsf(x[r]));
+    return half_max(m);
+}
+__device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
+// by how many powers of two the largest |dS|, scaled, has to be lowered; 0: it is in range
+__device__ __forceinline__ int lower_by(float mx) { return mx > DS_TOP ? DS_AT + 127 - (int)(__float_as_uint(mx) >> 23) : 0; }
+
 // ------------------------------------------------------------------------------------------- dQ
 // Four products of 32 x 32 x D per wave and half tile (S, dP, dQ twice) beside about 12 vector instructions a score; K and V tiles are
 // staged once for 128 queries, two workgroups a CU.  8,192 causal tokens, 12 query heads of 128 on 4, capped: 425 us (the three products
@@ -116,7 +138,8 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
     }
     delta = half_sum(delta);
     const int64_t row = (int64_t)bh * a.Tq + tc;
-    const float lse = a.lse[row];
+    int up = Half<T>::value ? DS_FROM : 0;            // dS and its sums are held at 2^up
+    float lse = a.lse[row] - up;
     if (t < a.Tq && h == 0 && grp == 0) a.delta[row] = -delta;  // as attn_dkv starts its products
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
@@ -198,6 +221,20 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
                 cols(u, 1);
                 cols(u, 2);
                 probs<CAP, BIAS>(s, dp, a, slope, p, j0, h, all, [&](int) { return f32x4{lse, lse, lse, lse}; }, [&]() { return seen16(see, j0, h, j0 < mk.prefix, docs ? a.ids + idb + j0 : nullptr, dq); });
+                if constexpr (Half<T>::value) {
+                    const int e = lower_by(max_abs(dp));
+                    if (__any(e < 0)) {
+                        up += e;
+                        lse = a.lse[(int64_t)bh * a.Tq + tc] - up;
+                        const float f = pow2(e);
+#pragma unroll
+                        for (int r = 0; r < 16; r++) dp[r] *= f;
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                            for (int r = 0; r < 16; r++) acc[dt][r] *= f;
+                    }
+                }
                 // dS in two parts, its rounding and what that took away: a row's dS sum to zero, so that what the keys with the large
                 // weights have in common (they lie along the query) cancels in dQ, but not the roundings of their dS.
                 const uint4 ds[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
@@ -216,9 +253,12 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
         }
     }
     if constexpr (GR == 2) {
-        float4* so = reinterpret_cast<float4*>(smem);                 // [4 DT][thread]
+        float4* so = reinterpret_cast<float4*>(smem);                 // [4 DT][thread], then the rows' powers of two
+        int* su = reinterpret_cast<int*>(so + 4 * DT * BT);
+        static_assert((16 * DT + 1) * BT * 4 <= (int)sizeof(smem), "a group's sums fit");
         __syncthreads();
         if (grp) {
+            su[tid] = up;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -226,15 +266,22 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
         }
         __syncthreads();
         if (grp) return;
+        float f0 = 1.f, f1 = 1.f;                     // to the smaller of the groups' powers of two
+        if constexpr (Half<T>::value) {
+            const int u1 = su[tid], u = min(up, u1);
+            f0 = pow2(u - up);
+            f1 = pow2(u - u1);
+            up = u;
+        }
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 const float4 x = so[(4 * dt + g) * BT + tid];
-                acc[dt][4 * g] += x.x;
-                acc[dt][4 * g + 1] += x.y;
-                acc[dt][4 * g + 2] += x.z;
-                acc[dt][4 * g + 3] += x.w;
+                acc[dt][4 * g] = fmaf(x.x, f1, acc[dt][4 * g] * f0);
+                acc[dt][4 * g + 1] = fmaf(x.y, f1, acc[dt][4 * g + 1] * f0);
+                acc[dt][4 * g + 2] = fmaf(x.z, f1, acc[dt][4 * g + 2] * f0);
+                acc[dt][4 * g + 3] = fmaf(x.w, f1, acc[dt][4 * g + 3] * f0);
             }
     }
     float bad = 0.f;
@@ -271,7 +318,7 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
     }
     if (t < a.Tq && !bit(rows, lane & 31)) {
         T* out = (T*)a.dq + (((int64_t)b * a.Tq + t) * a.Hq + hq) * D;
-        const float f = a.scale;
+        const float f = a.scale * pow2(-up);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -454,6 +501,7 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
         cur = nxt;
         nxt = nn;
     };
+    int up = !Half<T>::value ? 0 : role ? DS_FROM + P_UP : P_UP;      // the sums are held at 2^up
     // (a loop for each kind of wave, with the same barriers: in one loop the sums were copied where its branches meet)
     if (!role) {
         while (cur.x >= 0) {
@@ -466,7 +514,10 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
             for (int i = 0; i < 4; i++) col(tile + STAGE, i);
             f32x4 L[4];
 #pragma unroll
-            for (int g = 0; g < 4; g++) L[g] = lds4f(lst + slot * 2 * QT * 4 + 32 * g + 16 * h);
+            for (int g = 0; g < 4; g++) {
+                L[g] = lds4f(lst + slot * 2 * QT * 4 + 32 * g + 16 * h);
+                if constexpr (Half<T>::value) L[g] -= (float)P_UP;
+            }
             __builtin_amdgcn_sched_barrier(0);
             scores<CAP>(s, a);
             const float slope = BIAS ? a.slopes[hk * a.R + cur.y] * LOG2E : 0.f, d = (float)(j - t0 - off - 4 * h);
@@ -525,13 +576,28 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
                     dp[e] = p[e >> 2][e & 3] == 0.f ? 0.f : dp[e];
                 }
             }
+            if constexpr (Half<T>::value) {           // (P comes at 2^P_UP)
+                const float mx = max_abs(dp);
+                const int e = lower_by(mx * pow2(up - P_UP));
+                if (__any(e < 0)) {
+                    up += e;
+                    const float g = pow2(e);
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) sum[dt][r] *= g;
+                }
+                const float g = pow2(up - P_UP);
+#pragma unroll
+                for (int r = 0; r < 16; r++) dp[r] *= g;
+            }
             const uint4 y[2] = {pack8<T>(dp, 0), pack8<T>(dp, 1)};
             __builtin_amdgcn_sched_barrier(0);
             add(tile, y);
             leave();
         }
     }
-    const float f = role ? a.scale : 1.f;
+    const float one = role ? a.scale : 1.f, f = one * pow2(-up);
     float bad = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) bad = nonfinite(sum[dt], bad);
@@ -589,7 +655,7 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
                 add_rows<T, D>(o1, d, m, role ? qh + t1 * a.q_st : gh + t1 * a.do_st, role ? a.q_st : a.do_st, te - t1, lane);
             }
         }
-        for (int e = 0; e < D / 64; e++) o1[e] *= f;
+        for (int e = 0; e < D / 64; e++) o1[e] *= one;
         if (a.nsplit > 1) {
             for (int e = 0; e < D / 64; e++) po[i * D + lane * (D / 64) + e] = o1[e];
         } else {
