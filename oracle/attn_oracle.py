@@ -13,7 +13,7 @@ much of itself (times the scale) and dS by that much of P (|dO| |V|^T + delta').
 
 A capped score may be off by 2^-21 of the cap; with `strict` by 2^-20 of itself and no more, however far the cap is.  In fp16 small
 probabilities and dS lose bits, by half a step of 2^-24 each; with `strict` that step counts from the largest dS of a query (for dq) or of a key (for
-dk) at 2^10, P for dv from 1 at 2^14, and delta is off only by what two roundings of the output leave.
+dk) at 2^10, P for dv from 1 at 2^14 and for the output from a row's largest at 2^7, and delta is off only by what two roundings of the output leave.
 """
 import torch
 
@@ -78,6 +78,9 @@ def attention(q, k, v, scale=None, causal=True, window=None, cap=None, slopes=No
     tiny = 2.0 ** -30 if u == 0 else 2.0 ** -25 if half else 0.0
     a = p @ v.abs()
     res = {"out": (out, u * (a + out.abs()) * 1.02 + (p * amp) @ v.abs() + sub * ok.double() @ v.abs() + tiny)}
+    if strict and half:
+        few = 2.0 ** -32 * p.amax(-1, keepdim=True) * ok.double()
+        res["out"] = (out, u * (a + out.abs()) * 1.02 + (p * amp + few) @ v.abs() + tiny)
     if dout is None:
         return res
     g = torch.where(ok.any(-1).expand(B, Hq, Tq).unsqueeze(-1), dout.double(), 0.0)

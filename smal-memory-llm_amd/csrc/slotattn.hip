@@ -22,6 +22,10 @@ using slothost::al16;
 // A row's sums keep their reference maximum until a score passes it by this much (base 2): probabilities then reach 2^8, far
 // from any type's end, and the sums are rescaled a few times a row instead of in most tiles.
 #define LAZY 8.f
+// In fp16 the reference is 2^7 below the maximum, so that probabilities reach 2^7 to 2^15: fp16's smallest step is 2^-24, and below a largest
+// one of 1 those under 2^-25 would add to a row's sum but not to its output (8,192 of them at 2^-26: 1.2e-4 of the values).
+template <typename T> constexpr float HEAD = 0.f;
+template <> constexpr float HEAD<f16_t> = 7.f;
 
 namespace {
 
@@ -175,7 +179,7 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
-            mx = half_max(mx) * F;
+            mx = half_max(mx) * F - HEAD<T>;
             if (__any(mx > m + LAZY)) {
                 const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_(m - mn);
                 m = mn;
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
         float mx = x[0];
 #pragma unroll
         for (int r = 1; r < 16; r++) mx = fmaxf(mx, x[r]);
-        mx = half_max(mx) * F;
+        mx = half_max(mx) * F - HEAD<T>;
         if (__any(mx > m + LAZY)) {
             const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_(m - mn);
             m = mn;

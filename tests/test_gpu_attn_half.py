@@ -56,3 +56,16 @@ def test_gradients_past_the_range_of_scores():
     """dP past fp16's largest number, whose gradients are not."""
     q, k, v, do = attn_inputs(1, 2, 2, 400, 400, 64, HF, 64)
     _check((0.02 * q.float()).to(HF), (0.02 * k.float()).to(HF), (100 * v.float()).to(HF), (500 * do.float()).to(HF))
+
+
+@pytest.mark.parametrize("B,Hq,Hk,Tq,Tk,D", [(1, 2, 1, 3000, 3000, 64), (1, 2, 2, 2500, 2500, 128), (2, 4, 2, 1, 3000, 64), (1, 8, 1, 40, 2000, 128)])
+def test_many_small_probabilities_beside_a_large_one(B, Hq, Hk, Tq, Tk, D):
+    """Keys at 2^-26 of a row's largest probability, thousands of them, whose values are not the largest one's."""
+    print("small probabilities", B, Hq, Hk, Tq, Tk, D, flush=True)
+    q, k, v, do = attn_inputs(B, Hq, Hk, Tq, Tk, D, HF, 65)
+    q, k, v = ((0.25 * x.float()).to(HF) for x in (q, k, v))
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[:, :, 3, 0] = 18.0 * D ** 0.5 / 8.0
+    v = v + 1.0
+    v[:, :, 3] = 0.0
+    _check(q, k, v, do)
