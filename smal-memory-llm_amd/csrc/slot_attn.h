@@ -337,10 +337,11 @@ __device__ __forceinline__ bool bit(uint32_t m, int r) { return (m >> r & 1) != 
 
 // ---- rows next to infinities and NaN -----------------------------------------------------------------------
 // A masked pair has the weight 0 in its product, and 0 times an infinity or a NaN of the other operand is a NaN.  So a row whose
-// sums come out so, though all that it sees is finite, is formed again by its wave, one row at a time, from its visible pairs
-// alone; one that sees such a value keeps its sums.  Where all is finite that costs the tests, about 1 instruction per
-// value of the accumulators; a value seen by every row costs each wave one pass over the keys (8,192 tokens, 12 heads, forward: 2.1 ms),
-// one next to a tile's finite rows these rows one by one (the last token's value: 127 rows a head, 28 ms).
+// sums come out so is formed again by its wave, one row at a time, from its visible pairs alone, unless it sees a value that is not
+// finite and the sums are what that makes of them: no column holds such a value in a masked place only (Ill).  Where all is finite that
+// costs the tests, about 1 instruction per value of the accumulators.  8,192 tokens, 12 heads, forward (0.23 ms): a value that every row
+// sees costs each wave one pass over the keys, 2.0 ms, and 6.5 ms where every value is NaN; one next to a tile's finite rows costs
+// these rows one by one (the last token's value: 127 rows a head, 28 ms).
 __device__ __forceinline__ float nonfinite(const f32x16& x, float t) {            // t + 0 if all of x is finite, else NaN
 #pragma unroll
     for (int r = 0; r < 16; r++) t = fmaf(x[r], 0.f, t);
@@ -408,16 +409,44 @@ template <bool CAP, bool BIAS> __device__ __forceinline__ float score1(float x, 
 __device__ __forceinline__ bool sees1(const Sees& v, int j, const int* ids, int id) {
     return ((unsigned)j - v.first <= v.count || (unsigned)j < v.below) && (!ids || ids[j] == id);
 }
-// Whether the lane's row sees one of keys [lo, hi) whose two rows are not finite.  (In a wave: all lanes.)
-template <typename T, int D>
-__device__ __forceinline__ bool sees_nonfinite(const Sees& v, const int* ids, int id, const T* kb, int64_t k_st, const T* vb, int64_t v_st, int lo, int hi, int lane) {
-    bool hit = false;
+// What became of the lane's row where rows of the other side are not finite: whether it sees one, and, as bits over the columns that
+// are summed (lane D / 64 .. of them per lane), where one that it sees holds a NaN and where one met under a mask alone holds anything not finite.
+template <typename T, int D> struct Ill {
+    static constexpr int N = D / 64;
+    bool hit = false, lost = false;                   // lost: every column is NaN by what the row sees
+    uint64_t nan[N] = {}, odd[N] = {};
+    // row z (of the wave) of the summed operand.  met: its tile was multiplied; copies: and holds it again behind the last row
+    __device__ __forceinline__ void add(const T* z, bool sees, bool met, bool copies, int lane) {
+        hit = hit || sees;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float x = widen1(z[lane * N + i]);
+            const uint64_t n = __ballot(x != x), o = __ballot(!(fabsf(x) < INFINITY));
+            if (sees) nan[i] |= n;
+            if (met && (copies || !sees)) odd[i] |= o;
+        }
+    }
+    // the sums are those of the visible pairs as they are
+    __device__ __forceinline__ bool kept() const {
+        uint64_t x = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) x |= odd[i] & ~nan[i];
+        return lost || (hit && x == 0);
+    }
+};
+// The same for keys [lo, hi), whose two rows both count, in steps of 64: sees(j) for the lane's row, met(j) for the wave, j a key of the step.
+template <typename T, int D, class SEES, class MET>
+__device__ __forceinline__ bool keeps(const T* kb, int64_t k_st, const T* vb, int64_t v_st, const T* zb, int64_t z_st, int lo, int hi, int last, int lane,
+                                      SEES sees, MET met) {
+    Ill<T, D> ill;
     for (int j0 = lo; j0 < hi; j0 += 64) {
         const int j = j0 + lane;
-        for (uint64_t b = __ballot(j < hi && !(finite_row<T, D>(kb + j * k_st) && finite_row<T, D>(vb + j * v_st))); b; b &= b - 1)
-            hit = hit || sees1(v, j0 + __builtin_ctzll(b), ids, id);
+        for (uint64_t b = __ballot(j < hi && !(finite_row<T, D>(kb + j * k_st) && finite_row<T, D>(vb + j * v_st))); b; b &= b - 1) {
+            const int i = j0 + __builtin_ctzll(b);
+            ill.add(zb + i * z_st, sees(i), met(i), i == last, lane);
+        }
     }
-    return hit;
+    return ill.kept();
 }
 // rows of the wave (lanes l and l + 32 have row l) for which x holds, as bits
 __device__ __forceinline__ uint32_t row_bits(bool x) {
@@ -470,6 +499,12 @@ struct Walk {
         const int end = mk.causal ? min(mk.klen, max(sw.p1 + 1, mk.prefix)) : mk.klen;
         nt = (end + KT - 1) / KT;
         base = (mk.prefix > 0 ? 0 : (max(0, max(sw.p0, 0) - mk.W + 1) / KT) & ~63) - 64;
+    }
+    // whether the wave computes tile x (of the wave)
+    __device__ __forceinline__ bool computes(int x) const {
+        const int j0 = x * KT;
+        if (!(sv.p0 <= sv.p1 && mk.some(sv, j0, j0 + KT - 1))) return false;
+        return !range || (range_lo(range[x]) <= sv.hi && sv.lo <= range[x].y);
     }
     // the next visible tile (-1: none), whether this wave's rows see any of it and whether they see all of it
     __device__ __forceinline__ void next(int& jt, bool& some, bool& all) {

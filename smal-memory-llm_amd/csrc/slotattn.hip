@@ -243,8 +243,10 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
     float bad = l * 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) bad = nonfinite(o[dt], bad);
-    uint32_t rows = row_bits(bad != 0.f && t < a.Tq);
-    if (rows) rows &= ~row_bits(sees_nonfinite<T, D>(see, docs ? a.ids + idb : nullptr, dq, kb, a.k_st, vb, a.v_st, 0, mk.klen, lane));
+    uint32_t rows = row_bits(bad != 0.f && l == l && t < a.Tq);       // (a NaN in its sum makes all of a row NaN)
+    if (rows)
+        rows &= ~row_bits(keeps<T, D>(kb, a.k_st, vb, a.v_st, vb, a.v_st, 0, mk.klen, mk.klen % KT ? mk.klen - 1 : -1, lane,
+                                      [&](int j) { return sees1(see, j, docs ? a.ids + idb : nullptr, dq); }, [&](int j) { return walk.computes(j / KT); }));
     for (uint32_t left = rows; left; left &= left - 1) {
         const int i = __builtin_ctz(left), ti = t0 + 32 * w + i;
         float m1, l1, o1[D / 64], rest[D / 64];
@@ -417,7 +419,10 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < SW; i++) left |= s_bad[i];
     if (left) {                                       // the same in every wave
-        left &= ~row_bits(sees_nonfinite<T, D>(see, nullptr, 0, kb, a.k_st, vb, a.v_st, lo, hi, lane));
+        const int last = (klen - lo) % 32 ? klen - 1 : -1;            // keys past hi are in the last tile, too
+        left &= ~row_bits(Ls != Ls || keeps<T, D>(kb, a.k_st, vb, a.v_st, vb, a.v_st, lo, min(klen, lo + (hi - lo + 31) / 32 * 32), last, lane,
+                                                  [&](int j) { return j < hi && sees1(see, j, nullptr, 0); },
+                                                  [&](int j) { const int x = lo + (j - lo) / 32 * 32; return mk.some(s, x, x + 31); }));
         for (; left; left &= left - 1) {
             const int i = __builtin_ctz(left);
             if (i % SW != w) continue;

@@ -287,8 +287,11 @@ __global__ __launch_bounds__(BT * GR, 2) void attn_dq(AttnArgs a) {
     float bad = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) bad = nonfinite(acc[dt], bad);
-    uint32_t rows = row_bits(bad != 0.f && t < a.Tq);
-    if (rows) rows &= ~row_bits(sees_nonfinite<T, D>(see, docs ? a.ids + idb : nullptr, dq, kb, a.k_st, vb, a.v_st, 0, mk.klen, lane));
+    // (a NaN log-sum-exp or, where anything is visible, delta makes all of a row NaN)
+    uint32_t rows = row_bits(bad != 0.f && t < a.Tq && lse == lse && (delta == delta || lse == INFINITY));
+    if (rows)
+        rows &= ~row_bits(keeps<T, D>(kb, a.k_st, vb, a.v_st, kb, a.k_st, 0, mk.klen, mk.klen % KT ? mk.klen - 1 : -1, lane,
+                                      [&](int j) { return sees1(see, j, docs ? a.ids + idb : nullptr, dq); }, [&](int j) { return walk.computes(j / KT); }));
     for (uint32_t left = rows; left; left &= left - 1) {              // (exact_row's, with dS in the place of P)
         const int i = __builtin_ctz(left), ti = t0 + 32 * w + i, pi = ti + off, id = lane_of(dq, i);
         const T* q = (const T*)a.q + b * a.q_sb + hq * a.q_sh + ti * a.q_st;
@@ -411,6 +414,17 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
     const Sees see = Sees::key(mk, j, a.Tk - 1);
     // the walk: heads of the group x query tiles, those of this workgroup's part.  A tile: its number, twice, plus whether every
     // pair of the wave's keys is visible, and its head; -1: none
+    auto queries = [&](int x, bool in) {              // tile x's
+        Span s{x * QT + off, min(x * QT + QT, a.Tq) - 1 + off, 0, 0, true};
+        if (range && in) {
+            const int2 ra = range[s.p0 / KT], rb = range[s.p1 / KT];
+            s.lo = min(range_lo(ra), range_lo(rb));
+            s.hi = max(ra.y, rb.y);
+            s.one = range_one(ra) && range_one(rb) && ra.y == rb.y;
+        }
+        return s;
+    };
+    auto visited = [&](const Span& s) { return mk.some(s, j0, j1) && (!range || (s.lo <= kw.hi && kw.lo <= s.hi)); };
     int r = u0 / nx - 1, base = 0, xe = 0;
     uint64_t act = 0, full = 0;
     auto next = [&]() -> int2 {
@@ -423,14 +437,8 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
             }
             const int x = base + lane;
             const bool in = x < xe;
-            Span s{x * QT + off, min(x * QT + QT, a.Tq) - 1 + off, 0, 0, true};
-            if (range && in) {
-                const int2 ra = range[s.p0 / KT], rb = range[s.p1 / KT];
-                s.lo = min(range_lo(ra), range_lo(rb));
-                s.hi = max(ra.y, rb.y);
-                s.one = range_one(ra) && range_one(rb) && ra.y == rb.y;
-            }
-            act = __ballot(in && mk.some(s, j0, j1) && (!range || (s.lo <= kw.hi && kw.lo <= s.hi)));
+            const Span s = queries(x, in);
+            act = __ballot(in && visited(s));
             full = __ballot(in && x * QT + QT <= a.Tq && mk.all(s, jw, jw + 31) && (!range || (s.one && kv.one && s.lo == kv.lo)));
         }
         const int i = __builtin_ctzll(act);
@@ -535,7 +543,7 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     s[e] = bit(m, e) ? s[e] : 0.f;
-                    g[e] = bit(m, e) ? g[e] : 0.f;
+                    g[e] = bit(m, e) ? g[e] : -INFINITY;              // masked (a weight of 0 is something else)
                 }
             }
             unsigned char* ex = s_ex[n & 1][w] + 16 * lane;
@@ -573,7 +581,7 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     asm volatile("" : "+v"(dp[e]));   // (not ahead of the branch)
-                    dp[e] = p[e >> 2][e & 3] == 0.f ? 0.f : dp[e];
+                    dp[e] = p[e >> 2][e & 3] == -INFINITY ? 0.f : dp[e];
                 }
             }
             if constexpr (Half<T>::value) {           // (P comes at 2^P_UP)
@@ -602,25 +610,32 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) bad = nonfinite(sum[dt], bad);
     uint32_t rows = row_bits(bad != 0.f && j < a.Tk);
-    if (rows) {                                       // keys that see a query with something not finite keep their sums, too
-        bool hit = false;
-        for (int rr = u0 / nx; rr * nx < u1; rr++) {
+    if (rows) {
+        Ill<T, D> ill;
+        auto open = [&]() { return (rows & row_bits(!ill.lost)) != 0; };               // some row is not decided yet
+        for (int rr = u0 / nx; rr * nx < u1 && open(); rr++) {
             const int hq = hk * a.R + rr, te = min(min(x1, u1 - rr * nx) * QT, a.Tq);
             const T* qh = (const T*)a.q + b * a.q_sb + hq * a.q_sh;
             const T* gh = (const T*)a.dout + b * a.do_sb + hq * a.do_sh;
             const int64_t at = ((int64_t)b * a.Hq + hq) * a.Tq;
-            for (int t1 = max(x0, u0 - rr * nx) * QT; t1 < te; t1 += 64) {
+            for (int t1 = max(x0, u0 - rr * nx) * QT; t1 < te && open(); t1 += 64) {
                 const int t = t1 + lane;
-                bool ill = false;
+                bool is = false, gone = false;        // not finite; all of what it adds is NaN
                 if (t < te) {
-                    const float s = a.lse[at + t] * 0.f + (role ? a.delta[at + t] * 0.f : 0.f);   // (an infinite log-sum-exp: a query that sees nothing)
-                    ill = s != s || !finite_row<T, D>(qh + t * a.q_st) || !finite_row<T, D>(gh + t * a.do_st);
+                    const float L = a.lse[at + t], de = role ? a.delta[at + t] : 0.f;
+                    gone = L != L || de != de;
+                    is = gone || !(fabsf(de) < INFINITY) || !finite_row<T, D>(qh + t * a.q_st) || !finite_row<T, D>(gh + t * a.do_st);
                 }
-                for (uint64_t m = __ballot(ill); m; m &= m - 1)
-                    hit = hit || sees1(see, t1 + __builtin_ctzll(m) + off, docs ? a.ids + idb : nullptr, id);
+                const uint64_t all = __ballot(gone);
+                for (uint64_t m = __ballot(is); m; m &= m - 1) {
+                    const int i = __builtin_ctzll(m), ti = t1 + i;
+                    const bool sees = sees1(see, ti + off, docs ? a.ids + idb : nullptr, id);
+                    ill.lost = ill.lost || (sees && (all >> i & 1));
+                    ill.add(role ? qh + ti * a.q_st : gh + ti * a.do_st, sees, visited(queries(ti / QT, true)), ti == a.Tq - 1 && a.Tq % QT, lane);
+                }
             }
         }
-        rows &= ~row_bits(hit);
+        rows &= ~row_bits(ill.kept());
     }
     float* const po = a.part + ((int64_t)(part * a.tiles + jt) * kvh + bh) * 2 * BQ * D + (role ? 0 : BQ * D) + 32 * w * D;
     for (uint32_t left = rows; left; left &= left - 1) {              // a key's sums from the queries that see it, of this part
