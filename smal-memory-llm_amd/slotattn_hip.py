@@ -17,7 +17,7 @@ bf16 or fp16, D in {64, 128}; docs, prefix (B,) and lens (B,) int32, slopes fp32
 fp32; the probabilities and score gradients are rounded to the operands' type for their products.  What a query does not see
 never reaches its row, infinities and NaN included.  Operands may be any views whose rows are contiguous and 16-byte aligned
 (others are copied: a cache should not need that); results and gradients are token-major, seen as (B, H, T, D).  Gradients
-are bitwise reproducible; there is no second derivative.  No CPU path: a missing library raises.
+are bitwise reproducible; there is no second derivative and no forward-mode one.  No CPU path: a missing library raises.
 """
 import torch
 from torch.autograd.function import once_differentiable
@@ -53,6 +53,7 @@ def _check(q, k, v, scale, window, cap, slopes, prefix, what):
             raise ValueError(f"{what}: slopes must be fp32 ({q.shape[1]},) (got {slopes.dtype}, {tuple(slopes.shape)})")
         if slopes.requires_grad:
             raise NotImplementedError(f"{what}: the slopes are constants (no gradient)")
+    L.check_tangents(what, q, k, v, slopes)
     if prefix is not None and (prefix.dtype != torch.int32 or prefix.shape != (q.shape[0],)):
         raise ValueError(f"{what}: prefix must be int32 ({q.shape[0]},) (got {prefix.dtype}, {tuple(prefix.shape)})")
 

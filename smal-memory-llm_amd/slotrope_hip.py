@@ -15,8 +15,9 @@ does to its projected queries and keys before the attention (slotattn_hip, slotw
 
 bf16, fp16 or fp32 rows (q, k, v and the caches alike), D in {64, 128}, 2 len(freqs) a multiple of 16 up to D; freqs are
 float64, so that a far position keeps its angle.  Sums are fp32, results rounded once; the gains' gradients are summed in
-a fixed order.  Operands may be any views whose rows are contiguous and 16-byte aligned, such as slices of one fused
-projection (others are copied); results are token-major, seen as (B, H, T, D).  No CPU path: a missing library raises.
+a fixed order; there is no second derivative and no forward-mode one.  Operands may be any views whose rows are contiguous
+and 16-byte aligned, such as slices of one fused projection (others are copied); results are token-major, seen as
+(B, H, T, D).  No CPU path: a missing library raises.
 """
 import torch
 from torch.autograd.function import once_differentiable
@@ -50,6 +51,7 @@ def _check(q, k, wq, wk, freqs, what):
     for w in (wq, wk):
         if w is not None and (w.shape != (D,) or w.dtype not in L._TYPE_CODES):
             raise ValueError(f"{what}: a gain must be ({D},), bf16, fp16 or fp32 (got {tuple(w.shape)}, {w.dtype})")
+    L.check_tangents(what, q, k, wq, wk, freqs)
 
 
 def _same_device(what, *ts):
@@ -179,6 +181,7 @@ def qk_rope_cache(q, k, v, wq, wk, freqs, lens, kcache, vcache, eps=1e-6, interl
         raise ValueError(f"{what}: v must have k's shape and type (got {tuple(v.shape)}, {v.dtype})")
     check_caches(kcache, vcache, q, Hk, what)
     check_lens(lens, B, what)
+    L.check_tangents(what, v, kcache, vcache)
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, wq, wk, kcache, vcache)):
         raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
     for c in (kcache, vcache):

@@ -12,6 +12,7 @@ import ctypes
 import os
 
 import torch  # noqa: F401  -- must precede the CDLL below (shared HIP runtime)
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libslotscan.so")
@@ -159,6 +160,12 @@ def strided(x):
 def on(device):
     """Makes `device` the current one around a launch (a no-op where it is)."""
     return torch.cuda.device(device if device.index != torch.cuda.current_device() else -1)
+
+
+def check_tangents(what, *xs):
+    """Refuses a dual tensor: a kernel launched on its pointer would drop the tangent."""
+    if forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in xs):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 KERNEL_NAMES = ("chain_fwd", "rows_fwd", "rows_bwd", "chain_bwd", "reduce_parts", "read_fwd", "read_bwd", "mem_fwd",
