@@ -199,4 +199,7 @@ def qk_rope_cache(q, k, v, wq, wk, freqs, lens, kcache, vcache, eps=1e-6, interl
                                         kcache.shape[2], float(eps), L.ptr(qo), *L.strided(kcache), *L.strided(vcache),
                                         L.stream_of(q.device))
         L.check(rc, what)
+        written = [c for c in (kcache, vcache) if not c.is_inference()]               # (those have no version)
+        if written:
+            torch.autograd.graph.increment_version(written)
     return qo.transpose(1, 2)
