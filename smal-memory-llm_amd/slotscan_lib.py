@@ -135,25 +135,31 @@ def dtype_code(dt):
 _TYPE_CODES = {torch.float32: SLOTSCAN_F32, torch.bfloat16: SLOTSCAN_BF16, torch.float16: SLOTSCAN_F16}
 
 
+def _strides(x):
+    """Strides of batch, head, token and row; 0 for the first three where the dimension has size 1: torch leaves odd ones there,
+    and none of them matters."""
+    s = x.stride()
+    if (s[0] | s[1] | s[2]) % 8 or s[2] >= 1 << 25:
+        s = (*(a if n > 1 else 0 for a, n in zip(s[:3], x.shape)), s[3])
+    return s
+
+
 def in_place(x):
     """Whether x (batch, head, token, D) is as the kernels read it: D values of a row contiguous, every row 16-byte aligned and
     tokens fewer than 2^25 elements apart."""
     n = 16 // x.element_size()
-    s = x.stride()
+    s = _strides(x)
     return s[3] == 1 and not (s[0] % n or s[1] % n or s[2] % n) and s[2] < 1 << 25 and not x.data_ptr() % 16
 
 
 def rows(x):
     """x as the kernels read it (in_place), itself or a copy."""
-    if in_place(x):
-        return x
-    x = x.contiguous()
-    return x.clone(memory_format=torch.contiguous_format) if x.data_ptr() % 16 else x
+    return x if in_place(x) else x.clone(memory_format=torch.contiguous_format)
 
 
 def strided(x):
     """Pointer and strides (batch, head, token) of rows(x), as the entry points take them."""
-    s = x.stride()
+    s = _strides(x)
     return x.data_ptr(), s[0], s[1], s[2]
 
 

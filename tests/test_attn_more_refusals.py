@@ -40,3 +40,33 @@ def test_forward_mode_derivatives(which, at):
         xs[which] = forward_ad.make_dual(xs[which], torch.ones_like(xs[which]))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             _calls(*xs)[at]()
+
+
+def _views():
+    """Views whose dimensions of size 1 have strides of their own, and the rows' alignment (elements) of each."""
+    wide = torch.arange(4 * 644, dtype=torch.float32).to(BF).view(4, 644)
+    yield wide[:, :640].unflatten(1, (2, 5, 64)).split(1)[0]                          # one sequence of rows of 644
+    yield wide[:1, :640].view(1, 5, 2, 64).transpose(1, 2)
+    yield torch.arange(5 * 2 * 3 * 65.0).to(BF).as_strided((2, 1, 5, 64), (960, 3, 64, 1))
+    yield torch.arange(4096.0).to(BF).as_strided((2, 3, 1, 64), (640, 64, 1 << 26, 1))  # one token, far from the next
+    yield torch.arange(4096.0).to(BF).as_strided((1, 1, 1, 64), (7, 5, 3, 1))
+
+
+@pytest.mark.parametrize("i", range(5))
+def test_strides_of_single_items_do_not_matter(i):
+    """A dimension of size 1 has no stride that could be odd: the rows are read where they are."""
+    x = list(_views())[i]
+    y = L.rows(x)
+    p, *s = L.strided(y)
+    assert p % 16 == 0 and all(v % 8 == 0 and 0 <= v < 1 << 25 for v in s), s
+    flat = y.as_strided((y.shape[0], y.shape[1], y.shape[2], 64), (*s, 1))
+    assert torch.equal(flat, x)
+    if x.data_ptr() % 16 == 0:
+        assert L.in_place(x) and y is x
+
+
+@pytest.mark.parametrize("x", [z(2, 2, 5, 65)[..., :64], z(2 * 2 * 5 * 64 + 1)[1:].view(2, 2, 5, 64), z(2, 2, 64, 5).transpose(2, 3),
+                               z(1, 2, 5, 64).expand(3, 2, 5, 64), z(2, 5, 2, 64).transpose(1, 2), z(3, 2, 8, 64)[:, :, ::2], z(2, 2, 5, 1).expand(2, 2, 5, 64)])
+def test_rows_are_aligned(x):
+    y = L.rows(x)
+    assert L.in_place(y) and torch.equal(x, y)
