@@ -51,7 +51,7 @@ def _check(q, k, v, scale, window, cap, slopes, prefix, what):
     if slopes is not None:
         if slopes.shape != (q.shape[1],) or slopes.dtype != torch.float32:
             raise ValueError(f"{what}: slopes must be fp32 ({q.shape[1]},) (got {slopes.dtype}, {tuple(slopes.shape)})")
-        if slopes.requires_grad:
+        if slopes.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError(f"{what}: the slopes are constants (no gradient)")
     L.check_tangents(what, q, k, v, slopes)
     if prefix is not None and (prefix.dtype != torch.int32 or prefix.shape != (q.shape[0],)):

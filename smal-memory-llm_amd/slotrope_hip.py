@@ -46,7 +46,7 @@ def _check(q, k, wq, wk, freqs, what):
         raise ValueError(f"{what}: freqs must be a float64 vector (got {freqs.dtype}, {tuple(freqs.shape)})")
     if freqs.numel() % 8 or 2 * freqs.numel() > D:
         raise NotImplementedError(f"{what} rotates a multiple of 16 values, at most D (got 2 x {freqs.numel()})")
-    if freqs.requires_grad:
+    if freqs.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{what}: the frequencies are constants")
     for w in (wq, wk):
         if w is not None and (w.shape != (D,) or w.dtype not in L._TYPE_CODES):

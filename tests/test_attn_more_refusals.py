@@ -70,3 +70,16 @@ def test_strides_of_single_items_do_not_matter(i):
 def test_rows_are_aligned(x):
     y = L.rows(x)
     assert L.in_place(y) and torch.equal(x, y)
+
+
+def test_constants_may_ask_for_gradients_where_none_are_formed():
+    """Slopes and frequencies are constants: refused where autograd is on and would miss them, and only there."""
+    q, k, n = z(2, 4, 3, 64), z(2, 2, 3, 64), torch.tensor([3, 3], dtype=torch.int32)
+    s, fr = z(4, dt=torch.float32).requires_grad_(), R.frequencies(64).requires_grad_()
+    calls = [lambda: A.attend(q, k, k, slopes=s), lambda: A.attend_cache(q, k, k, n, slopes=s), lambda: R.qk_rope(q, k, None, None, fr),
+             lambda: R.qk_rope_cache(q, k, k, None, None, fr, n, z(2, 2, 9, 64), z(2, 2, 9, 64))]
+    for f in calls:
+        with pytest.raises((NotImplementedError, RuntimeError), match="constants|no backward"):
+            f()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU tensors only"):
+            f()
