@@ -10,7 +10,7 @@ does to its projected queries and keys before the attention (slotattn_hip, slotw
         the serving form, forward only: the T tokens are the newest of lens[b] (int32 (B,), the new ones included), token
         t at position lens[b] - T + t; the prepared keys and the values are written into rows `position` of kcache, vcache
         (B, Hk, S, D), everything else in them stays.  A token of negative position (a batch padded on the left) or of
-        one past the cache writes nothing.
+        one past the cache writes nothing.  The caches share no memory with each other or with the operands.
     frequencies(rot, theta=10000.0, device=None) -> (rot / 2,) float64: theta^(-2 i / rot)
 
 bf16, fp16 or fp32 rows (q, k, v and the caches alike), D in {64, 128}, 2 len(freqs) a multiple of 16 up to D; freqs are
@@ -156,14 +156,27 @@ def check_caches(kcache, vcache, like, Hk, what):
         raise NotImplementedError(f"{what}: the caches must have the queries' type {like.dtype} (got {kcache.dtype}, {vcache.dtype})")
 
 
-def _apart(c):
-    """Whether no two rows of c (B, H, S, D) share memory: every dimension steps over all that the closer ones reach."""
+def _apart(c, steps=()):
+    """Whether no two rows of c (B, H, S, D) share memory: every dimension steps over all that the closer ones reach.  steps:
+    further dimensions, as (stride, size)."""
     reach = c.size(3)
-    for st, n in sorted((c.stride(i), c.size(i)) for i in range(3) if c.size(i) > 1):
+    for st, n in sorted([(c.stride(i), c.size(i)) for i in range(3) if c.size(i) > 1] + list(steps)):
         if st < reach:
             return False
         reach += st * (n - 1)
     return True
+
+
+def _overlap(a, b):
+    """Whether two caches of one shape share memory.  Where the memory that they reach over does not meet they do not; where it does
+    they may lie side by side, as two parts of one buffer with the same strides; anything else counts as sharing."""
+    d, n, st, size = b.data_ptr() - a.data_ptr(), a.element_size(), a.stride(), a.shape
+    if d < 0:
+        return _overlap(b, a)
+    if d >= n * (1 + (size[0] - 1) * st[0] + (size[1] - 1) * st[1] + (size[2] - 1) * st[2] + (size[3] - 1) * st[3]) or not a.numel():
+        return False
+    same = all(st[i] == b.stride(i) for i in range(3) if size[i] > 1)
+    return not (same and d % n == 0 and _apart(a, [(d // n, 2)]))
 
 
 def check_lens(lens, B, what):
@@ -187,6 +200,8 @@ def qk_rope_cache(q, k, v, wq, wk, freqs, lens, kcache, vcache, eps=1e-6, interl
     for c in (kcache, vcache):
         if not _apart(c) or not L.in_place(c):
             raise ValueError(f"{what}: a cache is written in place: its rows must be contiguous, 16-byte aligned and apart")
+    if _overlap(kcache, vcache):
+        raise ValueError(f"{what}: the two caches share memory")
     _same_device(what, q, k, v, wq, wk, freqs, lens, kcache, vcache)
     q_, k_, v_ = L.rows(q), L.rows(k), L.rows(v)
     wq_, wk_, wt = _gains(wq, wk)

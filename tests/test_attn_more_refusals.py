@@ -83,3 +83,28 @@ def test_constants_may_ask_for_gradients_where_none_are_formed():
             f()
         with torch.no_grad(), pytest.raises(RuntimeError, match="GPU tensors only"):
             f()
+
+
+def _pair(a, b):
+    q, n = z(2, 4, 3, 64), torch.tensor([3, 3], dtype=torch.int32)
+    with torch.no_grad():
+        R.qk_rope_cache(q, a[:, :, :3].contiguous(), a[:, :, :3].contiguous(), None, None, R.frequencies(64), n, a, b)
+
+
+@pytest.mark.parametrize("kind", range(5))
+def test_caches_that_share_memory_with_each_other(kind):
+    buf = z(2, 2, 12, 64)
+    far = z(2 * 2 * 9 * 128)
+    a, b = [(buf, buf), (buf[:, :, :9], buf[:, :, 3:]), (buf[:, :, :9], buf[:, :, 1:10]),
+            (far.as_strided((2, 2, 9, 64), (2304, 1152, 128, 1)), far.as_strided((2, 2, 9, 64), (2304, 1152, 128, 1), 32)),
+            (far.as_strided((2, 2, 9, 64), (2304, 1152, 128, 1)), far.as_strided((2, 2, 9, 64), (1152, 576, 64, 1)))][kind]
+    with pytest.raises(ValueError, match="share memory"):
+        _pair(a, b)
+
+
+@pytest.mark.parametrize("kind", range(6))
+def test_caches_side_by_side_in_one_buffer(kind):
+    a, b = [z(2, 2, 2, 9, 64).unbind(0), z(2, 2, 2, 9, 64).unbind(1), z(2, 2, 2, 9, 64).unbind(2), z(2, 9, 2, 2, 64).transpose(1, 3).unbind(2),
+            z(2, 9, 2, 128).transpose(1, 2).split(64, 3), (z(2, 2, 18, 64)[:, :, :9], z(2, 2, 18, 64)[:, :, 9:])][kind]
+    with pytest.raises(RuntimeError, match="GPU tensors only"):       # taken, as far as a CPU tensor is
+        _pair(a, b)
