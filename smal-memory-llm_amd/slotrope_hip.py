@@ -159,11 +159,13 @@ def check_caches(kcache, vcache, like, Hk, what):
 def _apart(c, steps=()):
     """Whether no two rows of c (B, H, S, D) share memory: every dimension steps over all that the closer ones reach.  steps:
     further dimensions, as (stride, size)."""
-    reach = c.size(3)
-    for st, n in sorted([(c.stride(i), c.size(i)) for i in range(3) if c.size(i) > 1] + list(steps)):
-        if st < reach:
-            return False
-        reach += st * (n - 1)
+    st, size = c.stride(), c.shape
+    reach = size[3]
+    for s, n in sorted([(st[0], size[0]), (st[1], size[1]), (st[2], size[2]), *steps]):
+        if n > 1:
+            if s < reach:
+                return False
+            reach += s * (n - 1)
     return True
 
 
