@@ -787,8 +787,8 @@ extern "C" int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q
     if (int r = slotattn_host::check(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, dtype, B, Tq, Tk, Hq, Hk, D, scale, window, cap)) return r;
     if (Tq > Tk) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: more queries than keys");
     if (!out || !res || !lse || !dout || !delta || !dq || !dk || !dv) return fail(SLOTSCAN_ERR_NULL, "slotattn_bwd: a required pointer is NULL");
-    if (!al16(out) || !al16(res) || !al16(dout) || !al16(dq) || !al16(dk) || !al16(dv) || !al16(docs) || (do_sb | do_sh | do_st) % 8)
-        return fail(SLOTSCAN_ERR_ALIGN, "slotattn_bwd: rows of out, res, dout, dq, dk and dv, and docs, must be 16-byte aligned");
+    if (!al16(out) || !al16(res) || !al16(dout) || !al16(dq) || !al16(dk) || !al16(dv) || !al16(docs) || !al16(workspace) || (do_sb | do_sh | do_st) % 8)
+        return fail(SLOTSCAN_ERR_ALIGN, "slotattn_bwd: rows of out, res, dout, dq, dk and dv, docs and the workspace must be 16-byte aligned");
     if (do_st < 0 || do_st >= SLOTATTN_MAX_ST) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: token strides must be in [0, 2^25)");
     if ((Tq + BQ - 1) / BQ * B * Hq > 0x7fffffffLL || (Tk + BQ - 1) / BQ * B * Hk > 0x7fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_bwd: shape too large");
     AttnArgs a = slotattn_host::args(q, q_sb, q_sh, q_st, k, k_sb, k_sh, k_st, v, v_sb, v_sh, v_st, B, Tq, Tk, Hq, Hk, scale, causal, window, cap,

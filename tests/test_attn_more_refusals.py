@@ -108,3 +108,10 @@ def test_caches_side_by_side_in_one_buffer(kind):
             z(2, 9, 2, 128).transpose(1, 2).split(64, 3), (z(2, 2, 18, 64)[:, :, :9], z(2, 2, 18, 64)[:, :, 9:])][kind]
     with pytest.raises(RuntimeError, match="GPU tensors only"):       # taken, as far as a CPU tensor is
         _pair(a, b)
+
+
+@pytest.mark.parametrize("at", [4, 8])
+def test_workspace_of_the_backward_is_aligned(at):
+    s = (512, 64, 128)
+    assert L.lib().slotattn_bwd(P, *s, P, *s, P, *s, 1, 1, 4, 4, 2, 2, 64, 0.1, 1, 5, 0.0, None, None, None, P, P, P, P, *s, P + at, P, P, P, P,
+                                None) == 4
