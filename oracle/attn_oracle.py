@@ -13,7 +13,7 @@ much of itself (times the scale) and dS by that much of P (|dO| |V|^T + delta').
 
 A capped score may be off by 2^-21 of the cap; with `strict` by 2^-20 of itself and no more, however far the cap is.  In fp16 small
 probabilities and dS lose bits, by half a step of 2^-24 each; with `strict` that step counts from the largest dS of a query (for dq) or of a key (for
-dk) at 2^10, P for dv from 1 at 2^14 and for the output from a row's largest at 2^7, and delta is off only by what two roundings of the output leave.
+dk) at 2^10, P for dv from 1 at 2^14 and for the output from a row's largest at 2^7, and delta is off by what the probabilities' rounding does to the output and its own two roundings leave.
 """
 import torch
 
@@ -67,7 +67,7 @@ def attention(q, k, v, scale=None, causal=True, window=None, cap=None, slopes=No
     f = D * 2.0 ** -24
     # how far a probability may be off, relative: its score's absolute sum, the exponential's argument (2^-23 of it), both for
     # the score and for the row's log-sum-exp; and what the cap's tanh is off by
-    amp = f * scale * (q.abs() @ k.abs().transpose(-1, -2)) + 2.0 ** -21 * torch.where(ok, s, 0.0).abs() + tanh_err
+    amp = f * (abs(scale) if strict else scale) * (q.abs() @ k.abs().transpose(-1, -2)) + 2.0 ** -21 * torch.where(ok, s, 0.0).abs() + tanh_err
     if strict and cap:                                   # a capped score is off by the cap's range at most
         amp = amp.clamp_max(2.0 * cap)
     amp = torch.where(ok, amp, 0.0)
@@ -104,7 +104,8 @@ def attention(q, k, v, scale=None, causal=True, window=None, cap=None, slopes=No
     if strict:
         step = 2.0 ** -25 if half else 0.0
         d = ok.double()
-        e0 = u * 1.02 * ds.abs() + p * (2 * u * u * d1 + step * g.abs().sum(-1, keepdim=True)
+        # delta is formed from the output, in which each probability was rounded: off by u sum_j p_j |dp_j|
+        e0 = u * 1.02 * (ds.abs() + p * (p * dp.abs()).sum(-1, keepdim=True)) + p * (2 * u * u * d1 + step * g.abs().sum(-1, keepdim=True)
                                         + f * (pa + d1) + (amp + (2 * amp / cap if cap else 0.0)) * (dp.abs() + d1))
         at = lambda dim: step * 2.0 ** -10 * d * ds.abs().amax(dim, keepdim=True)
         res["dq"] = (dq, sc * ((e0 + at(-1)) @ k.abs()) + u * dq.abs() * 1.02 + tiny)
