@@ -420,9 +420,10 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
     for (int i = 0; i < SW; i++) left |= s_bad[i];
     if (left) {                                       // the same in every wave
         const int last = (klen - lo) % 32 ? klen - 1 : -1;            // keys past hi are in the last tile, too
-        left &= ~row_bits(Ls != Ls || keeps<T, D>(kb, a.k_st, vb, a.v_st, vb, a.v_st, lo, min(klen, lo + (hi - lo + 31) / 32 * 32), last, lane,
-                                                  [&](int j) { return j < hi && sees1(see, j, nullptr, 0); },
-                                                  [&](int j) { const int x = lo + (j - lo) / 32 * 32; return mk.some(s, x, x + 31); }));
+        const bool kept = keeps<T, D>(kb, a.k_st, vb, a.v_st, vb, a.v_st, lo, min(klen, lo + (hi - lo + 31) / 32 * 32), last, lane,
+                                      [&](int j) { return j < hi && sees1(see, j, nullptr, 0); },
+                                      [&](int j) { const int x = lo + (j - lo) / 32 * 32; return mk.some(s, x, x + 31); });      // (by all lanes)
+        left &= ~row_bits(kept || Ls != Ls);
         for (; left; left &= left - 1) {
             const int i = __builtin_ctz(left);
             if (i % SW != w) continue;

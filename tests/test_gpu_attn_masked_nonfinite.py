@@ -133,3 +133,23 @@ def test_every_place_of_a_cache(places, B, Hq, Hk, Tq, Tk, D, dt, lens, opt):
         out = A.attend_cache(q.cuda(), k.cuda(), v.cuda(), n.cuda(), **{m: x.cuda() if torch.is_tensor(x) else x for m, x in o.items()})
     for b in range(B):
         _same(out[b], *_reference(q, k, v, None, ok[b], b, U[dt])["out"], "out")
+
+
+@pytest.mark.parametrize("Tq,Tk,D,dt,opt", [(5, 5, 64, BF, {}), (2, 900, 128, HF, {}), (40, 170, 64, BF, dict(window=30)), (9, 33, 128, HF, dict(prefix=7))])
+def test_rows_beside_rows_that_are_lost(Tq, Tk, D, dt, opt):
+    """Queries that are NaN, and keys that make a later row NaN, beside rows that keep a finite part."""
+    print("lost rows", Tq, Tk, D, opt, flush=True)
+    q, k, v, do = _poisoned([("v", Tk - Tq, 3, NAN), ("v", -1, 5, INF), ("v", -1, 2, -INF)], attn_inputs(2, 2, 1, Tq, Tk, D, dt, 53))
+    q[0, 0, Tq - 2, 7] = NAN
+    k[1, :, Tk - 2, 7] = NAN
+    o = dict(opt)
+    if "prefix" in o:
+        o["prefix"] = torch.full((2,), o["prefix"], dtype=torch.int32)
+    ok, _ = AO.visible(2, Tq, Tk, **o)
+    leaves = [x.cuda().requires_grad_() for x in (q, k, v)]
+    out = A.attend(*leaves, **{m: x.cuda() if torch.is_tensor(x) else x for m, x in o.items()})
+    got = dict(zip(("out", "dq", "dk", "dv"), [out, *torch.autograd.grad(out, leaves, do.cuda())]))
+    for b in range(2):
+        ref = _reference(q, k, v, do, ok[b % len(ok)], b, U[dt])
+        for n, x in got.items():
+            _same(x[b], *ref[n], n)
