@@ -135,11 +135,12 @@ def test_every_place_of_a_cache(places, B, Hq, Hk, Tq, Tk, D, dt, lens, opt):
         _same(out[b], *_reference(q, k, v, None, ok[b], b, U[dt])["out"], "out")
 
 
-@pytest.mark.parametrize("Tq,Tk,D,dt,opt", [(5, 5, 64, BF, {}), (2, 900, 128, HF, {}), (40, 170, 64, BF, dict(window=30)), (9, 33, 128, HF, dict(prefix=7))])
+@pytest.mark.parametrize("Tq,Tk,D,dt,opt", [(5, 5, 64, BF, {}), (2, 898, 128, HF, {}), (9, 73, 128, HF, dict(prefix=7)), (20, 1044, 64, BF, {}), (150, 150, 128, BF, {})])
 def test_rows_beside_rows_that_are_lost(Tq, Tk, D, dt, opt):
-    """Queries that are NaN, and keys that make a later row NaN, beside rows that keep a finite part."""
+    """A query that is NaN, or a key that makes the later rows NaN, beside rows that keep a finite part; and a value that those do not
+    see at the key of the lost query's place in its tile."""
     print("lost rows", Tq, Tk, D, opt, flush=True)
-    q, k, v, do = _poisoned([("v", Tk - Tq, 3, NAN), ("v", -1, 5, INF), ("v", -1, 2, -INF)], attn_inputs(2, 2, 1, Tq, Tk, D, dt, 53))
+    q, k, v, do = _poisoned([("v", Tk - Tq, 3, NAN), ("v", -2, 5, INF), ("v", -2, 2, -INF)], attn_inputs(2, 1, 1, Tq, Tk, D, dt, 53))
     q[0, 0, Tq - 2, 7] = NAN
     k[1, :, Tk - 2, 7] = NAN
     o = dict(opt)
