@@ -22,6 +22,9 @@ using slothost::al16;
 // A row's sums keep their reference maximum until a score passes it by this much (base 2): probabilities then reach 2^8, far
 // from any type's end, and the sums are rescaled a few times a row instead of in most tiles.
 #define LAZY 8.f
+// Scores are taken to base 2 and from their reference by one multiply-add.  The reference's own product is rounded, which moves a row's
+// probabilities by a common factor of up to 2^(|reference| 2^-24): nothing, until scores of millions.  From FAR on the difference is formed first.
+#define FAR 4194304.f
 // In fp16 the reference is 2^7 below the maximum, so that probabilities reach 2^7 to 2^15: fp16's smallest step is 2^-24, and below a largest
 // one of 1 those under 2^-25 would add to a row's sum but not to its output (8,192 of them at 2^-26: 1.2e-4 of the values).
 template <typename T> constexpr float HEAD = 0.f;
@@ -106,7 +109,9 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) o[dt] = zero16();
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, mu = 0.f, l = 0.f;           // a row's reference, the same in base 2, its sum
+    const float lazy = LAZY / F, head = HEAD<T> / F;
+    bool far = false;
     // this group's next tile, and whether any group has one
     auto next = [&](int& jt, bool& some, bool& all) -> bool {
         walk.next(jt, some, all);
@@ -179,23 +184,35 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
-            mx = half_max(mx) * F - HEAD<T>;
-            if (__any(mx > m + LAZY)) {
-                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_(m - mn);
+            mx = half_max(mx) - head;
+            if (__any(mx > m + lazy)) {
+                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_((m - mn) * F);
                 m = mn;
+                mu = m == -INFINITY ? 0.f : m * F;
+                far = __any(fabsf(mu) > FAR);
                 l *= f;
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++)
 #pragma unroll
                     for (int r = 0; r < 16; r++) o[dt][r] *= f;
             }
-            const float mu = m == -INFINITY ? 0.f : m;
+            if (far) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[u][r] = (s[u][r] - (m == -INFINITY ? 0.f : m)) * F;
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[u][r] = fmaf(s[u][r], F, -mu);
+            }
             uint4 pf[2][2];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    s[u][r] = exp2_(fmaf(s[u][r], F, -mu));
+                    s[u][r] = exp2_(s[u][r]);
                     l += s[u][r];
                 }
                 pf[u][0] = pack8<T>(s[u], 0);
@@ -210,6 +227,7 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
         }
     }
     l = half_sum(l);
+    m = m == -INFINITY ? m : mu;                      // in base 2 from here on
     if constexpr (GR == 2) {
         float4* so = reinterpret_cast<float4*>(smem);                 // [4 DT][thread], then the rows' maxima and sums
         float* sm = reinterpret_cast<float*>(so + 4 * DT * FT);
@@ -331,7 +349,9 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) o[dt] = zero16();
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, mu = 0.f, l = 0.f;           // a row's reference, the same in base 2, its sum
+    const float lazy = LAZY / F, head = HEAD<T> / F;
+    bool far = false;
     // Keys and values are fetched two tiles ahead, each into the place that it has just been read from: a wave has one and a
     // half to two tiles (24 to 32 KB at D = 128) on their way while it computes.
     int j1 = j0 < hi ? seen(j0 + 32 * SW) : hi;
@@ -357,20 +377,28 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
         float mx = x[0];
 #pragma unroll
         for (int r = 1; r < 16; r++) mx = fmaxf(mx, x[r]);
-        mx = half_max(mx) * F - HEAD<T>;
-        if (__any(mx > m + LAZY)) {
-            const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_(m - mn);
+        mx = half_max(mx) - head;
+        if (__any(mx > m + lazy)) {
+            const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_((m - mn) * F);
             m = mn;
+            mu = m == -INFINITY ? 0.f : m * F;
+            far = __any(fabsf(mu) > FAR);
             l *= f;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[dt][r] *= f;
         }
-        const float mu = m == -INFINITY ? 0.f : m;
+        if (far) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) x[r] = (x[r] - (m == -INFINITY ? 0.f : m)) * F;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; r++) x[r] = fmaf(x[r], F, -mu);
+        }
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-            x[r] = exp2_(fmaf(x[r], F, -mu));
+            x[r] = exp2_(x[r]);
             l += x[r];
         }
         const uint4 pf[2] = {pack8<T>(x, 0), pack8<T>(x, 1)};
@@ -389,6 +417,7 @@ __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {
         j1 = j2;
     }
     l = half_sum(l);
+    m = m == -INFINITY ? m : mu;                      // in base 2 from here on
     // the waves' parts: (m, l) of every row to all, then the weighted sums through LDS (its tiles are read)
     if (h == 0) { s_m[w][lane] = m; s_l[w][lane] = l; }
     __syncthreads();

@@ -6,18 +6,21 @@ are not enough -- packed documents, long windows, prompts read both ways, capped
         queries are the last Tq <= Tk of the keys' positions.  For query position i and key j:
             s = scale <q, k>  (default 1 / sqrt(D));   cap: s = cap tanh(s / cap);   slopes (Hq,): s -= slopes[h] |i - j|
         then the softmax over the visible keys: 0 <= i - j < window (causal) or |i - j| < window (not; None: no bound), and
-        whatever the band says the first prefix[b] keys; with docs (B, Tk) only keys of the query's own document, a negative
-        id being padding.  A query that sees nothing gets 0.  Autograd gives dq, dk, dv; slopes are constants.
+        whatever the band says the first prefix[b] keys of the row; with docs (B, Tk) of all these only keys of the query's
+        own document (so that a prefix reaches the row's first documents alone), a negative id being padding.  A query that
+        sees nothing, or scores of -inf alone, gets 0.  Autograd gives dq, dk, dv; slopes are constants.
     attend_cache(q, kcache, vcache, lens, scale=None, window=None, cap=None, slopes=None, prefix=None) -> (B, Hq, T, D)
         the serving form, forward only and causal: q holds the newest T of each sequence's lens[b] tokens, whose keys and
         values (the new ones included) are the first lens[b] rows of kcache, vcache (B, Hk, S, D).  What lies behind them
         is not read.  A query of negative position (lens[b] < T) gets 0.
 
 bf16 or fp16, D in {64, 128}; docs, prefix (B,) and lens (B,) int32, slopes fp32.  Scores, softmax statistics and sums are
-fp32; the probabilities and score gradients are rounded to the operands' type for their products.  What a query does not see
-never reaches its row, infinities and NaN included.  Operands may be any views whose rows are contiguous and 16-byte aligned
-(others are copied: a cache should not need that); results and gradients are token-major, seen as (B, H, T, D).  Gradients
-are bitwise reproducible; there is no second derivative and no forward-mode one.  No CPU path: a missing library raises.
+fp32; the probabilities and score gradients are rounded to the operands' type for their products.  The gradients take the
+probabilities from the rows' fp32 log-sum-exp, which moves them by about 2^-24 of the row's largest score (fine for scores
+up to tens of thousands, no longer for millions).  What a query does not see never reaches its row, infinities and NaN
+included.  Operands may be any views whose rows are contiguous and 16-byte aligned (others are copied: a cache should not
+need that); results and gradients are token-major, seen as (B, H, T, D).  Gradients are bitwise reproducible; there is no
+second derivative and no forward-mode one.  No CPU path: a missing library raises.
 """
 import torch
 from torch.autograd.function import once_differentiable

@@ -61,3 +61,29 @@ def test_ends_of_the_range(cap, scale):
     out = A.attend(q.cuda(), k.cuda(), v.cuda(), cap=cap, scale=scale)
     assert bool(out.isfinite().all())
     near(out, *ref, "out")
+
+
+def _whole(B, Hq, Hk, Tq, Tk, D, dt, seed):
+    """Queries and keys of small whole numbers: their products are exact, the largest ones often met several times."""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda h, t: torch.randint(-2, 3, (B, h, t, D), generator=g).to(dt)
+    return r(Hq, Tq), r(Hk, Tk), torch.randn(B, Hk, Tk, D, generator=g).to(dt)
+
+
+@pytest.mark.parametrize("scale", [1e4, 1e7, 3e8, 1e12, -1e20, 1e27])
+@pytest.mark.parametrize("B,Hq,Hk,Tq,Tk,D,dt,lens,opt", [
+    (1, 2, 1, 150, 150, 64, BF, None, {}), (70, 4, 2, 140, 140, 64, HF, None, dict(window=60)), (2, 2, 2, 130, 130, 128, HF, None, {}),
+    (2, 8, 2, 1, 900, 128, BF, (900, 333), {}), (1, 4, 4, 3, 5000, 64, HF, (4800,), {}), (1, 2, 2, 70, 70, 64, BF, None, dict(cap=1e30))])
+def test_scores_of_any_size(scale, B, Hq, Hk, Tq, Tk, D, dt, lens, opt):
+    """Scores far past the range in which a 32-bit number resolves their differences: the largest share the weight.  The scores are
+    exact, so the bounds are the probabilities' rounding and the result's alone."""
+    print("far scores", scale, B, Hq, Hk, Tq, Tk, D, flush=True)
+    if "cap" in opt and scale < 0:
+        scale = -scale
+    q, k, v = _whole(B, Hq, Hk, Tq, Tk, D, dt, 75)
+    n = None if lens is None else torch.tensor(lens, dtype=torch.int32)
+    with torch.no_grad():
+        x = [y.cuda() for y in (q, k, v)]
+        out = A.attend(*x, scale=scale, **opt) if n is None else A.attend_cache(*x, n.cuda(), scale=scale, **opt)
+    want, size = (AO.attention(q, k, y, lens=n, scale=scale, window=opt.get("window"))["out"][0] for y in (v, v.abs()))
+    near(out, want, 1.02 * U[dt] * (size + want.abs()) + 2.0 ** -20, "out")
