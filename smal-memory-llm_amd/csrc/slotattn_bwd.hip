@@ -414,17 +414,6 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
     const Sees see = Sees::key(mk, j, a.Tk - 1);
     // the walk: heads of the group x query tiles, those of this workgroup's part.  A tile: its number, twice, plus whether every
     // pair of the wave's keys is visible, and its head; -1: none
-    auto queries = [&](int x, bool in) {              // tile x's
-        Span s{x * QT + off, min(x * QT + QT, a.Tq) - 1 + off, 0, 0, true};
-        if (range && in) {
-            const int2 ra = range[s.p0 / KT], rb = range[s.p1 / KT];
-            s.lo = min(range_lo(ra), range_lo(rb));
-            s.hi = max(ra.y, rb.y);
-            s.one = range_one(ra) && range_one(rb) && ra.y == rb.y;
-        }
-        return s;
-    };
-    auto visited = [&](const Span& s) { return mk.some(s, j0, j1) && (!range || (s.lo <= kw.hi && kw.lo <= s.hi)); };
     int r = u0 / nx - 1, base = 0, xe = 0;
     uint64_t act = 0, full = 0;
     auto next = [&]() -> int2 {
@@ -437,8 +426,14 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
             }
             const int x = base + lane;
             const bool in = x < xe;
-            const Span s = queries(x, in);
-            act = __ballot(in && visited(s));
+            Span s{x * QT + off, min(x * QT + QT, a.Tq) - 1 + off, 0, 0, true};
+            if (range && in) {
+                const int2 ra = range[s.p0 / KT], rb = range[s.p1 / KT];
+                s.lo = min(range_lo(ra), range_lo(rb));
+                s.hi = max(ra.y, rb.y);
+                s.one = range_one(ra) && range_one(rb) && ra.y == rb.y;
+            }
+            act = __ballot(in && mk.some(s, j0, j1) && (!range || (s.lo <= kw.hi && kw.lo <= s.hi)));
             full = __ballot(in && x * QT + QT <= a.Tq && mk.all(s, jw, jw + 31) && (!range || (s.one && kv.one && s.lo == kv.lo)));
         }
         const int i = __builtin_ctzll(act);
@@ -543,7 +538,7 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     s[e] = bit(m, e) ? s[e] : 0.f;
-                    g[e] = bit(m, e) ? g[e] : -INFINITY;              // masked (a weight of 0 is something else)
+                    g[e] = bit(m, e) ? g[e] : -1.f;   // masked (a weight of 0 is something else; none is negative)
                 }
             }
             unsigned char* ex = s_ex[n & 1][w] + 16 * lane;
@@ -581,7 +576,7 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     asm volatile("" : "+v"(dp[e]));   // (not ahead of the branch)
-                    dp[e] = p[e >> 2][e & 3] == -INFINITY ? 0.f : dp[e];
+                    dp[e] = p[e >> 2][e & 3] < 0.f ? 0.f : dp[e];
                 }
             }
             if constexpr (Half<T>::value) {           // (P comes at 2^P_UP)
@@ -612,6 +607,13 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
     uint32_t rows = row_bits(bad != 0.f && j < a.Tk);
     if (rows) {
         Ill<T, D> ill;
+        auto met = [&](int x) {                       // tile x was walked
+            const Span s{x * QT + off, min(x * QT + QT, a.Tq) - 1 + off, 0, 0, true};
+            if (!mk.some(s, j0, j1)) return false;
+            if (!range) return true;
+            const int2 ra = range[s.p0 / KT], rb = range[s.p1 / KT];
+            return min(range_lo(ra), range_lo(rb)) <= kw.hi && kw.lo <= max(ra.y, rb.y);
+        };
         auto open = [&]() { return (rows & row_bits(!ill.lost)) != 0; };               // some row is not decided yet
         for (int rr = u0 / nx; rr * nx < u1 && open(); rr++) {
             const int hq = hk * a.R + rr, te = min(min(x1, u1 - rr * nx) * QT, a.Tq);
@@ -631,7 +633,7 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
                     const int i = __builtin_ctzll(m), ti = t1 + i;
                     const bool sees = sees1(see, ti + off, docs ? a.ids + idb : nullptr, id);
                     ill.lost = ill.lost || (sees && (all >> i & 1));
-                    ill.add(role ? qh + ti * a.q_st : gh + ti * a.do_st, sees, visited(queries(ti / QT, true)), ti == a.Tq - 1 && a.Tq % QT, lane);
+                    ill.add(role ? qh + ti * a.q_st : gh + ti * a.do_st, sees, met(ti / QT), ti == a.Tq - 1 && a.Tq % QT, lane);
                 }
             }
         }
