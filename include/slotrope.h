@@ -43,7 +43,8 @@ int slotrope_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const 
 
 /* The serving form: the tokens are the newest T of lens[b] tokens of sequence b (token t at position lens[b] - T + t).
  * qo (B, T, Hq, D) is written whole; the prepared keys and the values go to rows `position` of the caches kc, vc
- * (B, Hk, S, D) by strides.  A token whose position is negative (padding on the left) or >= S writes no cache row. */
+ * (B, Hk, S, D) by strides.  A token whose position is negative (a first prompt's padding on the left) or >= S writes no cache row; one
+ * of a sequence that has tokens already has a position of theirs and overwrites it. */
 int slotrope_cache(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
                    int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, int dtype, const void* wq,
                    const void* wk, int wdtype, const double* freqs, int64_t rot, int interleaved, const int32_t* lens,

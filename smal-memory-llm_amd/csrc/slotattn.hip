@@ -52,9 +52,9 @@ __global__ __launch_bounds__(64) void attn_docs(const int32_t* ids, int T, int n
 // ------------------------------------------------------------------------------------------- many rows
 // Per 64 keys a wave has 2 D / 16 + D / 8 matrix instructions of 32 cycles (S = K Q^T, O += V^T P^T; 1,024 cycles at D = 128) and
 // about 350 vector ones for the softmax of 32 x 64 scores; both share a SIMD's issue, so two waves a SIMD (64 KB of LDS a
-// workgroup) fill one's gaps with the other's work.  Measured: 8,192 causal tokens, 12 query heads of 128 on 4, capped: 284 us
-// (1.45e12 bits of arithmetic in products: 726 TFLOP/s; the two products alone would take 149 us at the rate of a large
-// library product); 4 x 2,000 tokens with prefixes, capped: 98 us.
+// workgroup) fill one's gaps with the other's work.  Measured (kernel trace): 8,192 causal tokens, 12 query heads of 128 on 4, capped:
+// 284 us (2.06e11 operations in products: 726 TFLOP/s; they alone would take 149 us at the rate of a large library product);
+// 4 x 2,000 tokens with prefixes, capped: 104 us.
 // GR groups of 4 waves share a workgroup's rows, each taking every GR-th of their key tiles; their sums meet in LDS.  Two
 // groups halve the longest rows' steps where every tile has a CU of its own (up to 256 tiles); with more tiles their
 // lockstep costs more than the balance gives (8,192 tokens: 340 against 295 us).
@@ -296,8 +296,8 @@ __global__ __launch_bounds__(FT * GR, 2) void attn_fwd(AttnArgs a) {
 // Rows of a key/value head packed as (token, query head of the group); a workgroup takes `chunk` keys of 32 rows, its waves every
 // SW-th 32-key tile of them, each through a ring of its own of two tiles (no barrier in the loop); the waves' results meet
 // in LDS, the workgroups' in attn_join.  Bound by the bytes of the keys and values: two workgroups a CU keep about 100 KB
-// on their way.  Measured: 32 sequences of up to 8,192 tokens, 12 query heads of 128 on 4: 63 + 4 us (join), 4.6 TB/s;
-// one of 131,072: 43 + 8 us, 6.2 TB/s in the kernel.  (Four waves a workgroup, one workgroup a CU, tiles fetched one
+// on their way.  Measured (kernel trace): 32 sequences of up to 8,192 tokens, 12 query heads of 128 on 4: 66 + 5
+// us (join), 4.8 TB/s in the kernel; one of 131,072: 44 + 9 us, 6.1 TB/s.  (Four waves a workgroup, one workgroup a CU, tiles fetched one
 // ahead: 92 and 57 us.)
 template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(64 * SW) void attn_split(AttnArgs a) {

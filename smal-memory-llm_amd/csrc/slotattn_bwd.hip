@@ -103,7 +103,7 @@ __device__ __forceinline__ int lower_by(float mx) { return mx > DS_TOP ? DS_AT +
 
 // ------------------------------------------------------------------------------------------- dQ
 // Four products of 32 x 32 x D per wave and half tile (S, dP, dQ twice) beside about 12 vector instructions a score; K and V tiles are
-// staged once for 128 queries, two workgroups a CU.  8,192 causal tokens, 12 query heads of 128 on 4, capped: 425 us (the three products
+// staged once for 128 queries, two workgroups a CU.  8,192 causal tokens, 12 query heads of 128 on 4, capped: 435 us (kernel trace; the three products
 // that cannot be left out take 224 us at a large library product's rate; with dS rounded once 370 us).  (GR groups of waves as in
 // the forward.)
 template <typename T, int D, bool CAP, bool BIAS, int GR>
@@ -353,7 +353,7 @@ __device__ __forceinline__ bool meets(int x0, int x1, int nx, int u0, int u1) {
 // Two waves share 32 keys, on one SIMD: the first forms the scores and P, and sums dV = P^T dO; the second dP and dS, and sums
 // dK = dS^T Q, a tile behind, with P (times the cap's slope) handed over in LDS.  Each holds one operand and one sum -- one wave
 // with both had 250 registers and no room to read operands ahead: 3,100 cycles a tile of 32 x 32 pairs, with 1,024 of
-// matrix work -- and one's matrix instructions run beside the other's vector ones.  Measured (as above): 660 us, 624 TFLOP/s; 176 KB
+// matrix work -- and one's matrix instructions run beside the other's vector ones.  Measured (as above): 658 us, 627 TFLOP/s; 176 KB
 // pass through the LDS per step of four 32 x 32 tiles, which is about as long as their products take.  With dV summed by the
 // second wave, too: 698 us; one wave a SIMD with a pipeline of three tiles: 681 us.
 #define RING 4                                       // tiles: the two at work, two on their way

@@ -9,8 +9,9 @@ does to its projected queries and keys before the attention (slotattn_hip, slotw
     qk_rope_cache(q, k, v, wq, wk, freqs, lens, kcache, vcache, eps=1e-6, interleaved=False) -> q'
         the serving form, forward only: the T tokens are the newest of lens[b] (int32 (B,), the new ones included), token
         t at position lens[b] - T + t; the prepared keys and the values are written into rows `position` of kcache, vcache
-        (B, Hk, S, D), everything else in them stays.  A token of negative position (a batch padded on the left) or of
-        one past the cache writes nothing.  The caches share no memory with each other or with the operands.
+        (B, Hk, S, D), everything else in them stays.  A token of negative position or of one past the cache writes nothing,
+        so that first prompts of unlike lengths may be padded on the left.  Later calls may not: the padding's positions
+        would be those of earlier tokens, whose rows it would overwrite.  The caches share no memory with each other or with the operands.
     frequencies(rot, theta=10000.0, device=None) -> (rot / 2,) float64: theta^(-2 i / rot)
 
 bf16, fp16 or fp32 rows (q, k, v and the caches alike), D in {64, 128}, 2 len(freqs) a multiple of 16 up to D; freqs are
