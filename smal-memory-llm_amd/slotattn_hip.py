@@ -137,7 +137,7 @@ def attend(q, k, v, scale=None, causal=True, window=None, cap=None, slopes=None,
         docs = docs.contiguous()
     _same_device("attend", q, k, v, slopes, docs, prefix)
     if B * Tq == 0:
-        return q * 0                                     # no query: an empty result, and no gradient for the keys
+        return q * 0 + k[:, :0].sum() + v[:, :0].sum()   # no query: an empty result, and zeros as the gradients
     slopes, prefix = (None if x is None else x.contiguous() for x in (slopes, prefix))
     opts = _opts(q, scale, causal, window, cap)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

@@ -49,3 +49,13 @@ def test_views_of_a_buffer_and_inference_tensors():
     with torch.inference_mode():                         # and ordinary ones there
         _write(buf[:, :, 0].transpose(1, 2), buf[:, :, 1].transpose(1, 2), 5)
     assert bool(buf[:, 4].any())
+
+
+@pytest.mark.parametrize("B,Tq,Tk", [(0, 5, 5), (2, 0, 5), (2, 0, 0)])
+def test_no_query_gives_zero_gradients(B, Tq, Tk):
+    z = lambda h, t: torch.full((B, h, t, 64), float("nan"), device="cuda", dtype=BF, requires_grad=True)
+    leaves = [z(4, Tq), z(2, Tk), z(2, Tk)]
+    out = A.attend(*leaves)
+    assert out.shape == leaves[0].shape
+    for x, g in zip(leaves, torch.autograd.grad(out, leaves, torch.zeros_like(out))):
+        assert g.shape == x.shape and not bool(g.any())
