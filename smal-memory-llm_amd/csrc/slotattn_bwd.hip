@@ -364,6 +364,7 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
     typedef TileLoad<D, QT, BW> Load;
     __shared__ __align__(1024) unsigned char smem[RING * SLOT];      // [slot][queries, dout]
     __shared__ __align__(1024) unsigned char s_ex[2][BW][EX];        // P on its way: [tile % 2][pair][register quad][lane]
+    __shared__ uint32_t s_mk[2][BW][64];                             // which pairs of a masked tile are visible: [tile % 2][pair][lane]
     __shared__ __align__(16) float s_st[RING][2][QT];                // log-sum-exp, minus delta
     __shared__ __align__(16) int s_id[RING][2 * QT];                 // the queries' documents (twice)
     const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -531,16 +532,15 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
                 float x = fmaf(t, a.f, -L[e >> 2][e & 3]);
                 if constexpr (BIAS) x = fmaf(-slope, fabsf(d - (float)key_of(e, 0)), x);
                 s[e] = exp2_(x);
-                g[e] = CAP ? s[e] * fmaf(-t, t, 1.f) : s[e];
+                if constexpr (CAP) g[e] = s[e] * fmaf(-t, t, 1.f);
             }
             if (!(cur.x & 1)) {
                 const uint32_t m = seen16(see, t0 + off, h, false, docs ? s_id[slot] : nullptr, id);
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    s[e] = bit(m, e) ? s[e] : 0.f;
-                    g[e] = bit(m, e) ? g[e] : -1.f;   // masked (a weight of 0 is something else; none is negative)
-                }
+                for (int e = 0; e < 16; e++) s[e] = bit(m, e) ? s[e] : 0.f;
+                s_mk[n & 1][w][lane] = m;
             }
+            if constexpr (!CAP) g = s;
             unsigned char* ex = s_ex[n & 1][w] + 16 * lane;
 #pragma unroll
             for (int q = 0; q < 4; q++) *reinterpret_cast<float4*>(ex + 1024 * q) = make_float4(g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]);
@@ -572,11 +572,12 @@ __global__ __launch_bounds__(2 * BT, 2) void attn_dkv(AttnArgs a) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e = 0; e < 16; e++) dp[e] *= p[e >> 2][e & 3];
-            if (!(last.x & 1)) {                      // a masked pair's dP may be anything
+            if (!(last.x & 1)) {                      // a masked pair's dP, and with a cap its P, may be anything
+                const uint32_t m = s_mk[(n - 1) & 1][w][lane];
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     asm volatile("" : "+v"(dp[e]));   // (not ahead of the branch)
-                    dp[e] = p[e >> 2][e & 3] < 0.f ? 0.f : dp[e];
+                    dp[e] = __uint_as_float(__float_as_uint(dp[e]) & (uint32_t)((int)(m << (31 - e)) >> 31));
                 }
             }
             if constexpr (Half<T>::value) {           // (P comes at 2^P_UP)
