@@ -56,6 +56,22 @@ int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const 
                  const float* lse, const void* dout, int64_t do_sb, int64_t do_sh, int64_t do_st, void* workspace, float* delta, void* dq,
                  void* dk, void* dv, void* stream);
 
+/* The serving form over a cache in pages (slotpage.h): the newest tokens of R sequences, packed.  Row r's tokens are starts[r] .. starts[r + 1] - 1
+ * of the N, ascending (tokens of no row get 0); the i-th of its n is at position ends[r] - n + i and sees, by causality, window and prefix as
+ * above, keys of positions below ends[r] (ends[r] > M page reads M page keys; a query of negative position sees nothing).  The key at position j
+ * is row j % page of page table[r][j / page]; keys of a page outside [0, P) are not seen.
+ *   q by strides (head, token), k, v (P, Hk, page, D) by strides (page, head, row within the page), every row 16-byte aligned; page a power of two
+ *           in [16, 4096]; table rows t_sr elements apart; starts (R + 1), ends (R), prefix (R) int32; out (N, Hq, D) contiguous
+ *   most    an upper bound of the rows' numbers of tokens, or N.  It chooses between kernels; results do not depend on it but for rounding
+ * Nothing outside the tensors is read or written whatever table, starts and ends hold.  Rows must not share tokens (starts that fall).
+ * workspace: slotattn_pages_workspace(...) bytes, 256-byte aligned. */
+size_t slotattn_pages_workspace(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t most);
+int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sp, int64_t k_sh, int64_t k_st,
+                   const void* v, int64_t v_sp, int64_t v_sh, int64_t v_st, int dtype, const int32_t* table, int64_t t_sr,
+                   const int32_t* starts, const int32_t* ends, int64_t N, int64_t R, int64_t M, int64_t P, int64_t page,
+                   int64_t Hq, int64_t Hk, int64_t D, int64_t most, float scale, int64_t window, float cap, const float* slopes,
+                   const int32_t* prefix, void* workspace, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

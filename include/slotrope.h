@@ -52,6 +52,16 @@ int slotrope_cache(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, cons
                    int64_t kc_sb, int64_t kc_sh, int64_t kc_st, void* vc, int64_t vc_sb, int64_t vc_sh, int64_t vc_st,
                    void* stream);
 
+/* The serving form over a cache in pages (slotpage.h): N packed tokens, token i at position pos[i]; q, k, v by strides (head, token).  qo (N, Hq, D) is
+ * written whole; token i's prepared keys and values go to row slots[i] % page of page slots[i] / page of kp, vp (P, Hk, page, D) by strides
+ * (page, head, row within the page), unless slots[i] lies outside [0, P page).  page a power of two in [16, 4096].  Two tokens of one slot: either may
+ * remain, or a mixture. */
+int slotrope_pages(const void* q, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sh, int64_t k_st, const void* v,
+                   int64_t v_sh, int64_t v_st, int dtype, const void* wq, const void* wk, int wdtype, const double* freqs,
+                   int64_t rot, int interleaved, const int32_t* pos, const int64_t* slots, int64_t N, int64_t Hq, int64_t Hk,
+                   int64_t D, int64_t P, int64_t page, float eps, void* qo, void* kp, int64_t kp_sp, int64_t kp_sh,
+                   int64_t kp_st, void* vp, int64_t vp_sp, int64_t vp_sh, int64_t vp_st, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -274,7 +274,9 @@ int slotscan_gen_bwd(const void* k, const void* q, const void* v, int dtype, con
 #define SLOTSCAN_K_ATTN_DQ 20
 #define SLOTSCAN_K_ATTN_DKV 21
 #define SLOTSCAN_K_ATTN_JOIN 22
-#define SLOTSCAN_NK 23
+#define SLOTSCAN_K_PAGES 23
+#define SLOTSCAN_K_ATTN_PLAN 24
+#define SLOTSCAN_NK 25
 int slotscan_profile(int enable);
 int slotscan_profile_read(double* total_ms, int64_t* count, int nk);
 

@@ -5,7 +5,7 @@
 //               tiles with the running maximum and sum of the softmax.
 //   attn_split  few query rows against many keys (a generated token, a short chunk): the rows of a key/value head's query
 //               heads together, the keys split over waves and workgroups; attn_join combines the parts.
-#include "slot_attn.h"
+#include "slot_attn_rows.h"
 #include "slotscan.h"
 #include "slotattn.h"
 #include "slot_attn_host.h"
@@ -19,16 +19,6 @@ using slothost::al16;
 #define FT (64 * FW)
 #define FQ (32 * FW)                                 // query rows per workgroup
 #define SW 2                                         // waves per workgroup where the keys are split
-// A row's sums keep their reference maximum until a score passes it by this much (base 2): probabilities then reach 2^8, far
-// from any type's end, and the sums are rescaled a few times a row instead of in most tiles.
-#define LAZY 8.f
-// Scores are taken to base 2 and from their reference by one multiply-add.  The reference's own product is rounded, which moves a row's
-// probabilities by a common factor of up to 2^(|reference| 2^-24): nothing, until scores of millions.  From FAR on the difference is formed first.
-#define FAR 4194304.f
-// In fp16 the reference is 2^7 below the maximum, so that probabilities reach 2^7 to 2^15: fp16's smallest step is 2^-24, and below a largest
-// one of 1 those under 2^-25 would add to a row's sum but not to its output (8,192 of them at 2^-26: 1.2e-4 of the values).
-template <typename T> constexpr float HEAD = 0.f;
-template <> constexpr float HEAD<f16_t> = 7.f;
 
 namespace {
 

@@ -12,6 +12,7 @@
 #include "slot_common.h"
 #include "slotscan.h"
 #include "slotrope.h"
+#include "slotpage.h"
 #include "slot_host.h"
 
 using namespace slot;
@@ -94,6 +95,7 @@ struct RopeArgs {
     const void* pos;
     int64_t pos_sb;
     const int32_t* lens;
+    const int64_t* slots; int64_t places; int shift;  // pages: each token's place, P page, log2(page)
     int64_t BT;
     int T, Hq, Hk, S, hs;                            // hs: heads per workgroup (grid y)
     float eps;
@@ -161,8 +163,11 @@ template <int D, bool PAIRS> struct Turn {
 };
 
 // ------------------------------------------------------------------------------------------- forward
-template <typename T, int D, bool PAIRS, bool CACHE>
+// Where the prepared keys go: token-major outputs, rows of caches by position, rows of pages by slot (the last two with the values).
+enum { ROWS, CACHES, PAGES };
+template <typename T, int D, bool PAIRS, int INTO>
 __global__ __launch_bounds__(RT) void rope_fwd(RopeArgs a) {
+    constexpr bool CACHE = INTO != ROWS;
     constexpr int LPR = D / 8, GPB = RT / LPR;
     const int c = threadIdx.x % LPR, e0 = 8 * c;
     const int64_t tok = (int64_t)blockIdx.x * GPB + threadIdx.x / LPR;
@@ -178,10 +183,17 @@ __global__ __launch_bounds__(RT) void rope_fwd(RopeArgs a) {
     const T* xk = (const T*)a.k + b * a.k_sb + t * a.k_st + e0;
     const T* xv = CACHE ? (const T*)a.v + b * a.v_sb + t * a.v_st + e0 : nullptr;
     T* oq = (T*)a.qo + (tok * a.Hq) * D + e0;
-    const bool kept = !CACHE || (pos >= 0 && pos < a.S);
+    bool kept = true;
     T* ok;
     T* ov = nullptr;
-    if constexpr (CACHE) {
+    if constexpr (INTO == PAGES) {
+        const int64_t slot = a.slots[tok], in = (1 << a.shift) - 1;
+        kept = slot >= 0 && slot < a.places;
+        const int64_t page = kept ? slot >> a.shift : 0, row = kept ? slot & in : 0;
+        ok = (T*)a.ko + page * a.ko_sb + row * a.ko_st + e0;
+        ov = (T*)a.vo + page * a.vo_sb + row * a.vo_st + e0;
+    } else if constexpr (CACHE) {
+        kept = pos >= 0 && pos < a.S;
         ok = (T*)a.ko + b * a.ko_sb + (kept ? pos : 0) * a.ko_st + e0;
         ov = (T*)a.vo + b * a.vo_sb + (kept ? pos : 0) * a.vo_st + e0;
     } else {
@@ -330,8 +342,9 @@ __global__ __launch_bounds__(256) void rope_reduce(const float* part, int n, int
 
 template <typename T, int D, bool PAIRS>
 void launch_kind(const RopeArgs& a, int dir, dim3 grid, hipStream_t st) {
-    if (dir == 0) slothost::launch(rope_fwd<T, D, PAIRS, false>, grid, dim3(RT), 0, st, a);
-    else if (dir == 1) slothost::launch(rope_fwd<T, D, PAIRS, true>, grid, dim3(RT), 0, st, a);
+    if (dir == 0) slothost::launch(rope_fwd<T, D, PAIRS, ROWS>, grid, dim3(RT), 0, st, a);
+    else if (dir == 1) slothost::launch(rope_fwd<T, D, PAIRS, CACHES>, grid, dim3(RT), 0, st, a);
+    else if (dir == 3) slothost::launch(rope_fwd<T, D, PAIRS, PAGES>, grid, dim3(RT), 0, st, a);
     else slothost::launch(rope_bwd<T, D, PAIRS>, grid, dim3(RT), 0, st, a);
 }
 template <typename T>
@@ -476,4 +489,28 @@ extern "C" int slotrope_cache(const void* q, int64_t q_sb, int64_t q_sh, int64_t
     hipStream_t st = (hipStream_t)stream;
     slothost::Scope sc(SLOTSCAN_K_ROPE, st);
     return launch_rope(a, dtype, (int)D, interleaved, 1, dim3((unsigned)((B * T + gpb - 1) / gpb), (unsigned)((heads + a.hs - 1) / a.hs)), st);
+}
+
+extern "C" int slotrope_pages(const void* q, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sh, int64_t k_st, const void* v,
+                              int64_t v_sh, int64_t v_st, int dtype, const void* wq, const void* wk, int wdtype, const double* freqs,
+                              int64_t rot, int interleaved, const int32_t* pos, const int64_t* slots, int64_t N, int64_t Hq, int64_t Hk,
+                              int64_t D, int64_t P, int64_t page, float eps, void* qo, void* kp, int64_t kp_sp, int64_t kp_sh,
+                              int64_t kp_st, void* vp, int64_t vp_sp, int64_t vp_sh, int64_t vp_st, void* stream) {
+    if (int r = check_rope(q, k, dtype, wdtype, wq, wk, freqs, rot, 1, N, Hq, Hk, D, "slotrope_pages")) return r;
+    if (P < 1 || P > 0x7fffffffLL || page < SLOTPAGE_MIN || (page & (page - 1)) || page > SLOTPAGE_MAX)
+        return fail(SLOTSCAN_ERR_SHAPE, "slotrope_pages: P must be in [1, 2^31), page a power of two in [16, 4096]");
+    if (!v || !pos || !slots || !qo || !kp || !vp) return fail(SLOTSCAN_ERR_NULL, "slotrope_pages: a required pointer is NULL");
+    if (!al16(v) || !al16(qo) || !al16(kp) || !al16(vp) || !rows16(dtype, 0, q_sh, q_st) || !rows16(dtype, 0, k_sh, k_st) ||
+        !rows16(dtype, 0, v_sh, v_st) || !rows16(dtype, kp_sp, kp_sh, kp_st) || !rows16(dtype, vp_sp, vp_sh, vp_st))
+        return fail(SLOTSCAN_ERR_ALIGN, "slotrope_pages: rows of q, k, v, qo and the pages must be 16-byte aligned");
+    RopeArgs a = base_args(q, 0, q_sh, q_st, k, 0, k_sh, k_st, wq, wk, wdtype, freqs, rot, 1, N, Hq, Hk, eps);
+    a.v = v; a.v_sh = v_sh; a.v_st = v_st;
+    a.pos = pos; a.slots = slots; a.places = P * page; a.shift = __builtin_ctzll((unsigned long long)page);
+    a.qo = qo; a.ko = kp; a.vo = vp;
+    a.ko_sb = kp_sp; a.ko_sh = kp_sh; a.ko_st = kp_st; a.vo_sb = vp_sp; a.vo_sh = vp_sh; a.vo_st = vp_st;
+    const int heads = (int)(Hq + 2 * Hk), gpb = RT / (int)(D / 8);
+    a.hs = heads_per_group(N, heads, (int)D);
+    hipStream_t st = (hipStream_t)stream;
+    slothost::Scope sc(SLOTSCAN_K_ROPE, st);
+    return launch_rope(a, dtype, (int)D, interleaved, 3, dim3((unsigned)((N + gpb - 1) / gpb), (unsigned)((heads + a.hs - 1) / a.hs)), st);
 }

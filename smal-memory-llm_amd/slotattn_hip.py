@@ -14,6 +14,15 @@ are not enough -- packed documents, long windows, prompts read both ways, capped
         values (the new ones included) are the first lens[b] rows of kcache, vcache (B, Hk, S, D).  What lies behind them
         is not read.  A query of negative position (lens[b] < T) gets 0.
 
+    attend_pages(q, kpages, vpages, table, starts, ends, most=None, scale=None, window=None, cap=None, slopes=None, prefix=None)
+            -> (N, Hq, D)
+        the serving form over a cache in pages (slotpage_hip): q (N, Hq, D) holds the newest tokens of R sequences, packed --
+        one token each, a few, whole prompts, in any mixture; row r's are starts[r] .. starts[r + 1] - 1 (starts (R + 1,) int32,
+        ascending), the last of them at position ends[r] - 1 (ends (R,) int32).  Its keys and values are the first ends[r] rows of the
+        pages table[r] (table (R, M) int32) of kpages, vpages (P, Hk, page, D).  Keys of a page outside [0, P) are not seen; tokens
+        of no row, and of rows with ends[r] = 0, get 0.  `most` is an upper bound of the rows' numbers of tokens that the host knows
+        (None: N): it chooses between kernels, and results depend on it by rounding alone.
+
 bf16 or fp16, D in {64, 128}; docs, prefix (B,) and lens (B,) int32, slopes fp32.  Scores, softmax statistics and sums are
 fp32; the probabilities and score gradients are rounded to the operands' type for their products.  The gradients take the
 probabilities from the rows' fp32 log-sum-exp, which moves them by about 2^-24 of the row's largest score (fine for scores
@@ -26,7 +35,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 import slotscan_lib as L
-from slotrope_hip import _same_device, check_caches, check_lens
+from slotpage_hip import check_table, table_rows
+from slotrope_hip import _same_device, check_caches, check_ints, check_lens, check_pools
 
 _TYPES = (torch.bfloat16, torch.float16)
 _D = (64, 128)
@@ -39,17 +49,22 @@ def _check(q, k, v, scale, window, cap, slopes, prefix, what):
                          f"{tuple(v.shape)}")
     if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
         raise ValueError(f"{what}: the query heads must be a multiple of the key/value heads")
+    _check_options(q, k, v, scale, window, cap, slopes, prefix, k.shape[0], what)
+
+
+def _check_options(q, k, v, scale, window, cap, slopes, prefix, rows, what):
+    D = q.shape[-1]
     if q.dtype not in _TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise NotImplementedError(f"{what} computes in bf16 or fp16, all operands alike (got {q.dtype}, {k.dtype}, {v.dtype})")
-    if q.shape[3] not in _D:
-        raise NotImplementedError(f"{what} needs D in {_D} (got {q.shape[3]})")
+    if D not in _D:
+        raise NotImplementedError(f"{what} needs D in {_D} (got {D})")
     if window is not None and int(window) < 1:
         raise ValueError(f"{what}: window must be >= 1 or None (got {window})")
     if cap is not None and not 1e-30 <= float(cap) <= 1e30:
         raise ValueError(f"{what}: cap must be in [1e-30, 1e30] or None (got {cap})")
     if scale is not None and not 1e-30 <= abs(scale) <= 1e30:
         raise ValueError(f"{what}: |scale| must be in [1e-30, 1e30] (got {scale})")
-    if cap is not None and float(cap) > 1e36 * (q.shape[3] ** -0.5 if scale is None else abs(scale)):
+    if cap is not None and float(cap) > 1e36 * (D ** -0.5 if scale is None else abs(scale)):
         raise ValueError(f"{what}: cap must be at most 1e36 |scale| (got {cap}, scale {scale})")
     if slopes is not None:
         if slopes.shape != (q.shape[1],) or slopes.dtype != torch.float32:
@@ -57,8 +72,8 @@ def _check(q, k, v, scale, window, cap, slopes, prefix, what):
         if slopes.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError(f"{what}: the slopes are constants (no gradient)")
     L.check_tangents(what, q, k, v, slopes)
-    if prefix is not None and (prefix.dtype != torch.int32 or prefix.shape != (q.shape[0],)):
-        raise ValueError(f"{what}: prefix must be int32 ({q.shape[0]},) (got {prefix.dtype}, {tuple(prefix.shape)})")
+    if prefix is not None and (prefix.dtype != torch.int32 or prefix.shape != (rows,)):
+        raise ValueError(f"{what}: prefix must be int32 ({rows},) (got {prefix.dtype}, {tuple(prefix.shape)})")
 
 
 def _documents(docs, B, T):
@@ -120,7 +135,7 @@ class _Attend(torch.autograd.Function):
 
 
 def _opts(q, scale, causal, window, cap):
-    return (q.shape[3] ** -0.5 if scale is None else float(scale), int(bool(causal)),
+    return (q.shape[-1] ** -0.5 if scale is None else float(scale), int(bool(causal)),
             _NO_WINDOW if window is None else min(int(window), _NO_WINDOW), 0.0 if cap is None else float(cap))
 
 
@@ -162,3 +177,42 @@ def attend_cache(q, kcache, vcache, lens, scale=None, window=None, cap=None, slo
     with L.on(q.device):
         return _launch_fwd(L.rows(q), L.rows(kcache), L.rows(vcache), _opts(q, scale, True, window, cap), slopes, None, prefix, lens,
                            False)[0].transpose(1, 2)
+
+
+def attend_pages(q, kpages, vpages, table, starts, ends, most=None, scale=None, window=None, cap=None, slopes=None, prefix=None):
+    """Causal attention of packed newest tokens over a cache in pages (see the module docstring)."""
+    what = "attend_pages"
+    if q.dim() != 3 or kpages.dim() != 4 or table.dim() != 2:
+        raise ValueError(f"{what}: expected q (N, Hq, D), pages (P, Hk, page, D) and table (R, M); got {tuple(q.shape)}, "
+                         f"{tuple(kpages.shape)}, {tuple(table.shape)}")
+    N, Hq, D = q.shape
+    P, Hk, page, _ = kpages.shape
+    R, M = table.shape
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        raise ValueError(f"{what}: the query heads must be a multiple of the key/value heads")
+    _check_options(q, kpages, vpages, scale, window, cap, slopes, prefix, R, what)
+    check_pools(kpages, vpages, q, Hk, what)
+    check_table(table, what)
+    check_ints(starts, (R + 1,), torch.int32, what, "starts")
+    check_ints(ends, (R,), torch.int32, what, "ends")
+    if most is not None and int(most) < 0:
+        raise ValueError(f"{what}: most must be >= 0 or None (got {most})")
+    if torch.is_grad_enabled() and (q.requires_grad or kpages.requires_grad or vpages.requires_grad):
+        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
+    if not L.in_place(kpages) or not L.in_place(vpages):
+        raise ValueError(f"{what}: the pages are read in place: their rows must be contiguous and 16-byte aligned")
+    _same_device(what, q, kpages, vpages, table, starts, ends, slopes, prefix)
+    if N * R * M * P == 0:
+        return torch.zeros(N, Hq, D, device=q.device, dtype=q.dtype)
+    slopes, prefix = (None if x is None else x.contiguous() for x in (slopes, prefix))
+    most = N if most is None else min(max(int(most), 1), N)
+    scale, _, window, cap = _opts(q, scale, True, window, cap)
+    q_, lib = L.tokens(q), L.lib()
+    with L.on(q.device):
+        out = torch.empty(N, Hq, D, device=q.device, dtype=q.dtype)
+        ws = torch.empty(lib.slotattn_pages_workspace(N, R, M, page, Hq, Hk, D, most), device=q.device, dtype=torch.uint8)
+        rc = lib.slotattn_pages(*L.by_head(q_), *L.strided(kpages), *L.strided(vpages), L._TYPE_CODES[q.dtype], *table_rows(table),
+                                L.ptr(starts), L.ptr(ends), N, R, M, P, page, Hq, Hk, D, most, scale, window, cap, L.ptr(slopes),
+                                L.ptr(prefix), L.ptr(ws), L.ptr(out), L.stream_of(q.device))
+    L.check(rc, "slotattn_pages")
+    return out

@@ -12,6 +12,11 @@ does to its projected queries and keys before the attention (slotattn_hip, slotw
         (B, Hk, S, D), everything else in them stays.  A token of negative position or of one past the cache writes nothing,
         so that first prompts of unlike lengths may be padded on the left.  Later calls may not: the padding's positions
         would be those of earlier tokens, whose rows it would overwrite.  The caches share no memory with each other or with the operands.
+    qk_rope_pages(q, k, v, wq, wk, freqs, pos, slots, kpages, vpages, eps=1e-6, interleaved=False) -> q'
+        the serving form over a cache in pages (slotpage_hip), forward only: q (N, Hq, D), k, v (N, Hk, D) are packed tokens of many
+        sequences, pos and slots (N,) int32 and int64 their positions and places as page_extend gives them.  Token i's prepared key and
+        its value are written into row slots[i] % page of page slots[i] // page of kpages, vpages (P, Hk, page, D); a slot outside
+        of the pages (-1) writes nothing.  q' (N, Hq, D) is written whole.  Slots of one call are different.
     frequencies(rot, theta=10000.0, device=None) -> (rot / 2,) float64: theta^(-2 i / rot)
 
 bf16, fp16 or fp32 rows (q, k, v and the caches alike), D in {64, 128}, 2 len(freqs) a multiple of 16 up to D; freqs are
@@ -36,11 +41,15 @@ def frequencies(rot, theta=10000.0, device=None):
 def _check(q, k, wq, wk, freqs, what):
     if q.dim() != 4 or k.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
         raise ValueError(f"{what}: expected q (B, Hq, T, D) and k (B, Hk, T, D); got {tuple(q.shape)}, {tuple(k.shape)}")
+    _check_rows(q, k, wq, wk, freqs, what)
+
+
+def _check_rows(q, k, wq, wk, freqs, what):
     if q.shape[1] < 1 or k.shape[1] < 1:
         raise ValueError(f"{what}: needs at least one head of queries and of keys")
     if q.dtype not in L._TYPE_CODES or k.dtype != q.dtype:
         raise NotImplementedError(f"{what} takes bf16, fp16 or fp32 queries and keys of one type (got {q.dtype}, {k.dtype})")
-    D = q.shape[3]
+    D = q.shape[-1]
     if D not in _D:
         raise NotImplementedError(f"{what} needs D in {_D} (got {D})")
     if freqs.dim() != 1 or freqs.dtype != torch.float64:
@@ -200,11 +209,7 @@ def qk_rope_cache(q, k, v, wq, wk, freqs, lens, kcache, vcache, eps=1e-6, interl
     L.check_tangents(what, v, kcache, vcache)
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, wq, wk, kcache, vcache)):
         raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
-    for c in (kcache, vcache):
-        if not _apart(c) or not L.in_place(c):
-            raise ValueError(f"{what}: a cache is written in place: its rows must be contiguous, 16-byte aligned and apart")
-    if _overlap(kcache, vcache):
-        raise ValueError(f"{what}: the two caches share memory")
+    _check_written(kcache, vcache, what)
     _same_device(what, q, k, v, wq, wk, freqs, lens, kcache, vcache)
     q_, k_, v_ = L.rows(q), L.rows(k), L.rows(v)
     wq_, wk_, wt = _gains(wq, wk)
@@ -217,7 +222,76 @@ def qk_rope_cache(q, k, v, wq, wk, freqs, lens, kcache, vcache, eps=1e-6, interl
                                         kcache.shape[2], float(eps), L.ptr(qo), *L.strided(kcache), *L.strided(vcache),
                                         L.stream_of(q.device))
         L.check(rc, what)
-        written = [c for c in (kcache, vcache) if not c.is_inference()]               # (those have no version)
-        if written:
-            torch.autograd.graph.increment_version(written)
+        _written(kcache, vcache)
     return qo.transpose(1, 2)
+
+
+def _check_written(kcache, vcache, what):
+    for c in (kcache, vcache):
+        if not _apart(c) or not L.in_place(c):
+            raise ValueError(f"{what}: a cache is written in place: its rows must be contiguous, 16-byte aligned and apart")
+    if _overlap(kcache, vcache):
+        raise ValueError(f"{what}: the two caches share memory")
+
+
+def _written(*xs):
+    """Raises the versions of tensors that a kernel wrote."""
+    xs = [x for x in xs if not x.is_inference()]         # (those have no version)
+    if xs:
+        torch.autograd.graph.increment_version(xs)
+
+
+def check_pools(kpages, vpages, like, Hk, what):
+    """The shape, type and layout of the pages (P, Hk, page, D) of the keys and values, which are read or written in place."""
+    if kpages.dim() != 4 or vpages.shape != kpages.shape or kpages.shape[1] != Hk or kpages.shape[3] != like.shape[2]:
+        raise ValueError(f"{what}: expected pages (P, {Hk}, page, {like.shape[2]}); got {tuple(kpages.shape)}, {tuple(vpages.shape)}")
+    check_page(kpages.shape[2], what)
+    if kpages.dtype != like.dtype or vpages.dtype != like.dtype:
+        raise NotImplementedError(f"{what}: the pages must have the queries' type {like.dtype} (got {kpages.dtype}, {vpages.dtype})")
+
+
+def check_page(page, what):
+    if page < 16 or page > 4096 or page & (page - 1):
+        raise ValueError(f"{what}: a page must hold a power of two of tokens, 16 to 4096 (got {page})")
+
+
+def check_ints(x, shape, dtype, what, name):
+    if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {str(dtype)[6:]} {shape} (got {x.dtype}, {tuple(x.shape)})")
+
+
+def qk_rope_pages(q, k, v, wq, wk, freqs, pos, slots, kpages, vpages, eps=1e-6, interleaved=False):
+    """Prepared queries of packed tokens, their keys and values written into the pages (see the module docstring)."""
+    what = "qk_rope_pages"
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"{what}: expected q (N, Hq, D) and k (N, Hk, D); got {tuple(q.shape)}, {tuple(k.shape)}")
+    _check_rows(q, k, wq, wk, freqs, what)
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"{what}: v must have k's shape and type (got {tuple(v.shape)}, {v.dtype})")
+    N, Hq, D = q.shape
+    Hk = k.shape[1]
+    check_pools(kpages, vpages, q, Hk, what)
+    check_ints(pos, (N,), torch.int32, what, "pos")
+    check_ints(slots, (N,), torch.int64, what, "slots")
+    L.check_tangents(what, v, kpages, vpages)
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, wq, wk, kpages, vpages)):
+        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
+    P, page = kpages.shape[0], kpages.shape[2]
+    if P:
+        _check_written(kpages, vpages, what)
+    _same_device(what, q, k, v, wq, wk, freqs, pos, slots, kpages, vpages)
+    if not P:
+        raise ValueError(f"{what}: there are no pages to write into")
+    q_, k_, v_ = L.tokens(q), L.tokens(k), L.tokens(v)
+    wq_, wk_, wt = _gains(wq, wk)
+    freqs = freqs.contiguous()
+    qo = torch.empty(N, Hq, D, device=q.device, dtype=q.dtype)
+    if N:
+        with L.on(q.device):
+            rc = L.lib().slotrope_pages(*L.by_head(q_), *L.by_head(k_), *L.by_head(v_), L._TYPE_CODES[q.dtype], L.ptr(wq_), L.ptr(wk_),
+                                        wt, L.ptr(freqs), 2 * freqs.numel(), int(bool(interleaved)), L.ptr(pos), L.ptr(slots), N, Hq,
+                                        Hk, D, P, page, float(eps), L.ptr(qo), *L.strided(kpages), *L.strided(vpages),
+                                        L.stream_of(q.device))
+        L.check(rc, what)
+        _written(kpages, vpages)
+    return qo

@@ -1,5 +1,5 @@
 """ctypes binding of libslotscan.so (declarations: include/slotscan.h, slotread.h, slotmem.h, slotwin.h,
-slotproj.h, slotrope.h, slotattn.h).
+slotproj.h, slotrope.h, slotattn.h, slotpage.h).
 
 torch is imported BEFORE the library is opened: libslotscan.so needs libamdhip64.so.7 by SONAME, and with
 torch loaded first the dynamic loader binds it to torch's own HIP runtime, so the streams and device
@@ -24,6 +24,7 @@ SLOTSCAN_F16 = 2          # the attention of any range and its query and key pre
 _vp, _i64, _i32, _f32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
 
 _ROWS = [_vp, _i64, _i64, _i64]                          # rows by strides: batch, head, token
+_HEADS = [_vp, _i64, _i64]                               # packed tokens by strides: head, token
 _ROPE = _ROWS * 2 + [_i32, _vp, _vp, _i32, _vp, _i64, _i32]
 _ATTN = _ROWS * 3 + [_i32] + [_i64] * 6 + [_f32, _i32, _i64, _f32, _vp]
 
@@ -81,6 +82,12 @@ SIGNATURES = {
     "slotrope_bwd": (_i32, _ROPE + [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _f32] + _ROWS * 2 + [_vp] * 6),
     "slotrope_cache": (_i32, _ROWS * 3 + [_i32, _vp, _vp, _i32, _vp, _i64, _i32, _vp] + [_i64] * 6 + [_f32, _vp]
                        + _ROWS * 2 + [_vp]),
+    "slotrope_pages": (_i32, _HEADS * 3 + [_i32, _vp, _vp, _i32, _vp, _i64, _i32, _vp, _vp] + [_i64] * 6 + [_f32, _vp]
+                       + _ROWS * 2 + [_vp]),
+    "slotpage_extend": (_i32, [_vp, _vp, _vp, _i64, _vp] + [_i64] * 5 + [_vp] * 5),
+    "slotpage_trim": (_i32, [_vp, _vp, _vp, _i64, _vp] + [_i64] * 4 + [_vp]),
+    "slotattn_pages_workspace": (_sz, [_i64] * 8),
+    "slotattn_pages": (_i32, _HEADS + _ROWS * 2 + [_i32, _vp, _i64, _vp, _vp] + [_i64] * 9 + [_f32, _i64, _f32] + [_vp] * 5),
     "slotattn_docs_bytes": (_sz, [_i64, _i64]),
     "slotattn_docs": (_i32, [_vp, _i64, _i64, _vp, _vp]),
     "slotattn_fwd_workspace": (_sz, [_i64] * 6 + [_i32, _i64, _i32, _i32, _i32]),
@@ -163,6 +170,29 @@ def strided(x):
     return x.data_ptr(), s[0], s[1], s[2]
 
 
+def _token_strides(x):
+    """Strides of token and head of x (token, head, D); 0 where the dimension has size 1, as _strides."""
+    s = x.stride()
+    if (s[0] | s[1]) % 8 or s[0] >= 1 << 25:
+        s = (*(a if n > 1 else 0 for a, n in zip(s[:2], x.shape)), s[2])
+    return s
+
+
+def tokens(x):
+    """Packed tokens (token, head, D) as the kernels read them (contiguous rows, 16-byte aligned, tokens fewer than 2^25 elements
+    apart), themselves or a copy."""
+    n = 16 // x.element_size()
+    s = _token_strides(x)
+    ok = s[2] == 1 and not (s[0] % n or s[1] % n) and s[0] < 1 << 25 and not x.data_ptr() % 16
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
+
+
+def by_head(x):
+    """Pointer and strides (head, token) of tokens(x), as the entry points take them."""
+    s = _token_strides(x)
+    return x.data_ptr(), s[1], s[0]
+
+
 def on(device):
     """Makes `device` the current one around a launch (a no-op where it is)."""
     return torch.cuda.device(device if device.index != torch.cuda.current_device() else -1)
@@ -176,7 +206,7 @@ def check_tangents(what, *xs):
 
 KERNEL_NAMES = ("chain_fwd", "rows_fwd", "rows_bwd", "chain_bwd", "reduce_parts", "read_fwd", "read_bwd", "mem_fwd",
                 "mem_bwd", "win_fwd", "win_bwd", "gen_fwd", "gen_bwd", "proj", "proj_drd", "proj_dwo",
-                "proj_reduce", "rope", "rope_bwd", "attn_fwd", "attn_dq", "attn_dkv", "attn_join")
+                "proj_reduce", "rope", "rope_bwd", "attn_fwd", "attn_dq", "attn_dkv", "attn_join", "pages", "attn_plan")
 
 
 def profile(enable, kernels=None):
