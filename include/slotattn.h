@@ -64,8 +64,9 @@ int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const 
  *           in [16, 4096]; table rows t_sr elements apart; starts (R + 1), ends (R), prefix (R) int32; out (N, Hq, D) contiguous
  *   most    an upper bound of the rows' numbers of tokens, or N.  It chooses between kernels; results do not depend on it but for rounding
  * Nothing outside the tensors is read or written whatever table, starts and ends hold.  Rows must not share tokens (starts that fall).
- * workspace: slotattn_pages_workspace(...) bytes, 256-byte aligned. */
-size_t slotattn_pages_workspace(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t most);
+ * workspace: slotattn_pages_workspace(...) bytes (may be 0), 256-byte aligned. */
+size_t slotattn_pages_workspace(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t most,
+                                int64_t window, int has_prefix);
 int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sp, int64_t k_sh, int64_t k_st,
                    const void* v, int64_t v_sp, int64_t v_sh, int64_t v_st, int dtype, const int32_t* table, int64_t t_sr,
                    const int32_t* starts, const int32_t* ends, int64_t N, int64_t R, int64_t M, int64_t P, int64_t page,

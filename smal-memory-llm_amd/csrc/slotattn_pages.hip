@@ -5,8 +5,8 @@
 // ragged lengths nor causality leave a worker more than another.  A piece that is not a whole unit leaves its rows' maxima, sums and
 // weighted values in the workspace, two such pieces a worker at most, and pages_join combines a unit's pieces in order.
 //
-//   pages_plan   the units' costs and their running sums
-//   pages_many   128 rows a workgroup, 32 per wave, 64-key tiles
+//   pages_many   128 rows a workgroup, 32 per wave, 64-key tiles; pages_plan before it: the units' costs and their running sums
+//   pages_few    32 rows, 32-key tiles
 //   pages_join   pieces of one unit
 #include "slot_attn_rows.h"
 #include "slotscan.h"
@@ -24,6 +24,10 @@ using slothost::al16;
 #define MQ (32 * MW)                                 // its query rows
 #define MG 512                                       // workgroups: two a CU
 #define LT 1024                                      // threads of pages_plan
+#define FG 1024                                      // waves of pages_few that share all units
+#define FS 4                                         // tiles of one of them at least
+#define FW 4                                         // waves of pages_few that share one
+#define UNIT_KEYS 2048                               // keys of a row up to which they do
 
 namespace {
 
@@ -58,26 +62,50 @@ template <int STEP> __device__ __forceinline__ void keys_of(const PagedArgs& a, 
     hi = p1 < 0 ? lo : min(x.klen, max(p1 + 1, x.pre));
 }
 
-// A wave's 64 pages of a sequence from page wb on, one a lane.  An id outside of the pages stands for page 0, and its keys are not seen.
-struct Window {
+// A wave's 64 NR pages of a sequence from page wb on, NR a lane.  An id outside of the pages stands for page 0, and its keys are not seen.
+template <int NR> struct Window {
     const int32_t* tab;
-    int M, P, shift, used, lane, wb, ids;             // used: pages that hold keys
-    uint64_t bad;
+    int M, P, shift, used, lane, wb, ids[NR];         // used: pages that hold keys
+    uint64_t bad[NR];
+    __device__ __forceinline__ Window(const PagedArgs& a, int r, int klen, int l)
+        : tab(a.table + r * a.t_sr), M(a.M), P(a.P), shift(a.shift), used((klen + (1 << a.shift) - 1) >> a.shift), lane(l), wb(-65536) {}
     __device__ __forceinline__ void at(int j0, int keys) {
         const int first = j0 >> shift, last = (j0 + keys - 1) >> shift;
-        if (first >= wb && last - wb < 64) return;
+        if (first >= wb && last - wb < 64 * NR) return;
         wb = first;
-        const int i = wb + lane, id = tab[min(i, M - 1)];
-        const bool in = i < used, b = in && (unsigned)id >= (unsigned)P;
-        bad = __ballot(b);
-        ids = in && !b ? id : 0;
+#pragma unroll
+        for (int n = 0; n < NR; n++) ids[n] = tab[min(wb + 64 * n + lane, M - 1)];
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            const bool in = wb + 64 * n + lane < used, b = in && (unsigned)ids[n] >= (unsigned)P;
+            bad[n] = __ballot(b);
+            ids[n] = in && !b ? ids[n] : 0;
+        }
     }
-    __device__ __forceinline__ int page(int j) const { return __builtin_amdgcn_readlane(ids, (j >> shift) - wb); }    // j: of the wave
+    __device__ __forceinline__ int page(int j) const {                // j: of the wave
+        const int i = (j >> shift) - wb;
+        int x = __builtin_amdgcn_readlane(ids[0], i & 63);
+#pragma unroll
+        for (int n = 1; n < NR; n++) {
+            const int y = __builtin_amdgcn_readlane(ids[n], i & 63);
+            x = i >= 64 * n ? y : x;
+        }
+        return x;
+    }
     // the groups of 16 keys from j0 on, as bits, that lie in no page
     __device__ __forceinline__ uint32_t lost(int j0, int keys) const {
         uint32_t x = 0;
-        if (bad)
-            for (int g = 0; g < keys / 16; g++) x |= (uint32_t)(bad >> (((j0 + 16 * g) >> shift) - wb) & 1) << g;
+        uint64_t any = bad[0];
+#pragma unroll
+        for (int n = 1; n < NR; n++) any |= bad[n];
+        if (any)
+            for (int g = 0; g < keys / 16; g++) {
+                const int i = ((j0 + 16 * g) >> shift) - wb;
+                uint64_t b = bad[0];
+#pragma unroll
+                for (int n = 1; n < NR; n++) b = i >= 64 * n ? bad[n] : b;
+                x |= (uint32_t)(b >> (i & 63) & 1) << g;
+            }
         return x;
     }
 };
@@ -96,7 +124,7 @@ template <int D, int ROWS, int NW> struct PageLoad {
     __device__ __forceinline__ int row(int i) const { return RPL * (NW * i + w) + lane / Tile<D>::CH; }
     __device__ __forceinline__ int chunk(int i) const { return Tile<D>::pos(row(i), lane % Tile<D>::CH); }
     // keys j0 .. (a multiple of 32), `last` the sequence's last (>= j0), which stands for those behind it
-    template <typename T> __device__ __forceinline__ void issue(const T* base, const Window& win, int j0, int last, unsigned lds) const {
+    template <typename T, int NR> __device__ __forceinline__ void issue(const T* base, const Window<NR>& win, int j0, int last, unsigned lds) const {
         const int in = (1 << win.shift) - 1;
         if (last - j0 >= ROWS - 1) {
 #pragma unroll
@@ -296,8 +324,7 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
         const int j_end = min(hi, lo + kb * KT);
         const T* kbase = (const T*)a.k + hk * a.k_sh;
         const T* vbase = (const T*)a.v + hk * a.v_sh;
-        const int32_t* tab = a.table + r * a.t_sr;
-        Window win{tab, a.M, a.P, a.shift, (sq.klen + (1 << a.shift) - 1) >> a.shift, lane, -1000, 0, 0};
+        Window<1> win(a, r, sq.klen, lane);
         auto seen = [&](int j) {                      // the next tile that any of the workgroup's rows sees
             while (j < j_end && !mk.some(sw, j, j + KT - 1)) j += KT;
             return j;
@@ -397,7 +424,7 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
         for (uint32_t b = odd; b; b &= b - 1) {
             const int i = __builtin_ctz(b);
             float m1, l1, o1[D / 64];
-            exact_paged<T, D, CAP, BIAS>(a, (const T*)a.q + lane_of(hq, i) * a.q_sh + (int64_t)(sq.s + lane_of(tok, i)) * a.q_st, kbase, vbase, tab,
+            exact_paged<T, D, CAP, BIAS>(a, (const T*)a.q + lane_of(hq, i) * a.q_sh + (int64_t)(sq.s + lane_of(tok, i)) * a.q_st, kbase, vbase, win.tab,
                                          lane_of(see, i), lane_of(slope, i), lane_of(p, i), lo + ka * KT, j_end, lane, m1, l1, o1);
             if (whole) {
                 const float inv1 = l1 > 0.f || l1 != l1 ? 1.f / l1 : 0.f;
@@ -437,75 +464,388 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
     if (tid == 0) a.join[me] = left;
 }
 
-// ------------------------------------------------------------------------------------------- join
-// A group of D / 4 lanes per row: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the unit's pieces, in order
-template <typename T, int D>
-__global__ __launch_bounds__(256) void pages_join(PagedArgs a) {
-    constexpr int LN = D / 4, RW = 256 / LN;
-    const Unit u = a.join[blockIdx.x];
-    if (u.parts < 2) return;
-    const int c = threadIdx.x % LN, i = blockIdx.y * RW + threadIdx.x / LN, row = MQ * u.t + i;
-    if (row >= u.n * a.rep) return;
-    const int me = blockIdx.x;
-    auto slot = [&](int s) { return (int64_t)(s ? 2 * (me + s) : 2 * me + 1) * MQ + i; };
-    float M = -INFINITY, L = 0.f;
-    for (int s = 0; s < u.parts; s++) M = fmaxf(M, a.pm[slot(s)].x);
-    const float Mu = M == -INFINITY ? 0.f : M;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = 0; s < u.parts; s++) {
-        const float2 x = a.pm[slot(s)];
-        const float f = x.y != 0.f ? exp2_(x.x - Mu) : 0.f;           // otherwise nothing is visible in this piece
-        const float4 o = *reinterpret_cast<const float4*>(a.po + slot(s) * D + 4 * c);
-        L = fmaf(x.y, f, L);
-        acc.x = fmaf(o.x, f, acc.x);
-        acc.y = fmaf(o.y, f, acc.y);
-        acc.z = fmaf(o.z, f, acc.z);
-        acc.w = fmaf(o.w, f, acc.w);
+// ------------------------------------------------------------------------------------------- few rows
+// One 32-row tile of a key/value head (a generated token's query heads, a few tokens') against 32-key tiles, each wave through a ring of its own of
+// two tiles without a barrier in the loop.  NW = 1, STREAM: every wave is a worker with an equal share of all units' tiles.  Otherwise a
+// workgroup's NW waves share one unit, every NW-th tile each, and meet in LDS.
+__device__ __forceinline__ int scan_up(int x, int lane) {            // sum over the lanes up to this one
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x += y;
     }
-    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-    const int tok = row / a.rep, hq = u.hk * a.rep + row - tok * a.rep;
-    const int s = min(max(a.starts[u.r], 0), a.N);
-    put4<T>(a.out, nullptr, ((int64_t)(s + tok) * a.Hq + hq) * D + 4 * c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    return x;
+}
+// 32-row tiles of row r, and 32-key tiles of each (of its whole row, so that no table of them is needed)
+__device__ __forceinline__ int few_tiles(const PagedArgs& a, const Seq& x, int& per) {
+    int lo, hi;
+    keys_of<32>(a, x, x.end - x.n, x.end - 1, lo, hi);
+    per = max(1, (hi - lo + 31) >> 5);
+    return (x.n * a.rep + 31) >> 5;
+}
+__device__ __forceinline__ int few_cost(const PagedArgs& a, int r) {
+    if (r >= a.R) return 0;
+    int per;
+    const int t = few_tiles(a, seq_of(a, r), per);
+    return t * per;
+}
+
+template <typename T, int D, bool CAP, bool BIAS, int NW, bool STREAM>
+__global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
+    constexpr int KK = D / 16, DT = D / 32, ST = 32 * 2 * D;
+    typedef PageLoad<D, 32, 1> Load;
+    __shared__ __align__(1024) unsigned char smem[NW][2][2][ST];     // [wave][buffer][keys, values]
+    __shared__ float s_m[NW][32], s_l[NW][32];                       // the waves' maxima and sums of every row
+    __shared__ float s_M[32], s_L[32];                               // the workgroup's
+    __shared__ uint32_t s_bad[NW];
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int w = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
+    int r = 0, base = 0, me = 0, G = 1;               // base: tiles of one head in front of row r
+    int64_t x = 0, end = 1, total = 1;
+    Unit left{0, 0, 0, 0, 0};
+    if constexpr (STREAM) {
+        const int C = (a.R + 63) / 64;
+        int mine = 0;
+        for (int i = 0; i < C; i++) mine += few_cost(a, lane * C + i);
+        const int upto = scan_up(mine, lane);
+        total = (int64_t)lane_of(upto, 63) * a.Hk;
+        G = (int)min((int64_t)gridDim.x, max(total / FS, (int64_t)1));
+        me = blockIdx.x;
+        if (me < G) {
+            if (G % 8 == 0) me = (me & 7) * (G / 8) + (me >> 3);     // workers that follow each other run on one XCD
+            x = total * me / G;
+            end = total * (me + 1) / G;
+            const int y = (int)(x / a.Hk), L = 63 - __builtin_clzll(__ballot(upto - mine <= y) | 1);
+            base = lane_of(upto - mine, L);
+            r = L * C;
+            for (int i0 = 0; C > 1 && i0 < C; i0 += 64) {            // the row within the lane's rows
+                const int c = i0 + lane < C ? few_cost(a, r + i0 + lane) : 0, u = scan_up(c, lane), all = lane_of(u, 63);
+                if (base + all <= y) { base += all; continue; }
+                const int k = 63 - __builtin_clzll(__ballot(base + u - c <= y) | 1);
+                base += lane_of(u - c, k);
+                r += i0 + k;
+                break;
+            }
+        } else {
+            x = end;
+        }
+    }
+    const unsigned lds = lds_addr(smem[w]);
+    const Load lk(a.k_sp, a.k_st, 0, lane), lv(a.v_sp, a.v_st, 0, lane);
+    const Ops<D> ops(lane);
+    const float f2 = fabsf(a.s.f);
+    RowSums<T, D, BIAS> sum(f2);
+    int t = STREAM ? 0 : blockIdx.x, hk = STREAM ? 0 : blockIdx.y;
+    if constexpr (!STREAM) r = blockIdx.z;
+    while (x < end) {
+        Seq sq = seq_of(a, r);
+        sq = {uni(sq.s), uni(sq.n), uni(sq.end), uni(sq.klen), uni(sq.pre)};
+        const int rows = sq.n * a.rep, off = sq.end - sq.n;
+        int per, ka = 0, kb, lo, hi;
+        const int tiles = few_tiles(a, sq, per);
+        if constexpr (STREAM) {
+            const int64_t y = x - (int64_t)base * a.Hk;
+            const int cost = tiles * per;
+            if (y >= (int64_t)cost * a.Hk) {          // the next row
+                if (++r >= a.R) break;
+                base += cost;
+                continue;
+            }
+            hk = (int)(y / cost);
+            const int z = (int)(y - (int64_t)hk * cost);
+            t = z / per;
+            ka = z - t * per;
+            kb = (int)min((int64_t)per, ka + end - x);
+        } else {
+            if (t >= tiles) break;
+            kb = per;
+        }
+        keys_of<32>(a, sq, off, sq.end - 1, lo, hi);
+        const int r0 = 32 * t, row = min(r0 + (lane & 31), rows - 1);
+        const int tok = row / a.rep, hq = hk * a.rep + row - tok * a.rep, p = tok + off;
+        const Mask mk{1, a.W, sq.pre, sq.klen};
+        const Span s{r0 / a.rep + off, (min(r0 + 32, rows) - 1) / a.rep + off, 0, 0, true};
+        const int first = lo + 32 * ka;
+        hi = min(hi, lo + 32 * kb);
+        const T* kbase = (const T*)a.k + hk * a.k_sh;
+        const T* vbase = (const T*)a.v + hk * a.v_sh;
+        Window<2> win(a, r, sq.klen, lane);
+        auto seen = [&](int j) {                      // the next of this wave's tiles that any row sees
+            while (j < hi && !mk.some(s, j, j + 31)) j += 32 * NW;
+            return j;
+        };
+        auto keys = [&](int j, int buf) { lk.issue(kbase, win, j, sq.klen - 1, lds + (2 * buf) * ST); };
+        auto values = [&](int j, int buf) { lv.issue(vbase, win, j, sq.klen - 1, lds + (2 * buf + 1) * ST); };
+        // a tile's groups of 16 keys in no page; the window stands at the tile that is loaded last
+        auto look = [&](int j) -> uint32_t {
+            win.at(j, 32);
+            return win.lost(j, 32);
+        };
+        uint32_t lost0 = 0, lost1 = 0, lost2 = 0;
+        int j0 = seen(first + 32 * w);
+        if (j0 < hi) {
+            lost0 = look(j0);
+            keys(j0, 0);
+            values(j0, 0);
+        }
+        const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
+        const T* qrow = (const T*)a.q + hq * a.q_sh + (int64_t)(sq.s + tok) * a.q_st;
+        uint4 qf[KK];
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) qf[kk] = ld16(qrow + 8 * h + 16 * kk);
+        if (a.s.f < 0.f)                              // a negative scale: of the queries' sign, so that larger products are larger scores
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) { qf[kk].x ^= 0x80008000u; qf[kk].y ^= 0x80008000u; qf[kk].z ^= 0x80008000u; qf[kk].w ^= 0x80008000u; }
+        const Sees see = Sees::query(mk, p);
+        sum.clear();
+        // Keys and values are fetched two tiles ahead, each into the place that it has just been read from.
+        int j1 = j0 < hi ? seen(j0 + 32 * NW) : hi;
+        if (j1 < hi) {
+            lost1 = look(j1);
+            keys(j1, 1);
+            values(j1, 1);
+        }
+        for (int buf = 0; j0 < hi; buf ^= 1) {
+            const int j2 = j1 < hi ? seen(j1 + 32 * NW) : hi;
+            if (j2 < hi) lost2 = look(j2);
+            if (j1 < hi) wait_vm<3 * Load::N>();      // behind this tile's keys: its values, the next keys and values
+            else wait_vm<Load::N>();
+            asm volatile("" ::: "memory");
+            const unsigned bo = lds + (2 * buf) * ST, rk = bo + ops.row, c = bo + ops.col, c8 = bo + ops.col8;
+            f32x16 sc[1] = {zero16()};
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) sc[0] = mfma32<T>(lds16(Ops<D>::k_step(rk, kk)), qf[kk], sc[0]);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the keys are read before their place is filled again
+            if (j2 < hi) keys(j2, buf);
+            scores<CAP>(sc[0], a.s);
+            if constexpr (BIAS) bias(sc[0], f2, slope, p, j0, h);
+            if (lost0 || j0 + 32 > hi || !mk.all(s, j0, j0 + 31)) {
+                uint32_t ok = seen16(see, j0, h, j0 < mk.prefix, nullptr, 0);
+                if (bit(lost0, 0)) ok &= ~0xffu;      // registers 0 .. 7 are keys of the first 16
+                if (bit(lost0, 1)) ok &= 0xffu;
+#pragma unroll
+                for (int e = 0; e < 16; e++) sc[0][e] = j0 + key_of(e, h) < hi && bit(ok, e) ? sc[0][e] : -INFINITY;
+            }
+            uint4 pf[1][2];
+            sum.template weigh<1>(sc, pf);
+            if (j2 < hi) wait_vm<3 * Load::N>();      // behind the values: the next tile, the keys after it
+            else if (j1 < hi) wait_vm<2 * Load::N>();
+            else wait_vm<0>();
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int mm = 0; mm < 2; mm++)
+                    sum.o[dt] = mfma32<T>(Ops<D>::at_col(Ops<D>::block(c, dt), Ops<D>::block(c8, dt), ST + 16 * mm * Tile<D>::ROWB), pf[0][mm], sum.o[dt]);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the values, too
+            if (j2 < hi) values(j2, buf);
+            j0 = j1;
+            j1 = j2;
+            lost0 = lost1;
+            lost1 = lost2;
+        }
+        sum.close();
+        // the waves' parts: (m, l) of every row to all, then the weighted sums through LDS (its tiles are read)
+        if (h == 0) { s_m[w][lane] = sum.m; s_l[w][lane] = sum.l; }
+        __syncthreads();
+        float M = -INFINITY, Ls = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; i++) M = fmaxf(M, s_m[i][lane & 31]);
+        const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int i = 0; i < NW; i++) Ls += s_l[i][lane & 31] * exp2_(s_m[i][lane & 31] - Mu);
+        const float f = exp2_(sum.m - Mu);
+        float* so = reinterpret_cast<float*>(smem);   // [wave][row][D + 4]
+        constexpr int SO = D + 4;
+        static_assert(NW * 32 * SO * 4 <= (int)sizeof(smem), "the waves' sums fit");
+        const int used = min(32, rows - r0);
+        if ((lane & 31) < used) {
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    *reinterpret_cast<float4*>(so + (w * 32 + (lane & 31)) * SO + 32 * dt + 8 * g + 4 * h) =
+                        make_float4(sum.o[dt][4 * g] * f, sum.o[dt][4 * g + 1] * f, sum.o[dt][4 * g + 2] * f, sum.o[dt][4 * g + 3] * f);
+        }
+        if (w == 0 && h == 0) { s_M[lane] = M; s_L[lane] = Ls; }      // not over s_m and s_l, which the other waves may still read
+        float nf = sum.l * 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) nf = nonfinite(sum.o[dt], nf);
+        const uint32_t odd = row_bits(nf != 0.f && (lane & 31) < used);
+        if (lane == 0) s_bad[w] = odd;
+        __syncthreads();
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < NW; i++) bad |= s_bad[i];
+        if (bad) {                                    // rows next to infinities and NaN, from their visible pairs alone; the same in every wave
+            bad &= ~row_bits(Ls != Ls);
+            for (; bad; bad &= bad - 1) {
+                const int i = __builtin_ctz(bad);
+                if (i % NW != w) continue;
+                float m1, l1, o1[D / 64];
+                exact_paged<T, D, CAP, BIAS>(a, (const T*)a.q + lane_of(hq, i) * a.q_sh + (int64_t)(sq.s + lane_of(tok, i)) * a.q_st, kbase, vbase,
+                                             win.tab, lane_of(see, i), lane_of(slope, i), lane_of(p, i), first, hi, lane, m1, l1, o1);
+                for (int ww = 0; ww < NW; ww++)
+                    for (int e = 0; e < D / 64; e++) so[(ww * 32 + i) * SO + lane * (D / 64) + e] = ww ? 0.f : o1[e];
+                if (lane == 0) { s_M[i] = m1; s_L[i] = l1; }
+            }
+            __syncthreads();
+        }
+        const bool whole = ka == 0 && kb == per;
+        const int64_t part = (int64_t)(2 * me + (ka == 0)) * 32;      // a piece's rows
+        // used rows x D values: 8 lanes a row
+        for (int rr = tid >> 3; rr < used; rr += 8 * NW) {
+            const int c8 = tid & 7, g = r0 + rr;
+            const float lr = s_L[rr], inv = lr > 0.f || lr != lr ? 1.f / lr : 0.f;
+            const int gt = g / a.rep, gh = hk * a.rep + g - gt * a.rep;
+            const int64_t at = ((int64_t)(sq.s + gt) * a.Hq + gh) * D;
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) {
+                const int d = 4 * c8 + 32 * i;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int ww = 0; ww < NW; ww++) {
+                    const float4 y = *reinterpret_cast<const float4*>(so + (ww * 32 + rr) * SO + d);
+                    v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+                }
+                if (whole) put4<T>(a.out, nullptr, at + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                else *reinterpret_cast<float4*>(a.po + (part + rr) * D + d) = v;
+            }
+            if (!whole && c8 == 0) a.pm[part + rr] = make_float2(s_M[rr], lr);
+        }
+        if constexpr (STREAM) {
+            if (ka == 0 && kb < per) left = {r, hk, t, sq.n, (int)(((x + per) * G - 1) / total) - me + 1};
+            x += kb - ka;
+        } else {
+            t += gridDim.x;
+        }
+        __syncthreads();                              // the sums are read before the next unit's tiles take their place
+    }
+    // tokens of no row, by workers that are through
+    {
+        const int s0 = min(max(uni(a.starts[0]), 0), a.N), s1 = min(max(uni(a.starts[a.R]), s0), a.N);
+        const int64_t n = (int64_t)a.Hq * D / 8, n0 = s0 * n, n1 = n0 + (a.N - s1) * n, all = (int64_t)gridDim.x * gridDim.y * gridDim.z * 64 * NW;
+        for (int64_t i = ((int64_t)(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * 64 * NW + tid; i < n1; i += all)
+            reinterpret_cast<uint4*>(a.out)[i < n0 ? i : i - n0 + s1 * n] = make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (STREAM) {
+        if (tid == 0) a.join[me] = left;
+    }
+}
+
+// ------------------------------------------------------------------------------------------- join
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a unit's pieces.  A row is D / 4 lanes times NG groups, which take every NG-th piece: a
+// row of hundreds of pieces is as many short chains of loads.  Their sums meet in LDS in order.
+template <typename T, int D, int ROWS, int NG>
+__global__ __launch_bounds__(256) void pages_join(PagedArgs a) {
+    constexpr int LN = D / 4, RW = 256 / (LN * NG);
+    static_assert(RW >= 1, "whole rows");
+    __shared__ __align__(16) float s_o[NG > 1 ? NG : 1][D];
+    __shared__ float s_l[NG];
+    const int me = blockIdx.x;
+    const Unit u = a.join[me];
+    if (u.parts < 2) return;
+    const int c = threadIdx.x % LN, g = NG == 1 ? 0 : threadIdx.x / LN;
+    for (int i = blockIdx.y * RW + (NG == 1 ? threadIdx.x / LN : 0); i < ROWS; i += gridDim.y * RW) {
+        const int row = ROWS * u.t + i;
+        if (row >= u.n * a.rep) return;               // (with several groups: all threads alike)
+        auto slot = [&](int s) { return (int64_t)(s ? 2 * (me + s) : 2 * me + 1) * ROWS + i; };
+        float M = -INFINITY, L = 0.f;
+        if constexpr (NG == 1) {
+            for (int s = 0; s < u.parts; s++) M = fmaxf(M, a.pm[slot(s)].x);
+        } else {
+            for (int s = threadIdx.x & 63; s < u.parts; s += 64) M = fmaxf(M, a.pm[slot(s)].x);
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+        }
+        const float Mu = M == -INFINITY ? 0.f : M;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int s = g; s < u.parts; s += NG) {
+            const float2 x = a.pm[slot(s)];
+            const float f = x.y != 0.f ? exp2_(x.x - Mu) : 0.f;       // otherwise nothing is visible in this piece
+            const float4 o = *reinterpret_cast<const float4*>(a.po + slot(s) * D + 4 * c);
+            L = fmaf(x.y, f, L);
+            acc.x = fmaf(o.x, f, acc.x);
+            acc.y = fmaf(o.y, f, acc.y);
+            acc.z = fmaf(o.z, f, acc.z);
+            acc.w = fmaf(o.w, f, acc.w);
+        }
+        if constexpr (NG > 1) {
+            __syncthreads();                          // the last row's sums are read
+            *reinterpret_cast<float4*>(&s_o[g][4 * c]) = acc;
+            if (c == 0) s_l[g] = L;
+            __syncthreads();
+            if (g) continue;
+            acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            L = 0.f;
+#pragma unroll
+            for (int k = 0; k < NG; k++) {
+                const float4 o = *reinterpret_cast<const float4*>(&s_o[k][4 * c]);
+                L += s_l[k];
+                acc.x += o.x;
+                acc.y += o.y;
+                acc.z += o.z;
+                acc.w += o.w;
+            }
+        }
+        const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+        const int tok = row / a.rep, hq = u.hk * a.rep + row - tok * a.rep;
+        const int s = min(max(a.starts[u.r], 0), a.N);
+        put4<T>(a.out, nullptr, ((int64_t)(s + tok) * a.Hq + hq) * D + 4 * c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    }
+}
+
+// How a call runs.
+//   MANY    tiles of 128 query rows
+//   SHARED  one tile of 32 rows a key/value head (one or a few tokens of each sequence): equal shares of all keys, and a join
+//   SINGLE  the same where no row has many keys: a workgroup a unit, no join
+enum { MANY, SHARED, SINGLE };
+struct Plan { int kind, G; int64_t units; size_t join, pm, po, all; };
+Plan plan(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t most, int64_t W, bool prefix) {
+    Plan x{};
+    const int64_t rep = Hq / Hk, rows = std::min(N, R);
+    const int64_t keys = prefix ? M * page : std::min(M * page, W + most + 32);
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    x.kind = most * rep > 32 ? MANY : keys <= UNIT_KEYS ? SINGLE : SHARED;
+    if (x.kind == SINGLE && (R > 65535 || Hk > 65535)) x.kind = SHARED;
+    if (x.kind == SHARED && (N * rep / 32 + rows) * Hk * ((M * page + 31) / 32) > 0x3fffffffLL) x.kind = MANY;      // (its sums are 32-bit ones)
+    const int64_t Q = x.kind == MANY ? MQ : 32, K = x.kind == MANY ? KT : 32;
+    x.units = N * rep / Q + rows;
+    if (x.kind == SINGLE) return x;
+    const int64_t tiles = x.units * Hk * ((M * page + K - 1) / K);
+    x.G = x.kind == MANY ? (int)std::min<int64_t>(MG, (tiles + 3) / 4) : (int)std::min<int64_t>(FG, std::max<int64_t>(tiles / FS, 1));
+    x.join = x.kind == MANY ? up((size_t)(2 * (R + 1) + x.units + 1) * 4) : 0;
+    x.pm = x.join + up((size_t)x.G * sizeof(Unit));
+    x.po = x.pm + up((size_t)x.G * 2 * Q * sizeof(float2));
+    x.all = x.po + up((size_t)x.G * 2 * Q * D * sizeof(float));
+    return x;
 }
 
 template <typename T, int D, bool CAP, bool BIAS>
-void launch_one(const PagedArgs& a, int G, hipStream_t st) {
-    slothost::launch(pages_many<T, D, CAP, BIAS>, dim3((unsigned)G), dim3(MT), 0, st, a);
+void launch_one(const PagedArgs& a, const Plan& x, int tiles, hipStream_t st) {
+    if (x.kind == MANY) slothost::launch(pages_many<T, D, CAP, BIAS>, dim3((unsigned)x.G), dim3(MT), 0, st, a);
+    else if (x.kind == SHARED) slothost::launch(pages_few<T, D, CAP, BIAS, 1, true>, dim3((unsigned)x.G), dim3(64), 0, st, a);
+    else slothost::launch(pages_few<T, D, CAP, BIAS, FW, false>, dim3((unsigned)tiles, (unsigned)a.Hk, (unsigned)a.R), dim3(64 * FW), 0, st, a);
 }
 template <typename T, int D>
-void launch_attn(const PagedArgs& a, bool cap, int G, hipStream_t st) {
-    if (cap) a.slopes ? launch_one<T, D, true, true>(a, G, st) : launch_one<T, D, true, false>(a, G, st);
-    else a.slopes ? launch_one<T, D, false, true>(a, G, st) : launch_one<T, D, false, false>(a, G, st);
+void launch_attn(const PagedArgs& a, bool cap, const Plan& x, int tiles, hipStream_t st) {
+    if (cap) a.slopes ? launch_one<T, D, true, true>(a, x, tiles, st) : launch_one<T, D, true, false>(a, x, tiles, st);
+    else a.slopes ? launch_one<T, D, false, true>(a, x, tiles, st) : launch_one<T, D, false, false>(a, x, tiles, st);
 }
 template <typename T, int D>
-void launch_join(const PagedArgs& a, int G, hipStream_t st) {
-    slothost::launch(pages_join<T, D>, dim3((unsigned)G, (unsigned)(MQ * (D / 4) / 256)), dim3(256), 0, st, a);
-}
-
-// Room in the workspace: workers, units, and where its parts begin.
-struct Room { int G; int64_t units; size_t plan, join, pm, po, all; };
-Room room(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D) {
-    Room x;
-    x.units = N * (Hq / Hk) / MQ + std::min(N, R);
-    const int64_t tiles = x.units * Hk * ((M * page + KT - 1) / KT);
-    x.G = (int)std::min<int64_t>(MG, (tiles + 3) / 4);
-    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    x.plan = 0;
-    x.join = up((size_t)(2 * (R + 1) + x.units + 1) * 4);
-    x.pm = x.join + up((size_t)x.G * sizeof(Unit));
-    x.po = x.pm + up((size_t)x.G * 2 * MQ * sizeof(float2));
-    x.all = x.po + up((size_t)x.G * 2 * MQ * D * sizeof(float));
-    return x;
+void launch_join(const PagedArgs& a, const Plan& x, int rows, hipStream_t st) {
+    if (x.kind == MANY) slothost::launch(pages_join<T, D, MQ, 1>, dim3((unsigned)x.G, (unsigned)(MQ * (D / 4) / 256)), dim3(256), 0, st, a);
+    else slothost::launch(pages_join<T, D, 32, 1024 / D>, dim3((unsigned)x.G, (unsigned)std::min(rows, 8)), dim3(256), 0, st, a);
 }
 
 }  // namespace
 
 // ======================================================================================== C-ABI
-extern "C" size_t slotattn_pages_workspace(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t most) {
-    (void)most;
-    if (N < 1 || R < 1 || M < 1 || page < 1 || Hk < 1 || Hq < Hk || Hq % Hk || N > SLOTATTN_MAX_T) return 0;
-    return room(N, R, M, page, Hq, Hk, D).all;
+extern "C" size_t slotattn_pages_workspace(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t most,
+                                           int64_t window, int has_prefix) {
+    if (N < 1 || R < 1 || M < 1 || page < 1 || Hk < 1 || Hq < Hk || Hq % Hk || N > SLOTATTN_MAX_T || most < 1 || window < 1) return 0;
+    return plan(N, R, M, page, Hq, Hk, D, std::min(most, N), window, has_prefix).all;
 }
 
 extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sp, int64_t k_sh, int64_t k_st,
@@ -518,11 +858,12 @@ extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const v
     if (M * page > SLOTATTN_MAX_T || P > SLOTATTN_MAX_T || R > 1 << 24 || t_sr < 0 || most < 1)
         return fail(SLOTSCAN_ERR_SHAPE, "slotattn_pages: shape too large");
     if (int r = slotattn_host::check(q, 0, q_sh, q_st, k, k_sp, k_sh, k_st, v, v_sp, v_sh, v_st, dtype, 1, N, page, Hq, Hk, D, scale, window, cap)) return r;
-    if (!table || !starts || !ends || !out || !workspace) return fail(SLOTSCAN_ERR_NULL, "slotattn_pages: a required pointer is NULL");
+    if (!table || !starts || !ends || !out) return fail(SLOTSCAN_ERR_NULL, "slotattn_pages: a required pointer is NULL");
     if (!al16(out) || !al16(workspace)) return fail(SLOTSCAN_ERR_ALIGN, "slotattn_pages: out and workspace must be 16-byte aligned");
-    const Room x = room(N, R, M, page, Hq, Hk, D);
+    const Plan x = plan(N, R, M, page, Hq, Hk, D, std::min(most, N), window, prefix != nullptr);
+    if (x.all && !workspace) return fail(SLOTSCAN_ERR_NULL, "slotattn_pages: workspace is NULL");
     // running costs are 32-bit: tiles of all units of one head
-    if ((x.units + 1) * ((M * page + KT - 1) / KT) > 0x3fffffffLL || Hk > 65535) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_pages: shape too large");
+    if (x.kind == MANY && (x.units + 1) * ((M * page + KT - 1) / KT) > 0x3fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_pages: shape too large");
     PagedArgs a{};
     a.s = slotattn_host::args(q, 0, q_sh, q_st, k, k_sp, k_sh, k_st, v, v_sp, v_sh, v_st, 1, N, page, Hq, Hk, scale, 1, window, cap, slopes, nullptr, prefix);
     a.q = q; a.k = k; a.v = v;
@@ -535,24 +876,26 @@ extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const v
     a.out = out;
     hipStream_t st = (hipStream_t)stream;
     const bool cp = cap > 0.f;
+    const int tiles = (int)((std::min(most, N) * a.rep + 31) / 32), rows = (int)std::min<int64_t>(32, std::min(most, N) * a.rep);
     hipError_t e;
-    {
+    if (x.kind == MANY) {
         slothost::Scope sc(SLOTSCAN_K_ATTN_PLAN, st);
         slothost::launch(pages_plan, dim3(1), dim3(LT), 0, st, a);
         e = hipGetLastError();
+        if (e != hipSuccess) return hip_fail(e, "pages_plan launch");
     }
-    if (e != hipSuccess) return hip_fail(e, "pages_plan launch");
     {
         slothost::Scope sc(SLOTSCAN_K_ATTN, st);
-        if (dtype == SLOTSCAN_BF16) D == 128 ? launch_attn<bf16_t, 128>(a, cp, x.G, st) : launch_attn<bf16_t, 64>(a, cp, x.G, st);
-        else D == 128 ? launch_attn<f16_t, 128>(a, cp, x.G, st) : launch_attn<f16_t, 64>(a, cp, x.G, st);
+        if (dtype == SLOTSCAN_BF16) D == 128 ? launch_attn<bf16_t, 128>(a, cp, x, tiles, st) : launch_attn<bf16_t, 64>(a, cp, x, tiles, st);
+        else D == 128 ? launch_attn<f16_t, 128>(a, cp, x, tiles, st) : launch_attn<f16_t, 64>(a, cp, x, tiles, st);
         e = hipGetLastError();
     }
-    if (e != hipSuccess) return hip_fail(e, "pages_many launch");
+    if (e != hipSuccess) return hip_fail(e, "pages_many or pages_few launch");
+    if (x.kind == SINGLE) return 0;
     {
         slothost::Scope sc(SLOTSCAN_K_ATTN_JOIN, st);
-        if (dtype == SLOTSCAN_BF16) D == 128 ? launch_join<bf16_t, 128>(a, x.G, st) : launch_join<bf16_t, 64>(a, x.G, st);
-        else D == 128 ? launch_join<f16_t, 128>(a, x.G, st) : launch_join<f16_t, 64>(a, x.G, st);
+        if (dtype == SLOTSCAN_BF16) D == 128 ? launch_join<bf16_t, 128>(a, x, rows, st) : launch_join<bf16_t, 64>(a, x, rows, st);
+        else D == 128 ? launch_join<f16_t, 128>(a, x, rows, st) : launch_join<f16_t, 64>(a, x, rows, st);
         e = hipGetLastError();
     }
     return e == hipSuccess ? 0 : hip_fail(e, "pages_join launch");

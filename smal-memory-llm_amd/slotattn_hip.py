@@ -210,7 +210,8 @@ def attend_pages(q, kpages, vpages, table, starts, ends, most=None, scale=None, 
     q_, lib = L.tokens(q), L.lib()
     with L.on(q.device):
         out = torch.empty(N, Hq, D, device=q.device, dtype=q.dtype)
-        ws = torch.empty(lib.slotattn_pages_workspace(N, R, M, page, Hq, Hk, D, most), device=q.device, dtype=torch.uint8)
+        n = lib.slotattn_pages_workspace(N, R, M, page, Hq, Hk, D, most, window, prefix is not None)
+        ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
         rc = lib.slotattn_pages(*L.by_head(q_), *L.strided(kpages), *L.strided(vpages), L._TYPE_CODES[q.dtype], *table_rows(table),
                                 L.ptr(starts), L.ptr(ends), N, R, M, P, page, Hq, Hk, D, most, scale, window, cap, L.ptr(slopes),
                                 L.ptr(prefix), L.ptr(ws), L.ptr(out), L.stream_of(q.device))

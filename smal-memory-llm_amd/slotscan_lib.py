@@ -86,7 +86,7 @@ SIGNATURES = {
                        + _ROWS * 2 + [_vp]),
     "slotpage_extend": (_i32, [_vp, _vp, _vp, _i64, _vp] + [_i64] * 5 + [_vp] * 5),
     "slotpage_trim": (_i32, [_vp, _vp, _vp, _i64, _vp] + [_i64] * 4 + [_vp]),
-    "slotattn_pages_workspace": (_sz, [_i64] * 8),
+    "slotattn_pages_workspace": (_sz, [_i64] * 9 + [_i32]),
     "slotattn_pages": (_i32, _HEADS + _ROWS * 2 + [_i32, _vp, _i64, _vp, _vp] + [_i64] * 9 + [_f32, _i64, _f32] + [_vp] * 5),
     "slotattn_docs_bytes": (_sz, [_i64, _i64]),
     "slotattn_docs": (_i32, [_vp, _i64, _i64, _vp, _vp]),
