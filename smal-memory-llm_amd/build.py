@@ -26,7 +26,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = [os.path.join(CSRC, f) for f in ("slotscan.hip", "slotread.hip", "slotmem.hip", "slotwin.hip", "slotgen.hip",
                                                  "slotproj.hip", "slotrope.hip", "slotattn.hip", "slotattn_bwd.hip",
-                                                 "slotpage.hip", "slotattn_pages.hip")]
+                                                 "slotpage.hip", "slotattn_pages.hip", "slotattn_few.hip")]
 OUT = os.path.join(HERE, "libslotscan.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
