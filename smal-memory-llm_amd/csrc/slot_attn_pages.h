@@ -10,7 +10,11 @@
 
 namespace slotattn {
 
-struct Unit { int r, hk, t, n, parts; };             // what a worker leaves for the join: row, head, tile, tokens, pieces (0: nothing)
+// What is left for the join.  pages_many: of each worker, the unit that begins in it and goes on in the next (row, head, tile, tokens, pieces; 0: none).
+// pages_few: of each unit, the worker in which it begins and its pieces, at ((s rep) / 32 + row + tile) Hk + head, s its sequence's first token:
+// a place of its own for every tile of the batch.
+struct Unit { int r, hk, t, n, parts; };
+struct Piece { int me, parts; };
 
 struct PagedArgs {
     AttnArgs s;                                       // the scores' constants
@@ -20,7 +24,8 @@ struct PagedArgs {
     const int32_t* starts; const int32_t* ends; const int32_t* prefix; const float* slopes;
     int N, R, M, P, Hq, Hk, rep, W, shift, units;     // units: room for them in the plan
     int* plan;                                        // running costs of the rows (R + 1), first units of the rows (R + 1), running costs (units + 1)
-    Unit* join; float* po; float2* pm;                // of every worker; (worker, head or tail, row of the tile)
+    Unit* join; Piece* pieces;
+    float* po; float2* pm;                            // (worker, piece that it begins or goes on with, row of the tile)
     void* out;
 };
 

@@ -81,7 +81,6 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
     const int w = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
     Walker c{};                                       // the tiles that are computed
     int me = 0, total = 0, G = 1;
-    Unit left{0, 0, 0, 0, 0};
     if constexpr (SHARED) {
         const int C = (a.R + 63) / 64;
         int mine = 0;
@@ -241,7 +240,8 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
         const int32_t* tab = a.table + c.r * a.t_sr;
         if constexpr (SHARED) {
             finish<T, D, CAP, BIAS>(a, sum, rw, kb, vb, tab, c.lo + 32 * c.ka, c.hi, c.ka == 0 && c.kb == c.per, (int64_t)(2 * me + (c.ka == 0)) * 32, lane);
-            if (c.ka == 0 && c.kb < c.per) left = {c.r, c.hk, c.t, c.sq.n, Shares(total, G).owner(c.end + c.per - c.kb - 1) - me + 1};
+            if (c.ka == 0 && lane == 0)
+                a.pieces[(((c.sq.s * a.rep) >> 5) + c.r + c.t) * a.Hk + c.hk] = {me, c.kb == c.per ? 1 : Shares(total, G).owner(c.end + c.per - c.kb - 1) - me + 1};
         } else {
             // the waves' parts: (m, l) of every row to all, then the weighted sums through LDS (its tiles are read)
             __shared__ float s_m[NW][32], s_l[NW][32], s_M[32], s_L[32];     // the waves' maxima and sums of every row, the workgroup's
@@ -313,9 +313,6 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
         }
     }
     fill_rest<D>(a, ((int64_t)(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * 64 * NW + tid, (int64_t)gridDim.x * gridDim.y * gridDim.z * 64 * NW);
-    if constexpr (SHARED) {
-        if (tid == 0) a.join[me] = left;
-    }
 }
 
 template <typename T, int D, bool CAP, bool BIAS>

@@ -256,65 +256,111 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------- join
-// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a unit's pieces.  A row is D / 4 lanes times NG groups, which take every NG-th piece: a
-// row of hundreds of pieces is as many short chains of loads.  Their sums meet in LDS in order.
-template <typename T, int D, int ROWS, int NG>
+// A group of D / 4 lanes has 4 columns each of one row: pieces [0, parts) at rows row(s) of the workspace, every `step`-th from `s0` on, as maximum M, sum L and
+// weighted values.  Pieces are read four at a time: a row of many is a few round trips to memory.  (A piece in which nothing is visible has l = 0.)
+template <int D, class ROW> __device__ __forceinline__ void join_pieces(const PagedArgs& a, int s0, int step, int parts, int c, ROW row, float& M, float& L, float4& acc) {
+    M = -INFINITY;
+    L = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = s0; s < parts; s += 4 * step) {
+        float2 x[4];
+        float4 o[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int64_t at = row(min(s + k * step, parts - 1));
+            x[k] = a.pm[at];
+            o[k] = *reinterpret_cast<const float4*>(a.po + at * D + 4 * c);
+            if (s + k * step >= parts) x[k] = make_float2(-INFINITY, 0.f);
+        }
+        const float mn = fmaxf(fmaxf(fmaxf(M, x[0].x), fmaxf(x[1].x, x[2].x)), x[3].x), mu = mn == -INFINITY ? 0.f : mn, f0 = exp2_(M - mu);
+        L *= f0;
+        acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const bool any = x[k].y != 0.f;
+            const float f = any ? exp2_(x[k].x - mu) : 0.f;
+            if (!any) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            L = fmaf(x[k].y, f, L);
+            acc.x = fmaf(o[k].x, f, acc.x);
+            acc.y = fmaf(o[k].y, f, acc.y);
+            acc.z = fmaf(o[k].z, f, acc.z);
+            acc.w = fmaf(o[k].w, f, acc.w);
+        }
+        M = mn;
+    }
+}
+// Row `row` of sequence r's packed rows of head hk, columns 4 c ..
+template <typename T, int D> __device__ __forceinline__ void put_joined(const PagedArgs& a, int s, int hk, int row, int c, float L, const float4& o) {
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+    const int tok = row / a.rep, hq = hk * a.rep + row - tok * a.rep;
+    put4<T>(a.out, nullptr, ((int64_t)(s + tok) * a.Hq + hq) * D + 4 * c, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// Pieces of pages_many: a worker whose last unit goes on in the next ones; a group of lanes a row.
+template <typename T, int D>
 __global__ __launch_bounds__(256) void pages_join(PagedArgs a) {
-    constexpr int LN = D / 4, RW = 256 / (LN * NG);
-    static_assert(RW >= 1, "whole rows");
-    __shared__ __align__(16) float s_o[NG > 1 ? NG : 1][D];
-    __shared__ float s_l[NG];
+    constexpr int LN = D / 4, RW = 256 / LN;
     const int me = blockIdx.x;
     const Unit u = a.join[me];
-    if (u.parts < 2) return;
-    const int c = threadIdx.x % LN, g = NG == 1 ? 0 : threadIdx.x / LN;
-    for (int i = blockIdx.y * RW + (NG == 1 ? threadIdx.x / LN : 0); i < ROWS; i += gridDim.y * RW) {
-        const int row = ROWS * u.t + i;
-        if (row >= u.n * a.rep) return;               // (with several groups: all threads alike)
-        auto slot = [&](int s) { return (int64_t)(s ? 2 * (me + s) : 2 * me + 1) * ROWS + i; };
-        float M = -INFINITY, L = 0.f;
-        if constexpr (NG == 1) {
-            for (int s = 0; s < u.parts; s++) M = fmaxf(M, a.pm[slot(s)].x);
-        } else {
-            for (int s = threadIdx.x & 63; s < u.parts; s += 64) M = fmaxf(M, a.pm[slot(s)].x);
+    const int i = blockIdx.y * RW + threadIdx.x / LN, c = threadIdx.x % LN, row = MQ * u.t + i;
+    if (u.parts < 2 || row >= u.n * a.rep) return;
+    float M, L;
+    float4 acc;
+    join_pieces<D>(a, 0, 1, u.parts, c, [&](int s) { return (int64_t)(s ? 2 * (me + s) : 2 * me + 1) * MQ + i; }, M, L, acc);
+    put_joined<T, D>(a, min(max(a.starts[u.r], 0), a.N), u.hk, row, c, L, acc);
+}
+
+// Pieces of pages_few: a row may have hundreds.  A workgroup has `per` of the (row of the batch, head) pairs, and of their units every gridDim.y-th query
+// row, one at a time; its NG groups of lanes take every NG-th piece and meet in LDS in order.
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per) {
+    constexpr int LN = D / 4, NG = NT / LN;
+    __shared__ __align__(16) float s_o[NG][D];
+    __shared__ float2 s_m[NG];
+    const int lane = threadIdx.x & 63, c = threadIdx.x % LN, g = threadIdx.x / LN;
+    const int u0 = blockIdx.x * per, u1 = min(a.R * a.Hk, u0 + per);
+    for (int b0 = u0; b0 < u1; b0 += 64) {
+        const int u = b0 + lane, r = min(u, u1 - 1) / a.Hk, hk = min(u, u1 - 1) - r * a.Hk;
+        const Seq x = seq_of(a, r);
+        const int rows = x.n * a.rep, at = ((x.s * a.rep) >> 5) + r;
+        Piece p{0, 0};
+        if (rows && u < u1) p = a.pieces[at * a.Hk + hk];
+        for (uint64_t b = __ballot(u < u1 && (p.parts > 1 || rows > 32)); b; b &= b - 1) {
+            const int k = __builtin_ctzll(b), n = lane_of(rows, k), hd = lane_of(hk, k), s = lane_of(x.s, k), at0 = lane_of(at, k);
+            Piece q{lane_of(p.me, k), lane_of(p.parts, k)};
+            for (int t = 0; 32 * t < n; t++) {
+                if (t) q = a.pieces[(at0 + t) * a.Hk + hd];
+                if (q.parts < 2) continue;
+                for (int i = blockIdx.y; i < min(32, n - 32 * t); i += gridDim.y) {
+                    float M, L;
+                    float4 acc;
+                    join_pieces<D>(a, g, NG, q.parts, c, [&](int z) { return (int64_t)(z ? 2 * (q.me + z) : 2 * q.me + 1) * 32 + i; }, M, L, acc);
+                    __syncthreads();                  // the last row's sums are read
+                    *reinterpret_cast<float4*>(&s_o[g][4 * c]) = acc;
+                    if (c == 0) s_m[g] = make_float2(M, L);
+                    __syncthreads();
+                    if (g == 0) {
+                        M = -INFINITY;
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
-        }
-        const float Mu = M == -INFINITY ? 0.f : M;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int s = g; s < u.parts; s += NG) {
-            const float2 x = a.pm[slot(s)];
-            const float f = x.y != 0.f ? exp2_(x.x - Mu) : 0.f;       // otherwise nothing is visible in this piece
-            const float4 o = *reinterpret_cast<const float4*>(a.po + slot(s) * D + 4 * c);
-            L = fmaf(x.y, f, L);
-            acc.x = fmaf(o.x, f, acc.x);
-            acc.y = fmaf(o.y, f, acc.y);
-            acc.z = fmaf(o.z, f, acc.z);
-            acc.w = fmaf(o.w, f, acc.w);
-        }
-        if constexpr (NG > 1) {
-            __syncthreads();                          // the last row's sums are read
-            *reinterpret_cast<float4*>(&s_o[g][4 * c]) = acc;
-            if (c == 0) s_l[g] = L;
-            __syncthreads();
-            if (g) continue;
-            acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            L = 0.f;
+                        for (int z = 0; z < NG; z++) M = fmaxf(M, s_m[z].x);
+                        const float Mu = M == -INFINITY ? 0.f : M;
+                        L = 0.f;
+                        acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < NG; k++) {
-                const float4 o = *reinterpret_cast<const float4*>(&s_o[k][4 * c]);
-                L += s_l[k];
-                acc.x += o.x;
-                acc.y += o.y;
-                acc.z += o.z;
-                acc.w += o.w;
+                        for (int z = 0; z < NG; z++) {
+                            const float f = exp2_(s_m[z].x - Mu);
+                            const float4 o = *reinterpret_cast<const float4*>(&s_o[z][4 * c]);
+                            L = fmaf(s_m[z].y, f, L);
+                            acc.x = fmaf(o.x, f, acc.x);
+                            acc.y = fmaf(o.y, f, acc.y);
+                            acc.z = fmaf(o.z, f, acc.z);
+                            acc.w = fmaf(o.w, f, acc.w);
+                        }
+                        put_joined<T, D>(a, s, hd, 32 * t + i, c, L, acc);
+                    }
+                }
             }
         }
-        const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-        const int tok = row / a.rep, hq = u.hk * a.rep + row - tok * a.rep;
-        const int s = min(max(a.starts[u.r], 0), a.N);
-        put4<T>(a.out, nullptr, ((int64_t)(s + tok) * a.Hq + hq) * D + 4 * c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     }
 }
 
@@ -338,7 +384,7 @@ Plan plan(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk,
     const int64_t tiles = x.units * Hk * ((M * page + K - 1) / K);
     x.G = x.kind == MANY ? (int)std::min<int64_t>(MG, (tiles + 3) / 4) : (int)std::min<int64_t>(FG, std::max<int64_t>(tiles / FS, 1));
     x.join = x.kind == MANY ? up((size_t)(2 * (R + 1) + x.units + 1) * 4) : 0;
-    x.pm = x.join + up((size_t)x.G * sizeof(Unit));
+    x.pm = x.join + up(x.kind == MANY ? (size_t)x.G * sizeof(Unit) : (size_t)(N * rep / 32 + R) * Hk * sizeof(Piece));
     x.po = x.pm + up((size_t)x.G * 2 * Q * sizeof(float2));
     x.all = x.po + up((size_t)x.G * 2 * Q * D * sizeof(float));
     return x;
@@ -355,8 +401,15 @@ void launch_attn(const PagedArgs& a, bool cap, int G, hipStream_t st) {
 }
 template <typename T, int D>
 void launch_join(const PagedArgs& a, const Plan& x, int rows, hipStream_t st) {
-    if (x.kind == MANY) slothost::launch(pages_join<T, D, MQ, 1>, dim3((unsigned)x.G, (unsigned)(MQ * (D / 4) / 256)), dim3(256), 0, st, a);
-    else slothost::launch(pages_join<T, D, 32, 1024 / D>, dim3((unsigned)x.G, (unsigned)std::min(rows, 8)), dim3(256), 0, st, a);
+    if (x.kind == MANY) {
+        slothost::launch(pages_join<T, D>, dim3((unsigned)x.G, (unsigned)(MQ * (D / 4) / 256)), dim3(256), 0, st, a);
+        return;
+    }
+    // few units have many pieces each
+    const int pairs = a.R * a.Hk, per = (pairs + 2047) / 2048, grid = (pairs + per - 1) / per;
+    const dim3 blocks((unsigned)grid, (unsigned)std::max(1, std::min(rows, 4096 / grid)));
+    if (pairs <= 32) slothost::launch(pages_join_few<T, D, 1024>, blocks, dim3(1024), 0, st, a, per);
+    else slothost::launch(pages_join_few<T, D, 256>, blocks, dim3(256), 0, st, a, per);
 }
 
 }  // namespace
@@ -392,7 +445,7 @@ extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const v
     a.N = (int)N; a.R = (int)R; a.M = (int)M; a.P = (int)P; a.Hq = (int)Hq; a.Hk = (int)Hk; a.rep = (int)(Hq / Hk);
     a.W = a.s.W; a.shift = __builtin_ctzll((unsigned long long)page); a.units = (int)x.units;
     char* ws = (char*)workspace;
-    a.plan = (int*)ws; a.join = (Unit*)(ws + x.join); a.pm = (float2*)(ws + x.pm); a.po = (float*)(ws + x.po);
+    a.plan = (int*)ws; a.join = (Unit*)(ws + x.join); a.pieces = (Piece*)(ws + x.join); a.pm = (float2*)(ws + x.pm); a.po = (float*)(ws + x.po);
     a.out = out;
     hipStream_t st = (hipStream_t)stream;
     const bool cp = cap > 0.f;
