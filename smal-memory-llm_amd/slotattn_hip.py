@@ -204,16 +204,14 @@ def attend_pages(q, kpages, vpages, table, starts, ends, most=None, scale=None, 
     _same_device(what, q, kpages, vpages, table, starts, ends, slopes, prefix)
     if N * R * M * P == 0:
         return torch.zeros(N, Hq, D, device=q.device, dtype=q.dtype)
-    slopes, prefix = (None if x is None else x.contiguous() for x in (slopes, prefix))
+    slopes, prefix = None if slopes is None else slopes.contiguous(), None if prefix is None else prefix.contiguous()
     most = N if most is None else min(max(int(most), 1), N)
     scale, _, window, cap = _opts(q, scale, True, window, cap)
-    q_, lib = L.tokens(q), L.lib()
-    with L.on(q.device):
-        out = torch.empty(N, Hq, D, device=q.device, dtype=q.dtype)
-        n = lib.slotattn_pages_workspace(N, R, M, page, Hq, Hk, D, most, window, prefix is not None)
-        ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
-        rc = lib.slotattn_pages(*L.by_head(q_), *L.strided(kpages), *L.strided(vpages), L._TYPE_CODES[q.dtype], *table_rows(table),
-                                L.ptr(starts), L.ptr(ends), N, R, M, P, page, Hq, Hk, D, most, scale, window, cap, L.ptr(slopes),
-                                L.ptr(prefix), L.ptr(ws), L.ptr(out), L.stream_of(q.device))
-    L.check(rc, "slotattn_pages")
+    q_, lib, dev = L.tokens(q), L.lib(), q.device
+    out = torch.empty(N, Hq, D, device=dev, dtype=q.dtype)
+    n = lib.slotattn_pages_workspace(N, R, M, page, Hq, Hk, D, most, window, prefix is not None)
+    ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
+    L.call(lib.slotattn_pages, what, dev, *L.by_head(q_), *L.strided(kpages), *L.strided(vpages), L._TYPE_CODES[q.dtype], *table_rows(table),
+           starts.data_ptr(), ends.data_ptr(), N, R, M, P, page, Hq, Hk, D, most, scale, window, cap, L.ptr(slopes), L.ptr(prefix), L.ptr(ws),
+           out.data_ptr())
     return out

@@ -37,8 +37,8 @@ PageStep = namedtuple("PageStep", "starts ends slots pos")
 
 
 def check_table(table, what):
-    R, M = table.shape
-    if table.dtype != torch.int32 or M > 1 and table.stride(1) != 1 or R > 1 and table.stride(0) < M:
+    (R, M), (sr, sm) = table.shape, table.stride()
+    if table.dtype is not torch.int32 or M > 1 and sm != 1 or R > 1 and sr < M:
         raise ValueError(f"{what}: table must be int32 (R, M) with contiguous rows that are apart (got {table.dtype}, "
                          f"{tuple(table.shape)}, strides {table.stride()})")
 
@@ -77,15 +77,13 @@ def page_extend(new, lens, table, free, page, N):
     R, M, P = _check(new, "new", lens, table, free, page, what)
     if N < 0:
         raise ValueError(f"{what}: N must be >= 0 (got {N})")
-    dev = table.device
-    e = lambda n, dt=torch.int32: torch.empty(n, device=dev, dtype=dt)
-    step = PageStep(e(R + 1), e(R), e(N, torch.int64), e(N))
-    with L.on(dev):
-        rc = L.lib().slotpage_extend(L.ptr(new), L.ptr(lens), *table_rows(table), L.ptr(free), R, M, P, page, N, L.ptr(step.starts),
-                                     L.ptr(step.ends), L.ptr(step.slots), L.ptr(step.pos), L.stream_of(dev))
-    L.check(rc, what)
+    dev, i32 = table.device, torch.int32
+    slots, pos, starts, ends = torch.empty(3 * N + 2 * R + 1, device=dev, dtype=i32).split_with_sizes((2 * N, N, R + 1, R))   # one allocation
+    slots = slots.view(torch.int64)
+    L.call(L.lib().slotpage_extend, what, dev, new.data_ptr(), lens.data_ptr(), *table_rows(table), free.data_ptr(), R, M, P, page, N,
+           starts.data_ptr(), ends.data_ptr(), slots.data_ptr(), pos.data_ptr())
     _written(lens, table, free)
-    return step
+    return PageStep(starts, ends, slots, pos)
 
 
 def page_trim(keep, lens, table, free, page):
@@ -93,8 +91,5 @@ def page_trim(keep, lens, table, free, page):
     what = "page_trim"
     page = int(page)
     R, M, P = _check(keep, "keep", lens, table, free, page, what)
-    dev = table.device
-    with L.on(dev):
-        rc = L.lib().slotpage_trim(L.ptr(keep), L.ptr(lens), *table_rows(table), L.ptr(free), R, M, P, page, L.stream_of(dev))
-    L.check(rc, what)
+    L.call(L.lib().slotpage_trim, what, table.device, keep.data_ptr(), lens.data_ptr(), *table_rows(table), free.data_ptr(), R, M, P, page)
     _written(lens, table, free)

@@ -65,6 +65,13 @@ def _check_rows(q, k, wq, wk, freqs, what):
 
 
 def _same_device(what, *ts):
+    d = ts[0].get_device()                               # (numbers compare faster than devices)
+    if d >= 0:
+        for t in ts:
+            if t is not None and t.get_device() != d:
+                break
+        else:
+            return
     dev = ts[0].device
     for t in ts:
         if t is not None and t.device != dev:
@@ -227,6 +234,10 @@ def qk_rope_cache(q, k, v, wq, wk, freqs, lens, kcache, vcache, eps=1e-6, interl
 
 
 def _check_written(kcache, vcache, what):
+    n, d = kcache.numel() * kcache.element_size(), kcache.data_ptr() - vcache.data_ptr()
+    if kcache.is_contiguous() and vcache.is_contiguous() and (d >= n or -d >= n) and not (kcache.data_ptr() | vcache.data_ptr()) % 16 \
+            and kcache.shape[2] * kcache.shape[3] < 1 << 25:
+        return                                           # the common case (2 us less)
     for c in (kcache, vcache):
         if not _apart(c) or not L.in_place(c):
             raise ValueError(f"{what}: a cache is written in place: its rows must be contiguous, 16-byte aligned and apart")
@@ -236,9 +247,10 @@ def _check_written(kcache, vcache, what):
 
 def _written(*xs):
     """Raises the versions of tensors that a kernel wrote."""
-    xs = [x for x in xs if not x.is_inference()]         # (those have no version)
-    if xs:
-        torch.autograd.graph.increment_version(xs)
+    try:
+        torch._C._increment_version(xs)
+    except RuntimeError:                                 # inference tensors have none
+        torch._C._increment_version([x for x in xs if not x.is_inference()])
 
 
 def check_pools(kpages, vpages, like, Hk, what):
@@ -256,7 +268,7 @@ def check_page(page, what):
 
 
 def check_ints(x, shape, dtype, what, name):
-    if x.dtype != dtype or tuple(x.shape) != shape or not x.is_contiguous():
+    if x.dtype is not dtype or x.shape != shape or not x.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous {str(dtype)[6:]} {shape} (got {x.dtype}, {tuple(x.shape)})")
 
 
@@ -277,21 +289,17 @@ def qk_rope_pages(q, k, v, wq, wk, freqs, pos, slots, kpages, vpages, eps=1e-6, 
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, wq, wk, kpages, vpages)):
         raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
     P, page = kpages.shape[0], kpages.shape[2]
-    if P:
-        _check_written(kpages, vpages, what)
-    _same_device(what, q, k, v, wq, wk, freqs, pos, slots, kpages, vpages)
     if not P:
         raise ValueError(f"{what}: there are no pages to write into")
+    _check_written(kpages, vpages, what)
+    _same_device(what, q, k, v, wq, wk, freqs, pos, slots, kpages, vpages)
     q_, k_, v_ = L.tokens(q), L.tokens(k), L.tokens(v)
     wq_, wk_, wt = _gains(wq, wk)
     freqs = freqs.contiguous()
     qo = torch.empty(N, Hq, D, device=q.device, dtype=q.dtype)
     if N:
-        with L.on(q.device):
-            rc = L.lib().slotrope_pages(*L.by_head(q_), *L.by_head(k_), *L.by_head(v_), L._TYPE_CODES[q.dtype], L.ptr(wq_), L.ptr(wk_),
-                                        wt, L.ptr(freqs), 2 * freqs.numel(), int(bool(interleaved)), L.ptr(pos), L.ptr(slots), N, Hq,
-                                        Hk, D, P, page, float(eps), L.ptr(qo), *L.strided(kpages), *L.strided(vpages),
-                                        L.stream_of(q.device))
-        L.check(rc, what)
+        L.call(L.lib().slotrope_pages, what, q.device, *L.by_head(q_), *L.by_head(k_), *L.by_head(v_), L._TYPE_CODES[q.dtype], L.ptr(wq_),
+               L.ptr(wk_), wt, freqs.data_ptr(), 2 * freqs.numel(), int(bool(interleaved)), pos.data_ptr(), slots.data_ptr(), N, Hq, Hk, D,
+               P, page, float(eps), qo.data_ptr(), *L.strided(kpages), *L.strided(vpages))
         _written(kpages, vpages)
     return qo
