@@ -11,8 +11,8 @@
 namespace slotattn {
 
 // What is left for the join.  pages_many: of each worker, the unit that begins in it and goes on in the next (row, head, tile, tokens, pieces; 0: none).
-// pages_few: of each unit, the worker in which it begins and its pieces, at ((s rep) / 32 + row + tile) Hk + head, s its sequence's first token:
-// a place of its own for every tile of the batch.
+// pages_few: of each unit, the worker in which it begins and its pieces, at ((s rep) / QR + row + tile) Hk + head, s its sequence's first token:
+// a place of its own for every tile of QR rows of the batch.
 struct Unit { int r, hk, t, n, parts; };
 struct Piece { int me, parts; };
 
@@ -68,74 +68,120 @@ struct Shares {
     }
 };
 
-// The pages of a tile's groups of 16 keys from j0 on.  A number outside of the pool stands for page 0, and its group's bit says that its keys are
-// not seen; a group behind the sequence's last key has that key's page.
+// The pages of a tile's groups of 16 keys from j0 on.  fetch() asks for their numbers and check() looks at them, a tile later: a number outside of the
+// pool stands for page 0, and its group's bit says that its keys are not seen.  A group behind the sequence's last key has that key's page.
 template <int GROUPS> struct Pages {
     int id[GROUPS];
     uint32_t lost;
-    __device__ __forceinline__ void fetch(const PagedArgs& a, int64_t row, int j0, int klen) {
+    __device__ __forceinline__ void fetch(const PagedArgs& a, int64_t row, int j0, int last) {
+        id[0] = ld_uni(a.table, row + (j0 >> a.shift));
+        if (16 * GROUPS >> a.shift > 1) {
+#pragma unroll
+            for (int g = 1; g < GROUPS; g++) id[g] = ld_uni(a.table, row + (min(j0 + 16 * g, last) >> a.shift));
+        }
+    }
+    __device__ __forceinline__ void check(const PagedArgs& a) {
+        if (16 * GROUPS >> a.shift <= 1) {            // one page
+            const bool bad = (unsigned)id[0] >= (unsigned)a.P;
+            id[0] = bad ? 0 : id[0];
+            lost = bad ? (1u << GROUPS) - 1 : 0u;
+            return;
+        }
         lost = 0;
 #pragma unroll
         for (int g = 0; g < GROUPS; g++) {
-            id[g] = ld_uni(a.table, row + (min(j0 + 16 * g, klen - 1) >> a.shift));
-            if ((unsigned)id[g] >= (unsigned)a.P) {
-                id[g] = 0;
-                lost |= 1u << g;
-            }
+            const bool bad = (unsigned)id[g] >= (unsigned)a.P;
+            id[g] = bad ? 0 : id[g];
+            lost |= bad ? 1u << g : 0u;
         }
     }
 };
 
 // One direct load as dma16s's, whose base is in scalar registers already
-template <typename T> __device__ __forceinline__ const T* scalar_ptr(const T* x) {
-    const uint64_t p = (uint64_t)x;
-    return (const T*)(((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)p));
-}
-__device__ __forceinline__ void dma16b(const void* base, unsigned off, unsigned lds) {
+__device__ __forceinline__ void dma16b(uint64_t base, unsigned off, unsigned lds) {
     // five wait states for a base that the vector unit has just written
     asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" : : "{m0}"(lds), "v"(off), "s"(base) : "memory");
 }
-// Direct loads of a tile of ROWS keys by wave w of NW, laid out as TileLoad's.  A group of 16 keys is of one page: its base is formed once, and a
-// lane's offsets within a group are held in registers.
+// Direct loads of a tile of ROWS keys by wave w of NW, laid out as TileLoad's.  A group of 16 keys is of one page: its address is formed once, by
+// the scalar unit, and a lane's offsets within a group are held in registers.  (With 64-bit products for every load they were half of a wave's instructions.)
 template <int D, int ROWS, int NW> struct PageLoad {
     static constexpr int N = ROWS * 2 * D / 1024 / NW, RPL = 512 / D;  // loads per wave, rows per load
     static constexpr int VAR = RPL * NW >= 16 ? 1 : 16 / (RPL * NW);  // loads of one group
+    static constexpr int GROUPS = ROWS / 16, GPL = RPL * NW > 16 ? 2 : 1;                // groups of one load of all waves
     static_assert(NW == 1 || VAR == 1, "one load a group, or all of them");
-    unsigned off[VAR];
-    int64_t sp, st;
-    int w, lane, in;                                  // in: rows of a page, less one
-    __device__ __forceinline__ PageLoad(int64_t page_stride, int64_t stride, int shift, int wave, int l)
-        : sp(page_stride), st(stride), w(wave), lane(l), in((1 << shift) - 1) {
+    unsigned off[VAR], sp, st;                        // sp, st: bytes between pages and between rows
+    int w, lane, shift;
+    __device__ __forceinline__ PageLoad(int64_t page_stride, int64_t stride, int shift_, int wave, int l)
+        : sp((unsigned)(2 * page_stride)), st((unsigned)(2 * stride)), w(wave), lane(l), shift(shift_) {
 #pragma unroll
-        for (int i = 0; i < VAR; i++) off[i] = (unsigned)((RPL * (NW * i + w) & 15) + lane / Tile<D>::CH) * (unsigned)(2 * st) + 16 * chunk(i);
+        for (int i = 0; i < VAR; i++) off[i] = (unsigned)((RPL * (NW * i + w) & 15) + lane / Tile<D>::CH) * st + 16 * chunk(i);
     }
     __device__ __forceinline__ int row(int i) const { return RPL * (NW * i + w) + lane / Tile<D>::CH; }
     __device__ __forceinline__ int chunk(int i) const { return Tile<D>::pos(row(i), lane % Tile<D>::CH); }
-    // keys j0 .. (a multiple of 32), `last` the sequence's last (>= j0), which stands for those behind it
-    template <typename T> __device__ __forceinline__ void issue(const T* base, const Pages<ROWS / 16>& pg, int j0, int last, unsigned lds) const {
+    // keys j0 .. (a multiple of ROWS), `last` the sequence's last (>= j0), which stands for those behind it
+    template <typename T> __device__ __forceinline__ void issue(const T* base, const Pages<GROUPS>& pg, int j0, int last, unsigned lds) const {
+        const uint64_t p = (uint64_t)base;
+        const int in = (1 << shift) - 1;
+        uint64_t b[GROUPS];
+        b[0] = p + (uint64_t)(unsigned)pg.id[0] * sp + (uint64_t)(unsigned)(j0 & in) * st;
+        if (in >= ROWS - 1) {                         // the tile is of one page
+#pragma unroll
+            for (int g = 1; g < GROUPS; g++) b[g] = b[g - 1] + 16 * (uint64_t)st;
+        } else {                                      // it begins with a page
+#pragma unroll
+            for (int g = 1; g < GROUPS; g++) b[g] = p + (uint64_t)(unsigned)pg.id[g] * sp + (16 * g & in ? 16 * (uint64_t)st : 0);
+        }
         if (last - j0 >= ROWS - 1) {
-            const T* p = nullptr;
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                if (i % VAR == 0) {
-                    const int g = RPL * (NW * i + w) / 16;
-                    int id = pg.id[RPL * NW * i / 16];
-                    if constexpr (RPL * NW > 16) id = g & 1 ? pg.id[(RPL * NW * i / 16 + 1) % (ROWS / 16)] : id;     // (a load a wave over two groups)
-                    p = scalar_ptr(base + id * sp + ((j0 + 16 * g) & in) * st);
-                }
-                dma16b(p, off[i % VAR], lds + 1024u * (NW * i + w));
+                constexpr int S = RPL * NW / 16;
+                uint64_t x = b[RPL * NW * i / 16];
+                if constexpr (GPL == 2) x = w >= NW / 2 ? b[(S * i + 1) % GROUPS] : x;
+                dma16b(x, off[i % VAR], lds + 1024u * (NW * i + w));
             }
         } else {
+            const int gl = (last - j0) >> 4;          // the last key's group
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int g = RPL * (NW * i + w) / 16;
-                int id = pg.id[RPL * NW * i / 16];
-                if constexpr (RPL * NW > 16) id = g & 1 ? pg.id[(RPL * NW * i / 16 + 1) % (ROWS / 16)] : id;
-                const int j = min(j0 + row(i), last);
-                dma16(base + id * sp + (j & in) * st + 8 * chunk(i), lds + 1024u * (NW * i + w));
+                const int gi = min(RPL * (NW * i + w) / 16, gl);
+                uint64_t x = b[0];
+#pragma unroll
+                for (int g = 1; g < GROUPS; g++) x = gi == g ? b[g] : x;
+                dma16b(x, (unsigned)(min(row(i), last - j0) - 16 * gi) * st + 16 * chunk(i), lds + 1024u * (NW * i + w));
             }
         }
     }
+};
+
+// The way through a unit's tiles of STEP keys: [lo, hi) without the gap that may lie between a prefix and the band, from the first-th one on, NW tiles at
+// a time
+template <int STEP, int NW> struct Steps {
+    int j, hi, gap0, gap1;
+    __device__ __forceinline__ void enter(const PagedArgs& a, const Seq& x, int p0, int lo, int hi_, int first) {
+        j = lo + STEP * (first - NW);
+        hi = hi_;
+        gap0 = (x.pre + STEP - 1) & ~(STEP - 1);
+        gap1 = x.pre > 0 ? max(0, max(p0, 0) - a.W + 1) & ~(STEP - 1) : 0;
+    }
+    __device__ __forceinline__ bool next() {
+        j += STEP * NW;
+        if (j >= gap0 && j < gap1) j += (gap1 - j + STEP * NW - 1) / (STEP * NW) * (STEP * NW);
+        return j < hi;
+    }
+};
+// Keys of which rows at positions [p0, p1] see all: [f0, f1], and those up to f2.  Of any others they see some: [s0, s1], and those below s2.
+struct Sight {
+    int f0, f1, f2, s0, s1, s2;
+    __device__ __forceinline__ Sight(const PagedArgs& a, const Seq& x, int p0, int p1) {
+        f0 = max(0, p1 - a.W + 1);
+        f1 = min(p0, x.klen - 1);
+        f2 = p0 >= 0 ? min(x.pre, x.klen) - 1 : -1;
+        s0 = max(0, p0 - a.W + 1);
+        s1 = min(p1, x.klen - 1);
+        s2 = p1 >= 0 ? min(x.pre, x.klen) : 0;
+    }
+    __device__ __forceinline__ bool all(int j0, int j1) const { return (j0 >= f0 && j1 <= f1) || j1 <= f2; }
+    __device__ __forceinline__ bool some(int j0, int j1) const { return (j1 >= s0 && j0 <= s1) || j0 < s2; }
 };
 
 // One query's softmax over keys [lo, hi) from its visible pairs alone (slot_attn.h's exact_row, the rows found through the table)

@@ -1,8 +1,15 @@
 // Attention over a cache in pages where a sequence has few query rows: a generated token, a few guessed ones (slot_attn_pages.h).
 //
-// One 32-row tile of a key/value head against 32-key tiles, each wave through a ring of its own of two tiles without a barrier in the loop.
+// A unit is one tile of 16 NQ query rows of a key/value head, against 32-key tiles; each wave goes through a ring of its own of two tiles without a
+// barrier in the loop.
 //   SHARED  every wave is a worker with an equal share of all units' tiles; keys are fetched across the units' borders
 //   SINGLE  a workgroup's NW waves share one unit, every NW-th tile each, and meet in LDS: no join behind it
+//
+// Operands of v_mfma_f32_16x16x32 (16-bit inputs): lane l holds 8 consecutive k values 8 (l >> 4) .. + 7 of row (A) or column (B) l & 15; register r of
+// the result holds row 4 (l >> 4) + r of column l & 15.  With the keys as rows a lane's scores are one query's, and those of two blocks of 16 keys
+// are the B operand of the next product over 32 keys in the order that two transposing LDS reads give its A operand.  The keys of a block go to rows in the
+// order of key_row: a transposing read then meets every bank once (its lanes 0 .. 31 have rows 0 .. 3 and 8 .. 11).
+// One wave's 32 keys are about 450 instructions at D = 128 and 16 rows; with tiles of 32 x 32, whose rows are mostly empty, twice that.
 #include "slot_attn_pages.h"
 #include "slotscan.h"
 #include "slot_attn_few.h"
@@ -10,6 +17,106 @@
 using namespace slotattn;
 
 namespace {
+
+template <typename T> __device__ __forceinline__ f32x4 mfma16(const uint4& a, const uint4& b, f32x4 c);
+template <> __device__ __forceinline__ f32x4 mfma16<bf16_t>(const uint4& a, const uint4& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 mfma16<f16_t>(const uint4& a, const uint4& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ int swap12(int x) { return ((x & 1) << 1) | (x >> 1); }        // 0, 2, 1, 3
+__device__ __forceinline__ int key_row(int m) { return 4 * swap12(m >> 2) + (m & 3); }    // the key of row m of a block
+// over the four lanes of a query, l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float quad_max(float v) {
+    auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return half_max(fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1])));
+}
+
+// The scores' forms (slot_attn.h), for N values
+template <bool CAP, int N> __device__ __forceinline__ void scores_n(float (&s)[N], const AttnArgs& a) {
+    if constexpr (CAP) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) m = fmaxf(m, fabsf(s[i]));
+        if (__all(m <= a.lim)) {
+#pragma unroll
+            for (int i = 0; i < N; i++) s[i] = tanh_poly(s[i], a);
+        } else if (a.mix) {
+#pragma unroll
+            for (int i = 0; i < N; i++) s[i] = tanh_mix(s[i], a);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) s[i] = tanh_exp(s[i], a);
+        }
+    }
+}
+
+// A tile's rows: 16 query rows, one a lane and group of 16 lanes
+template <typename T, int D, bool BIAS> struct Rows16 {
+    static constexpr int DB = D / 16, KS = D / 32;
+    f32x4 o[DB];
+    float m, mu, l;                                   // a row's reference, the same in base 2, its sum
+    bool far;
+    uint4 q[KS];
+    int tok, hq, p;
+    Sees see;
+    float slope;
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < DB; i++) o[i] = {0.f, 0.f, 0.f, 0.f};
+        m = -INFINITY;
+        mu = l = 0.f;
+        far = false;
+    }
+    // 32 scores' worth of 8 values a lane become probabilities as an operand (slot_attn_rows.h)
+    __device__ __forceinline__ uint4 weigh(float (&s)[8], float F, float lazy, float head) {
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[i]);
+        mx = quad_max(mx) - head;
+        if (__any(mx > m + lazy)) {
+            const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_((m - mn) * F);
+            m = mn;
+            mu = m == -INFINITY ? 0.f : m * F;
+            far = __any(fabsf(mu) > FAR);
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < DB; i++) o[i] *= f;
+        }
+        if (far) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i] = (s[i] - (m == -INFINITY ? 0.f : m)) * F;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i] = fmaf(s[i], F, -mu);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            s[i] = exp2_(s[i]);
+            l += s[i];
+        }
+        return make_uint4(pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3]), pack2<T>(s[4], s[5]), pack2<T>(s[6], s[7]));
+    }
+    __device__ __forceinline__ void close() {
+        auto p2 = __builtin_amdgcn_permlane16_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = half_sum(__uint_as_float(p2[0]) + __uint_as_float(p2[1]));
+        m = m == -INFINITY ? m : mu;
+    }
+    __device__ __forceinline__ bool ill() const {     // a value that is not finite
+        float t = l * 0.f;
+#pragma unroll
+        for (int i = 0; i < DB; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) t = fmaf(o[i][r], 0.f, t);
+        return t != 0.f;
+    }
+};
+__device__ __forceinline__ uint32_t bits16(bool x) {                  // rows (lanes l, l ^ 16, l ^ 32, l ^ 48) for which x holds
+    uint64_t b = __ballot(x);
+    b |= b >> 32;
+    return (uint32_t)(b | b >> 16) & 0xffffu;
+}
 
 __device__ __forceinline__ int scan_up(int x, int lane) {            // sum over the lanes up to this one
 #pragma unroll
@@ -19,72 +126,71 @@ __device__ __forceinline__ int scan_up(int x, int lane) {            // sum over
     }
     return x;
 }
-// 32-row tiles of a sequence, and 32-key tiles of each: those that its tokens see together, so that no table of them is needed
-__device__ __forceinline__ int few_tiles(const PagedArgs& a, const Seq& x, int& per) {
+// Tiles of QR rows of a sequence, and 32-key tiles of each: as many as its tokens see together, so that no table of them is needed
+template <int QR> __device__ __forceinline__ int few_tiles(const PagedArgs& a, const Seq& x, int& per) {
     int lo, hi;
     keys_of<32>(a, x, x.end - x.n, x.end - 1, lo, hi);
     per = max(1, (hi - lo + 31) >> 5);
-    return (x.n * a.rep + 31) >> 5;
+    return (x.n * a.rep + QR - 1) / QR;
 }
-__device__ __forceinline__ int few_cost(const PagedArgs& a, int r) {
+template <int QR> __device__ __forceinline__ int few_cost(const PagedArgs& a, int r) {
     if (r >= a.R) return 0;
     int per;
-    const int t = few_tiles(a, seq_of(a, r), per);
+    const int t = few_tiles<QR>(a, seq_of(a, r), per);
     return t * per;
 }
 
-// A wave's way through its tiles.  unit() enters the next unit, tile() finds the next of its tiles (every `step` / 32-th) that any row sees.
-struct Walker {
-    int r, base, x, end;                              // row, tiles of one head in front of it, the worker's next tile and its end
+// A place in the worker's share: row, tiles of one head in front of it, the next tile and the share's end
+struct Place { int r, base, x, end; };
+// A unit: its sequence and head, tile of rows, and of its key tiles [ka, kb); positions of its rows; keys [lo, hi) up to the last of those tiles
+struct FewUnit {
     Seq sq;
-    int per, hk, t, ka, kb, lo, hi, j;
-    Span s;
-    __device__ __forceinline__ void enter(const PagedArgs& a) {       // tile rows t, key tiles [ka, kb)
-        const int rows = sq.n * a.rep, off = sq.end - sq.n, r0 = 32 * t;
-        keys_of<32>(a, sq, off, sq.end - 1, lo, hi);
-        s = {r0 / a.rep + off, (min(r0 + 32, rows) - 1) / a.rep + off, 0, 0, true};
+    int r, hk, t, per, ka, kb, p0, p1, lo, hi;
+    template <int QR> __device__ __forceinline__ void rows(const PagedArgs& a) {
+        const int n = sq.n * a.rep, off = sq.end - sq.n;
+        p0 = QR * t / a.rep + off;
+        p1 = (min(QR * (t + 1), n) - 1) / a.rep + off;
+        keys_of<32>(a, sq, p0, p1, lo, hi);
         hi = min(hi, lo + 32 * kb);
     }
-    __device__ __forceinline__ bool unit(const PagedArgs& a) {
-        while (x < end) {
-            sq = seq_uni(a, r);
-            const int cost = few_tiles(a, sq, per) * per, y = x - base * a.Hk;
+    // the next unit of a share
+    template <int QR> __device__ __forceinline__ bool next(const PagedArgs& a, Place& at) {
+        while (at.x < at.end) {
+            sq = seq_uni(a, at.r);
+            const int cost = few_tiles<QR>(a, sq, per) * per, y = at.x - at.base * a.Hk;
             if (y >= cost * a.Hk) {                   // the next row
-                if (++r >= a.R) return false;
-                base += cost;
+                if (++at.r >= a.R) return false;
+                at.base += cost;
                 continue;
             }
+            r = at.r;
             hk = y / cost;
             const int z = y - hk * cost;
             t = z / per;
             ka = z - t * per;
-            kb = min(per, ka + end - x);
-            x += kb - ka;
-            enter(a);
-            j = lo + 32 * ka - 32;
+            kb = min(per, ka + at.end - at.x);
+            at.x += kb - ka;
+            rows<QR>(a);
             return true;
         }
         return false;
     }
-    __device__ __forceinline__ bool tile(const Mask& mk, int step) {
-        do j += step; while (j < hi && !mk.some(s, j, j + 31));
-        return j < hi;
-    }
 };
-
-template <typename T, int D, bool CAP, bool BIAS, int NW, bool SHARED>
+template <typename T, int D, bool CAP, bool BIAS, int NQ, int NW, bool SHARED>
 __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
-    constexpr int KK = D / 16, DT = D / 32, ST = 32 * 2 * D;
+    constexpr int KS = D / 32, DB = D / 16, ST = 32 * 2 * D, QR = 16 * NQ;
     typedef PageLoad<D, 32, 1> Load;
+    typedef Tile<D> Ti;
     __shared__ __align__(1024) unsigned char smem[NW][2][2][ST];     // [wave][buffer][keys, values]
-    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
     const int w = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
-    Walker c{};                                       // the tiles that are computed
+    Place at{0, 0, 0, 0};                             // what is computed next
+    FewUnit u;
     int me = 0, total = 0, G = 1;
     if constexpr (SHARED) {
         const int C = (a.R + 63) / 64;
         int mine = 0;
-        for (int i = 0; i < C; i++) mine += few_cost(a, lane * C + i);
+        for (int i = 0; i < C; i++) mine += few_cost<QR>(a, lane * C + i);
         const int upto = scan_up(mine, lane);
         total = lane_of(upto, 63) * a.Hk;
         G = min((int)gridDim.x, max(total / FS, 1));
@@ -92,140 +198,179 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
         if (me < G) {
             if (G % 8 == 0) me = (me & 7) * (G / 8) + (me >> 3);     // workers that follow each other run on one XCD
             const Shares sh(total, G);
-            c.x = sh.begin(me);
-            c.end = sh.begin(me + 1);
-            const int y = c.x / a.Hk, L = 63 - __builtin_clzll(__ballot(upto - mine <= y) | 1);
-            c.base = lane_of(upto - mine, L);
-            c.r = L * C;
+            at.x = sh.begin(me);
+            at.end = sh.begin(me + 1);
+            const int y = at.x / a.Hk, L = 63 - __builtin_clzll(__ballot(upto - mine <= y) | 1);
+            at.base = lane_of(upto - mine, L);
+            at.r = L * C;
             for (int i0 = 0; C > 1 && i0 < C; i0 += 64) {            // the row within the lane's rows
-                const int cost = i0 + lane < C ? few_cost(a, c.r + i0 + lane) : 0, u = scan_up(cost, lane), all = lane_of(u, 63);
-                if (c.base + all <= y) { c.base += all; continue; }
-                const int k = 63 - __builtin_clzll(__ballot(c.base + u - cost <= y) | 1);
-                c.base += lane_of(u - cost, k);
-                c.r += i0 + k;
+                const int cost = i0 + lane < C ? few_cost<QR>(a, at.r + i0 + lane) : 0, v = scan_up(cost, lane), all = lane_of(v, 63);
+                if (at.base + all <= y) { at.base += all; continue; }
+                const int k = 63 - __builtin_clzll(__ballot(at.base + v - cost <= y) | 1);
+                at.base += lane_of(v - cost, k);
+                at.r += i0 + k;
                 break;
             }
         }
     } else {
-        c.r = blockIdx.z;
-        c.hk = blockIdx.y;
-        c.t = blockIdx.x;
+        u.r = blockIdx.z;
+        u.hk = blockIdx.y;
+        u.t = blockIdx.x;
     }
     const unsigned lds = lds_addr(smem[w]);
     const Load lk(a.k_sp, a.k_st, a.shift, 0, lane), lv(a.v_sp, a.v_st, a.shift, 0, lane);
-    const Ops<D> ops(lane);
-    const float f2 = fabsf(a.s.f);
-    RowSums<T, D, BIAS> sum(f2);
-    // the tiles that are loaded, two ahead
-    Walker f;
+    // a lane's operand addresses: chunk 4 ks + g of key row l & 15, and of a transposing read 4 columns of one of 4 keys
+    const int kr = key_row(lane & 15), vr = 4 * swap12(g) + ((lane & 15) >> 2);
+    const unsigned krow = kr * Ti::ROWB + 16 * Ti::pos(kr, g), vcol = vr * Ti::ROWB + 16 * Ti::pos(vr, (lane & 3) >> 1) + 8 * (lane & 1);
+    const int key0 = 4 * swap12(g);                   // the lane's keys of a block: key0 .. + 3
+    const float f2 = fabsf(a.s.f), F = BIAS ? 1.f : f2, lazy = LAZY / F, head = HEAD<T> / F;
+    Rows16<T, D, BIAS> row[NQ];
+    // what is fetched, two tiles ahead
+    Place ahead{0, 0, 0, 0};
+    Steps<32, NW> f;
     Pages<2> pg;
+    int64_t ftab = 0;
+    int flast = 0;
     const T* fk = nullptr;
     const T* fv = nullptr;
     bool open = false;                                // f is in a unit
+    auto enter = [&](const FewUnit& n) {
+        f.enter(a, n.sq, n.p0, n.lo, n.hi, n.ka + w);
+        ftab = n.r * a.t_sr;
+        flast = n.sq.klen - 1;
+        fk = (const T*)a.k + n.hk * a.k_sh;
+        fv = (const T*)a.v + n.hk * a.v_sh;
+        open = true;
+    };
     auto fetch = [&]() -> bool {
         for (;;) {
-            if (!open) {
-                if (!SHARED || !f.unit(a)) return false;
-                open = true;
-                fk = (const T*)a.k + f.hk * a.k_sh;
-                fv = (const T*)a.v + f.hk * a.v_sh;
-            }
-            if (f.tile(Mask{1, a.W, f.sq.pre, f.sq.klen}, 32 * NW)) break;
+            if (open && f.next()) break;
             open = false;
+            FewUnit n;
+            if (!SHARED || !n.next<QR>(a, ahead)) return false;
+            enter(n);
         }
-        pg.fetch(a, f.r * a.t_sr, f.j, f.sq.klen);
+        pg.fetch(a, ftab, f.j, flast);
         return true;
     };
-    auto keys = [&](int buf) { lk.issue(fk, pg, f.j, f.sq.klen - 1, lds + (2 * buf) * ST); };
-    auto values = [&](int buf) { lv.issue(fv, pg, f.j, f.sq.klen - 1, lds + (2 * buf + 1) * ST); };
-    bool e0 = false, e1 = false, e2 = false;          // this tile and the next are on their way, the one after them is known
+    auto keys = [&](int buf) {
+        pg.check(a);
+        lk.issue(fk, pg, f.j, flast, lds + (2 * buf) * ST);
+    };
+    auto values = [&](int buf) { lv.issue(fv, pg, f.j, flast, lds + (2 * buf + 1) * ST); };
+    bool e1 = false, e2 = false;                      // the next tile is on its way, the one after it is known
     uint32_t lost0 = 0, lost1 = 0;
     auto begin = [&]() {
-        e0 = fetch();
-        if (e0) {
-            keys(0);
-            values(0);
-            lost0 = pg.lost;
-            e1 = fetch();
-        }
-        if (e1) {
-            keys(1);
-            values(1);
-            lost1 = pg.lost;
-            e2 = fetch();
-        }
+        e1 = e2 = false;
+        if (!fetch()) return;
+        keys(0);
+        values(0);
+        lost0 = pg.lost;
+        e1 = fetch();
+        if (!e1) return;
+        keys(1);
+        values(1);
+        lost1 = pg.lost;
+        e2 = fetch();
     };
     int buf = 0;
     if constexpr (SHARED) {
-        f = c;
+        ahead = at;
         begin();
     }
     for (;;) {
         if constexpr (SHARED) {
-            if (!c.unit(a)) break;
+            if (!u.next<QR>(a, at)) break;
         } else {
-            c.sq = seq_uni(a, c.r);
-            if (c.t >= few_tiles(a, c.sq, c.per)) break;
-            c.ka = 0;
-            c.kb = c.per;
-            c.enter(a);
-            c.j = c.lo + 32 * (w - NW);
-            f = c;
-            open = true;
-            fk = (const T*)a.k + f.hk * a.k_sh;
-            fv = (const T*)a.v + f.hk * a.v_sh;
-            e1 = e2 = false;
+            u.sq = seq_uni(a, u.r);
+            if (u.t >= few_tiles<QR>(a, u.sq, u.per)) break;
+            u.ka = 0;
+            u.kb = u.per;
+            u.rows<QR>(a);
+            enter(u);
             buf = 0;
             begin();
         }
-        const int rows = c.sq.n * a.rep, off = c.sq.end - c.sq.n, r0 = 32 * c.t, row = min(r0 + (lane & 31), rows - 1);
-        const int tok = row / a.rep, hq = c.hk * a.rep + row - tok * a.rep, p = tok + off;
-        const Mask mk{1, a.W, c.sq.pre, c.sq.klen};
-        const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
-        uint4 qf[KK];
-        {
-            const T* q = (const T*)a.q + hq * a.q_sh + (int64_t)(c.sq.s + tok) * a.q_st + 8 * h;
+        const int rows = u.sq.n * a.rep, off = u.sq.end - u.sq.n, r0 = QR * u.t;
+        const Mask mk{1, a.W, u.sq.pre, u.sq.klen};
 #pragma unroll
-            for (int kk = 0; kk < KK; kk++) qf[kk] = ld16(q + 16 * kk);
+        for (int n = 0; n < NQ; n++) {
+            Rows16<T, D, BIAS>& x = row[n];
+            const int i = min(r0 + 16 * n + (lane & 15), rows - 1);
+            x.tok = i / a.rep;
+            x.hq = u.hk * a.rep + i - x.tok * a.rep;
+            x.p = x.tok + off;
+            const T* q = (const T*)a.q + x.hq * a.q_sh + (int64_t)(u.sq.s + x.tok) * a.q_st + 8 * g;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) x.q[ks] = ld16(q + 32 * ks);
+            if (a.s.f < 0.f)                          // a negative scale: of the queries' sign, so that larger products are larger scores
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) { x.q[ks].x ^= 0x80008000u; x.q[ks].y ^= 0x80008000u; x.q[ks].z ^= 0x80008000u; x.q[ks].w ^= 0x80008000u; }
+            x.slope = BIAS ? a.slopes[x.hq] * LOG2E : 0.f;
+            x.see = Sees::query(mk, x.p);
+            x.clear();
         }
-        if (a.s.f < 0.f)                              // a negative scale: of the queries' sign, so that larger products are larger scores
-#pragma unroll
-            for (int kk = 0; kk < KK; kk++) { qf[kk].x ^= 0x80008000u; qf[kk].y ^= 0x80008000u; qf[kk].z ^= 0x80008000u; qf[kk].w ^= 0x80008000u; }
-        const Rows rw{c.sq.s, tok, hq, p, min(32, rows - r0), Sees::query(mk, p), slope};
-        sum.clear();
+        const Sight sight(a, u.sq, u.p0, u.p1);
+        Steps<32, NW> c;
+        c.enter(a, u.sq, u.p0, u.lo, u.hi, u.ka + w);
         // Keys and values are fetched two tiles ahead, each into the place that it has just been read from: a wave has one and a half to two
         // tiles on their way while it computes.
-        for (; c.tile(mk, 32 * NW); buf ^= 1) {
+        for (; c.next(); buf ^= 1) {
             const int j0 = c.j;
             if (e1) wait_vm<3 * Load::N>();           // behind this tile's keys: its values, the next keys and values
             else wait_vm<Load::N>();
             asm volatile("" ::: "memory");
-            const unsigned bo = lds + (2 * buf) * ST, rk = bo + ops.row, cc = bo + ops.col, c8 = bo + ops.col8;
-            f32x16 sc[1] = {zero16()};
+            const unsigned bk = lds + (2 * buf) * ST + krow, bv = lds + (2 * buf + 1) * ST + vcol;
+            f32x4 s[NQ][2];
 #pragma unroll
-            for (int kk = 0; kk < KK; kk++) sc[0] = mfma32<T>(lds16(Ops<D>::k_step(rk, kk)), qf[kk], sc[0]);
+            for (int n = 0; n < NQ; n++) s[n][0] = s[n][1] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const uint4 k = lds16((bk ^ (64 * ks)) + 16 * b * Ti::ROWB);
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) s[n][b] = mfma16<T>(k, row[n].q[ks], s[n][b]);
+                }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the keys are read before their place is filled again
             if (e2) keys(buf);
-            scores<CAP>(sc[0], a.s);
-            if constexpr (BIAS) bias(sc[0], f2, slope, p, j0, h);
-            if (lost0 || j0 + 32 > c.hi || !mk.all(c.s, j0, j0 + 31)) {
-                uint32_t ok = seen16(rw.see, j0, h, j0 < mk.prefix, nullptr, 0);
-                if (bit(lost0, 0)) ok &= ~0xffu;      // registers 0 .. 7 are keys of the first 16
-                if (bit(lost0, 1)) ok &= 0xffu;
+            const bool all = lost0 == 0 && sight.all(j0, j0 + 31);
+            uint4 pf[NQ];
 #pragma unroll
-                for (int e = 0; e < 16; e++) sc[0][e] = j0 + key_of(e, h) < c.hi && bit(ok, e) ? sc[0][e] : -INFINITY;
+            for (int n = 0; n < NQ; n++) {
+                Rows16<T, D, BIAS>& x = row[n];
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = s[n][i >> 2][i & 3];
+                scores_n<CAP>(v, a.s);
+                if constexpr (BIAS) {
+                    const float d = (float)(x.p - j0 - key0);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = fmaf(-x.slope, fabsf(d - (float)(16 * (i >> 2) + (i & 3))), v[i] * f2);
+                }
+                if (!all) {
+                    const unsigned y = (unsigned)(j0 + key0), z = y - x.see.first;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const unsigned at8 = 16 * (i >> 2) + (i & 3);
+                        const bool ok = (z + at8 <= x.see.count || y + at8 < x.see.below) && !bit(lost0, i >> 2);
+                        v[i] = ok ? v[i] : -INFINITY;
+                    }
+                }
+                pf[n] = x.weigh(v, F, lazy, head);
             }
-            uint4 pf[1][2];
-            sum.template weigh<1>(sc, pf);
             if (e2) wait_vm<3 * Load::N>();           // behind the values: the next tile, the keys after it
             else if (e1) wait_vm<2 * Load::N>();
             else wait_vm<0>();
             asm volatile("" ::: "memory");
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++)
+            for (int d = 0; d < DB; d++) {
+                const unsigned v = bv ^ (32 * d);
+                const uint2 lo = lds_tr(v), hi = lds_tr(v + 16 * Ti::ROWB);
+                const uint4 vt = make_uint4(lo.x, lo.y, hi.x, hi.y);
 #pragma unroll
-                for (int mm = 0; mm < 2; mm++)
-                    sum.o[dt] = mfma32<T>(Ops<D>::at_col(Ops<D>::block(cc, dt), Ops<D>::block(c8, dt), ST + 16 * mm * Tile<D>::ROWB), pf[0][mm], sum.o[dt]);
+                for (int n = 0; n < NQ; n++) row[n].o[d] = mfma16<T>(vt, pf[n], row[n].o[d]);
+            }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the values, too
             lost0 = lost1;
             e1 = e2;
@@ -235,100 +380,140 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
                 e2 = fetch();
             }
         }
-        const T* kb = (const T*)a.k + c.hk * a.k_sh;
-        const T* vb = (const T*)a.v + c.hk * a.v_sh;
-        const int32_t* tab = a.table + c.r * a.t_sr;
+        const T* kb = (const T*)a.k + u.hk * a.k_sh;
+        const T* vb = (const T*)a.v + u.hk * a.v_sh;
+        const int32_t* tab = a.table + u.r * a.t_sr;
+        const int first = u.lo + 32 * u.ka;
+        auto exact = [&](const Rows16<T, D, BIAS>& x, int i, float& m1, float& l1, float (&o1)[D / 64]) {
+            exact_paged<T, D, CAP, BIAS>(a, (const T*)a.q + lane_of(x.hq, i) * a.q_sh + (int64_t)(u.sq.s + lane_of(x.tok, i)) * a.q_st, kb, vb, tab,
+                                         lane_of(x.see, i), lane_of(x.slope, i), lane_of(x.p, i), first, u.hi, lane, m1, l1, o1);
+        };
         if constexpr (SHARED) {
-            finish<T, D, CAP, BIAS>(a, sum, rw, kb, vb, tab, c.lo + 32 * c.ka, c.hi, c.ka == 0 && c.kb == c.per, (int64_t)(2 * me + (c.ka == 0)) * 32, lane);
-            if (c.ka == 0 && lane == 0)
-                a.pieces[(((c.sq.s * a.rep) >> 5) + c.r + c.t) * a.Hk + c.hk] = {me, c.kb == c.per ? 1 : Shares(total, G).owner(c.end + c.per - c.kb - 1) - me + 1};
+            const bool whole = u.ka == 0 && u.kb == u.per;
+            const int64_t part = (int64_t)(2 * me + (u.ka == 0)) * QR;
+            if (u.ka == 0 && lane == 0)
+                a.pieces[(u.sq.s * a.rep / QR + u.r + u.t) * a.Hk + u.hk] = {me, whole ? 1 : Shares(total, G).owner(at.end + u.per - u.kb - 1) - me + 1};
+#pragma unroll
+            for (int n = 0; n < NQ; n++) {
+                Rows16<T, D, BIAS>& x = row[n];
+                const int used = rows - r0 - 16 * n;
+                const bool in = (lane & 15) < used;
+                x.close();
+                const uint32_t odd = bits16(x.ill() && x.l == x.l && in);
+                for (uint32_t b = odd; b; b &= b - 1) {               // rows next to infinities and NaN, from their visible pairs alone
+                    const int i = __builtin_ctz(b);
+                    float m1, l1, o1[D / 64];
+                    exact(x, i, m1, l1, o1);
+                    if (whole) {
+                        const float inv1 = l1 > 0.f || l1 != l1 ? 1.f / l1 : 0.f;
+                        for (int e = 0; e < D / 64; e++) o1[e] *= inv1;
+                        put_row<T, D>((T*)a.out + ((int64_t)(u.sq.s + lane_of(x.tok, i)) * a.Hq + lane_of(x.hq, i)) * D, lane, o1);
+                    } else {
+                        for (int e = 0; e < D / 64; e++) a.po[(part + 16 * n + i) * D + lane * (D / 64) + e] = o1[e];
+                        if (lane == 0) a.pm[part + 16 * n + i] = make_float2(m1, l1);
+                    }
+                }
+                if (!in || bit(odd, lane & 15)) continue;
+                if (whole) {
+                    const int64_t o = ((int64_t)(u.sq.s + x.tok) * a.Hq + x.hq) * D + 4 * g;
+                    const float inv = x.l > 0.f || x.l != x.l ? 1.f / x.l : 0.f;
+#pragma unroll
+                    for (int d = 0; d < DB; d++) put4<T>(a.out, nullptr, o + 16 * d, x.o[d][0] * inv, x.o[d][1] * inv, x.o[d][2] * inv, x.o[d][3] * inv);
+                } else {
+                    const int64_t o = part + 16 * n + (lane & 15);
+#pragma unroll
+                    for (int d = 0; d < DB; d++) *reinterpret_cast<f32x4*>(a.po + o * D + 16 * d + 4 * g) = x.o[d];
+                    if (g == 0) a.pm[o] = make_float2(x.m, x.l);
+                }
+            }
         } else {
             // the waves' parts: (m, l) of every row to all, then the weighted sums through LDS (its tiles are read)
-            __shared__ float s_m[NW][32], s_l[NW][32], s_M[32], s_L[32];     // the waves' maxima and sums of every row, the workgroup's
+            __shared__ float s_m[NW][QR], s_l[NW][QR], s_L[QR];      // the waves' maxima and sums of every row, the workgroup's sums
             __shared__ uint32_t s_bad[NW];
-            sum.close();
-            if (h == 0) { s_m[w][lane] = sum.m; s_l[w][lane] = sum.l; }
-            __syncthreads();
-            float M = -INFINITY, Ls = 0.f;
-#pragma unroll
-            for (int i = 0; i < NW; i++) M = fmaxf(M, s_m[i][lane & 31]);
-            const float Mu = M == -INFINITY ? 0.f : M;
-#pragma unroll
-            for (int i = 0; i < NW; i++) Ls += s_l[i][lane & 31] * exp2_(s_m[i][lane & 31] - Mu);
-            const float fm = exp2_(sum.m - Mu);
             float* so = reinterpret_cast<float*>(smem);               // [wave][row][D + 4]
             constexpr int SO = D + 4;
-            static_assert(NW * 32 * SO * 4 <= (int)sizeof(smem), "the waves' sums fit");
-            if ((lane & 31) < rw.used) {
+            static_assert(NW * QR * SO * 4 <= (int)sizeof(smem), "the waves' sums fit");
+            const int used = min(QR, rows - r0);
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                    for (int g = 0; g < 4; g++)
-                        *reinterpret_cast<float4*>(so + (w * 32 + (lane & 31)) * SO + 32 * dt + 8 * g + 4 * h) =
-                            make_float4(sum.o[dt][4 * g] * fm, sum.o[dt][4 * g + 1] * fm, sum.o[dt][4 * g + 2] * fm, sum.o[dt][4 * g + 3] * fm);
+            for (int n = 0; n < NQ; n++) {
+                row[n].close();
+                if (g == 0) { s_m[w][16 * n + lane] = row[n].m; s_l[w][16 * n + lane] = row[n].l; }
             }
-            if (w == 0 && h == 0) s_L[lane] = Ls;     // not over s_l, which the other waves may still read
-            float nf = sum.l * 0.f;
+            __syncthreads();
+            uint32_t odd = 0;
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) nf = nonfinite(sum.o[dt], nf);
-            const uint32_t odd = row_bits(nf != 0.f && (lane & 31) < rw.used);
+            for (int n = 0; n < NQ; n++) {
+                Rows16<T, D, BIAS>& x = row[n];
+                const int i = 16 * n + (lane & 15);
+                float M = -INFINITY, Ls = 0.f;
+#pragma unroll
+                for (int k = 0; k < NW; k++) M = fmaxf(M, s_m[k][i]);
+                const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+                for (int k = 0; k < NW; k++) Ls += s_l[k][i] * exp2_(s_m[k][i] - Mu);
+                const float fm = exp2_(x.m - Mu);
+                odd |= bits16(x.ill() && Ls == Ls && i < used) << (16 * n);
+                if (i < used)
+#pragma unroll
+                    for (int d = 0; d < DB; d++) *reinterpret_cast<f32x4*>(so + (w * QR + i) * SO + 16 * d + 4 * g) = x.o[d] * fm;
+                if (w == 0 && g == 0) s_L[i] = Ls;    // not over s_l, which the other waves may still read
+            }
             if (lane == 0) s_bad[w] = odd;
             __syncthreads();
             uint32_t bad = 0;
 #pragma unroll
-            for (int i = 0; i < NW; i++) bad |= s_bad[i];
+            for (int k = 0; k < NW; k++) bad |= s_bad[k];
             if (bad) {                                // rows next to infinities and NaN, from their visible pairs alone; the same in every wave
-                bad &= ~row_bits(Ls != Ls);
                 for (; bad; bad &= bad - 1) {
                     const int i = __builtin_ctz(bad);
                     if (i % NW != w) continue;
                     float m1, l1, o1[D / 64];
-                    exact_paged<T, D, CAP, BIAS>(a, (const T*)a.q + lane_of(hq, i) * a.q_sh + (int64_t)(c.sq.s + lane_of(tok, i)) * a.q_st, kb, vb, tab,
-                                                 lane_of(rw.see, i), lane_of(slope, i), lane_of(p, i), c.lo, c.hi, lane, m1, l1, o1);
-                    for (int ww = 0; ww < NW; ww++)
-                        for (int e = 0; e < D / 64; e++) so[(ww * 32 + i) * SO + lane * (D / 64) + e] = ww ? 0.f : o1[e];
+                    exact(NQ == 2 && i >= 16 ? row[NQ - 1] : row[0], i & 15, m1, l1, o1);
+                    for (int k = 0; k < NW; k++)
+                        for (int e = 0; e < D / 64; e++) so[(k * QR + i) * SO + lane * (D / 64) + e] = k ? 0.f : o1[e];
                     if (lane == 0) s_L[i] = l1;
                 }
                 __syncthreads();
             }
             // used rows x D values: 8 lanes a row
-            for (int rr = tid >> 3; rr < rw.used; rr += 8 * NW) {
-                const int c4 = 4 * (tid & 7), g = r0 + rr;
-                const float lr = s_L[rr], inv = lr > 0.f || lr != lr ? 1.f / lr : 0.f;
-                const int gt = g / a.rep, gh = c.hk * a.rep + g - gt * a.rep;
-                const int64_t at = ((int64_t)(c.sq.s + gt) * a.Hq + gh) * D;
+            for (int i = tid >> 3; i < used; i += 8 * NW) {
+                const int c4 = 4 * (tid & 7), k = r0 + i;
+                const float lr = s_L[i], inv = lr > 0.f || lr != lr ? 1.f / lr : 0.f;
+                const int kt = k / a.rep, kh = u.hk * a.rep + k - kt * a.rep;
+                const int64_t o = ((int64_t)(u.sq.s + kt) * a.Hq + kh) * D;
 #pragma unroll
-                for (int i = 0; i < D / 32; i++) {
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int e = 0; e < D / 32; e++) {
+                    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int ww = 0; ww < NW; ww++) {
-                        const float4 y = *reinterpret_cast<const float4*>(so + (ww * 32 + rr) * SO + c4 + 32 * i);
-                        v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
-                    }
-                    put4<T>(a.out, nullptr, at + c4 + 32 * i, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                    for (int z = 0; z < NW; z++) v += *reinterpret_cast<const f32x4*>(so + (z * QR + i) * SO + c4 + 32 * e);
+                    put4<T>(a.out, nullptr, o + c4 + 32 * e, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
                 }
             }
-            c.t += gridDim.x;
+            u.t += gridDim.x;
             __syncthreads();                          // the sums are read before the next unit's tiles take their place
         }
     }
     fill_rest<D>(a, ((int64_t)(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * 64 * NW + tid, (int64_t)gridDim.x * gridDim.y * gridDim.z * 64 * NW);
 }
 
+template <typename T, int D, bool CAP, bool BIAS, int NQ>
+void launch_rows(const PagedArgs& a, int G, int tiles, hipStream_t st) {
+    if (G) slothost::launch(pages_few<T, D, CAP, BIAS, NQ, 1, true>, dim3((unsigned)G), dim3(64), 0, st, a);
+    else slothost::launch(pages_few<T, D, CAP, BIAS, NQ, FW, false>, dim3((unsigned)tiles, (unsigned)a.Hk, (unsigned)a.R), dim3(64 * FW), 0, st, a);
+}
 template <typename T, int D, bool CAP, bool BIAS>
-void launch_one(const PagedArgs& a, int G, int tiles, hipStream_t st) {
-    if (G) slothost::launch(pages_few<T, D, CAP, BIAS, 1, true>, dim3((unsigned)G), dim3(64), 0, st, a);
-    else slothost::launch(pages_few<T, D, CAP, BIAS, FW, false>, dim3((unsigned)tiles, (unsigned)a.Hk, (unsigned)a.R), dim3(64 * FW), 0, st, a);
+void launch_one(const PagedArgs& a, int QR, int G, int tiles, hipStream_t st) {
+    QR == 16 ? launch_rows<T, D, CAP, BIAS, 1>(a, G, tiles, st) : launch_rows<T, D, CAP, BIAS, 2>(a, G, tiles, st);
 }
 template <typename T, int D>
-void launch_attn(const PagedArgs& a, bool cap, int G, int tiles, hipStream_t st) {
-    if (cap) a.slopes ? launch_one<T, D, true, true>(a, G, tiles, st) : launch_one<T, D, true, false>(a, G, tiles, st);
-    else a.slopes ? launch_one<T, D, false, true>(a, G, tiles, st) : launch_one<T, D, false, false>(a, G, tiles, st);
+void launch_attn(const PagedArgs& a, bool cap, int QR, int G, int tiles, hipStream_t st) {
+    if (cap) a.slopes ? launch_one<T, D, true, true>(a, QR, G, tiles, st) : launch_one<T, D, true, false>(a, QR, G, tiles, st);
+    else a.slopes ? launch_one<T, D, false, true>(a, QR, G, tiles, st) : launch_one<T, D, false, false>(a, QR, G, tiles, st);
 }
 
 }  // namespace
 
-void slotattn_few::launch(const PagedArgs& a, int dtype, int D, bool cap, int G, int tiles, hipStream_t st) {
-    if (dtype == SLOTSCAN_BF16) D == 128 ? launch_attn<bf16_t, 128>(a, cap, G, tiles, st) : launch_attn<bf16_t, 64>(a, cap, G, tiles, st);
-    else D == 128 ? launch_attn<f16_t, 128>(a, cap, G, tiles, st) : launch_attn<f16_t, 64>(a, cap, G, tiles, st);
+void slotattn_few::launch(const PagedArgs& a, int dtype, int D, bool cap, int QR, int G, int tiles, hipStream_t st) {
+    if (dtype == SLOTSCAN_BF16) D == 128 ? launch_attn<bf16_t, 128>(a, cap, QR, G, tiles, st) : launch_attn<bf16_t, 64>(a, cap, QR, G, tiles, st);
+    else D == 128 ? launch_attn<f16_t, 128>(a, cap, QR, G, tiles, st) : launch_attn<f16_t, 64>(a, cap, QR, G, tiles, st);
 }

@@ -2,7 +2,7 @@
 // the work: slot_attn_pages.h.
 //
 //   pages_many   128 rows a workgroup, 32 per wave, 64-key tiles; pages_plan before it: the units' costs and their running sums
-//   pages_few    32 rows, 32-key tiles (slotattn_few.hip)
+//   pages_few    16 or 32 rows, 32-key tiles (slotattn_few.hip)
 //   pages_join   pieces of one unit
 #include "slot_attn_few.h"
 #include "slotscan.h"
@@ -19,7 +19,10 @@ using slothost::al16;
 #define MQ (32 * MW)                                 // its query rows
 #define MG 512                                       // workgroups: two a CU
 #define LT 1024                                      // threads of pages_plan
-#define UNIT_KEYS 2048                               // keys of a row up to which the waves of pages_few share one unit
+// The waves of a workgroup of pages_few share one unit up to this many keys and units (a round of workgroups); SINGLE / SHARED with its join, D = 128:
+// 32 units of 512 keys 11 / 18 us, 16 of 2,048 24 / 18, 1,024 of 512 54 / 51.
+#define UNIT_KEYS 1024
+#define UNIT_MOST 256
 
 namespace {
 
@@ -150,22 +153,23 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
         const int rows = sq.n * a.rep, off = sq.end - sq.n, row0 = MQ * t + 32 * w, row = min(row0 + (lane & 31), rows - 1);
         const int tok = row / a.rep, hq = hk * a.rep + row - tok * a.rep, p = tok + off;
         const Mask mk{1, a.W, sq.pre, sq.klen};
-        const Span sw{MQ * t / a.rep + off, (min(MQ * (t + 1), rows) - 1) / a.rep + off, 0, 0, true};
-        const bool mine = row0 < rows;
-        const Span sv{uni(row0 / a.rep + off), uni((min(row0 + 32, rows) - 1) / a.rep + off), 0, 0, true};
+        const int p0 = MQ * t / a.rep + off, p1 = (min(MQ * (t + 1), rows) - 1) / a.rep + off;
+        Sight sight(a, sq, row0 / a.rep + off, (min(row0 + 32, rows) - 1) / a.rep + off);
+        if (row0 >= rows) sight.s1 = -1, sight.s2 = 0;               // a wave without rows
         int lo, hi;
-        keys_of<KT>(a, sq, sw.p0, sw.p1, lo, hi);
-        const int j_end = min(hi, lo + kb * KT);
+        keys_of<KT>(a, sq, p0, p1, lo, hi);
+        hi = min(hi, lo + kb * KT);
         const T* kbase = (const T*)a.k + hk * a.k_sh;
         const T* vbase = (const T*)a.v + hk * a.v_sh;
-        auto seen = [&](int j) {                      // the next tile that any of the workgroup's rows sees
-            while (j < j_end && !mk.some(sw, j, j + KT - 1)) j += KT;
-            return j;
-        };
+        const int64_t tab = r * a.t_sr;
+        const int last = sq.klen - 1;
+        Steps<KT, 1> f;                               // the tile that is fetched
+        f.enter(a, sq, p0, lo, hi, ka);
         Pages<KT / 16> pg;
-        auto load = [&](int j, int buf) {
-            lk.issue(kbase, pg, j, sq.klen - 1, lds + (2 * buf) * STAGE);
-            lv.issue(vbase, pg, j, sq.klen - 1, lds + (2 * buf + 1) * STAGE);
+        auto load = [&](int buf) {
+            pg.check(a);
+            lk.issue(kbase, pg, f.j, last, lds + (2 * buf) * STAGE);
+            lv.issue(vbase, pg, f.j, last, lds + (2 * buf + 1) * STAGE);
         };
         const T* qrow = (const T*)a.q + hq * a.q_sh + (int64_t)(sq.s + tok) * a.q_st;
         uint4 qf[KK];
@@ -177,22 +181,31 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
         const float slope = BIAS ? a.slopes[hq] * LOG2E : 0.f;
         const Sees see = Sees::query(mk, p);
         sum.clear();
-        int j0 = seen(lo + ka * KT);
+        bool now = f.next(), more = false;            // a tile is on its way; the pages of the next one are known
+        int j0 = f.j, j1 = 0;
+        uint32_t lost = 0, lost1 = 0;
         __syncthreads();                              // the last unit's tiles are read
-        if (j0 < j_end) {
-            pg.fetch(a, r * a.t_sr, j0, sq.klen);
-            load(j0, 0);
+        if (now) {
+            pg.fetch(a, tab, f.j, last);
+            load(0);
+            lost = pg.lost;
+            more = f.next();
+            if (more) pg.fetch(a, tab, f.j, last);
         }
         // one barrier a tile: behind it the tile is there for every wave and the other buffer is read, so the next one's loads
         // run during this one's products
-        for (int buf = 0; j0 < j_end; buf ^= 1) {
-            const int j1 = seen(j0 + KT);
-            const uint32_t lost = pg.lost;
-            if (j1 < j_end) pg.fetch(a, r * a.t_sr, j1, sq.klen);
+        for (int buf = 0; now; buf ^= 1) {
             wait_vm<0>();
             tile_barrier();
-            if (j1 < j_end) load(j1, buf ^ 1);
-            if (mine && mk.some(sv, j0, j0 + KT - 1)) {
+            now = more;
+            if (more) {
+                load(buf ^ 1);
+                j1 = f.j;
+                lost1 = pg.lost;
+                more = f.next();
+                if (more) pg.fetch(a, tab, f.j, last);
+            }
+            if (sight.some(j0, j0 + KT - 1)) {
                 const unsigned bo = lds + (2 * buf) * STAGE, rk = bo + ops.row, cc = bo + ops.col, c8 = bo + ops.col8;
                 // operands are read three steps (six products) ahead: an LDS read takes as long as four or five products
                 f32x16 s[2] = {zero16(), zero16()};
@@ -225,7 +238,7 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
                     scores<CAP>(s[i], a.s);
                     if constexpr (BIAS) bias(s[i], f2, slope, p, j0 + 32 * i, h);
                 }
-                if (lost || !mk.all(sv, j0, j0 + KT - 1)) {
+                if (lost || !sight.all(j0, j0 + KT - 1)) {
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         uint32_t ok = seen16(see, j0 + 32 * i, h, j0 < mk.prefix, nullptr, 0);
@@ -245,9 +258,10 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
                 }
             }
             j0 = j1;
+            lost = lost1;
         }
         const Rows rw{sq.s, tok, hq, p, min(32, rows - row0), see, slope};
-        finish<T, D, CAP, BIAS>(a, sum, rw, kbase, vbase, a.table + r * a.t_sr, lo + ka * KT, j_end, ka == 0 && kb == c,
+        finish<T, D, CAP, BIAS>(a, sum, rw, kbase, vbase, a.table + r * a.t_sr, lo + ka * KT, hi, ka == 0 && kb == c,
                                 ((int64_t)(2 * me + (ka == 0)) * MW + w) * 32, lane);
         if (ka == 0 && kb < c) left = {r, hk, t, sq.n, sh.owner(x + c - 1) - me + 1};   // its other pieces: up to the worker of its last tile
         x += kb - ka;
@@ -313,7 +327,7 @@ __global__ __launch_bounds__(256) void pages_join(PagedArgs a) {
 // Pieces of pages_few: a row may have hundreds.  A workgroup has `per` of the (row of the batch, head) pairs, and of their units every gridDim.y-th query
 // row, one at a time; its NG groups of lanes take every NG-th piece and meet in LDS in order.
 template <typename T, int D, int NT>
-__global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per) {
+__global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per, int QR) {
     constexpr int LN = D / 4, NG = NT / LN;
     __shared__ __align__(16) float s_o[NG][D];
     __shared__ float2 s_m[NG];
@@ -322,19 +336,19 @@ __global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per) {
     for (int b0 = u0; b0 < u1; b0 += 64) {
         const int u = b0 + lane, r = min(u, u1 - 1) / a.Hk, hk = min(u, u1 - 1) - r * a.Hk;
         const Seq x = seq_of(a, r);
-        const int rows = x.n * a.rep, at = ((x.s * a.rep) >> 5) + r;
+        const int rows = x.n * a.rep, at = x.s * a.rep / QR + r;
         Piece p{0, 0};
         if (rows && u < u1) p = a.pieces[at * a.Hk + hk];
-        for (uint64_t b = __ballot(u < u1 && (p.parts > 1 || rows > 32)); b; b &= b - 1) {
+        for (uint64_t b = __ballot(u < u1 && (p.parts > 1 || rows > QR)); b; b &= b - 1) {
             const int k = __builtin_ctzll(b), n = lane_of(rows, k), hd = lane_of(hk, k), s = lane_of(x.s, k), at0 = lane_of(at, k);
             Piece q{lane_of(p.me, k), lane_of(p.parts, k)};
-            for (int t = 0; 32 * t < n; t++) {
+            for (int t = 0; QR * t < n; t++) {
                 if (t) q = a.pieces[(at0 + t) * a.Hk + hd];
                 if (q.parts < 2) continue;
-                for (int i = blockIdx.y; i < min(32, n - 32 * t); i += gridDim.y) {
+                for (int i = blockIdx.y; i < min(QR, n - QR * t); i += gridDim.y) {
                     float M, L;
                     float4 acc;
-                    join_pieces<D>(a, g, NG, q.parts, c, [&](int z) { return (int64_t)(z ? 2 * (q.me + z) : 2 * q.me + 1) * 32 + i; }, M, L, acc);
+                    join_pieces<D>(a, g, NG, q.parts, c, [&](int z) { return (int64_t)(z ? 2 * (q.me + z) : 2 * q.me + 1) * QR + i; }, M, L, acc);
                     __syncthreads();                  // the last row's sums are read
                     *reinterpret_cast<float4*>(&s_o[g][4 * c]) = acc;
                     if (c == 0) s_m[g] = make_float2(M, L);
@@ -356,7 +370,7 @@ __global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per) {
                             acc.z = fmaf(o.z, f, acc.z);
                             acc.w = fmaf(o.w, f, acc.w);
                         }
-                        put_joined<T, D>(a, s, hd, 32 * t + i, c, L, acc);
+                        put_joined<T, D>(a, s, hd, QR * t + i, c, L, acc);
                     }
                 }
             }
@@ -366,25 +380,26 @@ __global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per) {
 
 // How a call runs.
 //   MANY    tiles of 128 query rows
-//   SHARED  one tile of 32 rows a key/value head (one or a few tokens of each sequence): equal shares of all keys, and a join
+//   SHARED  one tile of at most 32 rows a key/value head (one or a few tokens of each sequence): equal shares of all keys, and a join
 //   SINGLE  the same where no row has many keys: a workgroup a unit, no join
 enum { MANY, SHARED, SINGLE };
-struct Plan { int kind, G; int64_t units; size_t join, pm, po, all; };
+struct Plan { int kind, QR, G; int64_t units; size_t join, pm, po, all; };
 Plan plan(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t most, int64_t W, bool prefix) {
     Plan x{};
     const int64_t rep = Hq / Hk, rows = std::min(N, R);
     const int64_t keys = prefix ? M * page : std::min(M * page, W + most + 32);
     auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    x.kind = most * rep > 32 ? MANY : keys <= UNIT_KEYS ? SINGLE : SHARED;
+    x.kind = most * rep > 32 ? MANY : keys <= UNIT_KEYS && rows * Hk <= UNIT_MOST ? SINGLE : SHARED;
     if (x.kind == SINGLE && (R > 65535 || Hk > 65535)) x.kind = SHARED;
-    if (x.kind == SHARED && (N * rep / 32 + rows) * Hk * ((M * page + 31) / 32) > 0x3fffffffLL) x.kind = MANY;      // (its sums are 32-bit ones)
-    const int64_t Q = x.kind == MANY ? MQ : 32, K = x.kind == MANY ? KT : 32;
+    if (x.kind == SHARED && (N * rep / 16 + rows) * Hk * ((M * page + 31) / 32) > 0x3fffffffLL) x.kind = MANY;      // (its sums are 32-bit ones)
+    x.QR = x.kind == MANY ? MQ : most * rep > 16 ? 32 : 16;
+    const int64_t Q = x.QR, K = x.kind == MANY ? KT : 32;
     x.units = N * rep / Q + rows;
     if (x.kind == SINGLE) return x;
     const int64_t tiles = x.units * Hk * ((M * page + K - 1) / K);
-    x.G = x.kind == MANY ? (int)std::min<int64_t>(MG, (tiles + 3) / 4) : (int)std::min<int64_t>(FG, std::max<int64_t>(tiles / FS, 1));
+    x.G = x.kind == MANY ? (int)std::min<int64_t>(MG, (tiles + 3) / 4) : (int)std::min<int64_t>(FG * 128 / D, std::max<int64_t>(tiles / FS, 1));
     x.join = x.kind == MANY ? up((size_t)(2 * (R + 1) + x.units + 1) * 4) : 0;
-    x.pm = x.join + up(x.kind == MANY ? (size_t)x.G * sizeof(Unit) : (size_t)(N * rep / 32 + R) * Hk * sizeof(Piece));
+    x.pm = x.join + up(x.kind == MANY ? (size_t)x.G * sizeof(Unit) : (size_t)(N * rep / Q + R) * Hk * sizeof(Piece));
     x.po = x.pm + up((size_t)x.G * 2 * Q * sizeof(float2));
     x.all = x.po + up((size_t)x.G * 2 * Q * D * sizeof(float));
     return x;
@@ -408,8 +423,8 @@ void launch_join(const PagedArgs& a, const Plan& x, int rows, hipStream_t st) {
     // few units have many pieces each
     const int pairs = a.R * a.Hk, per = (pairs + 2047) / 2048, grid = (pairs + per - 1) / per;
     const dim3 blocks((unsigned)grid, (unsigned)std::max(1, std::min(rows, 4096 / grid)));
-    if (pairs <= 32) slothost::launch(pages_join_few<T, D, 1024>, blocks, dim3(1024), 0, st, a, per);
-    else slothost::launch(pages_join_few<T, D, 256>, blocks, dim3(256), 0, st, a, per);
+    if (pairs <= 32) slothost::launch(pages_join_few<T, D, 1024>, blocks, dim3(1024), 0, st, a, per, x.QR);
+    else slothost::launch(pages_join_few<T, D, 256>, blocks, dim3(256), 0, st, a, per, x.QR);
 }
 
 }  // namespace
@@ -428,6 +443,7 @@ extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const v
                               const int32_t* prefix, void* workspace, void* out, void* stream) {
     if (N < 1 || R < 1 || M < 1 || P < 1) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_pages: N, R, M and P must be >= 1");
     if (page < SLOTPAGE_MIN || (page & (page - 1)) || page > SLOTPAGE_MAX) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_pages: page must be a power of two in [16, 4096]");
+    if (k_sp < 0 || v_sp < 0 || k_sp >> 31 || v_sp >> 31) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_pages: pages must be fewer than 2^31 elements apart");
     if (M * page > SLOTATTN_MAX_T || P > SLOTATTN_MAX_T || R > 1 << 24 || t_sr < 0 || most < 1)
         return fail(SLOTSCAN_ERR_SHAPE, "slotattn_pages: shape too large");
     if (int r = slotattn_host::check(q, 0, q_sh, q_st, k, k_sp, k_sh, k_st, v, v_sp, v_sh, v_st, dtype, 1, N, page, Hq, Hk, D, scale, window, cap)) return r;
@@ -449,7 +465,7 @@ extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const v
     a.out = out;
     hipStream_t st = (hipStream_t)stream;
     const bool cp = cap > 0.f;
-    const int tiles = (int)((std::min(most, N) * a.rep + 31) / 32), rows = (int)std::min<int64_t>(32, std::min(most, N) * a.rep);
+    const int tiles = (int)((std::min(most, N) * a.rep + x.QR - 1) / x.QR), rows = (int)std::min<int64_t>(x.QR, std::min(most, N) * a.rep);
     hipError_t e;
     if (x.kind == MANY) {
         slothost::Scope sc(SLOTSCAN_K_ATTN_PLAN, st);
@@ -459,7 +475,7 @@ extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const v
     }
     {
         slothost::Scope sc(SLOTSCAN_K_ATTN, st);
-        if (x.kind != MANY) slotattn_few::launch(a, dtype, (int)D, cp, x.G, tiles, st);
+        if (x.kind != MANY) slotattn_few::launch(a, dtype, (int)D, cp, x.QR, x.G, tiles, st);
         else if (dtype == SLOTSCAN_BF16) D == 128 ? launch_attn<bf16_t, 128>(a, cp, x.G, st) : launch_attn<bf16_t, 64>(a, cp, x.G, st);
         else D == 128 ? launch_attn<f16_t, 128>(a, cp, x.G, st) : launch_attn<f16_t, 64>(a, cp, x.G, st);
         e = hipGetLastError();
