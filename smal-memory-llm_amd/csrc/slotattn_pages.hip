@@ -18,6 +18,9 @@ using slothost::al16;
 #define MT (64 * MW)
 #define MQ (32 * MW)                                 // its query rows
 #define MG 512                                       // workgroups: two a CU
+#define ML 2                                         // what a unit costs beside its tiles, in tiles: its search, first loads and end take about 5 us
+#define MA 9                                         // shares of a CU's first and second workgroup
+#define MB 7
 #define LT 1024                                      // threads of pages_plan
 // The waves of a workgroup of pages_few share one unit up to this many keys and units (a round of workgroups); SINGLE / SHARED with its join, D = 128:
 // 32 units of 512 keys 11 / 18 us, 16 of 2,048 24 / 18, 1,024 of 512 54 / 51.
@@ -82,7 +85,7 @@ __global__ __launch_bounds__(LT) void pages_plan(PagedArgs a) {
             const int t = i - first[lo], off = x.end - x.n, last = min(MQ * (t + 1), x.n * a.rep) - 1;
             int k0, k1;
             keys_of<KT>(a, x, MQ * t / a.rep + off, last / a.rep + off, k0, k1);
-            c = max(1, (k1 - k0 + KT - 1) / KT);
+            c = ML + max(1, (k1 - k0 + KT - 1) / KT);
         }
         const int at = c0 + before_sum(c, s_sum, all);
         if (i < u0) {
@@ -111,6 +114,24 @@ __device__ __forceinline__ int find(const int* x, int lo, int hi, int mul, int y
 }
 
 // ------------------------------------------------------------------------------------------- many rows
+// Shares of pages_many's workers where two workgroups share each CU: a SIMD issues its older wave first, so the workgroups of the first half of
+// the grid have 1.83 us a tile and those of the second 2.35 (8,192 tokens of first prompts); with equal shares the second half ended 30 us later.
+// Worker w of an XCD's G / 8: the first half of them are of the grid's first half.
+struct PairShares {
+    int total, G, h;                                  // h: half of an XCD's workers; 0: equal shares
+    __device__ __forceinline__ PairShares(int t, int workers) : total(t), G(workers), h(workers == MG ? workers / 16 : 0) {}
+    __device__ __forceinline__ int begin(int w) const {
+        if (!h) return (int)((int64_t)total * w / G);
+        const int e = w / (2 * h), k = w - 2 * h * e, c = e * h * (MA + MB) + min(k, h) * MA + max(k - h, 0) * MB;
+        return (int)((int64_t)total * c / (8 * h * (MA + MB)));
+    }
+    __device__ __forceinline__ int owner(int x) const {               // of tile x
+        if (!h) return (int)(((int64_t)(x + 1) * G - 1) / total);
+        const int c = (int)(((int64_t)(x + 1) * (8 * h * (MA + MB)) - 1) / total), e = c / (h * (MA + MB)), k = c - e * h * (MA + MB);
+        return 2 * h * e + (k < h * MA ? k / MA : h + (k - h * MA) / MB);
+    }
+};
+
 template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
     constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
@@ -131,7 +152,7 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
         return;
     }
     if (G % 8 == 0) me = (me & 7) * (G / 8) + (me >> 3);
-    const Shares sh(total, G);
+    const PairShares sh(total, G);
     int x = sh.begin(me);
     const int end = sh.begin(me + 1);
     Unit left{0, 0, 0, 0, 0};
@@ -147,7 +168,10 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
         if (y >= per * a.Hk) { r++; continue; }
         const int hk = y / per, z = y - hk * per + cr;
         const int u0 = ld_uni(first, r), u = uni(find(cost, u0, ld_uni(first, r + 1), 1, z, lane));
-        const int cu = ld_uni(cost, u), c = ld_uni(cost, u + 1) - cu, ka = z - cu, kb = min(c, ka + end - x);
+        const int cu = ld_uni(cost, u), c = ld_uni(cost, u + 1) - cu - ML, y0 = z - cu, y1 = min(c + ML, y0 + end - x);
+        const int ka = max(0, y0 - ML), kb = max(0, y1 - ML);
+        x += y1 - y0;
+        if (kb <= ka) continue;                       // of this unit the worker's share is its beginning alone
         const int t = u - u0;
         const Seq sq = seq_uni(a, r);
         const int rows = sq.n * a.rep, off = sq.end - sq.n, row0 = MQ * t + 32 * w, row = min(row0 + (lane & 31), rows - 1);
@@ -263,8 +287,7 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
         const Rows rw{sq.s, tok, hq, p, min(32, rows - row0), see, slope};
         finish<T, D, CAP, BIAS>(a, sum, rw, kbase, vbase, a.table + r * a.t_sr, lo + ka * KT, hi, ka == 0 && kb == c,
                                 ((int64_t)(2 * me + (ka == 0)) * MW + w) * 32, lane);
-        if (ka == 0 && kb < c) left = {r, hk, t, sq.n, sh.owner(x + c - 1) - me + 1};   // its other pieces: up to the worker of its last tile
-        x += kb - ka;
+        if (ka == 0 && kb < c) left = {r, hk, t, sq.n, sh.owner(end + c - kb - 1) - me + 1};        // its other pieces: up to the worker of its last tile
     }
     if (tid == 0) a.join[me] = left;
 }
@@ -396,7 +419,7 @@ Plan plan(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk,
     const int64_t Q = x.QR, K = x.kind == MANY ? KT : 32;
     x.units = N * rep / Q + rows;
     if (x.kind == SINGLE) return x;
-    const int64_t tiles = x.units * Hk * ((M * page + K - 1) / K);
+    const int64_t tiles = x.units * Hk * ((M * page + K - 1) / K + ML);
     x.G = x.kind == MANY ? (int)std::min<int64_t>(MG, (tiles + 3) / 4) : (int)std::min<int64_t>(FG * 128 / D, std::max<int64_t>(tiles / FS, 1));
     x.join = x.kind == MANY ? up((size_t)(2 * (R + 1) + x.units + 1) * 4) : 0;
     x.pm = x.join + up(x.kind == MANY ? (size_t)x.G * sizeof(Unit) : (size_t)(N * rep / Q + R) * Hk * sizeof(Piece));
@@ -452,7 +475,7 @@ extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const v
     const Plan x = plan(N, R, M, page, Hq, Hk, D, std::min(most, N), window, prefix != nullptr);
     if (x.all && !workspace) return fail(SLOTSCAN_ERR_NULL, "slotattn_pages: workspace is NULL");
     // (the sums of all units' tiles are 32-bit ones)
-    if (x.kind == MANY && (x.units + 1) * Hk * ((M * page + KT - 1) / KT) > 0x3fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_pages: shape too large");
+    if (x.kind == MANY && (x.units + 1) * Hk * ((M * page + KT - 1) / KT + ML) > 0x3fffffffLL) return fail(SLOTSCAN_ERR_SHAPE, "slotattn_pages: shape too large");
     PagedArgs a{};
     a.s = slotattn_host::args(q, 0, q_sh, q_st, k, k_sp, k_sh, k_st, v, v_sp, v_sh, v_st, 1, N, page, Hq, Hk, scale, 1, window, cap, slopes, nullptr, prefix);
     a.q = q; a.k = k; a.v = v;
