@@ -69,8 +69,10 @@ template <typename T, int D, bool BIAS> struct Rows16 {
         mu = l = 0.f;
         far = false;
     }
-    // 32 scores' worth of 8 values a lane become probabilities as an operand (slot_attn_rows.h)
-    __device__ __forceinline__ uint4 weigh(float (&s)[8], float F, float lazy, float head) {
+    // 8 scores a lane become probabilities as an operand (slot_attn_rows.h), in bf16 as two of them, whose sum has 16 bits: one alone would be off by as
+    // much as the result's own rounding, and the products wait for memory anyway
+    static constexpr int PARTS = sizeof(T) == 2 && HEAD<T> == 0.f ? 2 : 1;
+    __device__ __forceinline__ void weigh(float (&s)[8], float F, float lazy, float head, uint4 (&pf)[PARTS]) {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[i]);
@@ -96,7 +98,13 @@ template <typename T, int D, bool BIAS> struct Rows16 {
             s[i] = exp2_(s[i]);
             l += s[i];
         }
-        return make_uint4(pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3]), pack2<T>(s[4], s[5]), pack2<T>(s[6], s[7]));
+        pf[0] = make_uint4(pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3]), pack2<T>(s[4], s[5]), pack2<T>(s[6], s[7]));
+        if constexpr (PARTS == 2) {
+            const uint32_t x[4] = {pf[0].x, pf[0].y, pf[0].z, pf[0].w};
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i] -= unpack<T>(x[i / 2], i & 1);
+            pf[1] = make_uint4(pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3]), pack2<T>(s[4], s[5]), pack2<T>(s[6], s[7]));
+        }
     }
     __device__ __forceinline__ void close() {
         auto p2 = __builtin_amdgcn_permlane16_swap(__float_as_uint(l), __float_as_uint(l), false, false);
@@ -335,7 +343,7 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the keys are read before their place is filled again
             if (e2) keys(buf);
             const bool all = lost0 == 0 && sight.all(j0, j0 + 31);
-            uint4 pf[NQ];
+            uint4 pf[NQ][Rows16<T, D, BIAS>::PARTS];
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
                 Rows16<T, D, BIAS>& x = row[n];
@@ -357,7 +365,7 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
                         v[i] = ok ? v[i] : -INFINITY;
                     }
                 }
-                pf[n] = x.weigh(v, F, lazy, head);
+                x.weigh(v, F, lazy, head, pf[n]);
             }
             if (e2) wait_vm<3 * Load::N>();           // behind the values: the next tile, the keys after it
             else if (e1) wait_vm<2 * Load::N>();
@@ -369,7 +377,9 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
                 const uint2 lo = lds_tr(v), hi = lds_tr(v + 16 * Ti::ROWB);
                 const uint4 vt = make_uint4(lo.x, lo.y, hi.x, hi.y);
 #pragma unroll
-                for (int n = 0; n < NQ; n++) row[n].o[d] = mfma16<T>(vt, pf[n], row[n].o[d]);
+                for (int n = 0; n < NQ; n++)
+#pragma unroll
+                    for (int i = 0; i < Rows16<T, D, BIAS>::PARTS; i++) row[n].o[d] = mfma16<T>(vt, pf[n][i], row[n].o[d]);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the values, too
             lost0 = lost1;
