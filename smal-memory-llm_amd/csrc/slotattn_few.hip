@@ -126,11 +126,12 @@ __device__ __forceinline__ uint32_t bits16(bool x) {                  // rows (l
     return (uint32_t)(b | b >> 16) & 0xffffu;
 }
 
-__device__ __forceinline__ int scan_up(int x, int lane) {            // sum over the lanes up to this one
+// Sum over the lanes up to this one, `most` at most (under 2^30).  (Rows that share tokens may add up to anything: the tiles behind `most` are nobody's.)
+__device__ __forceinline__ int scan_up(int x, int lane, int most) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
+        if (lane >= d) x = min(x + y, most);
     }
     return x;
 }
@@ -196,10 +197,10 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
     FewUnit u;
     int me = 0, total = 0, G = 1;
     if constexpr (SHARED) {
-        const int C = (a.R + 63) / 64;
+        const int C = (a.R + 63) / 64, most = 0x3fffffff / a.Hk;
         int mine = 0;
-        for (int i = 0; i < C; i++) mine += few_cost<QR>(a, lane * C + i);
-        const int upto = scan_up(mine, lane);
+        for (int i = 0; i < C; i++) mine = min(mine + few_cost<QR>(a, lane * C + i), most);
+        const int upto = scan_up(mine, lane, most);
         total = lane_of(upto, 63) * a.Hk;
         G = min((int)gridDim.x, max(total / FS, 1));
         me = blockIdx.x;
@@ -208,14 +209,14 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
             const Shares sh(total, G);
             at.x = sh.begin(me);
             at.end = sh.begin(me + 1);
-            const int y = at.x / a.Hk, L = 63 - __builtin_clzll(__ballot(upto - mine <= y) | 1);
-            at.base = lane_of(upto - mine, L);
+            const int y = at.x / a.Hk, up = __shfl_up(upto, 1), ahead0 = lane ? up : 0, L = 63 - __builtin_clzll(__ballot(ahead0 <= y) | 1);
+            at.base = lane_of(ahead0, L);
             at.r = L * C;
             for (int i0 = 0; C > 1 && i0 < C; i0 += 64) {            // the row within the lane's rows
-                const int cost = i0 + lane < C ? few_cost<QR>(a, at.r + i0 + lane) : 0, v = scan_up(cost, lane), all = lane_of(v, 63);
+                const int cost = i0 + lane < C ? few_cost<QR>(a, at.r + i0 + lane) : 0, v = scan_up(cost, lane, most), all = lane_of(v, 63);
                 if (at.base + all <= y) { at.base += all; continue; }
-                const int k = 63 - __builtin_clzll(__ballot(at.base + v - cost <= y) | 1);
-                at.base += lane_of(v - cost, k);
+                const int vp = __shfl_up(v, 1), v0 = lane ? vp : 0, k = 63 - __builtin_clzll(__ballot(at.base + v0 <= y) | 1);
+                at.base += lane_of(v0, k);
                 at.r += i0 + k;
                 break;
             }

@@ -31,14 +31,17 @@ namespace {
 
 // ------------------------------------------------------------------------------------------- plan
 // One workgroup: the rows' tiles of MQ query rows in a row (units), then their key tiles.  Latency: two running sums.
-__device__ __forceinline__ int before_sum(int x, int* s, int& all) {
+// (neither past `most`, under 2^30: rows that share tokens may add up to anything)
+__device__ __forceinline__ int before_sum(int x, int most, int* s, int& all) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     int v = x;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const int y = __shfl_up(v, d);
-        if (lane >= d) v += y;
+        if (lane >= d) v = min(v + y, most);
     }
+    int ex = __shfl_up(v, 1);
+    if (lane == 0) ex = 0;
     __syncthreads();
     if (lane == 63) s[w] = v;
     __syncthreads();
@@ -46,10 +49,10 @@ __device__ __forceinline__ int before_sum(int x, int* s, int& all) {
 #pragma unroll
     for (int i = 0; i < LT / 64; i++) {
         if (i == w) base = sum;
-        sum += s[i];
+        sum = min(sum + s[i], most);
     }
     all = sum;
-    return base + v - x;
+    return min(base + ex, most);
 }
 
 __global__ __launch_bounds__(LT) void pages_plan(PagedArgs a) {
@@ -66,7 +69,7 @@ __global__ __launch_bounds__(LT) void pages_plan(PagedArgs a) {
             const Seq x = seq_of(a, r);
             tiles = (x.n * a.rep + MQ - 1) / MQ;
         }
-        const int u = min(u0 + before_sum(tiles, s_sum, all), a.units);
+        const int u = min(u0 + before_sum(min(tiles, a.units), a.units, s_sum, all), a.units);
         if (r < a.R) first[r] = u;
         u0 = min(u0 + all, a.units);
     }
@@ -87,7 +90,7 @@ __global__ __launch_bounds__(LT) void pages_plan(PagedArgs a) {
             keys_of<KT>(a, x, MQ * t / a.rep + off, last / a.rep + off, k0, k1);
             c = ML + max(1, (k1 - k0 + KT - 1) / KT);
         }
-        const int at = c0 + before_sum(c, s_sum, all);
+        const int at = c0 + before_sum(c, 0x3fffffff, s_sum, all);
         if (i < u0) {
             cost[i] = at;
             if (i == first[lo]) cost_r[lo] = at;

@@ -74,9 +74,9 @@ def page_extend(new, lens, table, free, page, N):
     """New tokens and their pages for every row (see the module docstring)."""
     what = "page_extend"
     page, N = int(page), int(N)
-    R, M, P = _check(new, "new", lens, table, free, page, what)
     if N < 0:
         raise ValueError(f"{what}: N must be >= 0 (got {N})")
+    R, M, P = _check(new, "new", lens, table, free, page, what)
     dev, i32 = table.device, torch.int32
     slots, pos, starts, ends = torch.empty(3 * N + 2 * R + 1, device=dev, dtype=i32).split_with_sizes((2 * N, N, R + 1, R))   # one allocation
     slots = slots.view(torch.int64)
