@@ -214,13 +214,52 @@ __device__ __forceinline__ void exact_paged(const PagedArgs& a, const T* q, cons
             for (int i = 0; i < N; i++) o[i] = NAN;
             return;
         }
-        for (; b; b &= b - 1) {
-            const int k = __builtin_ctzll(b);
-            const T* z = vb + lane_of(id, k) * a.v_sp + ((j0 + k) & in) * a.v_st + lane * N;
-            const float y = lane_of(e, k);
-            for (int i = 0; i < N; i++) o[i] = fmaf(y, widen1(z[i]), o[i]);
+        for (int k0 = 0; k0 < 64; k0 += 16) {         // 16 loads on their way
+            if (!(b >> k0 & 0xffff)) continue;
+            T z[16][N];
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const T* r = vb + lane_of(ok ? id : 0, k0 + k) * a.v_sp + ((j0 + k0 + k) & in) * a.v_st + lane * N;
+#pragma unroll
+                for (int i = 0; i < N; i++) z[k][i] = r[i];
+            }
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const float y = lane_of(e, k0 + k);
+#pragma unroll
+                for (int i = 0; i < N; i++) o[i] = fmaf(y, b >> (k0 + k) & 1 ? widen1(z[k][i]) : 0.f, o[i]);
+            }
         }
     }
+}
+
+// Whether the lane's row keeps its sums although they are not finite (slot_attn.h's keeps, the rows found through the table): it sees a value that is
+// not, and no column holds one in a masked place only.  Keys [lo, hi); met(j): the wave multiplied key j; step: keys of a tile, whose last one may stand for
+// those behind it; parts: probabilities in two parts make a NaN of an infinity that is seen, so that such a row is formed again.
+template <typename T, int D, class MET>
+__device__ __forceinline__ bool keeps_paged(const PagedArgs& a, const T* kb, const T* vb, const int32_t* tab, const Sees& see, int lo, int hi, int klen, int step, bool parts,
+                                            int lane, MET met) {
+    Ill<T, D> ill;
+    const int in = (1 << a.shift) - 1, end = min(klen, lo + (hi - lo + step - 1) / step * step), last = klen % step ? klen - 1 : -1;
+    for (int j0 = lo; j0 < end; j0 += 64) {
+        const int j = j0 + lane, id = j < end ? tab[j >> a.shift] : -1;
+        const bool there = (unsigned)id < (unsigned)a.P;
+        const int64_t row = there ? id : 0;           // (a page that is not there: page 0 was multiplied in its place)
+        const bool odd = j < end && !(finite_row<T, D>(kb + row * a.k_sp + (j & in) * a.k_st) && finite_row<T, D>(vb + row * a.v_sp + (j & in) * a.v_st));
+        for (uint64_t b = __ballot(odd); b; b &= b - 1) {
+            const int k = __builtin_ctzll(b), i = j0 + k;
+            const T* z = vb + lane_of((int)row, k) * a.v_sp + (i & in) * a.v_st;
+            const bool sees = i < hi && lane_of((int)there, k) && sees1(see, i, nullptr, 0);
+            ill.add(z, sees, met(i), i == last, lane);
+            if (parts)
+#pragma unroll
+                for (int e = 0; e < D / 64; e++) {
+                    const uint64_t inf = __ballot(fabsf(widen1(z[lane * (D / 64) + e])) == INFINITY);
+                    if (sees) ill.odd[e] |= inf;
+                }
+        }
+    }
+    return ill.kept();
 }
 
 // The end of a piece: a wave's 32 rows, a row a lane and half.  Whole units are normalised and written, others leave their sums at row
@@ -230,9 +269,9 @@ struct Rows {
     Sees see;
     float slope;
 };
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, bool CAP, bool BIAS, class MET>
 __device__ __forceinline__ void finish(const PagedArgs& a, RowSums<T, D, BIAS>& sum, const Rows& w, const T* kb, const T* vb, const int32_t* tab, int lo, int hi,
-                                       bool whole, int64_t part, int lane) {
+                                       int klen, bool whole, int64_t part, int lane, MET met) {
     constexpr int DT = D / 32;
     const int h = lane >> 5;
     const bool in = (lane & 31) < w.used;
@@ -240,7 +279,8 @@ __device__ __forceinline__ void finish(const PagedArgs& a, RowSums<T, D, BIAS>& 
     float nf = sum.l * 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) nf = nonfinite(sum.o[dt], nf);
-    const uint32_t odd = row_bits(nf != 0.f && sum.l == sum.l && in);
+    uint32_t odd = row_bits(nf != 0.f && sum.l == sum.l && in);      // (a NaN in its sum makes all of a row NaN)
+    if (odd) odd &= ~row_bits(keeps_paged<T, D>(a, kb, vb, tab, w.see, lo, hi, klen, KT, false, lane, met));
     for (uint32_t b = odd; b; b &= b - 1) {
         const int i = __builtin_ctz(b);
         float m1, l1, o1[D / 64];

@@ -395,6 +395,11 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
         const T* vb = (const T*)a.v + u.hk * a.v_sh;
         const int32_t* tab = a.table + u.r * a.t_sr;
         const int first = u.lo + 32 * u.ka;
+        auto keeps = [&](const Rows16<T, D, BIAS>& x) {
+            const int g0 = (u.sq.pre + 31) & ~31, g1 = u.sq.pre > 0 ? max(0, max(u.p0, 0) - a.W + 1) & ~31 : 0;      // (the gap that Steps leaves out)
+            return keeps_paged<T, D>(a, kb, vb, tab, x.see, first, u.hi, u.sq.klen, 32, Rows16<T, D, BIAS>::PARTS == 2, lane,
+                                     [&](int j) { return (j & ~31) < g0 || (j & ~31) >= g1; });
+        };
         auto exact = [&](const Rows16<T, D, BIAS>& x, int i, float& m1, float& l1, float (&o1)[D / 64]) {
             exact_paged<T, D, CAP, BIAS>(a, (const T*)a.q + lane_of(x.hq, i) * a.q_sh + (int64_t)(u.sq.s + lane_of(x.tok, i)) * a.q_st, kb, vb, tab,
                                          lane_of(x.see, i), lane_of(x.slope, i), lane_of(x.p, i), first, u.hi, lane, m1, l1, o1);
@@ -410,7 +415,8 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
                 const int used = rows - r0 - 16 * n;
                 const bool in = (lane & 15) < used;
                 x.close();
-                const uint32_t odd = bits16(x.ill() && x.l == x.l && in);
+                uint32_t odd = bits16(x.ill() && x.l == x.l && in);
+                if (odd) odd &= ~bits16(keeps(x));
                 for (uint32_t b = odd; b; b &= b - 1) {               // rows next to infinities and NaN, from their visible pairs alone
                     const int i = __builtin_ctz(b);
                     float m1, l1, o1[D / 64];
@@ -475,6 +481,10 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
 #pragma unroll
             for (int k = 0; k < NW; k++) bad |= s_bad[k];
             if (bad) {                                // rows next to infinities and NaN, from their visible pairs alone; the same in every wave
+                uint32_t kept = 0;
+#pragma unroll
+                for (int n = 0; n < NQ; n++) kept |= bits16(keeps(row[n])) << (16 * n);
+                bad &= ~kept;
                 for (; bad; bad &= bad - 1) {
                     const int i = __builtin_ctz(bad);
                     if (i % NW != w) continue;

@@ -287,9 +287,13 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
             j0 = j1;
             lost = lost1;
         }
-        const Rows rw{sq.s, tok, hq, p, min(32, rows - row0), see, slope};
-        finish<T, D, CAP, BIAS>(a, sum, rw, kbase, vbase, a.table + r * a.t_sr, lo + ka * KT, hi, ka == 0 && kb == c,
-                                ((int64_t)(2 * me + (ka == 0)) * MW + w) * 32, lane);
+        // (a lane's row is found again rather than kept: the loop needs every register)
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int row1 = min(row0 + (ln & 31), rows - 1), tok1 = row1 / a.rep;
+        const Rows rw{sq.s, tok1, hk * a.rep + row1 - tok1 * a.rep, tok1 + off, min(32, rows - row0), see, slope};
+        finish<T, D, CAP, BIAS>(a, sum, rw, kbase, vbase, a.table + r * a.t_sr, lo + ka * KT, hi, sq.klen, ka == 0 && kb == c,
+                                ((int64_t)(2 * me + (ka == 0)) * MW + w) * 32, lane, [&](int j) { return sight.some(j & -KT, j | (KT - 1)); });
         if (ka == 0 && kb < c) left = {r, hk, t, sq.n, sh.owner(end + c - kb - 1) - me + 1};        // its other pieces: up to the worker of its last tile
     }
     if (tid == 0) a.join[me] = left;

@@ -203,6 +203,23 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(news, most,
             near(got[i][:, ~bad], ref[i][:, ~bad], bound[i][:, ~bad], "the other columns of the rows that see a NaN value")
 
 
+@pytest.mark.parametrize("news,ctxs,most", [([900], [0], None), ([1, 3], [6000, 9000], 3), ([1], [900], 1)])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_a_nan_that_every_row_sees_costs_one_pass(news, ctxs, most, dt):
+    """The rows keep their sums: the column with the NaN is NaN, the others are as without it."""
+    ends = [c + n for c, n in zip(ctxs, news)]
+    k, v, table = pool(ends, PO.up(max(ends), 32), 32, 2, 128, dt, 17)
+    clean = v.clone()
+    for r in range(len(news)):
+        v[table[r, 0], :, 0, 77] = float("nan")
+    q = queries(sum(news), 6, 128, dt, 18)
+    got = A.attend_pages(q.cuda(), k.cuda(), v.cuda(), table.cuda(), starts_of(news).cuda(), ints(*ends).cuda(), most=most).cpu().double()
+    ref, bound = reference(q, k, clean, table, news, ends, U[dt])
+    bad = torch.arange(128) == 77
+    assert bool(torch.isnan(got[..., bad]).all())
+    near(got[..., ~bad], ref[..., ~bad], bound[..., ~bad], "the other columns")
+
+
 def test_offsets_past_32_bits():
     """A pool of more than 2^32 bytes: its last pages are written and read."""
     page, Hk, D, n = 64, 4, 128, 70000                   # 65,536 bytes a page and pool
