@@ -210,7 +210,7 @@ extern "C" int slotpage_extend(const int32_t* new_, int32_t* lens, int32_t* tabl
     hipStream_t st = (hipStream_t)stream;
     slothost::Scope sc(SLOTSCAN_K_PAGES, st);
     slothost::launch(page_extend, dim3(1), dim3(PT), 0, st, a);
-    if (R > PR || N > PL) slothost::launch(page_tokens, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, st, a);
+    if (N > PL || (R > PR && N)) slothost::launch(page_tokens, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, st, a);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : hip_fail(e, "page_extend launch");
 }

@@ -139,3 +139,11 @@ def test_captured_steps_follow_the_lengths():
         assert [y.tolist() for y in step] == [list(y) for y in want]
         if i == 1:
             s.trim([3] * 7)
+
+
+def test_more_rows_than_fit_on_chip_and_no_batch():
+    """Room for no token: no row gets any, and there are no tokens to place."""
+    s = State(5000, 2, 7, 16)
+    s.extend([1] * 5000, 0)
+    s.extend([0] * 5000, 0)
+    s.extend([1] * 5000, 5000)
