@@ -9,7 +9,14 @@
 // the result holds row 4 (l >> 4) + r of column l & 15.  With the keys as rows a lane's scores are one query's, and those of two blocks of 16 keys
 // are the B operand of the next product over 32 keys in the order that two transposing LDS reads give its A operand.  The keys of a block go to rows in the
 // order of key_row: a transposing read then meets every bank once (its lanes 0 .. 31 have rows 0 .. 3 and 8 .. 11).
-// One wave's 32 keys are about 450 instructions at D = 128 and 16 rows; with tiles of 32 x 32, whose rows are mostly empty, twice that.
+// 16 query rows a product, not 32: of a group's 3 or 4 query heads and one token, tiles of 32 x 32 would be nearly empty, at twice the vector work.
+//
+// Bound by memory: a step reads each sequence's keys and values once (running maxima and sums, nothing stored between the products).  A call is 8 us, in
+// which the first keys are found (the rows' costs, a search, page numbers) and arrive, and its bytes at 6.2 TB/s (a large read alone: 5.8 with its
+// start).  32 sequences of 1,024 to 8,191 keys, 12 heads of 128 on 4, cap 50 (260 MB): 54 us, 4.8 TB/s; one of 131,072 keys (268 MB) 53; 256
+// with a window of 1,024 (315 MB) 74, where a unit is hardly longer than a share, so most are cut in two; 2 to 8 tokens of 16 sequences of up to
+// 16,000 (195 MB) 48, two tiles of rows and vector issue beside the loads.  1,024 waves, one a SIMD, each with two tiles on their way (32 KB at
+// D = 128); with 1,280 no change.
 #include "slot_attn_pages.h"
 #include "slotscan.h"
 #include "slot_attn_few.h"

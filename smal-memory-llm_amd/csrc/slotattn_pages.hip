@@ -30,7 +30,8 @@ using slothost::al16;
 namespace {
 
 // ------------------------------------------------------------------------------------------- plan
-// One workgroup: the rows' tiles of MQ query rows in a row (units), then their key tiles.  Latency: two running sums.
+// One workgroup: the rows' tiles of MQ query rows in a row (units), then their key tiles.  Latency: two running sums (4.3 us
+// for 8,192 tokens of two prompts); without it each of 512 workers would form both.
 // (neither past `most`, under 2^30: rows that share tokens may add up to anything)
 __device__ __forceinline__ int before_sum(int x, int most, int* s, int& all) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -135,6 +136,13 @@ struct PairShares {
     }
 };
 
+// As attn_fwd's: the score tile is K Qt, so that a lane has one query, and its probabilities, rounded to 16 bits, are the next product's operand where
+// they are; 64-key tiles by direct loads into two buffers, one barrier a tile.  What differs is where keys lie (a group of 16 keys is of one
+// page: its address is scalar) and who does what: 512 workers with equal shares of all key tiles, in which a unit may begin and end anywhere.
+// Bound by vector issue beside the matrix products where rows are many, by memory where a unit has a token alone (three waves of four then only load).
+// Two prompts of 4,096 tokens, 12 heads of 128 on 4: 132 to 149 us by the box, 690 to 780 TFLOP/s (attn_fwd at 8,192 tokens: 726, with a cap); 56 tokens and 4
+// prompts of 300 to 1,200 with 200 to 4,000 keys before them, pages of 16: 83 us, of which the prompts alone take 61, the tokens alone 28 (140 MB).  8 waves a
+// workgroup (256 rows, halves of it half a tile apart) read half the keys, but the barriers of both halves cost more: 152 us.
 template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
     constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
@@ -340,7 +348,7 @@ template <typename T, int D> __device__ __forceinline__ void put_joined(const Pa
     put4<T>(a.out, nullptr, ((int64_t)(s + tok) * a.Hq + hq) * D + 4 * c, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// Pieces of pages_many: a worker whose last unit goes on in the next ones; a group of lanes a row.
+// Pieces of pages_many: a worker whose last unit goes on in the next ones; a group of lanes a row.  Memory: 512 workers' pieces, 67 MB, 13 us.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void pages_join(PagedArgs a) {
     constexpr int LN = D / 4, RW = 256 / LN;
@@ -355,7 +363,8 @@ __global__ __launch_bounds__(256) void pages_join(PagedArgs a) {
 }
 
 // Pieces of pages_few: a row may have hundreds.  A workgroup has `per` of the (row of the batch, head) pairs, and of their units every gridDim.y-th query
-// row, one at a time; its NG groups of lanes take every NG-th piece and meet in LDS in order.
+// row, one at a time; its NG groups of lanes take every NG-th piece and meet in LDS in order.  Latency: 4 us for 32 sequences, 5.5 for the 1,024
+// pieces of one.
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per, int QR) {
     constexpr int LN = D / 4, NG = NT / LN;
@@ -412,6 +421,8 @@ __global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per, int Q
 //   MANY    tiles of 128 query rows
 //   SHARED  one tile of at most 32 rows a key/value head (one or a few tokens of each sequence): equal shares of all keys, and a join
 //   SINGLE  the same where no row has many keys: a workgroup a unit, no join
+// Calls of SHARED run as MANY, too; SHARED / MANY with plan and join, D = 128, three query heads a group: a token each of 32 sequences (cap) 58 / 74 us,
+// of 256 with a window of 1,024 80 / 79, 2 to 8 tokens of 16 sequences 52 / 52: as fast from two tiles of 16 rows on, and a launch less up to there.
 enum { MANY, SHARED, SINGLE };
 struct Plan { int kind, QR, G; int64_t units; size_t join, pm, po, all; };
 Plan plan(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t most, int64_t W, bool prefix) {
