@@ -140,9 +140,9 @@ struct PairShares {
 // they are; 64-key tiles by direct loads into two buffers, one barrier a tile.  What differs is where keys lie (a group of 16 keys is of one
 // page: its address is scalar) and who does what: 512 workers with equal shares of all key tiles, in which a unit may begin and end anywhere.
 // Bound by vector issue beside the matrix products where rows are many, by memory where a unit has a token alone (three waves of four then only load).
-// Two prompts of 4,096 tokens, 12 heads of 128 on 4: 132 to 149 us by the box, 690 to 780 TFLOP/s (attn_fwd at 8,192 tokens: 726, with a cap); 56 tokens and 4
-// prompts of 300 to 1,200 with 200 to 4,000 keys before them, pages of 16: 83 us, of which the prompts alone take 61, the tokens alone 28 (140 MB).  8 waves a
-// workgroup (256 rows, halves of it half a tile apart) read half the keys, but the barriers of both halves cost more: 152 us.
+// Two prompts of 4,096 tokens, 12 heads of 128 on 4: 132 to 159 us by the box, 650 to 780 TFLOP/s (attn_fwd at 8,192 tokens: 726, with a cap); 56 tokens and 4
+// prompts of 300 to 1,200 with 200 to 4,000 keys before them, pages of 16: 83 us, of which the prompts alone take 61, the tokens alone 28 (140 MB).  With 8
+// waves a workgroup (256 rows, halves of it half a tile apart) 153 where these took 150, and 127 instead of 79 for the mixture, whose units are small.
 template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
     constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;

@@ -4,7 +4,7 @@
 // each row its place in the packed batch and in the stack of free pages, so nothing depends on the order in which threads run.  All
 // of it is latency: a few dependent reads and four barriers per 1,024 rows.  The tokens' positions and slots follow from the rows' starts alone: the
 // same workgroup writes those of a small batch, a second kernel those of a large one.  256 rows of one token 4.7 us and 3.5 to trim
-// them, 57,000 tokens of 64 rows 7.5 and 3.4 (their positions and slots), 7.5 to trim them.
+// them, 23,000 tokens of 64 rows 7.2 and 3.5 (their positions and slots), 7.4 to trim them.
 #include "slot_common.h"
 #include "slotscan.h"
 #include "slotpage.h"
