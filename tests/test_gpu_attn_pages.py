@@ -125,3 +125,18 @@ def _masked(q, k, v, there, u):
             a, b = AO.attention(q[i: i + 1].transpose(0, 1).unsqueeze(0), k[:, :, keep], v[:, :, keep], lens=torch.tensor([m]), u=u)["out"]
             ref[i: i + 1], bound[i: i + 1] = a[0].transpose(0, 1), b[0].transpose(0, 1)
     return ref, bound
+
+
+@pytest.mark.parametrize("news,ctxs", [([1, 1, 2], [500, 90, 300]), ([1, 200, 50], [700, 100, 333])])
+@pytest.mark.parametrize("prefix", [2 ** 31 - 1, 2 ** 31 - 20, 400, -5])
+def test_prefixes_of_any_number(news, ctxs, prefix):
+    """A prefix past all keys beside a window: every key is seen; a negative one is none."""
+    ends = [c + n for c, n in zip(ctxs, news)]
+    k, v, table = pool(ends, 60, 16, 2, 64, BF, 12)
+    q = queries(sum(news), 4, 64, BF, 13)
+    pre = torch.full((3,), prefix, dtype=torch.int32)
+    ref, bound = reference(q, k, v, table, news, ends, U[BF], window=37, prefix=pre.long())
+    for most in (max(news), None):
+        got = A.attend_pages(q.cuda(), k.cuda(), v.cuda(), table.cuda(), starts_of(news).cuda(), torch.tensor(ends, dtype=torch.int32).cuda(), most=most,
+                             window=37, prefix=pre.cuda())
+        near(got, ref, bound, f"out {prefix}")
