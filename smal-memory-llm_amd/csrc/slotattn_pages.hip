@@ -146,6 +146,8 @@ struct PairShares {
 template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
     constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
+    constexpr int VA = CAP ? 2 : 4;                   // value operands read ahead: beside a cap's four of them registers would spill
+                                                     // in the loop (56 tokens and 4 prompts with a cap: 112 us, with two 108)
     typedef PageLoad<D, KT, MW> Load;
     __shared__ __align__(1024) unsigned char smem[2][2][STAGE];      // [buffer][keys, values]
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
@@ -260,14 +262,12 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
                     s[1] = mfma32<T>(kr[kk & 3][1], qf[kk], s[1]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                uint4 vr[5];                          // operand i: column block i % DT of 16 keys i / DT
+                uint4 vr[VA + 1];                     // operand i: column block i % DT of 16 keys i / DT
                 auto colop = [&](int i) {
-                    vr[i % 5] = Ops<D>::at_col(Ops<D>::block(cc, i % DT), Ops<D>::block(c8, i % DT), STAGE + 16 * (i / DT) * Tile<D>::ROWB);
+                    vr[i % (VA + 1)] = Ops<D>::at_col(Ops<D>::block(cc, i % DT), Ops<D>::block(c8, i % DT), STAGE + 16 * (i / DT) * Tile<D>::ROWB);
                 };
-                colop(0);
-                colop(1);
-                colop(2);
-                colop(3);
+#pragma unroll
+                for (int i = 0; i < VA; i++) colop(i);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     scores<CAP>(s[i], a.s);
@@ -287,8 +287,8 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
                 sum.template weigh<2>(s, pf);
 #pragma unroll
                 for (int i = 0; i < 4 * DT; i++) {
-                    sum.o[i % DT] = mfma32<T>(vr[i % 5], pf[i / DT >> 1][i / DT & 1], sum.o[i % DT]);
-                    if (i + 4 < 4 * DT) colop(i + 4);
+                    sum.o[i % DT] = mfma32<T>(vr[i % (VA + 1)], pf[i / DT >> 1][i / DT & 1], sum.o[i % DT]);
+                    if (i + VA < 4 * DT) colop(i + VA);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -394,12 +394,12 @@ __global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per, int Q
                     __syncthreads();
                     if (g == 0) {
                         M = -INFINITY;
-#pragma unroll
+#pragma unroll 8
                         for (int z = 0; z < NG; z++) M = fmaxf(M, s_m[z].x);
                         const float Mu = M == -INFINITY ? 0.f : M;
                         L = 0.f;
                         acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
+#pragma unroll 8
                         for (int z = 0; z < NG; z++) {
                             const float f = exp2_(s_m[z].x - Mu);
                             const float4 o = *reinterpret_cast<const float4*>(&s_o[z][4 * c]);
