@@ -21,6 +21,9 @@ using slothost::al16;
 #define ML 2                                         // what a unit costs beside its tiles, in tiles: its search, first loads and end take about 5 us
 #define MA 9                                         // shares of a CU's first and second workgroup
 #define MB 7
+#define LW 4                                         // whole units, one a workgroup, if none costs more than this beside LP % of an equal share
+#define LP 130
+#define LG 65536                                     // workgroups at most
 #define LT 1024                                      // threads of pages_plan
 // The waves of a workgroup of pages_few share one unit up to this many keys and units (a round of workgroups); SINGLE / SHARED with its join, D = 128:
 // 32 units of 512 keys 11 / 18 us, 16 of 2,048 24 / 18, 1,024 of 512 54 / 51.
@@ -57,7 +60,7 @@ __device__ __forceinline__ int before_sum(int x, int most, int* s, int& all) {
 }
 
 __global__ __launch_bounds__(LT) void pages_plan(PagedArgs a) {
-    __shared__ int s_sum[LT / 64];
+    __shared__ int s_sum[LT / 64], s_most, s_count[LT];
     int* cost_r = a.plan;                             // running costs in front of each row
     int* first = a.plan + a.R + 1;
     int* cost = first + a.R + 1;
@@ -74,35 +77,68 @@ __global__ __launch_bounds__(LT) void pages_plan(PagedArgs a) {
         if (r < a.R) first[r] = u;
         u0 = min(u0 + all, a.units);
     }
-    if (tid == 0) first[a.R] = u0;
+    if (tid == 0) first[a.R] = u0, s_most = 0;
+    s_count[tid] = 0;
     __syncthreads();
-    int c0 = 0;
+    auto row_of = [&](int i) -> int {                 // the last row whose first unit is at or before i
+        int lo = 0, hi = a.R;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first[mid] <= i) lo = mid; else hi = mid;
+        }
+        return lo;
+    };
+    int shift = 0;                                    // for the lists of units of about one cost, the longest ones first
+    while ((ML + (((a.M << a.shift) + KT - 1) / KT)) >> shift >= LT) shift++;
+    int c0 = 0, c1 = 0, lo1 = 0;                      // c1, lo1: of the thread's first unit
     for (int i0 = 0; i0 < u0; i0 += LT) {
         const int i = i0 + tid;
-        int c = 0, lo = 0, hi = a.R;
+        int c = 0, lo = 0;
         if (i < u0) {
-            while (hi - lo > 1) {                     // the last row whose first unit is at or before i
-                const int mid = (lo + hi) >> 1;
-                if (first[mid] <= i) lo = mid; else hi = mid;
-            }
+            lo = row_of(i);
             const Seq x = seq_of(a, lo);
             const int t = i - first[lo], off = x.end - x.n, last = min(MQ * (t + 1), x.n * a.rep) - 1;
             int k0, k1;
             keys_of<KT>(a, x, MQ * t / a.rep + off, last / a.rep + off, k0, k1);
             c = ML + max(1, (k1 - k0 + KT - 1) / KT);
+            atomicAdd(&s_count[LT - 1 - (c >> shift)], 1);
         }
+        int most = c;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d));
+        if ((tid & 63) == 0) atomicMax(&s_most, most);
         const int at = c0 + before_sum(c, 0x3fffffff, s_sum, all);
         if (i < u0) {
             cost[i] = at;
             if (i == first[lo]) cost_r[lo] = at;
         }
+        if (i0 == 0) c1 = c, lo1 = lo;
         c0 += all;
     }
     if (tid == 0) cost[u0] = c0;
     __syncthreads();
-    // rows without units stand where the next row stands
-    for (int r = tid; r <= a.R; r += LT)
-        if (r == a.R || first[r] == first[r + 1]) cost_r[r] = cost[first[r]];
+    // Whole units, one a workgroup, the longest first, where none is much longer than an equal share: no pieces, nothing to join
+    int* list = cost + a.units + 1;
+    const int64_t shares = min(a.G, max(c0 * a.Hk / 4, 1)), longest = LW + (int64_t)c0 * a.Hk * LP / (100 * shares);
+    const bool whole = s_most <= longest && (int64_t)u0 * a.Hk <= a.wgs;
+    if (tid == 0) list[0] = whole ? u0 : 0;
+    if (whole) {
+        const int at = before_sum(s_count[tid], 0x3fffffff, s_sum, all);
+        s_count[tid] = at;
+        __syncthreads();
+        for (int i = tid; i < u0; i += LT) {          // (units of one list in any order: each is computed by itself)
+            const int c = i < LT ? c1 : cost[i + 1] - cost[i], lo = i < LT ? lo1 : row_of(i);
+            const int k = atomicAdd(&s_count[LT - 1 - (c >> shift)], 1);
+            list[1 + 2 * k] = lo;
+            list[2 + 2 * k] = i - first[lo];
+        }
+        // (the row's costs are not read)
+    } else {
+        // rows without units stand where the next row stands
+        for (int r = tid; r < a.R; r += LT)
+            if (first[r] == first[r + 1]) cost_r[r] = cost[first[r]];
+    }
+    if (tid == 0) cost_r[a.R] = c0;
 }
 
 // the last i of [lo, hi) with mul x[i] <= y (x ascending, x[lo] does), by all lanes
@@ -157,19 +193,23 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
     const int* first = a.plan + a.R + 1;
     const int* cost = first + a.R + 1;
     const int total = ld_uni(cost_r, a.R) * a.Hk;
-    // workers that follow each other run on one XCD (workgroup i on XCD i % 8): they share keys
-    const int G = min((int)gridDim.x, max((total + 3) / 4, 1));
+    const int* list = cost + a.units + 1;
+    const int units = ld_uni(list, 0), G = units ? units * a.Hk : min(a.G, max((total + 3) / 4, 1));
     int me = blockIdx.x;
     if (me >= G) {
-        if (tid == 0) a.join[me].parts = 0;
+        if (tid == 0 && me < a.G) a.join[me].parts = 0;
         return;
     }
-    if (G % 8 == 0) me = (me & 7) * (G / 8) + (me >> 3);
     const PairShares sh(total, G);
-    int x = sh.begin(me);
-    const int end = sh.begin(me + 1);
+    int x = 0, end = 1, r = 0;
+    if (!units) {
+        // workers that follow each other run on one XCD (workgroup i on XCD i % 8): they share keys
+        if (G % 8 == 0) me = (me & 7) * (G / 8) + (me >> 3);
+        x = sh.begin(me);
+        end = sh.begin(me + 1);
+        r = uni(find(cost_r, 0, a.R, a.Hk, x, lane));
+    }
     Unit left{0, 0, 0, 0, 0};
-    int r = uni(find(cost_r, 0, a.R, a.Hk, x, lane));
     const unsigned lds = lds_addr(smem);
     const Load lk(a.k_sp, a.k_st, a.shift, w, lane), lv(a.v_sp, a.v_st, a.shift, w, lane);
     const Ops<D> ops(lane);
@@ -177,15 +217,27 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
     RowSums<T, D, BIAS> sum(f2);
     while (x < end) {
         // the unit of x, and this worker's key tiles [ka, kb) of its c
-        const int cr = ld_uni(cost_r, r), per = ld_uni(cost_r, r + 1) - cr, y = x - cr * a.Hk;
-        if (y >= per * a.Hk) { r++; continue; }
-        const int hk = y / per, z = y - hk * per + cr;
-        const int u0 = ld_uni(first, r), u = uni(find(cost, u0, ld_uni(first, r + 1), 1, z, lane));
-        const int cu = ld_uni(cost, u), c = ld_uni(cost, u + 1) - cu - ML, y0 = z - cu, y1 = min(c + ML, y0 + end - x);
-        const int ka = max(0, y0 - ML), kb = max(0, y1 - ML);
-        x += y1 - y0;
-        if (kb <= ka) continue;                       // of this unit the worker's share is its beginning alone
-        const int t = u - u0;
+        int hk, t, ka = 0, kb = 0xffffff, c = kb;        // (all of them)
+        if (units) {
+            const int i = me / a.Hk;
+            hk = me - i * a.Hk;
+            r = ld_uni(list, 1 + 2 * i);
+            t = ld_uni(list, 2 + 2 * i);
+            x = end;
+        } else {
+            const int cr = ld_uni(cost_r, r), per = ld_uni(cost_r, r + 1) - cr, y = x - cr * a.Hk;
+            if (y >= per * a.Hk) { r++; continue; }
+            hk = y / per;
+            const int z = y - hk * per + cr, u0 = ld_uni(first, r), u = uni(find(cost, u0, ld_uni(first, r + 1), 1, z, lane));
+            const int cu = ld_uni(cost, u), y0 = z - cu;
+            c = ld_uni(cost, u + 1) - cu - ML;
+            const int y1 = min(c + ML, y0 + end - x);
+            ka = max(0, y0 - ML);
+            kb = max(0, y1 - ML);
+            x += y1 - y0;
+            if (kb <= ka) continue;                   // of this unit the worker's share is its beginning alone
+            t = u - u0;
+        }
         const Seq sq = seq_uni(a, r);
         const int rows = sq.n * a.rep, off = sq.end - sq.n, row0 = MQ * t + 32 * w, row = min(row0 + (lane & 31), rows - 1);
         const int tok = row / a.rep, hq = hk * a.rep + row - tok * a.rep, p = tok + off;
@@ -304,7 +356,7 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
                                 ((int64_t)(2 * me + (ka == 0)) * MW + w) * 32, lane, [&](int j) { return sight.some(j & -KT, j | (KT - 1)); });
         if (ka == 0 && kb < c) left = {r, hk, t, sq.n, sh.owner(end + c - kb - 1) - me + 1};        // its other pieces: up to the worker of its last tile
     }
-    if (tid == 0) a.join[me] = left;
+    if (tid == 0 && me < a.G) a.join[me] = left;
 }
 
 // ------------------------------------------------------------------------------------------- join
@@ -424,7 +476,7 @@ __global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per, int Q
 // Calls of SHARED run as MANY, too; SHARED / MANY with plan and join, D = 128, three query heads a group: a token each of 32 sequences (cap) 58 / 74 us,
 // of 256 with a window of 1,024 80 / 79, 2 to 8 tokens of 16 sequences 52 / 52: as fast from two tiles of 16 rows on, and a launch less up to there.
 enum { MANY, SHARED, SINGLE };
-struct Plan { int kind, QR, G; int64_t units; size_t join, pm, po, all; };
+struct Plan { int kind, QR, G, wgs; int64_t units; size_t join, pm, po, all; };
 Plan plan(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t most, int64_t W, bool prefix) {
     Plan x{};
     const int64_t rep = Hq / Hk, rows = std::min(N, R);
@@ -439,7 +491,8 @@ Plan plan(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk,
     if (x.kind == SINGLE) return x;
     const int64_t tiles = x.units * Hk * ((M * page + K - 1) / K + ML);
     x.G = x.kind == MANY ? (int)std::min<int64_t>(MG, (tiles + 3) / 4) : (int)std::min<int64_t>(FG * 128 / D, std::max<int64_t>(tiles / FS, 1));
-    x.join = x.kind == MANY ? up((size_t)(2 * (R + 1) + x.units + 1) * 4) : 0;
+    x.join = x.kind == MANY ? up((size_t)(2 * (R + 1) + 3 * x.units + 2) * 4) : 0;
+    x.wgs = (int)std::max<int64_t>(x.G, std::min<int64_t>(x.units * Hk, LG));
     x.pm = x.join + up(x.kind == MANY ? (size_t)x.G * sizeof(Unit) : (size_t)(N * rep / Q + R) * Hk * sizeof(Piece));
     x.po = x.pm + up((size_t)x.G * 2 * Q * sizeof(float2));
     x.all = x.po + up((size_t)x.G * 2 * Q * D * sizeof(float));
@@ -500,7 +553,7 @@ extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const v
     a.q_sh = q_sh; a.q_st = q_st; a.k_sp = k_sp; a.k_sh = k_sh; a.k_st = k_st; a.v_sp = v_sp; a.v_sh = v_sh; a.v_st = v_st;
     a.table = table; a.t_sr = t_sr; a.starts = starts; a.ends = ends; a.prefix = prefix; a.slopes = slopes;
     a.N = (int)N; a.R = (int)R; a.M = (int)M; a.P = (int)P; a.Hq = (int)Hq; a.Hk = (int)Hk; a.rep = (int)(Hq / Hk);
-    a.W = a.s.W; a.shift = __builtin_ctzll((unsigned long long)page); a.units = (int)x.units;
+    a.W = a.s.W; a.shift = __builtin_ctzll((unsigned long long)page); a.units = (int)x.units; a.G = x.G; a.wgs = x.wgs;
     char* ws = (char*)workspace;
     a.plan = (int*)ws; a.join = (Unit*)(ws + x.join); a.pieces = (Piece*)(ws + x.join); a.pm = (float2*)(ws + x.pm); a.po = (float*)(ws + x.po);
     a.out = out;
@@ -517,8 +570,8 @@ extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const v
     {
         slothost::Scope sc(SLOTSCAN_K_ATTN, st);
         if (x.kind != MANY) slotattn_few::launch(a, dtype, (int)D, cp, x.QR, x.G, tiles, st);
-        else if (dtype == SLOTSCAN_BF16) D == 128 ? launch_attn<bf16_t, 128>(a, cp, x.G, st) : launch_attn<bf16_t, 64>(a, cp, x.G, st);
-        else D == 128 ? launch_attn<f16_t, 128>(a, cp, x.G, st) : launch_attn<f16_t, 64>(a, cp, x.G, st);
+        else if (dtype == SLOTSCAN_BF16) D == 128 ? launch_attn<bf16_t, 128>(a, cp, x.wgs, st) : launch_attn<bf16_t, 64>(a, cp, x.wgs, st);
+        else D == 128 ? launch_attn<f16_t, 128>(a, cp, x.wgs, st) : launch_attn<f16_t, 64>(a, cp, x.wgs, st);
         e = hipGetLastError();
     }
     if (e != hipSuccess) return hip_fail(e, "pages_many or pages_few launch");
