@@ -22,7 +22,7 @@ struct PagedArgs {
     int64_t q_sh, q_st, k_sp, k_sh, k_st, v_sp, v_sh, v_st;
     const int32_t* table; int64_t t_sr;
     const int32_t* starts; const int32_t* ends; const int32_t* prefix; const float* slopes;
-    int N, R, M, P, Hq, Hk, rep, W, shift, units, G, wgs;     // units: room for them in the plan; workers and workgroups of pages_many
+    int N, R, M, P, Hq, Hk, rep, W, shift, units, G, whole;   // units: room for them in the plan; pages_many's workers; whole units at most
     // running costs of the rows (R + 1), first units of the rows (R + 1), running costs (units + 1); then 0, or the number of units
     // and (row, tile of rows) of each, the longest first
     int* plan;

@@ -21,9 +21,12 @@ using slothost::al16;
 #define ML 2                                         // what a unit costs beside its tiles, in tiles: its search, first loads and end take about 5 us
 #define MA 9                                         // shares of a CU's first and second workgroup
 #define MB 7
-#define LW 4                                         // whole units, one a workgroup, if none costs more than this beside LP % of an equal share
-#define LP 130
-#define LG 65536                                     // workgroups at most
+// Units run whole, one a workgroup, if none costs more than LW tiles beside LP % of an equal share.  Plan, attention and join of whole units / of shares, 12
+// heads of 128 on 4: 8 x 1,024 tokens (the longest 1.1 times a share) 60 / 71 us, 2 x 4,096 (1.27) 157 / 171, 1 x 8,192 (1.3) 280 / 278, 1 x 6,000
+// (1.8) 187 / 157.  At D = 64, where pieces are half as large, never: 6 heads, 8 x 1,024 40 / 38, 200 x 33 37 / 35.
+#define LW 4
+#define LP 120
+#define LG 65536                                     // of them at most
 #define LT 1024                                      // threads of pages_plan
 // The waves of a workgroup of pages_few share one unit up to this many keys and units (a round of workgroups); SINGLE / SHARED with its join, D = 128:
 // 32 units of 512 keys 11 / 18 us, 16 of 2,048 24 / 18, 1,024 of 512 54 / 51.
@@ -120,7 +123,7 @@ __global__ __launch_bounds__(LT) void pages_plan(PagedArgs a) {
     // Whole units, one a workgroup, the longest first, where none is much longer than an equal share: no pieces, nothing to join
     int* list = cost + a.units + 1;
     const int64_t shares = min(a.G, max(c0 * a.Hk / 4, 1)), longest = LW + (int64_t)c0 * a.Hk * LP / (100 * shares);
-    const bool whole = s_most <= longest && (int64_t)u0 * a.Hk <= a.wgs;
+    const bool whole = s_most <= longest && (int64_t)u0 * a.Hk <= a.whole;
     if (tid == 0) list[0] = whole ? u0 : 0;
     if (whole) {
         const int at = before_sum(s_count[tid], 0x3fffffff, s_sum, all);
@@ -194,7 +197,7 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
     const int* cost = first + a.R + 1;
     const int total = ld_uni(cost_r, a.R) * a.Hk;
     const int* list = cost + a.units + 1;
-    const int units = ld_uni(list, 0), G = units ? units * a.Hk : min(a.G, max((total + 3) / 4, 1));
+    const int units = D == 128 ? ld_uni(list, 0) : 0, G = units ? units * a.Hk : min(a.G, max((total + 3) / 4, 1));
     int me = blockIdx.x;
     if (me >= G) {
         if (tid == 0 && me < a.G) a.join[me].parts = 0;
@@ -492,7 +495,7 @@ Plan plan(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk,
     const int64_t tiles = x.units * Hk * ((M * page + K - 1) / K + ML);
     x.G = x.kind == MANY ? (int)std::min<int64_t>(MG, (tiles + 3) / 4) : (int)std::min<int64_t>(FG * 128 / D, std::max<int64_t>(tiles / FS, 1));
     x.join = x.kind == MANY ? up((size_t)(2 * (R + 1) + 3 * x.units + 2) * 4) : 0;
-    x.wgs = (int)std::max<int64_t>(x.G, std::min<int64_t>(x.units * Hk, LG));
+    x.wgs = D == 128 ? (int)std::max<int64_t>(x.G, std::min<int64_t>(x.units * Hk, LG)) : x.G;
     x.pm = x.join + up(x.kind == MANY ? (size_t)x.G * sizeof(Unit) : (size_t)(N * rep / Q + R) * Hk * sizeof(Piece));
     x.po = x.pm + up((size_t)x.G * 2 * Q * sizeof(float2));
     x.all = x.po + up((size_t)x.G * 2 * Q * D * sizeof(float));
@@ -553,7 +556,7 @@ extern "C" int slotattn_pages(const void* q, int64_t q_sh, int64_t q_st, const v
     a.q_sh = q_sh; a.q_st = q_st; a.k_sp = k_sp; a.k_sh = k_sh; a.k_st = k_st; a.v_sp = v_sp; a.v_sh = v_sh; a.v_st = v_st;
     a.table = table; a.t_sr = t_sr; a.starts = starts; a.ends = ends; a.prefix = prefix; a.slopes = slopes;
     a.N = (int)N; a.R = (int)R; a.M = (int)M; a.P = (int)P; a.Hq = (int)Hq; a.Hk = (int)Hk; a.rep = (int)(Hq / Hk);
-    a.W = a.s.W; a.shift = __builtin_ctzll((unsigned long long)page); a.units = (int)x.units; a.G = x.G; a.wgs = x.wgs;
+    a.W = a.s.W; a.shift = __builtin_ctzll((unsigned long long)page); a.units = (int)x.units; a.G = x.G; a.whole = D == 128 ? x.wgs : 0;
     char* ws = (char*)workspace;
     a.plan = (int*)ws; a.join = (Unit*)(ws + x.join); a.pieces = (Piece*)(ws + x.join); a.pm = (float2*)(ws + x.pm); a.po = (float*)(ws + x.po);
     a.out = out;

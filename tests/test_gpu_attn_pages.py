@@ -140,3 +140,39 @@ def test_prefixes_of_any_number(news, ctxs, prefix):
         got = A.attend_pages(q.cuda(), k.cuda(), v.cuda(), table.cuda(), starts_of(news).cuda(), torch.tensor(ends, dtype=torch.int32).cuda(), most=most,
                              window=37, prefix=pre.cuda())
         near(got, ref, bound, f"out {prefix}")
+
+
+@pytest.mark.parametrize("Hq,Hk,dt,page", [(6, 2, BF, 16), (4, 4, HF, 64), (12, 1, BF, 32)])
+@pytest.mark.parametrize("o", [{}, dict(cap=20.0, window=70), dict(slopes=True, prefix=True), dict(prefix=True, window=33)])
+def test_units_of_about_one_length(Hq, Hk, dt, page, o):
+    """Units that run whole, a workgroup each; rows without tokens and without earlier keys between them."""
+    news = [(37 * r) % 41 + 5 for r in range(60)]
+    ctxs = [(53 * r) % 200 for r in range(60)]
+    news[3] = news[30] = news[59] = 0
+    run(news, ctxs, page, Hq, Hk, 128, dt, 14, pad=3, by_token=page == 32, **o)
+    run([128] * 7, [0] * 7, page, Hq, Hk, 128, dt, 15, **o)
+
+
+def test_replays_follow_the_lengths_from_alike_rows_to_unlike_ones():
+    """One captured call whose rows are alike, unlike and alike again: what is whole and what is shared out is decided on the GPU."""
+    sets = [([40] * 30, [100] * 30), ([1] * 29 + [1171], [900] + [3] * 28 + [500]), ([40] * 30, [0] * 30)]
+    ends = [[c + n for c, n in zip(ctxs, news)] for news, ctxs in sets]
+    most = [max(e[r] for e in ends) for r in range(30)]
+    k, v, table = pool(most, max(PO.up(e, 16) for e in most), 16, 2, 128, BF, 16)
+    q = queries(1200, 6, 128, BF, 17)
+    kc, vc, tc, qc = k.cuda(), v.cuda(), table.cuda(), q.cuda()
+    starts, end = starts_of(sets[0][0]).cuda(), torch.tensor(ends[0], dtype=torch.int32).cuda()
+    call = lambda: A.attend_pages(qc, kc, vc, tc, starts, end)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for (news, _), e in zip(sets, ends):
+        starts.copy_(starts_of(news))
+        end.copy_(torch.tensor(e, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref, bound = reference(q, k, v, table, news, e, U[BF])
+        near(out, ref, bound, f"replay {news[-1]}")
+        assert torch.equal(out, call())
