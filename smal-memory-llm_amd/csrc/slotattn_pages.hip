@@ -36,8 +36,8 @@ using slothost::al16;
 namespace {
 
 // ------------------------------------------------------------------------------------------- plan
-// One workgroup: the rows' tiles of MQ query rows in a row (units), then their key tiles.  Latency: two running sums (4.3 us
-// for 8,192 tokens of two prompts); without it each of 512 workers would form both.
+// One workgroup: the rows' tiles of MQ query rows in a row (units), then their key tiles.  Latency: two running sums (4.5 us
+// for 8,192 tokens of two prompts, 6 with the list of whole units); without it each of 512 workers would form both.
 // (neither past `most`, under 2^30: rows that share tokens may add up to anything)
 __device__ __forceinline__ int before_sum(int x, int most, int* s, int& all) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -177,11 +177,12 @@ struct PairShares {
 
 // As attn_fwd's: the score tile is K Qt, so that a lane has one query, and its probabilities, rounded to 16 bits, are the next product's operand where
 // they are; 64-key tiles by direct loads into two buffers, one barrier a tile.  What differs is where keys lie (a group of 16 keys is of one
-// page: its address is scalar) and who does what: 512 workers with equal shares of all key tiles, in which a unit may begin and end anywhere.
+// page: its address is scalar) and who does what: a workgroup a whole unit, or 512 workers with equal shares of all key tiles, in which a unit may begin and
+// end anywhere; pages_plan chooses.
 // Bound by vector issue beside the matrix products where rows are many, by memory where a unit has a token alone (three waves of four then only load).
-// Two prompts of 4,096 tokens, 12 heads of 128 on 4: 132 to 159 us by the box, 650 to 780 TFLOP/s (attn_fwd at 8,192 tokens: 726, with a cap); 56 tokens and 4
-// prompts of 300 to 1,200 with 200 to 4,000 keys before them, pages of 16: 83 us, of which the prompts alone take 61, the tokens alone 28 (140 MB).  With 8
-// waves a workgroup (256 rows, halves of it half a tile apart) 153 where these took 150, and 127 instead of 79 for the mixture, whose units are small.
+// Two prompts of 4,096 tokens, 12 heads of 128 on 4: 140 to 147 us by the box, 700 to 740 TFLOP/s (attn_fwd without pages 122 to 130); 56 tokens and 4
+// prompts of 300 to 1,200 with 200 to 4,000 keys before them, pages of 16: 85 us, of which the prompts alone take 61, the tokens alone 28 (140 MB).  With 8
+// waves a workgroup (256 rows, halves of it half a tile apart) 153 where shares took 150, and 127 instead of 79 for the mixture, whose units are small.
 template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
     constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
