@@ -4,6 +4,7 @@
 // that it sees is a unit, and all units' key tiles in a row are shared out to the workers in equal contiguous pieces, so that neither
 // ragged lengths nor causality leave a worker more than another.  A piece that is not a whole unit leaves its rows' maxima, sums and
 // weighted values in the workspace, two such pieces a worker at most, and pages_join combines a unit's pieces in order.
+// (pages_many takes whole units, a workgroup each, where they are much alike.)
 #pragma once
 #include "slot_attn_rows.h"
 #include "slot_attn_host.h"

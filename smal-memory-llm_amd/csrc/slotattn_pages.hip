@@ -187,7 +187,8 @@ template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
     constexpr int KK = D / 16, DT = D / 32, STAGE = KT * 2 * D;
     constexpr int VA = CAP ? 2 : 4;                   // value operands read ahead: beside a cap's four of them registers would spill
-                                                     // in the loop (56 tokens and 4 prompts with a cap: 112 us, with two 108)
+                                                     // in the loop (56 tokens and 4 prompts with a cap: 112 us, with two 108; what spills then is set up
+                                                     // once a unit)
     typedef PageLoad<D, KT, MW> Load;
     __shared__ __align__(1024) unsigned char smem[2][2][STAGE];      // [buffer][keys, values]
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
