@@ -3,8 +3,8 @@
 // One workgroup walks the rows, a row a thread: running sums over the rows (DPP-free shuffles within a wave, then the waves' sums in LDS) give
 // each row its place in the packed batch and in the stack of free pages, so nothing depends on the order in which threads run.  All
 // of it is latency: a few dependent reads and four barriers per 1,024 rows.  The tokens' positions and slots follow from the rows' starts alone: the
-// same workgroup writes those of a small batch, a second kernel those of a large one.  256 rows of one token 4.7 us and 3.5 to trim
-// them, 23,000 tokens of 64 rows 7.2 and 3.5 (their positions and slots), 7.4 to trim them.
+// same workgroup writes those of a small batch, a second kernel those of a large one.  256 rows of one token 4.8 us and 3.9 to trim
+// them, 23,000 tokens of 64 rows 5.2 to 5.7 and 3.5 (their positions and slots), 4 to 4.5 to trim them.
 #include "slot_common.h"
 #include "slotscan.h"
 #include "slotpage.h"
@@ -18,7 +18,6 @@ using slothost::hip_fail;
 #define PW (PT / 64)
 #define PL 8192                                      // tokens that it writes itself
 #define PR 4096                                      // rows whose starts it keeps in LDS for that
-#define SERIAL 4                                     // pages of a row that its own thread moves
 
 namespace {
 
@@ -55,6 +54,16 @@ __device__ __forceinline__ uint32_t before(uint32_t x, uint32_t top, uint32_t* s
     return satsum(base, ex, top);
 }
 
+// Page p of a round of rows, which begin at pages off[0 .. rows) (ascending): the last row that begins at or before it.
+__device__ __forceinline__ int row_of(const uint32_t* off, int rows, uint32_t p) {
+    int lo = 0, hi = rows;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (off[mid] <= p) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
 // Token i of the packed batch: its row is the last one that starts at or before it.
 __device__ __forceinline__ void put_token(const PageArgs& a, const int32_t* starts, int i) {
     int lo = 0, hi = a.R;                             // starts[lo] <= i < starts[hi]
@@ -76,9 +85,10 @@ __device__ __forceinline__ void put_token(const PageArgs& a, const int32_t* star
 
 __global__ __launch_bounds__(PT) void page_extend(PageArgs a) {
     __shared__ uint32_t s_sum[PW + 1];
-    __shared__ int32_t s_start[PR + 1];
+    __shared__ int32_t s_start[PR + 1], s_first[PT];  // rows' first tokens; of a round's rows the number of the first new page, -1: none
+    __shared__ uint32_t s_off[PT];                    // and the pages asked for before them
     __shared__ uint32_t s_taken;                      // pages handed out: those up to the last row that got any
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x;
     const int n = min(max(a.free_[0], 0), a.P);
     const uint32_t topN = (uint32_t)a.N + 1, topP = (uint32_t)n + 1;
     uint32_t at = 0, off = 0;                         // of the rows of earlier rounds: tokens, pages asked for
@@ -99,7 +109,7 @@ __global__ __launch_bounds__(PT) void page_extend(PageArgs a) {
         const bool fits = want > 0 && s1 <= (uint32_t)a.N && have >= 0 && (int64_t)have + want <= (int64_t)a.M << a.shift;
         const int first = up(max(have, 0), a.shift), need = fits ? up(have + want, a.shift) - first : 0;
         const uint32_t y = min((uint32_t)need, topP);
-        const uint32_t o0 = satsum(off, before(y, topP, s_sum, all), topP);
+        const uint32_t o0 = satsum(off, before(y, topP, s_sum, all), topP), begin = off;
         off = satsum(off, all, topP);
         const bool got = fits && (need == 0 || satsum(o0, y, topP) <= (uint32_t)n);
         if (got && need) atomicMax(&s_taken, o0 + y);
@@ -110,15 +120,17 @@ __global__ __launch_bounds__(PT) void page_extend(PageArgs a) {
             a.ends[r] = got ? have + want : 0;
             if (got) a.lens[r] = have + want;
         }
-        // the row's new pages, from the top of the stack down
-        const int src = n - (int)o0, todo = got ? need : 0;
-        if (todo <= SERIAL)
-            for (int i = 0; i < todo; i++) a.table[r * a.t_sr + first + i] = a.free_[src - i];
-        for (uint64_t b = __ballot(todo > SERIAL); b; b &= b - 1) {
-            const int k = __builtin_ctzll(b), f = __builtin_amdgcn_readlane(first, k), c = __builtin_amdgcn_readlane(todo, k),
-                      from = __builtin_amdgcn_readlane(src, k);
-            int32_t* t = a.table + (r0 + (tid & ~63) + k) * a.t_sr + f;
-            for (int i = lane; i < c; i += 64) t[i] = a.free_[from - i];
+        // The round's new pages, from the top of the stack down: a thread each (58 rows of 400 tokens: 5.2 us, row after row by a wave 7.2), or
+        // each by its row's thread where no row has two (256 rows of a token: 4.8, else 5.1)
+        s_off[tid] = o0;
+        s_first[tid] = got ? first : -1;
+        if (!__syncthreads_or(got && need > 1)) {
+            if (got && need) a.table[r * a.t_sr + first] = a.free_[n - (int)o0];
+            continue;
+        }
+        for (uint32_t p = begin + tid; p < min(off, (uint32_t)n); p += PT) {
+            const int k = row_of(s_off, min(PT, a.R - r0), p);
+            if (s_first[k] >= 0) a.table[(r0 + k) * a.t_sr + s_first[k] + (int)(p - s_off[k])] = a.free_[n - (int)p];
         }
     }
     __syncthreads();                                  // the table, the ends and the starts are written
@@ -133,8 +145,9 @@ __global__ __launch_bounds__(256) void page_tokens(PageArgs a) {
 }
 
 __global__ __launch_bounds__(PT) void page_trim(PageArgs a) {
-    __shared__ uint32_t s_sum[PW + 1];
-    const int tid = threadIdx.x, lane = tid & 63;
+    __shared__ uint32_t s_sum[PW + 1], s_off[PT];     // pages that come back from the rows before a round's
+    __shared__ int32_t s_first[PT];                   // the number of a row's first page that does
+    const int tid = threadIdx.x;
     const int n = min(max(a.free_[0], 0), a.P);
     const uint32_t top = 0x7ffffffe;
     auto row = [&](int r, int& first, int& keep) -> int {             // pages that row r gives back, from its page `first` on
@@ -161,21 +174,22 @@ __global__ __launch_bounds__(PT) void page_trim(PageArgs a) {
         int first, keep;
         uint32_t all;
         const int c = row(r, first, keep);
-        const uint32_t o0 = satsum(off, before((uint32_t)c, top, s_sum, all), top);
+        const uint32_t o0 = satsum(off, before((uint32_t)c, top, s_sum, all), top), begin = off;
         off = satsum(off, all, top);
         if (r < a.R) a.lens[r] = keep;
-        const int dst = end - (int)o0;                // in [1, P] unless pages come back that were never handed out
-        auto give = [&](int32_t* t, int to) {
+        s_off[tid] = o0;
+        s_first[tid] = first;
+        auto give = [&](int32_t* t, int to) {         // to in [1, P] unless pages come back that were never handed out
             if (to >= 1 && to <= a.P) a.free_[to] = *t;
             *t = -1;
         };
-        if (c <= SERIAL)
-            for (int i = 0; i < c; i++) give(a.table + r * a.t_sr + first + i, dst - i);
-        for (uint64_t b = __ballot(c > SERIAL); b; b &= b - 1) {
-            const int k = __builtin_ctzll(b), f = __builtin_amdgcn_readlane(first, k), cc = __builtin_amdgcn_readlane(c, k),
-                      d = __builtin_amdgcn_readlane(dst, k);
-            int32_t* t = a.table + (r0 + (tid & ~63) + k) * a.t_sr + f;
-            for (int i = lane; i < cc; i += 64) give(t + i, d - i);
+        if (!__syncthreads_or(c > 1)) {
+            if (c) give(a.table + r * a.t_sr + first, end - (int)o0);
+            continue;
+        }
+        for (uint32_t p = begin + tid; p < off; p += PT) {
+            const int k = row_of(s_off, min(PT, a.R - r0), p);
+            give(a.table + (r0 + k) * a.t_sr + s_first[k] + (int)(p - s_off[k]), end - (int)p);
         }
     }
     __syncthreads();
