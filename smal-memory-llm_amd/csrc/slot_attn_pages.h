@@ -45,7 +45,7 @@ __device__ __forceinline__ Seq make_seq(const PagedArgs& a, int s0, int s1, int 
     x.n = min(max(s1, x.s), a.N) - x.s;
     x.end = min(max(end, 0), (1 << 30) - 1);
     x.klen = min(x.end, a.M << a.shift);
-    x.pre = min(pre, x.klen);                         // (any number: sums with it stay in range)
+    x.pre = max(0, min(pre, x.klen));                 // (any number: sums and differences with it stay in range)
     return x;
 }
 __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int r) {                       // a row of the lane's

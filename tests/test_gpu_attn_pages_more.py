@@ -101,3 +101,17 @@ def test_scores_of_any_size(Hq, Hk, D, dt, scale, o):
         got = A.attend_pages(q.cuda(), k.cuda(), v.cuda(), table.cuda(), starts_of(news).cuda(), ints(ends), most=most, scale=scale, **o)
         want, size = (reference(q, k, y, table, news, ends, U[dt], scale=scale, window=o.get("window"))[0] for y in (v, v.abs()))
         near(got, want, 1.02 * U[dt] * (size + want.abs()) + 2.0 ** -20, "out")
+
+
+@pytest.mark.parametrize("news,ctxs", [([1, 1, 2], [500, 90, 300]), ([1, 200, 50], [700, 100, 333]), ([1], [3000])])
+@pytest.mark.parametrize("window", [None, 37])
+def test_the_least_prefix_is_none(news, ctxs, window):
+    """-2^31, of which nothing can be taken: as any other negative prefix."""
+    ends = [c + n for c, n in zip(ctxs, news)]
+    k, v, table = pool(ends, 200, 16, 2, 64, BF, 30)
+    q = queries(sum(news), 4, 64, BF, 31)
+    ref, bound = reference(q, k, v, table, news, ends, U[BF], window=window)
+    for most in (max(news), None):
+        got = A.attend_pages(q.cuda(), k.cuda(), v.cuda(), table.cuda(), starts_of(news).cuda(), ints(ends), most=most, window=window,
+                             prefix=ints([-2 ** 31] * len(news)))
+        near(got, ref, bound, "out")
