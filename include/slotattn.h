@@ -63,7 +63,8 @@ int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const 
  *   q by strides (head, token), k, v (P, Hk, page, D) by strides (page, head, row within the page), every row 16-byte aligned; page a power of two
  *           in [16, 4096]; table rows t_sr elements apart; starts (R + 1), ends (R), prefix (R) int32; out (N, Hq, D) contiguous
  *   most    an upper bound of the rows' numbers of tokens, or N.  It chooses between kernels; results do not depend on it but for rounding
- * Nothing outside the tensors is read or written whatever table, starts and ends hold.  Rows must not share tokens (starts that fall).
+ * Nothing outside the tensors is read or written whatever table, starts and ends hold.  Rows must not share tokens (starts that fall): what these
+ * get is not defined.
  * workspace: slotattn_pages_workspace(...) bytes (may be 0), 256-byte aligned. */
 size_t slotattn_pages_workspace(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t most,
                                 int64_t window, int has_prefix);

@@ -15,7 +15,12 @@ namespace slotattn {
 // pages_few: of each unit, the worker in which it begins and its pieces, at ((s rep) / QR + row + tile) Hk + head, s its sequence's first token:
 // a place of its own for every tile of QR rows of the batch.
 struct Unit { int r, hk, t, n, parts; };
-struct Piece { int me, parts; };
+struct Piece {
+    int me, parts;
+    // Pieces to read of those of `workers` workers.  Rows that share tokens can ask for more tiles than are handed out; units behind those leave nothing
+    // here, and what the workspace held before counts only where it names workers: the join then reads pieces of other units, but none outside.
+    __host__ __device__ __forceinline__ int there(int workers) const { return me >= 0 && parts <= workers - me ? parts : 0; }
+};
 
 struct PagedArgs {
     AttnArgs s;                                       // the scores' constants

@@ -435,11 +435,12 @@ __global__ __launch_bounds__(NT) void pages_join_few(PagedArgs a, int per, int Q
         const int rows = x.n * a.rep, at = x.s * a.rep / QR + r;
         Piece p{0, 0};
         if (rows && u < u1) p = a.pieces[at * a.Hk + hk];
+        p.parts = p.there(a.G);
         for (uint64_t b = __ballot(u < u1 && (p.parts > 1 || rows > QR)); b; b &= b - 1) {
             const int k = __builtin_ctzll(b), n = lane_of(rows, k), hd = lane_of(hk, k), s = lane_of(x.s, k), at0 = lane_of(at, k);
             Piece q{lane_of(p.me, k), lane_of(p.parts, k)};
             for (int t = 0; QR * t < n; t++) {
-                if (t) q = a.pieces[(at0 + t) * a.Hk + hd];
+                if (t) q = a.pieces[(at0 + t) * a.Hk + hd], q.parts = q.there(a.G);
                 if (q.parts < 2) continue;
                 for (int i = blockIdx.y; i < min(QR, n - QR * t); i += gridDim.y) {
                     float M, L;
