@@ -490,7 +490,8 @@ Plan plan(int64_t N, int64_t R, int64_t M, int64_t page, int64_t Hq, int64_t Hk,
     auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     x.kind = most * rep > 32 ? MANY : keys <= UNIT_KEYS && rows * Hk <= UNIT_MOST ? SINGLE : SHARED;
     if (x.kind == SINGLE && (R > 65535 || Hk > 65535)) x.kind = SHARED;
-    if (x.kind == SHARED && (N * rep / 16 + rows) * Hk * ((M * page + 31) / 32) > 0x3fffffffLL) x.kind = MANY;      // (its sums are 32-bit ones)
+    // (its sums of tiles and its numbers of pieces are 32-bit ones)
+    if (x.kind == SHARED && ((N * rep / 16 + rows) * Hk * ((M * page + 31) / 32) > 0x3fffffffLL || (N * rep / 16 + R) * Hk > 0x3fffffffLL)) x.kind = MANY;
     x.QR = x.kind == MANY ? MQ : most * rep > 16 ? 32 : 16;
     const int64_t Q = x.QR, K = x.kind == MANY ? KT : 32;
     x.units = N * rep / Q + rows;
