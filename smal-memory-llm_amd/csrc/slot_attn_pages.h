@@ -44,7 +44,7 @@ __device__ __forceinline__ int ld_uni(const int32_t* p, int64_t i) { return ((co
 
 // A sequence's part of the batch, whatever the tensors hold: tokens s .. s + n - 1 of [0, N), the first at position end - n
 struct Seq { int s, n, end, klen, pre; };
-__device__ __forceinline__ Seq make_seq(const PagedArgs& a, int s0, int s1, int end, int pre) {
+__host__ __device__ __forceinline__ Seq make_seq(const PagedArgs& a, int s0, int s1, int end, int pre) {
     Seq x;
     x.s = min(max(s0, 0), a.N);
     x.n = min(max(s1, x.s), a.N) - x.s;
@@ -59,18 +59,35 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs& a, int r) {              
 __device__ __forceinline__ Seq seq_uni(const PagedArgs& a, int r) {                      // a row of the wave's
     return make_seq(a, ld_uni(a.starts, r), ld_uni(a.starts, r + 1), ld_uni(a.ends, r), a.prefix ? ld_uni(a.prefix, r) : 0);
 }
-// Keys that positions [p0, p1] see lie in [lo, hi), lo a multiple of STEP
-template <int STEP> __device__ __forceinline__ void keys_of(const PagedArgs& a, const Seq& x, int p0, int p1, int& lo, int& hi) {
-    lo = x.pre > 0 ? 0 : max(0, max(p0, 0) - a.W + 1) & ~(STEP - 1);
-    hi = p1 < 0 ? lo : min(x.klen, max(p1 + 1, x.pre));
-}
+// The tiles of STEP keys that positions [p0, p1] see: [lo, hi) from a multiple of STEP on, without the `gap` keys from `at` on that may lie between
+// a prefix and the band.  Tiles are numbered, counted and shared out without the gap.
+template <int STEP> struct Reach {
+    int lo, hi, at, gap;
+    Reach() = default;
+    __host__ __device__ __forceinline__ Reach(const PagedArgs& a, const Seq& x, int p0, int p1) {
+        const int band = max(0, max(p0, 0) - a.W + 1) & ~(STEP - 1);
+        lo = x.pre > 0 ? 0 : band;
+        hi = p1 < 0 ? lo : min(x.klen, max(p1 + 1, x.pre));
+        at = (x.pre + STEP - 1) & ~(STEP - 1);
+        gap = x.pre > 0 ? max(0, band - at) : 0;
+    }
+    __host__ __device__ __forceinline__ int key(int i) const {        // the i-th tile's first
+        const int y = lo + STEP * i;
+        return y + (y >= at ? gap : 0);
+    }
+    __host__ __device__ __forceinline__ int tiles() const {
+        const int n = (hi - lo + STEP - 1) / STEP;
+        return max(0, n - max(0, min(gap, lo + STEP * n - at)) / STEP);
+    }
+    __host__ __device__ __forceinline__ void upto(int n) { hi = min(hi, key(n - 1) + STEP); }      // the first n tiles alone (n >= 1)
+};
 
 // Equal shares of `total` tiles for G workers: worker w has those from begin(w) on.
 struct Shares {
     int G, q, rem;
-    __device__ __forceinline__ Shares(int total, int workers) : G(workers), q(total / workers), rem(total - q * workers) {}
-    __device__ __forceinline__ int begin(int w) const { return w * q + min(w, rem); }
-    __device__ __forceinline__ int owner(int x) const {               // of tile x
+    __host__ __device__ __forceinline__ Shares(int total, int workers) : G(workers), q(total / workers), rem(total - q * workers) {}
+    __host__ __device__ __forceinline__ int begin(int w) const { return w * q + min(w, rem); }
+    __host__ __device__ __forceinline__ int owner(int x) const {      // of tile x
         const int big = rem * (q + 1);
         return x < big ? x / (q + 1) : rem + (x - big) / q;
     }
@@ -161,19 +178,18 @@ template <int D, int ROWS, int NW> struct PageLoad {
     }
 };
 
-// The way through a unit's tiles of STEP keys: [lo, hi) without the gap that may lie between a prefix and the band, from the first-th one on, NW tiles at
-// a time
+// The way through a unit's tiles from the first-th one on, NW tiles at a time
 template <int STEP, int NW> struct Steps {
-    int j, hi, gap0, gap1;
-    __device__ __forceinline__ void enter(const PagedArgs& a, const Seq& x, int p0, int lo, int hi_, int first) {
-        j = lo + STEP * (first - NW);
-        hi = hi_;
-        gap0 = (x.pre + STEP - 1) & ~(STEP - 1);
-        gap1 = x.pre > 0 ? max(0, max(p0, 0) - a.W + 1) & ~(STEP - 1) : 0;
+    int y, j, hi, at, gap;                            // y: j without the gap
+    __host__ __device__ __forceinline__ void enter(const Reach<STEP>& x, int first) {
+        y = x.lo + STEP * (first - NW);
+        hi = x.hi;
+        at = x.at;
+        gap = x.gap;
     }
-    __device__ __forceinline__ bool next() {
-        j += STEP * NW;
-        if (j >= gap0 && j < gap1) j += (gap1 - j + STEP * NW - 1) / (STEP * NW) * (STEP * NW);
+    __host__ __device__ __forceinline__ bool next() {
+        y += STEP * NW;
+        j = y + (y >= at ? gap : 0);
         return j < hi;
     }
 };

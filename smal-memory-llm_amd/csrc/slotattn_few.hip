@@ -144,9 +144,7 @@ __device__ __forceinline__ int scan_up(int x, int lane, int most) {
 }
 // Tiles of QR rows of a sequence, and 32-key tiles of each: as many as its tokens see together, so that no table of them is needed
 template <int QR> __device__ __forceinline__ int few_tiles(const PagedArgs& a, const Seq& x, int& per) {
-    int lo, hi;
-    keys_of<32>(a, x, x.end - x.n, x.end - 1, lo, hi);
-    per = max(1, (hi - lo + 31) >> 5);
+    per = max(1, Reach<32>(a, x, x.end - x.n, x.end - 1).tiles());
     return (x.n * a.rep + QR - 1) / QR;
 }
 template <int QR> __device__ __forceinline__ int few_cost(const PagedArgs& a, int r) {
@@ -158,16 +156,17 @@ template <int QR> __device__ __forceinline__ int few_cost(const PagedArgs& a, in
 
 // A place in the worker's share: row, tiles of one head in front of it, the next tile and the share's end
 struct Place { int r, base, x, end; };
-// A unit: its sequence and head, tile of rows, and of its key tiles [ka, kb); positions of its rows; keys [lo, hi) up to the last of those tiles
+// A unit: its sequence and head, tile of rows, and of its key tiles [ka, kb); positions of its rows; its keys up to the last of those tiles
 struct FewUnit {
     Seq sq;
-    int r, hk, t, per, ka, kb, p0, p1, lo, hi;
+    int r, hk, t, per, ka, kb, p0, p1;
+    Reach<32> reach;
     template <int QR> __device__ __forceinline__ void rows(const PagedArgs& a) {
         const int n = sq.n * a.rep, off = sq.end - sq.n;
         p0 = QR * t / a.rep + off;
         p1 = (min(QR * (t + 1), n) - 1) / a.rep + off;
-        keys_of<32>(a, sq, p0, p1, lo, hi);
-        hi = min(hi, lo + 32 * kb);
+        reach = Reach<32>(a, sq, p0, p1);
+        reach.upto(kb);
     }
     // the next unit of a share
     template <int QR> __device__ __forceinline__ bool next(const PagedArgs& a, Place& at) {
@@ -251,7 +250,7 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
     const T* fv = nullptr;
     bool open = false;                                // f is in a unit
     auto enter = [&](const FewUnit& n) {
-        f.enter(a, n.sq, n.p0, n.lo, n.hi, n.ka + w);
+        f.enter(n.reach, n.ka + w);
         ftab = n.r * a.t_sr;
         flast = n.sq.klen - 1;
         fk = (const T*)a.k + n.hk * a.k_sh;
@@ -328,7 +327,7 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
         }
         const Sight sight(a, u.sq, u.p0, u.p1);
         Steps<32, NW> c;
-        c.enter(a, u.sq, u.p0, u.lo, u.hi, u.ka + w);
+        c.enter(u.reach, u.ka + w);
         // Keys and values are fetched two tiles ahead, each into the place that it has just been read from: a wave has one and a half to two
         // tiles on their way while it computes.
         for (; c.next(); buf ^= 1) {
@@ -401,15 +400,14 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
         const T* kb = (const T*)a.k + u.hk * a.k_sh;
         const T* vb = (const T*)a.v + u.hk * a.v_sh;
         const int32_t* tab = a.table + u.r * a.t_sr;
-        const int first = u.lo + 32 * u.ka;
+        const int first = u.reach.key(u.ka);
         auto keeps = [&](const Rows16<T, D, BIAS>& x) {
-            const int g0 = (u.sq.pre + 31) & ~31, g1 = u.sq.pre > 0 ? max(0, max(u.p0, 0) - a.W + 1) & ~31 : 0;      // (the gap that Steps leaves out)
-            return keeps_paged<T, D>(a, kb, vb, tab, x.see, first, u.hi, u.sq.klen, 32, Rows16<T, D, BIAS>::PARTS == 2, lane,
-                                     [&](int j) { return (j & ~31) < g0 || (j & ~31) >= g1; });
+            return keeps_paged<T, D>(a, kb, vb, tab, x.see, first, u.reach.hi, u.sq.klen, 32, Rows16<T, D, BIAS>::PARTS == 2, lane,
+                                     [&](int j) { return (j & ~31) < u.reach.at || (j & ~31) >= u.reach.at + u.reach.gap; });
         };
         auto exact = [&](const Rows16<T, D, BIAS>& x, int i, float& m1, float& l1, float (&o1)[D / 64]) {
             exact_paged<T, D, CAP, BIAS>(a, (const T*)a.q + lane_of(x.hq, i) * a.q_sh + (int64_t)(u.sq.s + lane_of(x.tok, i)) * a.q_st, kb, vb, tab,
-                                         lane_of(x.see, i), lane_of(x.slope, i), lane_of(x.p, i), first, u.hi, lane, m1, l1, o1);
+                                         lane_of(x.see, i), lane_of(x.slope, i), lane_of(x.p, i), first, u.reach.hi, lane, m1, l1, o1);
         };
         if constexpr (SHARED) {
             const bool whole = u.ka == 0 && u.kb == u.per;

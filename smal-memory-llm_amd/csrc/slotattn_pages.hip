@@ -101,9 +101,7 @@ __global__ __launch_bounds__(LT) void pages_plan(PagedArgs a) {
             lo = row_of(i);
             const Seq x = seq_of(a, lo);
             const int t = i - first[lo], off = x.end - x.n, last = min(MQ * (t + 1), x.n * a.rep) - 1;
-            int k0, k1;
-            keys_of<KT>(a, x, MQ * t / a.rep + off, last / a.rep + off, k0, k1);
-            c = ML + max(1, (k1 - k0 + KT - 1) / KT);
+            c = ML + max(1, Reach<KT>(a, x, MQ * t / a.rep + off, last / a.rep + off).tiles());
             atomicAdd(&s_count[LT - 1 - (c >> shift)], 1);
         }
         int most = c;
@@ -250,15 +248,14 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
         const int p0 = MQ * t / a.rep + off, p1 = (min(MQ * (t + 1), rows) - 1) / a.rep + off;
         Sight sight(a, sq, row0 / a.rep + off, (min(row0 + 32, rows) - 1) / a.rep + off);
         if (row0 >= rows) sight.s1 = -1, sight.s2 = 0;               // a wave without rows
-        int lo, hi;
-        keys_of<KT>(a, sq, p0, p1, lo, hi);
-        hi = min(hi, lo + kb * KT);
+        Reach<KT> reach(a, sq, p0, p1);
+        reach.upto(kb);
         const T* kbase = (const T*)a.k + hk * a.k_sh;
         const T* vbase = (const T*)a.v + hk * a.v_sh;
         const int64_t tab = r * a.t_sr;
         const int last = sq.klen - 1;
         Steps<KT, 1> f;                               // the tile that is fetched
-        f.enter(a, sq, p0, lo, hi, ka);
+        f.enter(reach, ka);
         Pages<KT / 16> pg;
         auto load = [&](int buf) {
             pg.check(a);
@@ -357,7 +354,7 @@ __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {
         asm volatile("" : "+v"(ln));
         const int row1 = min(row0 + (ln & 31), rows - 1), tok1 = row1 / a.rep;
         const Rows rw{sq.s, tok1, hk * a.rep + row1 - tok1 * a.rep, tok1 + off, min(32, rows - row0), see, slope};
-        finish<T, D, CAP, BIAS>(a, sum, rw, kbase, vbase, a.table + r * a.t_sr, lo + ka * KT, hi, sq.klen, ka == 0 && kb == c,
+        finish<T, D, CAP, BIAS>(a, sum, rw, kbase, vbase, a.table + r * a.t_sr, reach.key(ka), reach.hi, sq.klen, ka == 0 && kb == c,
                                 ((int64_t)(2 * me + (ka == 0)) * MW + w) * 32, lane, [&](int j) { return sight.some(j & -KT, j | (KT - 1)); });
         if (ka == 0 && kb < c) left = {r, hk, t, sq.n, sh.owner(end + c - kb - 1) - me + 1};        // its other pieces: up to the worker of its last tile
     }

@@ -115,3 +115,21 @@ def test_the_least_prefix_is_none(news, ctxs, window):
         got = A.attend_pages(q.cuda(), k.cuda(), v.cuda(), table.cuda(), starts_of(news).cuda(), ints(ends), most=most, window=window,
                              prefix=ints([-2 ** 31] * len(news)))
         near(got, ref, bound, "out")
+
+
+@pytest.mark.parametrize("Hq,Hk,D,dt,page", [(6, 2, 128, BF, 16), (4, 1, 64, HF, 128)])
+@pytest.mark.parametrize("news,ctxs,most", [([1, 1, 1, 1], [5000, 900, 64, 2777], 1), ([3, 1, 6], [4000, 2500, 30], 6), ([200, 1, 40, 300], [3000, 2000, 1500, 0], None),
+                                            ([1], [9000], 1), ([128] * 6, [2500] * 6, None)])
+@pytest.mark.parametrize("window,prefix", [(1, 1), (33, 65), (200, 300), (64, 900)])
+def test_a_prefix_far_before_the_window(Hq, Hk, D, dt, page, news, ctxs, most, window, prefix):
+    """Most keys lie between the two and are nobody's; they hold NaN here, but for those in the tiles at both ends."""
+    ends = [c + n for c, n in zip(ctxs, news)]
+    k, v, table = pool(ends, PO.up(max(ends), page) + 1, page, Hk, D, dt, 32)
+    for r, (n, end) in enumerate(zip(news, ends)):
+        for j in range(-(-prefix // 64) * 64, (end - n - window + 1) // 64 * 64):
+            k[table[r, j // page], :, j % page] = v[table[r, j // page], :, j % page] = float("nan")
+    q = queries(sum(news), Hq, D, dt, 33)
+    pre = torch.full((len(news),), prefix, dtype=torch.int32)
+    got = A.attend_pages(q.cuda(), k.cuda(), v.cuda(), table.cuda(), starts_of(news).cuda(), ints(ends), most=most, window=window, prefix=pre.cuda())
+    ref, bound = reference(q, k, v, table, news, ends, U[dt], window=window, prefix=pre.long())
+    near(got, ref, bound, "out")

@@ -51,3 +51,94 @@ int main() {
     }
 }
 """)
+
+
+def test_shares_count_the_tiles_that_are_visited(tmp_path):
+    """With a prefix and a window far behind it, the tiles between them cost nothing and are nobody's: a unit's number of tiles is that of the tiles in which
+    one of its rows sees a key, its parts visit them all once, each as many as its share has, and four waves of a workgroup visit them, too."""
+    _run(tmp_path, """
+#include <vector>
+#include <algorithm>
+template <int STEP> void look(const PagedArgs& a, const Seq& x, int p0, int p1) {
+    std::vector<int> want;                            // the first keys of tiles that somebody sees
+    const int lo = std::max(0, std::max(p0, 0) - a.W + 1), hi = std::min(x.klen, p1 + 1), pre = p1 >= 0 ? std::min(x.pre, x.klen) : 0;
+    for (int j = 0; j < x.klen; j += STEP)
+        if ((lo < hi && j < hi && j + STEP > lo) || j < pre) want.push_back(j);
+    const Reach<STEP> all(a, x, p0, p1);
+    CHECK(all.tiles() == (int)want.size());
+    const int n = std::max(1, all.tiles());
+    std::vector<int> got;
+    for (int ka = 0; ka < n;) {
+        const int kb = std::min(n, ka + rnd(1, std::max(1, n / 3)));
+        Reach<STEP> part = all;
+        part.upto(kb);
+        Steps<STEP, 1> s;
+        s.enter(part, ka);
+        const size_t before = got.size();
+        while (s.next()) got.push_back(s.j);
+        CHECK(want.empty() ? got.empty() : (int)(got.size() - before) == kb - ka && got[before] == all.key(ka));
+        ka = kb;
+    }
+    CHECK(got == want);
+    got.clear();
+    for (int w = 0; w < 4; w++) {
+        Steps<STEP, 4> s;
+        s.enter(all, w);
+        while (s.next()) got.push_back(s.j);
+    }
+    std::sort(got.begin(), got.end());
+    CHECK(got == want);
+    Reach<STEP> far = all;                            // a bound past every tile
+    far.upto(0xffffff);
+    CHECK(far.hi == all.hi);
+}
+int main() {
+    for (int i = 0; i < 20000; i++) {
+        PagedArgs a{};
+        a.shift = rnd(4, 8);
+        a.M = rnd(1, 4000 >> a.shift);
+        a.N = 1000;
+        const int end = rnd(0, 3) ? rnd(0, a.M << a.shift) : rnd(0, 9000), n = rnd(1, rnd(0, 1) ? 3 : 400);
+        a.W = rnd(0, 3) ? rnd(1, rnd(0, 1) ? 40 : 2000) : 1 << 30;
+        const Seq x = make_seq(a, 5, 5 + n, end, rnd(0, 3) ? rnd(-3, rnd(0, 1) ? 100 : 5000) : rnd(0, 1) ? INT_MIN : INT_MAX);
+        const int p0 = x.end - x.n + rnd(0, x.n - 1), p1 = std::min(x.end - 1, p0 + rnd(0, 40));
+        look<32>(a, x, p0, p1);
+        look<64>(a, x, p0, p1);
+        // no unit has more tiles than the number that all units of a sequence of few rows have
+        const int most = std::max(1, Reach<32>(a, x, x.end - x.n, x.end - 1).tiles());
+        CHECK((Reach<32>(a, x, p0, p1).tiles() <= most));
+    }
+    // the far ends: no sum leaves 32 bits (an overflow traps)
+    for (int pre : {INT_MIN, -1, 0, 1, 1 << 29, INT_MAX})
+        for (int W : {1, 2, 1 << 29, 1 << 30})
+            for (int end : {INT_MIN, 0, 1, 1 << 29, (1 << 30) - 1, INT_MAX}) {
+                PagedArgs a{};
+                a.shift = 12; a.M = 0x3fffffff >> 12; a.N = 1 << 20; a.W = W;
+                const Seq x = make_seq(a, 0, 1 << 20, end, pre);
+                for (int p0 : {x.end - x.n, x.end - 1}) {
+                    Reach<64> r(a, x, p0, x.end - 1);
+                    CHECK(r.tiles() >= 0 && r.tiles() <= (1 << 24) && r.key(0xffffff - 1) >= 0);
+                    r.upto(0xffffff);
+                    Steps<64, 4> s;
+                    s.enter(r, std::max(0, r.tiles() - 2));
+                    for (int i = 0; i < 3 && s.next(); i++) CHECK(s.j >= 0 && s.j < x.klen);
+                }
+            }
+}
+""")
+
+
+def test_equal_shares_meet_end_to_end(tmp_path):
+    _run(tmp_path, """
+int main() {
+    for (int i = 0; i < 3000; i++) {
+        const int G = rnd(1, 2048), total = rnd(G, rnd(0, 1) ? 20000 : 0x3fffffff);
+        const Shares s(total, G);
+        CHECK(s.begin(0) == 0 && s.begin(G) == total && s.owner(0) == 0 && s.owner(total - 1) == G - 1);
+        for (int k = 0; k < 20; k++) {
+            const int w = rnd(0, G - 1);
+            CHECK(s.begin(w) < s.begin(w + 1) && s.owner(s.begin(w)) == w && s.owner(s.begin(w + 1) - 1) == w);
+        }
+    }
+}
+""")
