@@ -60,7 +60,8 @@ int slotattn_bwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const 
  * of the N, ascending (tokens of no row get 0); the i-th of its n is at position ends[r] - n + i and sees, by causality, window and prefix as
  * above, keys of positions below ends[r] (ends[r] > M page reads M page keys; a query of negative position sees nothing).  The key at position j
  * is row j % page of page table[r][j / page]; keys of a page outside [0, P) are not seen.
- *   q by strides (head, token), k, v (P, Hk, page, D) by strides (page, head, row within the page), every row 16-byte aligned; page a power of two
+ *   q by strides (head, token), k, v (P, Hk, page, D) by strides (page, head, row within the page), every row 16-byte aligned, pages fewer than
+ *           2^31 elements apart and rows fewer than 2^25; page a power of two
  *           in [16, 4096]; table rows t_sr elements apart; starts (R + 1), ends (R), prefix (R) int32; out (N, Hq, D) contiguous
  *   most    an upper bound of the rows' numbers of tokens, or N.  It chooses between kernels; results do not depend on it but for rounding
  * Nothing outside the tensors is read or written whatever table, starts and ends hold.  Rows must not share tokens (starts that fall): what these

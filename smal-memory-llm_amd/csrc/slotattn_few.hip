@@ -11,12 +11,14 @@
 // order of key_row: a transposing read then meets every bank once (its lanes 0 .. 31 have rows 0 .. 3 and 8 .. 11).
 // 16 query rows a product, not 32: of a group's 3 or 4 query heads and one token, tiles of 32 x 32 would be nearly empty, at twice the vector work.
 //
-// Bound by memory: a step reads each sequence's keys and values once (running maxima and sums, nothing stored between the products).  A call is 8 us, in
-// which the first keys are found (the rows' costs, a search, page numbers) and arrive, and its bytes at 6.2 TB/s (a large read alone: 5.8 with its
-// start).  32 sequences of 1,024 to 8,191 keys, 12 heads of 128 on 4, cap 50 (260 MB): 54 us, 4.8 TB/s; one of 131,072 keys (268 MB) 53; 256
-// with a window of 1,024 (315 MB) 74, where a unit is hardly longer than a share, so most are cut in two; 2 to 8 tokens of 16 sequences of up to
-// 16,000 (195 MB) 48, two tiles of rows and vector issue beside the loads.  1,024 waves, one a SIMD, each with two tiles on their way (32 KB at
-// D = 128); with 1,280 no change.
+// Bound by memory: a step reads each sequence's keys and values once (running maxima and sums, nothing stored between the products).  One sequence of 131,072,
+// 262,144 and 524,288 keys takes 52, 96 and 184 us: 8 us, in which the first keys are found (the rows' costs, a search, page numbers) and arrive, and its
+// bytes at 6.1 TB/s (a large read alone: 5.8 with its start).  32 sequences of 1,024 to 8,191 keys, 12 heads of 128 on 4, cap 50 (260 MB): 55 us, 4.8
+// TB/s; one of 131,072 keys (268 MB) 53; 256 with a window of 1,024 (315 MB) 74, where a unit is hardly longer than a share, so most are cut in two; 2 to 8
+// tokens of 16 sequences of up to 16,000 (195 MB) 46: two tiles of rows, both computed also where a sequence's rows fit into one.  1,024 waves, one a SIMD,
+// each with a ring of two tiles (32 KB at D = 128); with 1,280 no change.
+// Each wave goes through the rows' lengths by itself, 64 at a time.  Rows of 512 keys: 256 46 us, 1,024 197, 8,192 1,535 (5.6 TB/s); on pages_many with its
+// plan 53, 202 and 1,541.
 #include "slot_attn_pages.h"
 #include "slotscan.h"
 #include "slot_attn_few.h"
@@ -328,8 +330,10 @@ __global__ __launch_bounds__(64 * NW) void pages_few(PagedArgs a) {
         const Sight sight(a, u.sq, u.p0, u.p1);
         Steps<32, NW> c;
         c.enter(u.reach, u.ka + w);
-        // Keys and values are fetched two tiles ahead, each into the place that it has just been read from: a wave has one and a half to two
-        // tiles on their way while it computes.
+        // Keys and values are fetched two tiles ahead, each into the place that it has just been read from.  With slopes the counted waits are the loop's only
+        // ones, and a wave has one and a half to two tiles on their way while it computes.  Without them it has less: the compiler does not know that the counted
+        // waits cover the query rows' loads and waits for these where they are first used, in the loop, which in every tile is a wait for all that is
+        // outstanding.  This tile's values and the whole next tile are there before its first product, and only the tile after that comes in beside the rest.
         for (; c.next(); buf ^= 1) {
             const int j0 = c.j;
             if (e1) wait_vm<3 * Load::N>();           // behind this tile's keys: its values, the next keys and values

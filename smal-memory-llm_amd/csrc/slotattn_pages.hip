@@ -177,9 +177,12 @@ struct PairShares {
 // they are; 64-key tiles by direct loads into two buffers, one barrier a tile.  What differs is where keys lie (a group of 16 keys is of one
 // page: its address is scalar) and who does what: a workgroup a whole unit, or 512 workers with equal shares of all key tiles, in which a unit may begin and
 // end anywhere; pages_plan chooses.
-// Bound by vector issue beside the matrix products where rows are many, by memory where a unit has a token alone (three waves of four then only load).
-// Two prompts of 4,096 tokens, 12 heads of 128 on 4: 140 to 147 us by the box, 700 to 740 TFLOP/s (attn_fwd without pages 122 to 130); 56 tokens and 4
-// prompts of 300 to 1,200 with 200 to 4,000 keys before them, pages of 16: 85 us, of which the prompts alone take 61, the tokens alone 28 (140 MB).  With 8
+// Bound by issue beside the matrix products where rows are many, by memory where a unit has a token alone (three waves of four then only load; the unit's tiles
+// count as any other's).  Two prompts of 4,096 tokens, 12 heads of 128 on 4: 120 us call after call, 860 TFLOP/s (attn_fwd without pages, in the same process,
+// 113); 151 in the first calls of a process, under the profiler.  Of its cycles the matrix units are busy 41 %, vector instructions are issued in 44 % and scalar
+// ones in 21 %.  Some of both are the register allocator's: 141 to 196 scalar registers are kept in lanes of vector registers (attn_fwd: 37 to 109), and read
+// back in every tile.  56 tokens and 4 prompts of 300 to 1,200 with 200 to 4,000 keys before them, pages of 16: 89 us in such first calls; measured apart
+// before, the prompts took 61 and the tokens 28 (140 MB) of 85.  With 8
 // waves a workgroup (256 rows, halves of it half a tile apart) 153 where shares took 150, and 127 instead of 79 for the mixture, whose units are small.
 template <typename T, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(MT, 2) void pages_many(PagedArgs a) {

@@ -19,7 +19,7 @@ are not enough -- packed documents, long windows, prompts read both ways, capped
         the serving form over a cache in pages (slotpage_hip): q (N, Hq, D) holds the newest tokens of R sequences, packed --
         one token each, a few, whole prompts, in any mixture; row r's are starts[r] .. starts[r + 1] - 1 (starts (R + 1,) int32,
         ascending), the last of them at position ends[r] - 1 (ends (R,) int32).  Its keys and values are the first ends[r] rows of the
-        pages table[r] (table (R, M) int32) of kpages, vpages (P, Hk, page, D).  Keys of a page outside [0, P) are not seen; tokens
+        pages table[r] (table (R, M) int32) of kpages, vpages (P, Hk, page, D), pages fewer than 2^31 elements apart.  Keys of a page outside [0, P) are not seen; tokens
         of no row, and of rows with ends[r] = 0, get 0.  `most` is an upper bound of the rows' numbers of tokens that the host knows
         (None: N): it chooses between kernels, and results depend on it by rounding alone.
 
